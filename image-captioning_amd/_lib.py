@@ -198,6 +198,9 @@ SIGNATURES = {
     "mic_lstm_cell_ln": (C.c_int, [vp, vp, vp, vp, C.c_int, vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, vp]),
     "mic_gather_rows": (C.c_int, [vp, vp, vp, C.c_int, C.c_int, vp]),
     "mic_gather_rows_multi": (C.c_int, [vp, vp, vp, C.c_int, vp, C.c_int, vp]),
+    "mic_embed_rows": (C.c_int, [vp, C.c_int, vp, i64, vp, i64, vp, C.c_int, C.c_int, f32, i64, C.c_int, C.c_int, C.c_int, vp]),
+    "mic_embed_grad_workspace_bytes": (C.c_int64, [i64, C.c_int, C.c_int, C.c_int, C.c_int]),
+    "mic_embed_grad": (C.c_int, [vp, C.c_int, vp, vp, vp, C.c_int, C.c_int, f32, i64, C.c_int, C.c_int, C.c_int, vp, i64, vp]),
     "mic_logsoftmax_topk": (C.c_int, [vp, C.c_int, C.c_int, C.c_int, C.c_int, f32, C.c_int, vp, vp, vp, vp]),
     "mic_sample_multinomial": (C.c_int, [vp, C.c_int, C.c_int, C.c_int, f32, vp, vp, vp, vp]),
     "mic_beam_select": (C.c_int, [P(BeamState), P(BeamState), vp, vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int,

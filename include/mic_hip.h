@@ -493,6 +493,29 @@ int mic_sample_update(const float* val, const int32_t* idx, int32_t* tokens, int
                       void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Teacher-forced operators: whole caption sequences at once, each with its gradient.  What a training step of the decoder
+ * (train.py:163-206 cross entropy, train.py:209-262 reward-weighted) runs where the step kernels above take one position.
+ * Workspaces: caller-allocated device memory of at least *_workspace_bytes(same sizes) bytes, 16-byte aligned, contents
+ * arbitrary before and after; two calls that may overlap in time need two workspaces.  Sums are taken in fp32 in a fixed order
+ * (no atomics on values): the same inputs give the same bits.
+ * ---------------------------------------------------------------------------------------- */
+
+/* out[n, :] = scale * table[ids[n], :] + pos[n mod T, :], rounded once to out_dtype (SeqEmbedding.forward over a whole caption,
+ * models/transformer.py:44-50; nn.Embedding at models/basic.py:43, models/intermediate.py:59).  ids: ids_bits 32 or 64; ids
+ * outside [0, vocab) read the nearest row of the table, as in mic_embed_pos.  table [vocab][ld_table], pos [T][ld_pos] or NULL,
+ * both table_dtype; out [n][H] out_dtype.  n < 2^31. */
+int mic_embed_rows(const void* ids, int ids_bits, const void* table, int64_t ld_table, const void* pos, int64_t ld_pos, void* out,
+                   int table_dtype, int out_dtype, float scale, int64_t n, int T, int H, int vocab, void* stream);
+
+/* Gradient of mic_embed_rows: d_table [vocab][H] = scale * the sum of g's rows [n][H] per word (zero rows for words that do not
+ * occur), and d_pos [T][H] = the sum over sequences (NULL = not wanted; n must then be a multiple of T).  g is g_dtype, both
+ * outputs out_dtype.  The tokens are sorted by word, so no row is summed by atomics.  n < 2^30; n = 0 clears the outputs.
+ * mic_embed_grad_workspace_bytes returns MIC_ERR_ARG for sizes the gradient would refuse. */
+int64_t mic_embed_grad_workspace_bytes(int64_t n, int T, int H, int vocab, int want_pos);
+int mic_embed_grad(const void* ids, int ids_bits, const void* g, void* d_table, void* d_pos, int g_dtype, int out_dtype, float scale,
+                   int64_t n, int T, int H, int vocab, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Whole-path drivers: the same kernels chained natively so the host issues one call per phase.
  * ---------------------------------------------------------------------------------------- */
 
