@@ -67,6 +67,13 @@ class AttnFusedDesc(C.Structure):
                 ("S", i32), ("rows_per_image", i32), ("t", i32), ("t_cap", i32)]
 
 
+class AttnSeqDesc(C.Structure):
+    _fields_ = [("q", vp), ("k", vp), ("v", vp), ("o", vp), ("lse", vp), ("key_mask", vp), ("grad_o", vp), ("dq", vp), ("dk", vp), ("dv", vp),
+                ("q_stride", i64 * 3), ("k_stride", i64 * 3), ("v_stride", i64 * 3), ("o_stride", i64 * 3), ("g_stride", i64 * 3),
+                ("mask_stride", i64), ("dtype", i32), ("B", i32), ("Tq", i32), ("Tk", i32), ("Hq", i32), ("Hkv", i32), ("D", i32),
+                ("causal", i32), ("scale", f32), ("workspace", vp), ("workspace_bytes", i64)]
+
+
 class BeamState(C.Structure):
     _fields_ = [("score", vp), ("len", vp), ("seq", vp), ("anc", vp)]
 
@@ -201,6 +208,9 @@ SIGNATURES = {
     "mic_embed_rows": (C.c_int, [vp, C.c_int, vp, i64, vp, i64, vp, C.c_int, C.c_int, f32, i64, C.c_int, C.c_int, C.c_int, vp]),
     "mic_embed_grad_workspace_bytes": (C.c_int64, [i64, C.c_int, C.c_int, C.c_int, C.c_int]),
     "mic_embed_grad": (C.c_int, [vp, C.c_int, vp, vp, vp, C.c_int, C.c_int, f32, i64, C.c_int, C.c_int, C.c_int, vp, i64, vp]),
+    "mic_attn_seq_workspace_bytes": (C.c_int64, [P(AttnSeqDesc), C.c_int]),
+    "mic_attn_seq": (C.c_int, [P(AttnSeqDesc), vp]),
+    "mic_attn_seq_grad": (C.c_int, [P(AttnSeqDesc), vp]),
     "mic_logsoftmax_topk": (C.c_int, [vp, C.c_int, C.c_int, C.c_int, C.c_int, f32, C.c_int, vp, vp, vp, vp]),
     "mic_sample_multinomial": (C.c_int, [vp, C.c_int, C.c_int, C.c_int, f32, vp, vp, vp, vp]),
     "mic_beam_select": (C.c_int, [P(BeamState), P(BeamState), vp, vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int,

@@ -1,0 +1,192 @@
+// Pieces shared by the whole-sequence attention kernels (attn_seq_fwd.hip, attn_seq_dq.hip, attn_seq_dkv.hip): arguments, the
+// LDS tile image, MFMA fragments and tile staging.
+//
+// Query heads that share a key head are packed: a "row" r of key head hk is query i = r / group of query head
+// hk * group + r % group, so one pass over the keys serves the whole group, and the gradients of a shared key head are sums over
+// its rows.
+//
+// All products run on 32x32 MFMA tiles.  Lane l, half h = l >> 5: operand A holds row l & 31, B column l & 31, both the eight
+// reduction indices 8h..8h+7 of a step of 16; the result holds column l & 31 and rows 8*(r >> 2) + 4h + (r & 3) of register r.
+// Eight consecutive result registers therefore are one B operand of the next product if its reduction index is taken in the
+// order 4h..4h+3, 8+4h..8+4h+3: the probabilities go from one product into the next without leaving their lanes, and the
+// other operand is read from LDS in that order (a transposing read in bf16, eight scalar reads in fp32).
+#pragma once
+#include "mic_common.h"
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+struct AttnSeqArgs {
+    const void *q, *k, *v, *g;      // g: gradient of the output
+    void *o, *dq, *dk, *dv;
+    float *lse, *delta, *part, *part_ml;
+    const unsigned char* mask;      // [B][Tk], non-zero = the key may be seen, or NULL
+    long long mask_sb;
+    long long q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh, o_sb, o_st, o_sh, g_sb, g_st, g_sh;  // element strides
+    int B, Tq, Tk, Hq, Hkv, D, group, R;  // R = Tq * group rows per key head
+    int causal, off;                // query i sees keys up to i + off
+    float scale, scale_log2;
+    int splits, tiles_per_split;
+};
+
+namespace {
+
+constexpr float ATTN_LOG2E = 1.4426950408889634f, ATTN_LN2 = 0.6931471805599453f;
+
+template <typename T> struct Frag8;
+template <> struct Frag8<bf16_t> {
+    bf16x8_t v;
+};
+template <> struct Frag8<float> {
+    float v[8];
+};
+
+__device__ __forceinline__ void mma32(const Frag8<bf16_t>& a, const Frag8<bf16_t>& b, f32x16_t& c) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, b.v, c, 0, 0, 0);
+}
+// 32x32x2 takes one reduction index per half: step e pairs indices e of both halves, as the bf16 fragment lays them out
+__device__ __forceinline__ void mma32(const Frag8<float>& a, const Frag8<float>& b, f32x16_t& c) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[e], b.v[e], c, 0, 0, 0);
+}
+
+template <typename T> __device__ __forceinline__ Frag8<T> frag_zero() {
+    Frag8<T> f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f.v[e] = (T)0.f;
+    return f;
+}
+// registers 8j..8j+7 of a result tile as the B operand of the next product
+template <typename T> __device__ __forceinline__ Frag8<T> frag_of(const f32x16_t& p, int j) {
+    Frag8<T> f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f.v[e] = (T)p[8 * j + e];
+    return f;
+}
+
+// LDS image of a tile of rows of DP elements: 16-byte chunk c of row r is stored at chunk c ^ tile_swizzle(r).  Both kinds of
+// read then spread over all 64 banks: the same chunk of 16 consecutive rows (row operands), and 32 columns of the 4 rows a
+// transposing read takes together.
+template <typename T, int DP> struct Tile {
+    static constexpr int E = 16 / (int)sizeof(T);     // elements per chunk
+    static constexpr int CPR = DP / E;                // chunks per row
+    __device__ static __forceinline__ int swizzle(int r) {
+        if constexpr (CPR == 4) return (r >> 2) & 3;
+        else if constexpr (CPR == 8) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+        else return ((r & 3) << 2) | ((r >> 2) & 3);
+    }
+    __device__ static __forceinline__ int at(int r, int c) { return r * DP + ((c ^ swizzle(r)) * E); }
+};
+
+// row operand: row r, reduction step c (16 columns)
+template <int DP> __device__ __forceinline__ Frag8<bf16_t> read_row(const bf16_t* t, int r, int c, int h) {
+    Frag8<bf16_t> f;
+    f.v = *reinterpret_cast<const bf16x8_t*>(t + Tile<bf16_t, DP>::at(r, 2 * c + h));
+    return f;
+}
+template <int DP> __device__ __forceinline__ Frag8<float> read_row(const float* t, int r, int c, int h) {
+    Frag8<float> f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const float4 x = *reinterpret_cast<const float4*>(t + Tile<float, DP>::at(r, 4 * c + 2 * h + k));
+        f.v[4 * k] = x.x; f.v[4 * k + 1] = x.y; f.v[4 * k + 2] = x.z; f.v[4 * k + 3] = x.w;
+    }
+    return f;
+}
+// column operand: column d0 + (lane & 31), rows r0 + {4h..4h+3, 8+4h..8+4h+3}
+typedef short v4i16_t __attribute__((ext_vector_type(4)));
+template <int DP> __device__ __forceinline__ Frag8<bf16_t> read_col(const bf16_t* t, int d0, int r0, int lane) {
+    // every 16 lanes exchange a 4 x 16 block: lane j reads row j / 4, columns 4 (j mod 4)..+3 and receives column j of the four rows
+    const int h = lane >> 5, j = lane & 15, col = d0 + ((lane >> 4) & 1) * 16 + (j & 3) * 4, row = r0 + 4 * h + (j >> 2);
+    typedef __attribute__((address_space(3))) v4i16_t* lds_t;
+    const v4i16_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(t + Tile<bf16_t, DP>::at(row, col >> 3) + (col & 7)));
+    const v4i16_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(t + Tile<bf16_t, DP>::at(row + 8, col >> 3) + (col & 7)));
+    typedef short v8i16_t __attribute__((ext_vector_type(8)));
+    Frag8<bf16_t> f;
+    f.v = __builtin_bit_cast(bf16x8_t, (v8i16_t)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    return f;
+}
+template <int DP> __device__ __forceinline__ Frag8<float> read_col(const float* t, int d0, int r0, int lane) {
+    const int h = lane >> 5, col = d0 + (lane & 31);
+    Frag8<float> f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f.v[e] = t[Tile<float, DP>::at(r0 + 4 * h + (e & 3) + (e >> 2) * 8, col >> 2) + (col & 3)];
+    return f;
+}
+
+// fp32 with more than 128 columns: the wave's own operands do not fit the registers next to the sums, they are read again for
+// every tile
+template <typename T, int DP> struct InRegs {
+    static constexpr bool value = sizeof(T) == 2 || DP <= 128;
+};
+
+// eight consecutive elements of a row in memory, zero past the head's D columns
+template <typename T> __device__ __forceinline__ Frag8<T> load_frag(const T* row, int col, int D) {
+    Frag8<T> f = frag_zero<T>();
+    if constexpr (sizeof(T) == 2) {
+        if (row && col < D) f.v = *reinterpret_cast<const bf16x8_t*>(row + col);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            if (row && col + 4 * k < D) {
+                const float4 x = *reinterpret_cast<const float4*>(row + col + 4 * k);
+                f.v[4 * k] = x.x; f.v[4 * k + 1] = x.y; f.v[4 * k + 2] = x.z; f.v[4 * k + 3] = x.w;
+            }
+    }
+    return f;
+}
+
+// ROWS rows into a tile; row_ptr(r) is the row's address or NULL for a row of zeros
+template <typename T, int DP, int ROWS, int THREADS, typename P> __device__ __forceinline__ void stage(T* tile, int D, P row_ptr) {
+    using L = Tile<T, DP>;
+    constexpr int ALL = ROWS * L::CPR, N = (ALL + THREADS - 1) / THREADS;
+    constexpr int G = N < 8 ? N : 8;  // loads in flight per thread
+    static_assert(N % G == 0 && (N == 1 || ALL % THREADS == 0), "whole rounds");
+#pragma unroll
+    for (int n0 = 0; n0 < N; n0 += G) {
+        uint4 x[G];
+#pragma unroll
+        for (int n = 0; n < G; ++n) {
+            const int i = threadIdx.x + (n0 + n) * THREADS, r = i / L::CPR, c = i % L::CPR;
+            const T* p = ALL >= THREADS || i < ALL ? row_ptr(r) : nullptr;
+            x[n] = p && c * L::E < D ? *reinterpret_cast<const uint4*>(p + c * L::E) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int n = 0; n < G; ++n) {
+            const int i = threadIdx.x + (n0 + n) * THREADS, r = i / L::CPR, c = i % L::CPR;
+            if (ALL >= THREADS || i < ALL) *reinterpret_cast<uint4*>(tile + L::at(r, c)) = x[n];
+        }
+    }
+}
+
+// four consecutive columns of a result, rounded once
+template <typename T> __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
+    if constexpr (sizeof(T) == 2) {
+        typedef bf16_t v4 __attribute__((ext_vector_type(4)));
+        *reinterpret_cast<v4*>(p) = v4{(bf16_t)a, (bf16_t)b, (bf16_t)c, (bf16_t)d};
+    } else {
+        *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
+    }
+}
+
+// bit j: key k0 + j exists and may be seen (causality aside); the same word in every lane
+__device__ __forceinline__ unsigned key_bits(const AttnSeqArgs& a, int b, int k0, int lane) {
+    const int key = k0 + (lane & 31);
+    bool ok = key < a.Tk;
+    if (ok && a.mask) ok = a.mask[b * a.mask_sb + key] != 0;
+    return (unsigned)__ballot(ok);
+}
+__device__ __forceinline__ bool key_seen(const AttnSeqArgs& a, int b, int key) { return key < a.Tk && (!a.mask || a.mask[b * a.mask_sb + key] != 0); }
+
+}  // namespace
+
+// rows of a workgroup of the forward and query-gradient kernels, keys of one of the key-gradient kernel
+#define ATTN_SEQ_BLOCK 128
+
+// keys per tile of the forward and query-gradient kernels
+template <typename T, int DP> struct KeyTile {
+    static constexpr int value = DP * sizeof(T) <= 256 ? 64 : 32;
+};
+
+int mic_attn_seq_fwd_launch(const AttnSeqArgs& a, int dtype, hipStream_t s);
+int mic_attn_seq_dq_launch(const AttnSeqArgs& a, int dtype, hipStream_t s);
+int mic_attn_seq_dkv_launch(const AttnSeqArgs& a, int dtype, hipStream_t s);

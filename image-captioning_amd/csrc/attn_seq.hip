@@ -1,0 +1,147 @@
+// Whole-sequence attention: argument checks, the rules that split the work, and the entry points.
+#include "attn_seq.h"
+
+namespace {
+
+constexpr long long MAX_STRIDE = 1ll << 40;
+
+int head_columns(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256; }
+
+int check_tensor(const char* who, const char* name, const void* p, const int64_t st[3], int dtype, bool empty) {
+    if (empty) return 0;
+    MIC_ARG_CHECK(p, "%s: %s is a null pointer", who, name);
+    const int e = 16 / (int)mic_dtype_size(dtype);
+    MIC_ARG_CHECK(((uintptr_t)p & 15) == 0, "%s: %s is not 16-byte aligned", who, name);
+    for (int i = 0; i < 3; ++i)
+        MIC_ARG_CHECK(st[i] >= 0 && st[i] < MAX_STRIDE && st[i] % e == 0, "%s: stride %lld of %s is not a multiple of 16 bytes", who, (long long)st[i], name);
+    return 0;
+}
+
+int check_sizes(const char* who, const mic_attn_seq_desc* d) {
+    MIC_ARG_CHECK(d, "%s: null descriptor", who);
+    MIC_ARG_CHECK(d->dtype == MIC_F32 || d->dtype == MIC_BF16, "%s: bad dtype %d", who, d->dtype);
+    MIC_ARG_CHECK(d->B >= 0 && d->Tq >= 0 && d->Tk >= 0 && d->Hq > 0 && d->Hkv > 0 && d->D > 0, "%s: bad sizes B=%d Tq=%d Tk=%d Hq=%d Hkv=%d D=%d", who, d->B, d->Tq,
+                  d->Tk, d->Hq, d->Hkv, d->D);
+    MIC_ARG_CHECK(d->Hq % d->Hkv == 0, "%s: %d query heads do not share %d key heads evenly", who, d->Hq, d->Hkv);
+    MIC_ARG_CHECK(d->D <= 256 && d->D % (16 / (int)mic_dtype_size(d->dtype)) == 0, "%s: heads of %d columns (at most 256, whole 16 bytes)", who, d->D);
+    const long long lim = 1ll << 30;  // row and key numbers are 32-bit, grids as well
+    const long long group = d->Hq / d->Hkv, R = d->Tq * group;
+    MIC_ARG_CHECK(R < lim && d->Tk < lim && ((R + 127) / 128 + 1) * d->Hkv * (long long)d->B < lim && (((long long)d->Tk + 127) / 128 + 1) * d->Hkv * (long long)d->B < lim,
+                  "%s: too many rows (B=%d Tq=%d Tk=%d Hq=%d)", who, d->B, d->Tq, d->Tk, d->Hq);
+    return 0;
+}
+
+AttnSeqArgs args_of(const mic_attn_seq_desc* d) {
+    AttnSeqArgs a = {};
+    a.q = d->q; a.k = d->k; a.v = d->v; a.g = d->grad_o;
+    a.o = d->o; a.dq = d->dq; a.dk = d->dk; a.dv = d->dv;
+    a.lse = d->lse;
+    a.mask = d->key_mask; a.mask_sb = d->mask_stride;
+    a.q_sb = d->q_stride[0]; a.q_st = d->q_stride[1]; a.q_sh = d->q_stride[2];
+    a.k_sb = d->k_stride[0]; a.k_st = d->k_stride[1]; a.k_sh = d->k_stride[2];
+    a.v_sb = d->v_stride[0]; a.v_st = d->v_stride[1]; a.v_sh = d->v_stride[2];
+    a.o_sb = d->o_stride[0]; a.o_st = d->o_stride[1]; a.o_sh = d->o_stride[2];
+    a.g_sb = d->g_stride[0]; a.g_st = d->g_stride[1]; a.g_sh = d->g_stride[2];
+    a.B = d->B; a.Tq = d->Tq; a.Tk = d->Tk; a.Hq = d->Hq; a.Hkv = d->Hkv; a.D = d->D;
+    a.group = d->Hq / d->Hkv;
+    a.R = d->Tq * a.group;
+    a.causal = d->causal != 0;
+    a.off = d->Tk - d->Tq;
+    a.scale = d->scale;
+    a.scale_log2 = d->scale * ATTN_LOG2E;
+    a.splits = 1;
+    return a;
+}
+
+// The forward shares the keys of a row tile out over workgroups when there are fewer row tiles than compute units: one tile of keys
+// per workgroup at least, 512 workgroups at most.
+void split_keys(AttnSeqArgs& a, int dtype) {
+    const int BK = head_columns(a.D) * (int)mic_dtype_size(dtype) <= 256 ? 64 : 32;
+    const long long base = (long long)((a.R + ATTN_SEQ_BLOCK - 1) / ATTN_SEQ_BLOCK) * a.Hkv * a.B;
+    const int tiles = (a.Tk + BK - 1) / BK;
+    a.splits = 1;
+    a.tiles_per_split = tiles;
+    if (base == 0 || base >= 256 || tiles < 4) return;
+    const int want = (int)((512 + base - 1) / base);
+    const int s = want < tiles ? want : tiles;
+    a.tiles_per_split = (tiles + s - 1) / s;
+    a.splits = (tiles + a.tiles_per_split - 1) / a.tiles_per_split;
+}
+// The key gradients share the rows out in the same way, at least four tiles of 32 rows to a workgroup.
+void split_rows(AttnSeqArgs& a) {
+    const long long base = (long long)((a.Tk + ATTN_SEQ_BLOCK - 1) / ATTN_SEQ_BLOCK) * a.Hkv * a.B;
+    const int tiles = (a.R + 31) / 32;
+    a.splits = 1;
+    a.tiles_per_split = tiles;
+    if (base == 0 || base >= 512 || tiles < 8) return;
+    const int want = (int)((512 + base - 1) / base);
+    const int s = want < tiles / 4 ? want : tiles / 4;
+    if (s < 2) return;
+    a.tiles_per_split = (tiles + s - 1) / s;
+    a.splits = (tiles + a.tiles_per_split - 1) / a.tiles_per_split;
+}
+
+long long up256(long long b) { return (b + 255) / 256 * 256; }
+long long fwd_rows(const AttnSeqArgs& a) { return (long long)a.splits * a.B * a.Hkv * a.R; }
+long long fwd_bytes(const AttnSeqArgs& a) { return a.splits > 1 ? up256(fwd_rows(a) * a.D * 4) + up256(fwd_rows(a) * 8) : 0; }
+long long delta_bytes(const AttnSeqArgs& a) { return up256((long long)a.B * a.Hq * a.Tq * 4); }
+long long grad_bytes(const AttnSeqArgs& a) { return delta_bytes(a) + (a.splits > 1 ? up256(2ll * a.splits * a.B * a.Tk * a.Hkv * a.D * 4) : 0); }
+
+}  // namespace
+
+extern "C" int64_t mic_attn_seq_workspace_bytes(const mic_attn_seq_desc* d, int grad) {
+    MIC_TRY(check_sizes("mic_attn_seq_workspace_bytes", d));
+    AttnSeqArgs a = args_of(d);
+    if (grad) {
+        split_rows(a);
+        return grad_bytes(a);
+    }
+    split_keys(a, d->dtype);
+    return fwd_bytes(a);
+}
+
+extern "C" int mic_attn_seq(const mic_attn_seq_desc* d, void* stream) {
+    const char* who = "mic_attn_seq";
+    MIC_TRY(check_sizes(who, d));
+    AttnSeqArgs a = args_of(d);
+    const bool no_rows = d->B == 0 || d->Tq == 0, no_keys = d->B == 0 || d->Tk == 0;
+    if (no_rows) return 0;
+    MIC_TRY(check_tensor(who, "q", d->q, d->q_stride, d->dtype, false));
+    MIC_TRY(check_tensor(who, "k", d->k, d->k_stride, d->dtype, no_keys));
+    MIC_TRY(check_tensor(who, "v", d->v, d->v_stride, d->dtype, no_keys));
+    MIC_TRY(check_tensor(who, "o", d->o, d->o_stride, d->dtype, false));
+    MIC_ARG_CHECK(d->lse, "%s: lse is a null pointer", who);
+    split_keys(a, d->dtype);
+    const long long need = fwd_bytes(a);
+    MIC_ARG_CHECK(need == 0 || (d->workspace && d->workspace_bytes >= need && ((uintptr_t)d->workspace & 15) == 0), "%s: workspace of %lld bytes, %lld needed", who,
+                  (long long)d->workspace_bytes, need);
+    if (need) {
+        a.part = (float*)d->workspace;
+        a.part_ml = (float*)((char*)d->workspace + up256(fwd_rows(a) * a.D * 4));
+    }
+    return mic_attn_seq_fwd_launch(a, d->dtype, (hipStream_t)stream);
+}
+
+extern "C" int mic_attn_seq_grad(const mic_attn_seq_desc* d, void* stream) {
+    const char* who = "mic_attn_seq_grad";
+    MIC_TRY(check_sizes(who, d));
+    AttnSeqArgs a = args_of(d);
+    const bool no_rows = d->B == 0 || d->Tq == 0, no_keys = d->B == 0 || d->Tk == 0;
+    MIC_TRY(check_tensor(who, "q", d->q, d->q_stride, d->dtype, no_rows));
+    MIC_TRY(check_tensor(who, "k", d->k, d->k_stride, d->dtype, no_keys));
+    MIC_TRY(check_tensor(who, "v", d->v, d->v_stride, d->dtype, no_keys));
+    MIC_TRY(check_tensor(who, "o", d->o, d->o_stride, d->dtype, no_rows));
+    MIC_TRY(check_tensor(who, "grad_o", d->grad_o, d->g_stride, d->dtype, no_rows));
+    MIC_ARG_CHECK(no_rows || (d->lse && d->dq), "%s: lse or dq is a null pointer", who);
+    MIC_ARG_CHECK(no_keys || (d->dk && d->dv), "%s: dk or dv is a null pointer", who);
+    MIC_ARG_CHECK((((uintptr_t)d->dq | (uintptr_t)d->dk | (uintptr_t)d->dv) & 15) == 0, "%s: a gradient is not 16-byte aligned", who);
+    split_rows(a);
+    const long long need = grad_bytes(a);
+    MIC_ARG_CHECK(need == 0 || (d->workspace && d->workspace_bytes >= need && ((uintptr_t)d->workspace & 15) == 0), "%s: workspace of %lld bytes, %lld needed", who,
+                  (long long)d->workspace_bytes, need);
+    a.delta = (float*)d->workspace;
+    a.part = (float*)((char*)d->workspace + delta_bytes(a));
+    if (!no_rows) MIC_TRY(mic_attn_seq_dq_launch(a, d->dtype, (hipStream_t)stream));
+    if (!no_keys) MIC_TRY(mic_attn_seq_dkv_launch(a, d->dtype, (hipStream_t)stream));
+    return 0;
+}

@@ -1,0 +1,175 @@
+// Whole-sequence attention, forward:  o = softmax(scale * q k^T, masked) v  in one pass over the keys with a running maximum and
+// sum, and lse = log sum exp of every row for the gradient.  See attn_seq.h for the layouts.
+//
+// A workgroup of four waves takes 128 rows of one key head; a wave keeps 32 rows' queries as B operands in registers and computes
+// S^T = K Q^T, so a lane owns one row (query) and the statistics of a row are 16 registers of one lane and one exchange with
+// the lane 32 away.  P^T then is the B operand of O^T = V^T P^T.
+#include "attn_seq.h"
+
+namespace {
+
+template <typename T, int DP, int BK, bool SPLIT> __global__ __launch_bounds__(256) void attn_seq_fwd_kernel(AttnSeqArgs a) {
+    constexpr int NC = DP / 16, ND = DP / 32, KT = BK / 32, NR = InRegs<T, DP>::value ? NC : 1;
+    __shared__ __attribute__((aligned(16))) T sk[BK * DP];
+    __shared__ __attribute__((aligned(16))) T sv[BK * DP];
+    const int lane = threadIdx.x & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int tiles_r = (a.R + ATTN_SEQ_BLOCK - 1) / ATTN_SEQ_BLOCK;
+    int id = blockIdx.x;
+    const int split = SPLIT ? id % a.splits : 0;
+    if (SPLIT) id /= a.splits;
+    // the last rows, which see the most keys, first
+    const int rt = tiles_r - 1 - id % tiles_r, hk = id / tiles_r % a.Hkv, b = id / tiles_r / a.Hkv;
+    const int r0 = rt * ATTN_SEQ_BLOCK + wave * 32, r = r0 + (lane & 31);
+    const bool row_ok = r < a.R;
+    const int qi = row_ok ? r / a.group : 0, qh = hk * a.group + (row_ok ? r - qi * a.group : 0);
+    const T* qrow = row_ok ? (const T*)a.q + b * a.q_sb + qi * a.q_st + qh * a.q_sh : nullptr;
+    Frag8<T> qf[NR];
+#pragma unroll
+    for (int c = 0; c < NR; ++c) qf[c] = load_frag<T>(qrow, 16 * c + 8 * h, a.D);
+
+    const int last = min(rt * ATTN_SEQ_BLOCK + ATTN_SEQ_BLOCK, a.R) - 1;
+    const int k_end = a.causal ? min(a.Tk, last / a.group + a.off + 1) : a.Tk;  // keys any row of the workgroup may see
+    const int w_last = min(r0 + 31, a.R - 1);
+    const int w_end = r0 < a.R ? (a.causal ? min(a.Tk, w_last / a.group + a.off + 1) : a.Tk) : 0;  // any row of the wave
+    const int lim = a.causal ? qi + a.off : a.Tk - 1;  // last key this lane's row sees
+    int t0 = 0, t1 = k_end > 0 ? (k_end + BK - 1) / BK : 0;
+    if (SPLIT) {
+        t0 = split * a.tiles_per_split;
+        t1 = min(t1, t0 + a.tiles_per_split);
+    }
+    f32x16_t acc[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) acc[d] = f32x16_t{};
+    float m = -INFINITY, l = 0.f;
+    const T* kb = (const T*)a.k + b * a.k_sb + hk * a.k_sh;
+    const T* vb = (const T*)a.v + b * a.v_sb + hk * a.v_sh;
+    for (int t = t0; t < t1; ++t) {
+        const int k0 = t * BK;
+        __syncthreads();
+        // rows no query may see are zeros: whatever they hold, infinities and NaN included, stays out of the products
+        stage<T, DP, BK, 256>(sk, a.D, [&](int x) { return key_seen(a, b, k0 + x) ? kb + (long long)(k0 + x) * a.k_st : nullptr; });
+        stage<T, DP, BK, 256>(sv, a.D, [&](int x) { return key_seen(a, b, k0 + x) ? vb + (long long)(k0 + x) * a.v_st : nullptr; });
+        __syncthreads();
+        f32x16_t s[KT];
+        float top = -INFINITY;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+            s[kt] = f32x16_t{};
+            if (k0 + kt * 32 >= w_end) continue;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+                mma32(read_row<DP>(sk, kt * 32 + (lane & 31), c, h), InRegs<T, DP>::value ? qf[c % NR] : load_frag<T>(qrow, 16 * c + 8 * h, a.D), s[kt]);
+            const unsigned bits = key_bits(a, b, k0 + kt * 32, lane) >> (4 * h);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int j = 8 * (e >> 2) + (e & 3);
+                const bool seen = ((bits >> j) & 1) && k0 + kt * 32 + 4 * h + j <= lim;
+                s[kt][e] = seen ? s[kt][e] * a.scale_log2 : -INFINITY;
+                top = fmaxf(top, s[kt][e]);
+            }
+        }
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float m_new = fmaxf(m, top), m_use = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = __builtin_amdgcn_exp2f(m - m_use);
+        m = m_new;
+        float sum = 0.f;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+            if (k0 + kt * 32 >= w_end) continue;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                s[kt][e] = __builtin_amdgcn_exp2f(s[kt][e] - m_use);
+                sum += s[kt][e];
+            }
+        }
+        l = l * alpha + sum + __shfl_xor(sum, 32, 64);
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[d][e] *= alpha;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+            if (k0 + kt * 32 >= w_end) continue;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const Frag8<T> p = frag_of<T>(s[kt], j);  // bf16: the probabilities are rounded for the product, the sum l is not
+#pragma unroll
+                for (int d = 0; d < ND; ++d) mma32(read_col<DP>(sv, d * 32, kt * 32 + 16 * j, lane), p, acc[d]);
+            }
+        }
+    }
+    if (!row_ok) return;
+    if (SPLIT) {
+        const long long at = (((long long)split * a.B + b) * a.Hkv + hk) * a.R + r;
+        float* o = a.part + at * a.D;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int col = d * 32 + 8 * e + 4 * h;
+                if (col < a.D) store4<float>(o + col, acc[d][4 * e], acc[d][4 * e + 1], acc[d][4 * e + 2], acc[d][4 * e + 3]);
+            }
+        if (h == 0) {
+            a.part_ml[2 * at] = m;
+            a.part_ml[2 * at + 1] = l;
+        }
+        return;
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    T* o = (T*)a.o + b * a.o_sb + qi * a.o_st + qh * a.o_sh;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int col = d * 32 + 8 * e + 4 * h;
+            if (col < a.D) store4<T>(o + col, acc[d][4 * e] * inv, acc[d][4 * e + 1] * inv, acc[d][4 * e + 2] * inv, acc[d][4 * e + 3] * inv);
+        }
+    if (h == 0) a.lse[((long long)b * a.Hq + qh) * a.Tq + qi] = l == 0.f ? -INFINITY : (m + log2f(l)) * ATTN_LN2;
+}
+
+// joins the key ranges of a row: one wave per row
+template <typename T> __global__ __launch_bounds__(256) void attn_seq_join_kernel(AttnSeqArgs a) {
+    const int lane = threadIdx.x & 63;
+    const long long rows = (long long)a.B * a.Hkv * a.R, row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    float m = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[2 * (s * rows + row)]);
+    const float m_use = m == -INFINITY ? 0.f : m;
+    float l = 0.f, acc[4] = {};
+    const int col = lane * 4;
+    for (int s = 0; s < a.splits; ++s) {
+        const float w = __builtin_amdgcn_exp2f(a.part_ml[2 * (s * rows + row)] - m_use);
+        l += w * a.part_ml[2 * (s * rows + row) + 1];
+        if (col < a.D) {
+            const float4 x = *reinterpret_cast<const float4*>(a.part + (s * rows + row) * a.D + col);
+            acc[0] += w * x.x; acc[1] += w * x.y; acc[2] += w * x.z; acc[3] += w * x.w;
+        }
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    const int r = (int)(row % a.R), hk = (int)(row / a.R % a.Hkv), qi = r / a.group, qh = hk * a.group + r - qi * a.group;
+    const long long b = row / a.R / a.Hkv;
+    if (col < a.D) store4<T>((T*)a.o + b * a.o_sb + qi * a.o_st + qh * a.o_sh + col, acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+    if (lane == 0) a.lse[(b * a.Hq + qh) * a.Tq + qi] = l == 0.f ? -INFINITY : (m + log2f(l)) * ATTN_LN2;
+}
+
+template <typename T, int DP> int launch(const AttnSeqArgs& a, hipStream_t s) {
+    constexpr int BK = KeyTile<T, DP>::value;
+    const long long blocks = (long long)((a.R + ATTN_SEQ_BLOCK - 1) / ATTN_SEQ_BLOCK) * a.Hkv * a.B;
+    if (a.splits > 1) {
+        MIC_LAUNCH((attn_seq_fwd_kernel<T, DP, BK, true>), dim3((unsigned)(blocks * a.splits)), dim3(256), 0, s, a);
+        const long long rows = (long long)a.B * a.Hkv * a.R;
+        MIC_LAUNCH((attn_seq_join_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
+    } else {
+        MIC_LAUNCH((attn_seq_fwd_kernel<T, DP, BK, false>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+    }
+    return 0;
+}
+template <typename T> int launch_d(const AttnSeqArgs& a, hipStream_t s) {
+    return a.D <= 32 ? launch<T, 32>(a, s) : a.D <= 64 ? launch<T, 64>(a, s) : a.D <= 128 ? launch<T, 128>(a, s) : launch<T, 256>(a, s);
+}
+
+}  // namespace
+
+int mic_attn_seq_fwd_launch(const AttnSeqArgs& a, int dtype, hipStream_t s) {
+    return dtype == MIC_BF16 ? launch_d<bf16_t>(a, s) : launch_d<float>(a, s);
+}

@@ -11,13 +11,15 @@ types, devices) or ``_lib.MicError`` (what the library refuses).
 """
 from __future__ import annotations
 
+import ctypes as C
+import math
 from typing import Optional
 
 import torch
 
 from . import _lib as L
 
-__all__ = ["embedding", "embedding_forward", "embedding_grad"]
+__all__ = ["embedding", "embedding_forward", "embedding_grad", "attention", "attention_forward", "attention_grad"]
 
 
 def _device(name: str, *tensors) -> torch.device:
@@ -142,3 +144,113 @@ class _Embedding(torch.autograd.Function):
 def embedding(ids, table, pos=None, *, scale: float = 1.0, dtype=None) -> torch.Tensor:
     """``embedding_forward`` that ``torch.autograd`` can differentiate with respect to ``table`` and ``pos``."""
     return _Embedding.apply(ids, table, pos, scale, dtype)
+
+
+# ---- attention --------------------------------------------------------------------------------------------------------
+def _heads(t: torch.Tensor) -> torch.Tensor:
+    """The tensor itself where the kernels can read it in place (columns consecutive, everything on 16-byte boundaries)."""
+    e = 16 // t.element_size()
+    if t.data_ptr() % 16 == 0 and (t.stride(3) == 1 or t.shape[3] == 1) and all(s % e == 0 for s in _strides(t)):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _strides(t: torch.Tensor):
+    """Strides of (batch, position, head); a dimension of one entry has none to speak of."""
+    return (C.c_int64 * 3)(*(t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)))
+
+
+def _attn_desc(name, q, k, v, causal, key_mask, scale):
+    dev = _device(name, q, k, v, key_mask)
+    _need(q.dim() == 4 and k.dim() == 4 and v.dim() == 4, name, "q, k and v must be (batch, positions, heads, columns)")
+    B, Tq, Hq, D = q.shape
+    Tk, Hkv = k.shape[1], k.shape[2]
+    _need(k.shape == v.shape and k.shape[0] == B and k.shape[3] == D and Hq > 0 and Hkv > 0 and D > 0, name,
+          f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit")
+    _need(k.dtype == q.dtype and v.dtype == q.dtype, name, f"q, k and v are {q.dtype}, {k.dtype} and {v.dtype}")
+    d = L.AttnSeqDesc()
+    d.dtype = _float_code(name, "q", q.dtype)
+    q, k, v = _heads(q), _heads(k), _heads(v)
+    if key_mask is not None:
+        _need(key_mask.dtype in (torch.bool, torch.uint8) and key_mask.shape == (B, Tk), name,
+              f"key_mask must be bool ({B}, {Tk}), got {key_mask.dtype} {tuple(key_mask.shape)}")
+        if Tk > 1 and key_mask.stride(1) != 1:
+            key_mask = key_mask.contiguous()
+        d.key_mask, d.mask_stride = key_mask.data_ptr(), key_mask.stride(0)
+    d.q, d.k, d.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    d.q_stride, d.k_stride, d.v_stride = _strides(q), _strides(k), _strides(v)
+    d.B, d.Tq, d.Tk, d.Hq, d.Hkv, d.D, d.causal = B, Tq, Tk, Hq, Hkv, D, int(bool(causal))
+    d.scale = scale if scale is not None else 1.0 / math.sqrt(D)
+    return d, dev, (q, k, v, key_mask)
+
+
+def _attn_workspace(name, d, grad, dev):
+    size = int(L.lib.mic_attn_seq_workspace_bytes(C.byref(d), grad))
+    if size < 0:
+        L.check(size, name)
+    if size == 0:
+        return None
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    d.workspace, d.workspace_bytes = ws.data_ptr(), size
+    return ws
+
+
+def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool = False, key_mask: Optional[torch.Tensor] = None,
+                      scale: Optional[float] = None):
+    """softmax(scale * q k^T) v over whole sequences (models/transformer.py:81-86,130-140): returns ``(o, lse)``.
+
+    q (B, Tq, Hq, D); k, v (B, Tk, Hkv, D), Hq a multiple of Hkv (query head h reads key head h // (Hq // Hkv)); any strides, e.g.
+    slices of one packed projection.  ``causal``: query i sees keys up to i + Tk - Tq.  key_mask (B, Tk) bool: True where a key may
+    be seen; what k and v hold elsewhere is never used.  A query that sees nothing gets zeros.  scale defaults to D ** -0.5.
+    o (B, Tq, Hq, D) in q's dtype, lse (B, Hq, Tq) fp32.  D at most 256 and a multiple of 8 (bf16) or 4 (fp32)."""
+    name = "attention_forward"
+    d, dev, keep = _attn_desc(name, q, k, v, causal, key_mask, scale)
+    o = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    lse = torch.empty(q.shape[0], q.shape[2], q.shape[1], dtype=torch.float32, device=dev)
+    d.o, d.o_stride, d.lse = o.data_ptr(), _strides(o), lse.data_ptr()
+    with torch.cuda.device(dev):
+        ws = _attn_workspace(name, d, 0, dev)  # noqa: F841  (alive until the launch is enqueued)
+        L.check(L.lib.mic_attn_seq(C.byref(d), _stream(dev)), "mic_attn_seq")
+    return o, lse
+
+
+def attention_grad(grad: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor, *,
+                   causal: bool = False, key_mask: Optional[torch.Tensor] = None, scale: Optional[float] = None):
+    """Gradients ``(dq, dk, dv)`` of ``attention_forward`` for the gradient of o, from its inputs and both results.  The probabilities
+    are recomputed; gradients of shared key heads are summed over their query heads in a fixed order."""
+    name = "attention_grad"
+    d, dev, keep = _attn_desc(name, q, k, v, causal, key_mask, scale)
+    _device(name, q, grad, o, lse)
+    _need(grad.shape == q.shape and o.shape == q.shape and grad.dtype == q.dtype and o.dtype == q.dtype, name,
+          f"grad {tuple(grad.shape)} {grad.dtype} and o {tuple(o.shape)} {o.dtype} do not fit q {tuple(q.shape)} {q.dtype}")
+    _need(lse.shape == (q.shape[0], q.shape[2], q.shape[1]) and lse.dtype == torch.float32, name, f"lse {tuple(lse.shape)} {lse.dtype} does not fit q")
+    o, grad, lse = _heads(o), _heads(grad), lse.contiguous()
+    dq, dk, dv = (torch.empty(t.shape, dtype=q.dtype, device=dev) for t in (q, k, v))
+    d.o, d.o_stride, d.lse = o.data_ptr(), _strides(o), lse.data_ptr()
+    d.grad_o, d.g_stride = grad.data_ptr(), _strides(grad)
+    d.dq, d.dk, d.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+    with torch.cuda.device(dev):
+        ws = _attn_workspace(name, d, 1, dev)  # noqa: F841
+        L.check(L.lib.mic_attn_seq_grad(C.byref(d), _stream(dev)), "mic_attn_seq_grad")
+    return dq, dk, dv
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, causal, key_mask, scale):
+        o, lse = attention_forward(q, k, v, causal=causal, key_mask=key_mask, scale=scale)
+        ctx.save_for_backward(q, k, v, o, lse, key_mask)
+        ctx.meta = (causal, scale)
+        return o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        q, k, v, o, lse, key_mask = ctx.saved_tensors
+        causal, scale = ctx.meta
+        return (*attention_grad(grad, q, k, v, o, lse, causal=causal, key_mask=key_mask, scale=scale), None, None, None)
+
+
+def attention(q, k, v, *, causal: bool = False, key_mask=None, scale: Optional[float] = None) -> torch.Tensor:
+    """The output of ``attention_forward``, differentiable by ``torch.autograd`` with respect to q, k and v."""
+    return _Attention.apply(q, k, v, causal, key_mask, scale)

@@ -515,6 +515,38 @@ int64_t mic_embed_grad_workspace_bytes(int64_t n, int T, int H, int vocab, int w
 int mic_embed_grad(const void* ids, int ids_bits, const void* g, void* d_table, void* d_pos, int g_dtype, int out_dtype, float scale,
                    int64_t n, int T, int H, int vocab, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* Attention over whole sequences with shared key heads, and its gradient, which recomputes the probabilities from lse
+ * (the attention inside nn.MultiheadAttention of CausalSelfAttention and CrossAttention over a whole caption,
+ * models/transformer.py:81-86,130-140):
+ *     o[b, i, h] = sum_j p_ij v[b, j, h / (Hq/Hkv)],   p_ij = exp(scale * q_i . k_j - lse_i) over the keys j that i sees,
+ *     lse[b, h, i] = log sum_j exp(scale * q_i . k_j).
+ * Query i sees key j when key_mask[b, j] != 0 (NULL: always) and, with causal != 0, j <= i + Tk - Tq (the last query sees every
+ * key).  A row that sees no key has o = 0, lse = -infinity and zero gradients.  Keys hidden by key_mask never enter a product,
+ * whatever k and v hold there (infinities and NaN included); k and v of every other key must be finite, also where causality
+ * hides them from some rows.
+ * q, o, grad_o [B][Tq][Hq][D], k, v [B][Tk][Hkv][D] of dtype, addressed by element strides (batch, position, head), the D columns of
+ * a head consecutive; pointers and strides multiples of 16 bytes.  lse fp32 [B][Hq][Tq]; key_mask bytes [B][mask_stride].  The
+ * gradients dq [B][Tq][Hq][D], dk, dv [B][Tk][Hkv][D] are written whole and contiguous.  D <= 256, D * element size a multiple of 16 bytes.
+ * bf16: scores, statistics and sums in fp32; probabilities and their gradients are rounded to bf16 for the second products only.
+ * Sizes of zero are allowed.  mic_attn_seq_workspace_bytes(d, grad) looks at dtype and sizes alone (an argument error is negative). */
+typedef struct mic_attn_seq_desc {
+    const void *q, *k, *v;
+    void* o;              /* written by mic_attn_seq, read by mic_attn_seq_grad */
+    float* lse;           /* the same */
+    const uint8_t* key_mask;
+    const void* grad_o;
+    void *dq, *dk, *dv;
+    int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3], g_stride[3];
+    int64_t mask_stride;
+    int32_t dtype, B, Tq, Tk, Hq, Hkv, D, causal;
+    float scale;
+    void* workspace;
+    int64_t workspace_bytes;
+} mic_attn_seq_desc;
+int64_t mic_attn_seq_workspace_bytes(const mic_attn_seq_desc* d, int grad);
+int mic_attn_seq(const mic_attn_seq_desc* d, void* stream);
+int mic_attn_seq_grad(const mic_attn_seq_desc* d, void* stream);
+
 /* ------------------------------------------------------------------------------------------
  * Whole-path drivers: the same kernels chained natively so the host issues one call per phase.
  * ---------------------------------------------------------------------------------------- */

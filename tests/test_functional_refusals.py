@@ -74,3 +74,56 @@ def test_python_layer_refuses_cpu_tensors(F):
         F.embedding_forward(torch.zeros(2, 3, dtype=torch.long), torch.zeros(5, 8))
     with pytest.raises(ValueError, match="HIP device"):
         F.embedding_grad(torch.zeros(2, 3, 8), torch.zeros(2, 3, dtype=torch.long), 5)
+
+
+def attn_desc(L, **kw):
+    d = L.AttnSeqDesc()
+    for n in ("q", "k", "v", "o", "lse", "grad_o", "dq", "dk", "dv", "workspace"):
+        setattr(d, n, P)
+    for n in ("q_stride", "k_stride", "v_stride", "o_stride", "g_stride"):
+        for i, v in enumerate((1 << 20, 64, 32)):
+            getattr(d, n)[i] = v
+    d.dtype, d.B, d.Tq, d.Tk, d.Hq, d.Hkv, d.D, d.scale = L.BF16, 2, 3, 5, 2, 1, 32, 0.2
+    d.workspace_bytes = 1 << 30
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+def test_attn_seq_refuses(L):
+    import ctypes as C
+    calls = [L.lib.mic_attn_seq, L.lib.mic_attn_seq_grad]
+    for f in calls:
+        refused(L, f(None, None), b"null descriptor")
+        refused(L, f(C.byref(attn_desc(L, dtype=3)), None), b"dtype")
+        for kw in (dict(B=-1), dict(Tq=-1), dict(Tk=-2), dict(Hq=0), dict(Hkv=0), dict(D=0)):
+            refused(L, f(C.byref(attn_desc(L, **kw)), None), b"bad sizes")
+        refused(L, f(C.byref(attn_desc(L, Hq=3, Hkv=2)), None), b"evenly")
+        refused(L, f(C.byref(attn_desc(L, D=264)), None), b"columns")
+        refused(L, f(C.byref(attn_desc(L, D=36)), None), b"columns")
+        assert L.lib.mic_attn_seq_workspace_bytes(C.byref(attn_desc(L, dtype=L.F32, D=36)), 0) >= 0  # 36 floats are whole 16 bytes
+        refused(L, f(C.byref(attn_desc(L, B=1 << 20, Tq=1 << 20)), None), b"too many rows")
+        refused(L, f(C.byref(attn_desc(L, Tq=1 << 30)), None), b"too many rows")
+        for n in ("q", "k", "v", "o", "lse"):
+            refused(L, f(C.byref(attn_desc(L, **{n: None})), None), b"null pointer")
+        refused(L, f(C.byref(attn_desc(L, k=P + 8)), None), b"aligned")
+        for s in ("q_stride", "k_stride", "v_stride", "o_stride"):
+            d = attn_desc(L)
+            getattr(d, s)[1] = 33
+            refused(L, f(C.byref(d), None), b"stride")
+            getattr(d, s)[1] = -64
+            refused(L, f(C.byref(d), None), b"stride")
+    for n in ("dq", "dk", "dv"):
+        refused(L, L.lib.mic_attn_seq_grad(C.byref(attn_desc(L, **{n: None})), None), b"null pointer")
+    refused(L, L.lib.mic_attn_seq_grad(C.byref(attn_desc(L, dv=P + 4)), None), b"aligned")
+    d = attn_desc(L)
+    need = L.lib.mic_attn_seq_workspace_bytes(C.byref(d), 1)
+    assert need >= 2 * 2 * 3 * 4
+    for kw in (dict(workspace_bytes=need - 1), dict(workspace=None), dict(workspace=P + 8)):
+        refused(L, L.lib.mic_attn_seq_grad(C.byref(attn_desc(L, **kw)), None), b"workspace")
+    long = dict(B=1, Tq=1, Tk=8192)  # one row over many keys: shared out, which needs scratch
+    need = L.lib.mic_attn_seq_workspace_bytes(C.byref(attn_desc(L, **long)), 0)
+    assert need > 0
+    refused(L, L.lib.mic_attn_seq(C.byref(attn_desc(L, workspace_bytes=need - 1, **long)), None), b"workspace")
+    assert L.lib.mic_attn_seq(C.byref(attn_desc(L, B=0)), None) == 0 and L.lib.mic_attn_seq_grad(C.byref(attn_desc(L, B=0)), None) == 0
+    refused(L, L.lib.mic_attn_seq_workspace_bytes(C.byref(attn_desc(L, D=300)), 0), b"columns")

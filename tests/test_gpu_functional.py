@@ -145,3 +145,209 @@ def test_embedding_autograd_and_refusals(F):
         F.embedding_grad(g.to(DEV)[:2], ids.to(DEV), 11)
     with pytest.raises(ValueError):
         F.embedding_grad(g.to(DEV), ids.to(DEV), 11, positions=2)
+
+
+# ---- attention ----------------------------------------------------------------------------------------------------------
+def attn_ref(q, k, v, g, causal, mask, scale, dtype):
+    """Results in 64 bits and how far an fp32 evaluation (with probabilities rounded to `dtype`) may be from them.
+
+    Scores: a sum of D products and two roundings of the scaled value, es; a probability, exp of a score less lse, is off by the
+    errors of both (2 es) and of exp and the conversions (16 u); in bf16 by half a step more.  delta = g . o takes o as it was
+    rounded.  Every further product adds the fp32 error of its own sum."""
+    q, k, v, g = (t.double().transpose(1, 2) for t in (q, k, v, g))
+    group = q.shape[1] // k.shape[1]
+    k, v = k.repeat_interleave(group, 1), v.repeat_interleave(group, 1)
+    B, Hq, Tq, D = q.shape
+    Tk = k.shape[2]
+    hp, ho = (half(dtype) if dtype == BF16 else 0.0), half(dtype)
+    see = torch.ones(B, 1, Tq, Tk, dtype=torch.bool)
+    if causal:
+        see = see & torch.ones(Tq, Tk, dtype=torch.bool).tril(Tk - Tq)
+    if mask is not None:
+        see = see & mask.bool()[:, None, None, :]
+        hide = ~mask.bool()[:, None, :, None]
+        k, v = k.masked_fill(hide, 0.0), v.masked_fill(hide, 0.0)
+    s = q @ k.mT * scale
+    mag = q.abs() @ k.abs().mT * abs(scale)
+    es = ((D + 4) * U * mag).masked_fill(~see, 0.0).amax(-1, keepdim=True) if Tk else torch.zeros(B, Hq, Tq, 1).double()
+    s = s.masked_fill(~see, -math.inf)
+    lse = torch.logsumexp(s, -1)
+    some = see.any(-1) if Tk else torch.zeros(B, 1, Tq, dtype=torch.bool)
+    p = torch.exp(s - torch.where(some, lse, 0.0)[..., None])
+    rel = 2 * es + (16 + Tk) * U + hp
+    o = p @ v
+    e_o = rel * (p @ v.abs()) + Tk * U * (p @ v.abs()) + ho * o.abs() + 1e-30
+    e_lse = es[..., 0] + (8 + Tk) * U + 4 * U * torch.where(some, lse, 0.0).abs()
+    dp = g @ v.mT
+    delta = (g * o).sum(-1, keepdim=True)
+    ds = p * (dp - delta)
+    e_dp = D * U * (g.abs() @ v.abs().mT)
+    e_delta = (g.abs() * (e_o + D * U * o.abs())).sum(-1, keepdim=True)
+    e_ds = ds.abs() * (rel + 4 * U) + p * (e_dp + e_delta)
+    R = Tq * group
+    dv, e_dv = p.mT @ g, (p * (rel + R * U)).mT @ g.abs()
+    dq, e_dq = scale * ds @ k, abs(scale) * (e_ds + Tk * U * ds.abs()) @ k.abs()
+    dk, e_dk = scale * ds.mT @ q, abs(scale) * (e_ds + R * U * ds.abs()).mT @ q.abs()
+    fold = lambda t: t.reshape(B, Hq // group, group, Tk, D).sum(2)  # noqa: E731
+    dk, e_dk, dv, e_dv = fold(dk), fold(e_dk), fold(dv), fold(e_dv)
+    out = {}
+    for name, t, e in (("o", o, e_o), ("dq", dq, e_dq), ("dk", dk, e_dk), ("dv", dv, e_dv)):
+        out[name] = (t.transpose(1, 2), 1.01 * (e + ho * t.abs()).transpose(1, 2) + 1e-30)
+    out["lse"] = (lse, 1.01 * e_lse)
+    return out
+
+
+def check_lse(got, ref, tol):
+    got = got.double().cpu()
+    none = ref == -math.inf
+    assert torch.equal(got == -math.inf, none)
+    within(got[~none], ref[~none], tol[~none], "lse")
+
+
+def attn_inputs(B, Tq, Tk, Hq, Hkv, D, dtype, mask, seed=0):
+    g = gen(seed)
+    q, k, v, go = (torch.randn(*s, generator=g).to(dtype) for s in ((B, Tq, Hq, D), (B, Tk, Hkv, D), (B, Tk, Hkv, D), (B, Tq, Hq, D)))
+    m = None
+    if mask == "padded":
+        n = torch.randint(0, Tk + 1, (B, 1), generator=g)
+        n[0] = 0  # the first sequence has no key
+        m = torch.arange(Tk) < n
+    elif mask == "holes":
+        m = torch.rand(B, Tk, generator=g) < 0.6
+    return q, k, v, go, m
+
+
+def attn_run(F, q, k, v, go, causal, m, scale=None):
+    o, lse = F.attention_forward(q, k, v, causal=causal, key_mask=m, scale=scale)
+    return {"o": o, "lse": lse, **dict(zip(("dq", "dk", "dv"), F.attention_grad(go, q, k, v, o, lse, causal=causal, key_mask=m, scale=scale)))}
+
+
+def attn_check(got, ref):
+    check_lse(got["lse"], *ref["lse"])
+    for n in ("o", "dq", "dk", "dv"):
+        within(got[n], *ref[n], n)
+
+
+ATTN = [
+    # B, Tq, Tk, Hq, Hkv, D, causal, mask
+    (1, 1, 1, 1, 1, 32, False, None),
+    (2, 1, 5, 4, 1, 64, True, None),
+    (3, 29, 29, 2, 2, 256, True, None),
+    (2, 29, 49, 2, 2, 256, False, "holes"),
+    (2, 32, 64, 2, 1, 128, False, None),
+    (2, 33, 65, 2, 2, 40, False, "padded"),
+    (1, 129, 129, 2, 1, 72, True, "holes"),
+    (3, 17, 200, 4, 2, 96, True, "padded"),
+    (1, 200, 17, 2, 2, 64, True, None),       # more queries than keys: the first see none
+    (1, 140, 300, 8, 1, 128, True, None),     # eight query heads to a key head
+    (1, 1, 700, 8, 2, 128, True, "holes"),    # keys shared out over workgroups
+    (2, 3, 1031, 2, 1, 256, False, "padded"),
+    (1, 700, 40, 4, 2, 64, False, None),      # rows shared out over workgroups in the key gradients
+    (1, 300, 300, 1, 1, 160, True, None),
+    (4, 64, 128, 3, 3, 32, False, "padded"),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("B,Tq,Tk,Hq,Hkv,D,causal,mask", ATTN)
+def test_attention(F, B, Tq, Tk, Hq, Hkv, D, causal, mask, dtype):
+    q, k, v, go, m = attn_inputs(B, Tq, Tk, Hq, Hkv, D, dtype, mask)
+    ref = attn_ref(q, k, v, go, causal, m, 1 / math.sqrt(D), dtype)
+    got = attn_run(F, *(None if t is None else t.to(DEV) for t in (q, k, v, go)), causal, None if m is None else m.to(DEV))
+    assert got["o"].dtype == dtype and got["dk"].dtype == dtype
+    attn_check(got, ref)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_attention_hidden_keys_may_hold_anything(F, dtype):
+    q, k, v, go, m = attn_inputs(3, 50, 90, 4, 2, 64, dtype, "holes", seed=3)
+    m[1] = False
+    ref = attn_ref(q, k, v, go, False, m, 0.125, dtype)
+    bad = torch.tensor([math.nan, math.inf, -math.inf, torch.finfo(dtype).min])
+    fill = bad[torch.randint(0, 4, k.shape, generator=gen(4))].to(dtype)
+    k, v = torch.where(m[:, :, None, None], k, fill), torch.where(m[:, :, None, None], v, fill)
+    got = attn_run(F, q.to(DEV), k.to(DEV), v.to(DEV), go.to(DEV), False, m.to(DEV))
+    attn_check(got, ref)
+    assert not got["dk"][~m.to(DEV)].any() and not got["dv"][~m.to(DEV)].any() and not got["o"][1].any() and not got["dq"][1].any()
+
+
+def test_attention_large_scores_and_scale(F):
+    """Scores in the hundreds: the running maximum has to carry; the softmax is nearly one-hot."""
+    q, k, v, go, _ = attn_inputs(1, 70, 150, 2, 2, 64, F32, None, seed=5)
+    q = q * 8
+    for scale in (1.0, -0.7):
+        ref = attn_ref(q, k, v, go, False, None, float(torch.tensor(scale)), F32)
+        attn_check(attn_run(F, *(t.to(DEV) for t in (q, k, v, go)), False, None, scale), ref)
+
+
+def test_attention_strides(F):
+    """Slices of one packed projection, heads before positions, a broadcast key, odd offsets, a strided mask."""
+    g = gen(6)
+    B, T, H, D = 2, 45, 2, 64
+    packed = torch.randn(B, T, 3 * H * D, generator=g).to(BF16)
+    q, k, v = (packed[..., i * H * D:(i + 1) * H * D].unflatten(-1, (H, D)) for i in range(3))
+    go = torch.randn(B, H, T, D, generator=g).to(BF16).transpose(1, 2)
+    ref = attn_ref(q, k, v, go, True, None, 0.125, BF16)
+    dev = packed.to(DEV)
+    dq, dk, dv = (dev[..., i * H * D:(i + 1) * H * D].unflatten(-1, (H, D)) for i in range(3))
+    dgo = go.transpose(1, 2).contiguous().to(DEV).transpose(1, 2)
+    attn_check(attn_run(F, dq, dk, dv, dgo, True, None), ref)
+    # off a 16-byte boundary: copied first
+    flat = torch.randn(B * T * H * D + 1, generator=g).to(BF16)
+    q1 = flat[1:].view(B, T, H, D)
+    attn_check(attn_run(F, flat.to(DEV)[1:].view(B, T, H, D), dk, dv, dgo, True, None), attn_ref(q1, k, v, go, True, None, 0.125, BF16))
+    # one key sequence for the whole batch; a mask whose rows are columns
+    k0, v0 = k[:1].expand(B, T, H, D), v[:1].expand(B, T, H, D)
+    m = torch.rand(T, B, generator=g) < 0.7
+    got = attn_run(F, dq, dk[:1].expand(B, T, H, D), dv[:1].expand(B, T, H, D), dgo, False, m.to(DEV).t())
+    attn_check(got, attn_ref(q, k0, v0, go, False, m.t(), 0.125, BF16))
+
+
+def test_attention_empty(F):
+    e = lambda *s: torch.zeros(*s, dtype=BF16, device=DEV)  # noqa: E731
+    got = attn_run(F, e(2, 0, 2, 64), e(2, 5, 2, 64), e(2, 5, 2, 64), e(2, 0, 2, 64), False, None)
+    assert got["o"].shape == (2, 0, 2, 64) and not got["dk"].any() and not got["dv"].any()
+    got = attn_run(F, e(2, 3, 2, 64) + 1, e(2, 0, 2, 64), e(2, 0, 2, 64), e(2, 3, 2, 64) + 1, True, None)
+    assert not got["o"].any() and (got["lse"] == -math.inf).all() and not got["dq"].any() and got["dk"].shape == (2, 0, 2, 64)
+    got = attn_run(F, e(0, 3, 2, 64), e(0, 4, 2, 64), e(0, 4, 2, 64), e(0, 3, 2, 64), True, None)
+    assert got["o"].shape == (0, 3, 2, 64) and got["dv"].shape == (0, 4, 2, 64)
+
+
+def test_attention_is_the_same_every_time(F):
+    q, k, v, go, _ = (None if t is None else t.to(DEV) for t in attn_inputs(1, 900, 300, 8, 2, 64, BF16, None, seed=8))
+    first = attn_run(F, q, k, v, go, False, None)
+    for _ in range(4):
+        again = attn_run(F, q, k, v, go, False, None)
+        assert all(torch.equal(again[n], first[n]) for n in first)
+
+
+def test_attention_autograd_against_differences(F):
+    """The gradient against central differences of the 64-bit definition, and what the differentiable call refuses."""
+    q, k, v, go, m = attn_inputs(1, 6, 9, 2, 1, 32, F32, "holes", seed=10)
+    m[:, :2] = True
+    leaves = [t.to(DEV).requires_grad_() for t in (q, k, v)]
+    F.attention(*leaves, causal=True, key_mask=m.to(DEV)).backward(go.to(DEV))
+    scale = 1 / math.sqrt(32)
+
+    def loss(q, k, v):
+        return (attn_ref(q, k, v, go, True, m, scale, F32)["o"][0] * go.double()).sum()
+    for leaf, i in zip(leaves, range(3)):
+        direction = torch.randn(leaf.shape, generator=gen(11 + i), dtype=torch.float64)
+        args = [q.double(), k.double(), v.double()]
+        eps = 1e-5
+        hi, lo = list(args), list(args)
+        hi[i], lo[i] = args[i] + eps * direction, args[i] - eps * direction
+        diff = (loss(*hi) - loss(*lo)) / (2 * eps)  # off by eps^2 times a third derivative, about 1e-9 here
+        got = (leaf.grad.double().cpu() * direction).sum()
+        ref = attn_ref(q, k, v, go, True, m, scale, F32)[("dq", "dk", "dv")[i]]
+        assert abs(got - diff) <= (ref[1] * direction.abs()).sum() + 1e-7
+    with pytest.raises(ValueError):
+        F.attention_forward(q.to(DEV), k.to(DEV), v.to(DEV, BF16))
+    with pytest.raises(ValueError):
+        F.attention_forward(q.to(DEV), k.to(DEV), v.to(DEV)[:, :3])
+    with pytest.raises(ValueError):
+        F.attention_forward(q.to(DEV), k.to(DEV), v.to(DEV), key_mask=m[:, :4].to(DEV))
+    with pytest.raises(Exception, match="evenly"):
+        F.attention_forward(torch.zeros(1, 2, 3, 32, device=DEV), torch.zeros(1, 2, 2, 32, device=DEV), torch.zeros(1, 2, 2, 32, device=DEV))
+    with pytest.raises(Exception, match="columns"):
+        F.attention_forward(*(torch.zeros(1, 2, 1, 260, device=DEV) for _ in range(3)))
