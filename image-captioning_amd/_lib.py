@@ -74,6 +74,12 @@ class AttnSeqDesc(C.Structure):
                 ("causal", i32), ("scale", f32), ("workspace", vp), ("workspace_bytes", i64)]
 
 
+class VocabLossDesc(C.Structure):
+    _fields_ = [("x", vp), ("w", vp), ("bias", vp), ("targets", vp), ("loss", vp), ("lse", vp), ("grad_rows", vp), ("dx", vp), ("dw", vp),
+                ("db", vp), ("ld_x", i64), ("ld_w", i64), ("dtype", i32), ("N", i32), ("H", i32), ("V", i32), ("target_bits", i32),
+                ("n_ignore", i32), ("ignore", i32 * 4), ("workspace", vp), ("workspace_bytes", i64)]
+
+
 class BeamState(C.Structure):
     _fields_ = [("score", vp), ("len", vp), ("seq", vp), ("anc", vp)]
 
@@ -211,6 +217,9 @@ SIGNATURES = {
     "mic_attn_seq_workspace_bytes": (C.c_int64, [P(AttnSeqDesc), C.c_int]),
     "mic_attn_seq": (C.c_int, [P(AttnSeqDesc), vp]),
     "mic_attn_seq_grad": (C.c_int, [P(AttnSeqDesc), vp]),
+    "mic_vocab_loss_workspace_bytes": (C.c_int64, [P(VocabLossDesc), C.c_int]),
+    "mic_vocab_loss": (C.c_int, [P(VocabLossDesc), vp]),
+    "mic_vocab_loss_grad": (C.c_int, [P(VocabLossDesc), vp]),
     "mic_logsoftmax_topk": (C.c_int, [vp, C.c_int, C.c_int, C.c_int, C.c_int, f32, C.c_int, vp, vp, vp, vp]),
     "mic_sample_multinomial": (C.c_int, [vp, C.c_int, C.c_int, C.c_int, f32, vp, vp, vp, vp]),
     "mic_beam_select": (C.c_int, [P(BeamState), P(BeamState), vp, vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int,

@@ -1,0 +1,135 @@
+// Tiled matrix product of the vocabulary loss:  out[q][p] = sum_k Q(q, k) P(p, k), 128 x 128 tiles, four waves of 64 x 64.
+//
+// Each operand lies in memory either with k consecutive (a row per index: "row" operand) or with its index consecutive (a row per
+// k: "column" operand), and goes to LDS as it lies; a column operand is read from LDS by a transposing read (bf16) or scalar
+// reads (fp32).  So logits (x w^T), dx (d w) and dw (d^T x) run on the same tiles without a transposed copy of anything.
+// The result tile holds a lane per q and eight-row groups of p in registers: a row of the output (a token's logits) belongs to
+// two lanes, whose statistics need one exchange.
+#pragma once
+#include "attn_seq.h"
+
+namespace {
+
+// rows r0 + 8h..8h+7 of column d0 + (lane & 31): the order in which read_row takes k
+template <int DP> __device__ __forceinline__ Frag8<bf16_t> read_col_k(const bf16_t* t, int d0, int r0, int lane) {
+    const int h = lane >> 5, j = lane & 15, col = d0 + ((lane >> 4) & 1) * 16 + (j & 3) * 4, row = r0 + 8 * h + (j >> 2);
+    typedef __attribute__((address_space(3))) v4i16_t* lds_t;
+    const v4i16_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(t + Tile<bf16_t, DP>::at(row, col >> 3) + (col & 7)));
+    const v4i16_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(t + Tile<bf16_t, DP>::at(row + 4, col >> 3) + (col & 7)));
+    typedef short v8i16_t __attribute__((ext_vector_type(8)));
+    Frag8<bf16_t> f;
+    f.v = __builtin_bit_cast(bf16x8_t, (v8i16_t)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    return f;
+}
+template <int DP> __device__ __forceinline__ Frag8<float> read_col_k(const float* t, int d0, int r0, int lane) {
+    const int h = lane >> 5, col = d0 + (lane & 31);
+    Frag8<float> f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f.v[e] = t[Tile<float, DP>::at(r0 + 8 * h + e, col >> 2) + (col & 3)];
+    return f;
+}
+
+constexpr int VT = 128;  // tile edge
+
+struct Operand {
+    const void* p;
+    long long ld;  // elements between rows in memory
+    int n;         // how many indices there are
+};
+
+// One operand's tile of 128 indices x KS steps of k: fetched to registers, later stored to LDS.
+template <typename T, bool COL> struct OperandTile {
+    static constexpr int KS = 128 / (int)sizeof(T);
+    static constexpr int DP = COL ? VT : KS;
+    using L = Tile<T, DP>;
+    static constexpr int ROUNDS = VT * KS / L::E / 256;
+    uint4 x[ROUNDS];
+    __device__ __forceinline__ void fetch(const Operand& o, int i0, int k0, int k_end) {
+#pragma unroll
+        for (int n = 0; n < ROUNDS; ++n) {
+            const int i = threadIdx.x + n * 256, r = i / L::CPR, c = i % L::CPR * L::E;
+            const int idx = COL ? i0 + c : i0 + r, k = COL ? k0 + r : k0 + c;
+            const T* p = (const T*)o.p + (COL ? k * o.ld + idx : idx * o.ld + k);
+            x[n] = idx < o.n && k < k_end ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
+        }
+    }
+    __device__ __forceinline__ void put(T* tile) const {
+#pragma unroll
+        for (int n = 0; n < ROUNDS; ++n) {
+            const int i = threadIdx.x + n * 256;
+            *reinterpret_cast<uint4*>(tile + L::at(i / L::CPR, i % L::CPR)) = x[n];
+        }
+    }
+    // indices i0..i0+31 of the tile, 16 steps of k from 16 * s
+    __device__ static __forceinline__ Frag8<T> frag(const T* tile, int i0, int s, int lane) {
+        if constexpr (COL) return read_col_k<DP>(tile, i0, 16 * s, lane);
+        else return read_row<DP>(tile, i0 + (lane & 31), s, lane >> 5);
+    }
+};
+
+struct GemmShape {
+    Operand p, q;
+    int K, tiles_p, tiles_q, slices;
+};
+
+// Epi::run(args, acc, p0, q0, lane, tile_p, tile_q, wave, slice): acc[i][j] = p0 + 32 i.., q0 + 32 j..
+template <typename T, bool PCOL, bool QCOL, typename Epi> __global__ __launch_bounds__(256) void vocab_gemm_kernel(GemmShape g, typename Epi::Args ea) {
+    using TP = OperandTile<T, PCOL>;
+    using TQ = OperandTile<T, QCOL>;
+    constexpr int KS = TP::KS;
+    __shared__ __attribute__((aligned(16))) T sp[2][VT * KS];
+    __shared__ __attribute__((aligned(16))) T sq[2][VT * KS];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wp = wave >> 1, wq = wave & 1;
+    // workgroups b and b + 8 share an XCD and its L2: every XCD takes a contiguous range of tiles
+    int id;
+    {
+        const int n = gridDim.x, o = blockIdx.x, per = n >> 3, rest = n & 7, xcd = o & 7;
+        id = (xcd < rest ? xcd * (per + 1) : rest * (per + 1) + (xcd - rest) * per) + (o >> 3);
+    }
+    const int slice = id % g.slices;
+    id /= g.slices;
+    const int tq = id % g.tiles_q, tp = id / g.tiles_q;
+    const int p0 = tp * VT, q0 = tq * VT;
+    const int nk = (g.K + KS - 1) / KS, kb = (int)((long long)nk * slice / g.slices), ke = (int)((long long)nk * (slice + 1) / g.slices);
+    f32x16_t acc[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = f32x16_t{};
+    TP fp;
+    TQ fq;
+    if (kb < ke) {
+        fp.fetch(g.p, p0, kb * KS, g.K);
+        fq.fetch(g.q, q0, kb * KS, g.K);
+        fp.put(sp[0]);
+        fq.put(sq[0]);
+    }
+    for (int t = kb; t < ke; ++t) {
+        const int cur = (t - kb) & 1;
+        __syncthreads();
+        if (t + 1 < ke) {
+            fp.fetch(g.p, p0, (t + 1) * KS, g.K);
+            fq.fetch(g.q, q0, (t + 1) * KS, g.K);
+        }
+#pragma unroll
+        for (int s = 0; s < KS / 16; ++s) {
+            Frag8<T> a[2], b[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                a[i] = TP::frag(sp[cur], wp * 64 + i * 32, s, lane);
+                b[i] = TQ::frag(sq[cur], wq * 64 + i * 32, s, lane);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) mma32(a[i], b[j], acc[i][j]);
+        }
+        if (t + 1 < ke) {
+            fp.put(sp[cur ^ 1]);
+            fq.put(sq[cur ^ 1]);
+        }
+    }
+    Epi::run(ea, acc, p0 + wp * 64, q0 + wq * 64, lane, tp * 2 + wp, tq * 2 + wq, slice);
+}
+
+}  // namespace

@@ -19,7 +19,8 @@ import torch
 
 from . import _lib as L
 
-__all__ = ["embedding", "embedding_forward", "embedding_grad", "attention", "attention_forward", "attention_grad"]
+__all__ = ["embedding", "embedding_forward", "embedding_grad", "attention", "attention_forward", "attention_grad",
+           "vocab_loss", "vocab_loss_forward", "vocab_loss_grad"]
 
 
 def _device(name: str, *tensors) -> torch.device:
@@ -254,3 +255,101 @@ class _Attention(torch.autograd.Function):
 def attention(q, k, v, *, causal: bool = False, key_mask=None, scale: Optional[float] = None) -> torch.Tensor:
     """The output of ``attention_forward``, differentiable by ``torch.autograd`` with respect to q, k and v."""
     return _Attention.apply(q, k, v, causal, key_mask, scale)
+
+
+# ---- vocabulary loss ----------------------------------------------------------------------------------------------------
+def _vocab_desc(name, x, w, targets, bias, ignore):
+    dev = _device(name, x, w, targets, bias)
+    _need(x.dim() == 2 and w.dim() == 2 and x.shape[1] == w.shape[1] and x.shape[1] > 0 and w.shape[0] > 0, name,
+          f"x {tuple(x.shape)} and w {tuple(w.shape)} do not fit")
+    _need(x.dtype == w.dtype, name, f"x is {x.dtype}, w {w.dtype}")
+    N, H = x.shape
+    V = w.shape[0]
+    _need(targets.shape == (N,), name, f"targets {tuple(targets.shape)} do not fit {N} rows")
+    d = L.VocabLossDesc()
+    d.dtype = _float_code(name, "x", x.dtype)
+    x = x if x.stride(1) == 1 and (N <= 1 or x.stride(0) >= H) else x.contiguous()
+    w = w if w.stride(1) == 1 and (V <= 1 or w.stride(0) >= H) else w.contiguous()
+    targets = _ids(name, "targets", targets)
+    if bias is not None:
+        _need(bias.shape == (V,) and bias.dtype == torch.float32, name, f"bias must be float32 ({V},), got {bias.dtype} {tuple(bias.shape)}")
+        bias = bias.contiguous()
+    ignore = tuple(int(i) for i in ignore)
+    _need(len(ignore) <= 4, name, f"{len(ignore)} ignored words (at most 4)")
+    d.x, d.w, d.bias, d.targets = x.data_ptr(), w.data_ptr(), L.ptr(bias), targets.data_ptr()
+    d.ld_x, d.ld_w = (x.stride(0) if N > 1 else H), (w.stride(0) if V > 1 else H)
+    d.N, d.H, d.V, d.target_bits, d.n_ignore = N, H, V, 64 if targets.dtype == torch.int64 else 32, len(ignore)
+    for i, v in enumerate(ignore):
+        _need(-(1 << 31) <= v < (1 << 31), name, f"ignored word {v}")
+        d.ignore[i] = v
+    return d, dev, (x, w, targets, bias)
+
+
+def _vocab_workspace(name, d, grad, dev):
+    size = int(L.lib.mic_vocab_loss_workspace_bytes(C.byref(d), grad))
+    if size < 0:
+        L.check(size, name)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    d.workspace, d.workspace_bytes = ws.data_ptr(), size
+    return ws
+
+
+def vocab_loss_forward(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, *, bias: Optional[torch.Tensor] = None, ignore=()):
+    """Cross entropy of every row of x (N, H) against the vocabulary w (V, H) without keeping the logits x w^T + bias (the output
+    layer and loss of models/transformer.py:293, train.py:318-354): returns ``(loss, lse)``, both fp32 (N,).
+
+    targets (N,) int32 / int64; rows whose target is in ``ignore`` (at most four words, e.g. padding) or outside the vocabulary
+    have loss 0.  bias (V,) fp32."""
+    name = "vocab_loss_forward"
+    d, dev, keep = _vocab_desc(name, x, w, targets, bias, ignore)
+    loss = torch.empty(x.shape[0], dtype=torch.float32, device=dev)
+    lse = torch.empty_like(loss)
+    d.loss, d.lse = loss.data_ptr(), lse.data_ptr()
+    with torch.cuda.device(dev):
+        ws = _vocab_workspace(name, d, 0, dev)  # noqa: F841  (alive until the launches are enqueued)
+        L.check(L.lib.mic_vocab_loss(C.byref(d), _stream(dev)), "mic_vocab_loss")
+    return loss, lse
+
+
+def vocab_loss_grad(grad: torch.Tensor, x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, lse: torch.Tensor, *,
+                    bias: Optional[torch.Tensor] = None, ignore=()):
+    """Gradients ``(dx, dw, dbias or None)`` of ``vocab_loss_forward`` for the gradient ``grad`` (N,) fp32 of its losses (a scalar tensor is
+    taken for every row), from its inputs and lse.  Rows that do not count get zeros."""
+    name = "vocab_loss_grad"
+    d, dev, keep = _vocab_desc(name, x, w, targets, bias, ignore)
+    _device(name, x, grad, lse)
+    N = x.shape[0]
+    _need(grad.dtype == torch.float32 and grad.shape in ((N,), ()), name, f"grad must be float32 ({N},), got {grad.dtype} {tuple(grad.shape)}")
+    _need(lse.dtype == torch.float32 and lse.shape == (N,), name, f"lse must be float32 ({N},), got {lse.dtype} {tuple(lse.shape)}")
+    grad, lse = grad.expand(N).contiguous(), lse.contiguous()
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    dw = torch.empty(w.shape, dtype=w.dtype, device=dev)
+    db = None if bias is None else torch.empty(w.shape[0], dtype=torch.float32, device=dev)
+    d.grad_rows, d.lse = grad.data_ptr(), lse.data_ptr()
+    d.dx, d.dw, d.db = dx.data_ptr(), dw.data_ptr(), L.ptr(db)
+    with torch.cuda.device(dev):
+        ws = _vocab_workspace(name, d, 1, dev)  # noqa: F841
+        L.check(L.lib.mic_vocab_loss_grad(C.byref(d), _stream(dev)), "mic_vocab_loss_grad")
+    return dx, dw, db
+
+
+class _VocabLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, targets, bias, ignore):
+        loss, lse = vocab_loss_forward(x, w, targets, bias=bias, ignore=ignore)
+        ctx.save_for_backward(x, w, targets, bias, lse)
+        ctx.ignore = ignore
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        x, w, targets, bias, lse = ctx.saved_tensors
+        dx, dw, db = vocab_loss_grad(grad, x, w, targets, lse, bias=bias, ignore=ctx.ignore)
+        return dx, dw, None, db, None
+
+
+def vocab_loss(x, w, targets, *, bias=None, ignore=()) -> torch.Tensor:
+    """The losses (N,) of ``vocab_loss_forward``, differentiable by ``torch.autograd`` with respect to x, w and bias; sum, average or
+    weight them as the training step wants (train.py:346-352 averages over the counted rows)."""
+    return _VocabLoss.apply(x, w, targets, bias, tuple(ignore))

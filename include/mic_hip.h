@@ -547,6 +547,36 @@ int64_t mic_attn_seq_workspace_bytes(const mic_attn_seq_desc* d, int grad);
 int mic_attn_seq(const mic_attn_seq_desc* d, void* stream);
 int mic_attn_seq_grad(const mic_attn_seq_desc* d, void* stream);
 
+/* Softmax cross entropy of the output layer without keeping its logits (models/transformer.py:293 followed by the loss of
+ * train.py:318-354; with row weights the reward-weighted loss of train.py:209-262):
+ *     z = x w^T + bias,   lse[n] = log sum_v exp z[n, v],   loss[n] = lse[n] - z[n, targets[n]]
+ * and, for row weights a = grad_rows, d = a[n] (exp(z - lse) - onehot(target)):   dx = d w,  dw = d^T x,  db = column sums of d.
+ * A row whose target is one of the `ignore` words or outside [0, V) has loss 0 and no gradient; its lse is computed all the same.
+ * x [N][ld_x], w [V][ld_w] of dtype, bias fp32 [V] or NULL, targets int32 / int64; loss, lse, grad_rows fp32 [N]; dx [N][H] and
+ * dw [V][H] of dtype, db fp32 [V] or NULL (not wanted), written whole.  A bias may hide words with -infinity.  The gradient takes
+ * x, w, targets, bias and ignore as the loss did, and its lse; it computes the logits again, a piece of the vocabulary at a time
+ * (a piece of d takes up to 256 MiB of the workspace).  bf16: products and sums in fp32, d rounded to bf16 for the products with w and x,
+ * db summed before that.  H of any size; x and w whose rows are not whole 16 bytes on 16-byte boundaries are copied into
+ * the workspace first.  mic_vocab_loss_workspace_bytes(d, grad) looks at dtype, sizes, strides and the alignment of x, w and
+ * whether db is NULL (an argument error is negative). */
+typedef struct mic_vocab_loss_desc {
+    const void *x, *w;
+    const float* bias;
+    const void* targets;
+    float *loss, *lse;    /* written by mic_vocab_loss; lse is read by mic_vocab_loss_grad */
+    const float* grad_rows;
+    void *dx, *dw;
+    float* db;
+    int64_t ld_x, ld_w;
+    int32_t dtype, N, H, V, target_bits, n_ignore;
+    int32_t ignore[4];
+    void* workspace;
+    int64_t workspace_bytes;
+} mic_vocab_loss_desc;
+int64_t mic_vocab_loss_workspace_bytes(const mic_vocab_loss_desc* d, int grad);
+int mic_vocab_loss(const mic_vocab_loss_desc* d, void* stream);
+int mic_vocab_loss_grad(const mic_vocab_loss_desc* d, void* stream);
+
 /* ------------------------------------------------------------------------------------------
  * Whole-path drivers: the same kernels chained natively so the host issues one call per phase.
  * ---------------------------------------------------------------------------------------- */

@@ -127,3 +127,55 @@ def test_attn_seq_refuses(L):
     refused(L, L.lib.mic_attn_seq(C.byref(attn_desc(L, workspace_bytes=need - 1, **long)), None), b"workspace")
     assert L.lib.mic_attn_seq(C.byref(attn_desc(L, B=0)), None) == 0 and L.lib.mic_attn_seq_grad(C.byref(attn_desc(L, B=0)), None) == 0
     refused(L, L.lib.mic_attn_seq_workspace_bytes(C.byref(attn_desc(L, D=300)), 0), b"columns")
+
+
+def vocab_desc(L, **kw):
+    d = L.VocabLossDesc()
+    for n in ("x", "w", "bias", "targets", "loss", "lse", "grad_rows", "dx", "dw", "db", "workspace"):
+        setattr(d, n, P)
+    d.ld_x = d.ld_w = 64
+    d.dtype, d.N, d.H, d.V, d.target_bits, d.n_ignore, d.workspace_bytes = L.BF16, 10, 64, 300, 64, 1, 1 << 40
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+def test_vocab_loss_refuses(L):
+    import ctypes as C
+    for f in (L.lib.mic_vocab_loss, L.lib.mic_vocab_loss_grad):
+        refused(L, f(None, None), b"null descriptor")
+        refused(L, f(C.byref(vocab_desc(L, dtype=2)), None), b"dtype")
+        for kw in (dict(N=-1), dict(H=0), dict(V=0)):
+            refused(L, f(C.byref(vocab_desc(L, **kw)), None), b"bad sizes")
+        refused(L, f(C.byref(vocab_desc(L, N=1 << 30)), None), b"range")
+        refused(L, f(C.byref(vocab_desc(L, N=1 << 29, V=1 << 29)), None), b"range")
+        refused(L, f(C.byref(vocab_desc(L, target_bits=16)), None), b"bits")
+        refused(L, f(C.byref(vocab_desc(L, n_ignore=5)), None), b"ignored")
+        refused(L, f(C.byref(vocab_desc(L, n_ignore=-1)), None), b"ignored")
+        refused(L, f(C.byref(vocab_desc(L, ld_x=63)), None), b"row stride")
+        refused(L, f(C.byref(vocab_desc(L, ld_w=0)), None), b"row stride")
+        for n in ("x", "w", "targets", "lse"):
+            refused(L, f(C.byref(vocab_desc(L, **{n: None})), None), b"null pointer")
+    need = L.lib.mic_vocab_loss_workspace_bytes(C.byref(vocab_desc(L)), 0)
+    assert need > 0
+    refused(L, L.lib.mic_vocab_loss(C.byref(vocab_desc(L, workspace_bytes=need - 1)), None), b"workspace")
+    refused(L, L.lib.mic_vocab_loss(C.byref(vocab_desc(L, workspace=P + 8)), None), b"workspace")
+    refused(L, L.lib.mic_vocab_loss(C.byref(vocab_desc(L, loss=None)), None), b"null pointer")
+    for n in ("grad_rows", "dx", "dw"):
+        refused(L, L.lib.mic_vocab_loss_grad(C.byref(vocab_desc(L, **{n: None})), None), b"null pointer")
+    for n in ("dx", "dw", "db"):
+        refused(L, L.lib.mic_vocab_loss_grad(C.byref(vocab_desc(L, **{n: P + 4})), None), b"aligned")
+    need = L.lib.mic_vocab_loss_workspace_bytes(C.byref(vocab_desc(L)), 1)
+    refused(L, L.lib.mic_vocab_loss_grad(C.byref(vocab_desc(L, workspace_bytes=need - 1)), None), b"workspace")
+    assert L.lib.mic_vocab_loss(C.byref(vocab_desc(L, N=0, x=None, targets=None, lse=None)), None) == 0
+    refused(L, L.lib.mic_vocab_loss_workspace_bytes(C.byref(vocab_desc(L, V=-5)), 1), b"bad sizes")
+    assert L.lib.mic_vocab_loss_workspace_bytes(C.byref(vocab_desc(L, N=0)), 0) == 0
+    assert L.lib.mic_vocab_loss_workspace_bytes(C.byref(vocab_desc(L, N=0)), 1) == 0
+
+
+def test_workspace_sizes_of_empty_calls(L):
+    import ctypes as C
+    assert L.lib.mic_embed_grad_workspace_bytes(0, 1, 8, 5, 1) >= 0
+    for kw in (dict(B=0), dict(Tq=0), dict(Tk=0), dict(Tq=0, Tk=0)):
+        for grad in (0, 1):
+            assert L.lib.mic_attn_seq_workspace_bytes(C.byref(attn_desc(L, **kw)), grad) >= 0

@@ -351,3 +351,298 @@ def test_attention_autograd_against_differences(F):
         F.attention_forward(torch.zeros(1, 2, 3, 32, device=DEV), torch.zeros(1, 2, 2, 32, device=DEV), torch.zeros(1, 2, 2, 32, device=DEV))
     with pytest.raises(Exception, match="columns"):
         F.attention_forward(*(torch.zeros(1, 2, 1, 260, device=DEV) for _ in range(3)))
+
+
+# ---- vocabulary loss ----------------------------------------------------------------------------------------------------
+def vocab_inputs(N, H, V, dtype, bias, seed=0, ignore_share=0.3):
+    g = gen(seed)
+    x, w = torch.randn(N, H, generator=g).to(dtype), (2.0 / math.sqrt(H) * torch.randn(V, H, generator=g)).to(dtype)
+    b = 0.5 * torch.randn(V, generator=g) if bias else None
+    t = torch.randint(0, V, (N,), generator=g)
+    t = torch.where(torch.rand(N, generator=g) < ignore_share, torch.zeros_like(t), t)
+    return x, w, b, t, torch.randn(N, generator=g)
+
+
+def vocab_ref(x, w, b, t, a, ignore, dtype):
+    """Results in 64 bits and bounds of an fp32 evaluation with d rounded to `dtype` for its products (bf16).
+
+    A logit is a sum of H products and a bias, ez; lse is off by the largest ez and its own sum's error; a probability by both and
+    by the roundings of the exponent (4 u |z|) and of exp (16 u)."""
+    N, H = x.shape
+    V = w.shape[0]
+    hp, ho = (half(dtype) if dtype == BF16 else 0.0), half(dtype)
+    X, W = x.double(), w.double()
+    z = X @ W.T
+    ez = (H + 3) * U * (X.abs() @ W.abs().T)
+    if b is not None:
+        z, ez = z + b.double(), ez + U * b.double().abs().masked_fill(b == -math.inf, 0.0)
+    lse = torch.logsumexp(z, 1)
+    fin = z.masked_fill(z == -math.inf, 0.0)
+    e_lse = (ez + 4 * U * fin.abs()).amax(1) + (V + 16) * U + 2 * U * lse.abs()
+    counted = (t >= 0) & (t < V)
+    for i in ignore:
+        counted &= t != i
+    tt = t.clamp(0, V - 1)[:, None]
+    loss = torch.where(counted, lse - z.gather(1, tt)[:, 0], 0.0)
+    e_loss = torch.where(counted, e_lse + ez.gather(1, tt)[:, 0] + U * loss.abs() + U * fin.gather(1, tt)[:, 0].abs(), 0.0)
+    p = torch.exp(z - lse[:, None])
+    rel = ez + 4 * U * fin.abs() + e_lse[:, None] + 16 * U
+    aw = torch.where(counted, a.double(), 0.0)[:, None]
+    hot = torch.zeros_like(p).scatter_(1, tt, 1.0)
+    d = aw * (p - hot)
+    e_d = aw.abs() * p * rel + 3 * U * d.abs()
+    e_dr = e_d + hp * (d.abs() + e_d)
+    out = {"loss": (loss, 1.01 * e_loss + 1e-30), "lse": (lse, 1.01 * e_lse)}
+    dx, dw, db = d @ W, d.T @ X, d.sum(0)
+    out["dx"] = (dx, 1.01 * (e_dr @ W.abs() + V * U * (d.abs() @ W.abs()) + ho * dx.abs()) + 1e-30)
+    out["dw"] = (dw, 1.01 * (e_dr.T @ X.abs() + N * U * (d.abs().T @ X.abs()) + ho * dw.abs()) + 1e-30)
+    out["db"] = (db, 1.01 * (e_d.sum(0) + N * U * d.abs().sum(0) + U * db.abs()) + 1e-30) if b is not None else None
+    return out
+
+
+def vocab_run(F, x, w, b, t, a, ignore):
+    loss, lse = F.vocab_loss_forward(x, w, t, bias=b, ignore=ignore)
+    return {"loss": loss, "lse": lse, **dict(zip(("dx", "dw", "db"), F.vocab_loss_grad(a, x, w, t, lse, bias=b, ignore=ignore)))}
+
+
+def vocab_check(got, ref):
+    for n, r in ref.items():
+        if r is None:
+            assert got[n] is None
+        else:
+            within(got[n], *r, n)
+
+
+def on(*ts):
+    return [None if t is None else t.to(DEV) for t in ts]
+
+
+VOCAB = [
+    # N, H, V, bias
+    (1, 64, 300, True),
+    (1, 8, 1, False),
+    (24, 512, 3500, True),
+    (130, 200, 129, True),
+    (513, 64, 1031, False),
+    (257, 300, 777, True),   # rows that are not whole 16 bytes in bf16
+    (37, 33, 515, True),
+    (200, 1024, 384, False),
+    (700, 128, 128, True),
+    (1, 2048, 5000, False),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("N,H,V,bias", VOCAB)
+def test_vocab_loss(F, N, H, V, bias, dtype):
+    x, w, b, t, a = vocab_inputs(N, H, V, dtype, bias)
+    got = vocab_run(F, *on(x, w, b, t, a), (0,))
+    assert got["dx"].dtype == dtype and got["dw"].dtype == dtype
+    vocab_check(got, vocab_ref(x, w, b, t, a, (0,), dtype))
+
+
+def test_vocab_loss_in_pieces(F):
+    """So many rows that d takes several pieces of the vocabulary; the gradients against sums over row blocks in 64 bits."""
+    N, H, V = 100_000, 64, 3500
+    x, w, b, t, a = vocab_inputs(N, H, V, BF16, True, seed=4)
+    a = a / N
+    X, Wm, B, T, A = on(x, w, b, t, a)
+    got = vocab_run(F, X, Wm, B, T, A, (0,))
+    ref = vocab_ref(x[:1000], w, b, t[:1000], a[:1000], (0,), BF16)
+    for n in ("loss", "lse", "dx"):
+        within(got[n][:1000], *ref[n], n)
+    dw, db = torch.zeros(V, H, dtype=torch.float64, device=DEV), torch.zeros(V, dtype=torch.float64, device=DEV)
+    mag_w, mag_b = torch.zeros_like(dw), torch.zeros_like(db)
+    for lo in range(0, N, 10000):
+        r = slice(lo, lo + 10000)
+        z = X[r].double() @ Wm.double().T + B.double()
+        d = torch.softmax(z, 1)
+        d[torch.arange(d.shape[0]), T[r]] -= 1
+        d *= (A[r].double() * (T[r] != 0))[:, None]
+        dw += d.T @ X[r].double(); db += d.sum(0)
+        mag_w += d.abs().T @ X[r].double().abs(); mag_b += d.abs().sum(0)
+    # per element of d: a relative error below 2^-13 in fp32 (logits of up to 32, H = 64), then bf16 rounding for the products
+    within(got["dw"], dw.cpu(), ((half(BF16) + 2.0 ** -13 + N * U) * mag_w + half(BF16) * dw.abs()).cpu(), "dw")
+    within(got["db"], db.cpu(), ((2.0 ** -13 + N * U) * mag_b).cpu(), "db")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_vocab_loss_masks(F, dtype):
+    """Targets outside the vocabulary, several ignored words, words hidden by a bias of -infinity, rows that all do not count."""
+    x, w, b, t, a = vocab_inputs(150, 96, 400, dtype, True, seed=2)
+    t[3], t[7], t[11] = -100, 400, 1 << 40
+    hide = torch.rand(400, generator=gen(3)) < 0.3
+    hide[t.clamp(0, 399)] = False
+    hide[128:256] = True  # whole tiles of hidden words
+    t = torch.where((t >= 128) & (t < 256), torch.full_like(t, 2), t)
+    hide[2] = False
+    b = b.masked_fill(hide, -math.inf)
+    got = vocab_run(F, *on(x, w, b, t, a), (0, 1, 5, -7))
+    vocab_check(got, vocab_ref(x, w, b, t, a, (0, 1, 5, -7), dtype))
+    assert not got["dw"][hide.to(DEV)].any() and got["loss"][3] == 0
+    got = vocab_run(F, *on(x, w, b, torch.full_like(t, 5).int(), a), (5,))
+    assert not got["loss"].any() and not got["dx"].any() and not got["dw"].any() and not got["db"].any() and torch.isfinite(got["lse"]).all()
+
+
+def test_vocab_loss_strides_and_empty(F):
+    x, w, b, t, a = vocab_inputs(60, 64, 200, BF16, True, seed=5)
+    wide_x, wide_w = torch.randn(60, 104, generator=gen(6)).to(BF16), torch.randn(200, 80, generator=gen(7)).to(BF16)
+    for lo_x, lo_w in ((8, 16), (3, 1)):  # in place, and off a 16-byte boundary
+        wx, ww = wide_x[:, lo_x:lo_x + 64], wide_w[:, lo_w:lo_w + 64] * 0.2
+        dev_w = (wide_w * 0.2).to(DEV)[:, lo_w:lo_w + 64]
+        got = vocab_run(F, wide_x.to(DEV)[:, lo_x:lo_x + 64], dev_w, *on(b, t, a), (0,))
+        vocab_check(got, vocab_ref(wx, ww, b, t, a, (0,), BF16))
+    got = vocab_run(F, x.t().contiguous().to(DEV).t(), *on(w, b, t, a), (0,))  # columns first
+    vocab_check(got, vocab_ref(x, w, b, t, a, (0,), BF16))
+    got = vocab_run(F, *on(x[:0], w, b, t[:0], a[:0]), ())
+    assert got["loss"].shape == (0,) and got["dx"].shape == (0, 64) and not got["dw"].any() and not got["db"].any()
+
+
+def test_vocab_loss_is_the_same_every_time(F):
+    args = on(*vocab_inputs(300, 256, 5000, BF16, True, seed=8))
+    first = vocab_run(F, *args, (0,))
+    for _ in range(4):
+        again = vocab_run(F, *args, (0,))
+        assert all(torch.equal(again[n], first[n]) for n in first)
+
+
+def test_vocab_loss_autograd_against_differences(F):
+    x, w, b, t, a = vocab_inputs(7, 16, 40, F32, True, seed=9)
+    leaves = [v.to(DEV).requires_grad_() for v in (x, w, b)]
+    (F.vocab_loss(leaves[0], leaves[1], t.to(DEV), bias=leaves[2], ignore=(0,)) * a.to(DEV)).sum().backward()
+    ref = vocab_ref(x, w, b, t, a, (0,), F32)
+
+    def loss(x, w, b):
+        return (torch.nn.functional.cross_entropy(x @ w.T + b, t, reduction="none") * torch.where(t == 0, 0.0, a.double())).sum()
+    for i, n in enumerate(("dx", "dw", "db")):
+        args = [x.double(), w.double(), b.double()]
+        direction = torch.randn(args[i].shape, generator=gen(20 + i), dtype=torch.float64)
+        eps = 1e-5
+        hi, lo = list(args), list(args)
+        hi[i], lo[i] = args[i] + eps * direction, args[i] - eps * direction
+        diff = (loss(*hi) - loss(*lo)) / (2 * eps)  # off by eps^2 times a third derivative, about 1e-9 here
+        got = (leaves[i].grad.double().cpu() * direction).sum()
+        assert abs(got - diff) <= (ref[n][1] * direction.abs()).sum() + 1e-7
+    # a mean over the counted rows: one scalar gradient for every row
+    m = F.vocab_loss(leaves[0].detach().requires_grad_(), leaves[1], t.to(DEV), ignore=(0,)).sum()
+    m.backward()
+    with pytest.raises(ValueError):
+        F.vocab_loss_forward(x.to(DEV), w.to(DEV, BF16), t.to(DEV))
+    with pytest.raises(ValueError):
+        F.vocab_loss_forward(x.to(DEV), w.to(DEV), t.to(DEV).float())
+    with pytest.raises(ValueError):
+        F.vocab_loss_forward(x.to(DEV), w.to(DEV), t.to(DEV), ignore=(1, 2, 3, 4, 5))
+    with pytest.raises(ValueError):
+        F.vocab_loss_forward(x.to(DEV), w.to(DEV), t.to(DEV), bias=b.to(DEV, BF16))
+    with pytest.raises(ValueError):
+        F.vocab_loss_grad(a.double().to(DEV), x.to(DEV), w.to(DEV), t.to(DEV), a.to(DEV))
+
+
+# ---- all three in one step ----------------------------------------------------------------------------------------------
+class Chain:
+    """A one-layer decoder on the three operators: embedding + positions -> causal self-attention -> cross-attention to image
+    tokens -> vocabulary loss, the projections left out; forward and all gradients by the plain calls."""
+
+    def __init__(self, B=6, T=19, S=25, heads=2, D=64, V=700, dtype=BF16, seed=0):
+        g = gen(seed)
+        H = heads * D
+        self.shape = (B, T, S, heads, D, V)
+        self.ids = torch.randint(3, V, (B, T + 1), generator=g)
+        n = torch.randint(3, T + 2, (B, 1), generator=g)
+        self.ids = torch.where(torch.arange(T + 1) < n, self.ids, 0)
+        self.table = (0.7 * torch.randn(V, H, generator=g)).to(dtype)
+        self.pos = (0.7 * torch.randn(T, H, generator=g)).to(dtype)
+        self.image = torch.randn(B, S, heads, D, generator=g).to(dtype)
+        self.w = (0.3 * torch.randn(V, H, generator=g)).to(dtype)
+
+    def cuda(self):
+        for n in ("ids", "table", "pos", "image", "w"):
+            setattr(self, n, getattr(self, n).to(DEV))
+        return self
+
+    def step(self, F):
+        B, T, S, heads, D, V = self.shape
+        ids, targets = self.ids[:, :-1], self.ids[:, 1:].reshape(-1)
+        seen = ids != 0
+        x = F.embedding_forward(ids, self.table, self.pos, scale=1.5)
+        h = x.view(B, T, heads, D)
+        o1, l1 = F.attention_forward(h, h, h, causal=True, key_mask=seen)
+        o2, l2 = F.attention_forward(o1, self.image, self.image)
+        y = o2.view(B * T, heads * D)
+        loss, lse = F.vocab_loss_forward(y, self.w, targets, ignore=(0,))
+        ones = torch.ones_like(loss)
+        dy, dw, _ = F.vocab_loss_grad(ones, y, self.w, targets, lse, ignore=(0,))
+        do1, dk2, dv2 = F.attention_grad(dy.view(B, T, heads, D), o1, self.image, self.image, o2, l2)
+        dq, dk, dv = F.attention_grad(do1, h, h, h, o1, l1, causal=True, key_mask=seen)
+        dx = (dq.float() + dk.float() + dv.float()).view(B, T, heads * D)
+        dt, dp = F.embedding_grad(dx, ids, V, scale=1.5, positions=T, dtype=torch.float32)
+        return {"loss": loss, "dw": dw, "dk2": dk2, "dv2": dv2, "dt": dt, "dp": dp}
+
+    def reference(self):
+        """The same in 64 bits by torch's automatic differentiation."""
+        B, T, S, heads, D, V = self.shape
+        table, pos, w = (t.double().requires_grad_() for t in (self.table, self.pos, self.w))
+        k2, v2 = (self.image.double().requires_grad_() for _ in range(2))
+        ids, targets = self.ids[:, :-1], self.ids[:, 1:].reshape(-1)
+        h = (1.5 * table[ids] + pos).view(B, T, heads, D).transpose(1, 2)
+
+        def attend(q, k, v, see):
+            s = (q @ k.mT / math.sqrt(D)).masked_fill(~see, -1e300)
+            return torch.softmax(s, -1) * see.any(-1, keepdim=True) @ v
+        see = torch.ones(T, T, dtype=torch.bool).tril() & (ids != 0)[:, None, None, :]
+        o1 = attend(h, h, h, see)
+        o2 = attend(o1, k2.transpose(1, 2), v2.transpose(1, 2), torch.ones(T, S, dtype=torch.bool))
+        z = o2.transpose(1, 2).reshape(B * T, heads * D) @ w.T
+        loss = torch.nn.functional.cross_entropy(z, targets, reduction="none", ignore_index=0)
+        loss.sum().backward()
+        return {"loss": loss.detach(), "dw": w.grad, "dk2": k2.grad, "dv2": v2.grad, "dt": table.grad, "dp": pos.grad}
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_chain(F, dtype):
+    """Rounded intermediate tensors (eight roundings to `dtype` between the table and the gradients) and fp32 sums of a few
+    thousand terms: relative error in norm below 16 half steps, plus 2^-14 for the sums."""
+    c = Chain(dtype=dtype)
+    ref = c.reference()
+    got = c.cuda().step(F)
+    for n, r in ref.items():
+        err = (got[n].double().cpu() - r).norm() / r.norm()
+        assert err <= 16 * half(dtype) + 2.0 ** -14, (n, float(err))
+
+
+def test_chain_in_a_graph(F):
+    """Captured once, replayed with other inputs between eager steps: every replay equals the eager step, bit for bit."""
+    c = Chain(seed=1).cuda()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        c.step(F)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = c.step(F)
+    for k in range(4):
+        other = Chain(seed=10 + k).cuda()
+        for n in ("ids", "table", "pos", "image", "w"):
+            getattr(c, n).copy_(getattr(other, n))
+        graph.replay()
+        eager = other.step(F)
+        torch.cuda.synchronize()
+        for n in eager:
+            assert torch.equal(held[n], eager[n]), (k, n)
+
+
+def test_chain_on_two_streams(F):
+    """Two steps in flight at once, each on its own stream, against the same steps one after another."""
+    cs = [Chain(seed=s, B=9, T=60).cuda() for s in (5, 6)]
+    alone = [c.step(F) for c in cs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cs]
+    for _ in range(3):
+        got = []
+        for c, s in zip(cs, streams):
+            with torch.cuda.stream(s):
+                got.append(c.step(F))
+        torch.cuda.synchronize()
+        for g, a in zip(got, alone):
+            for n in a:
+                assert torch.equal(g[n], a[n]), n
