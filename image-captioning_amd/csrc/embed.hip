@@ -7,7 +7,8 @@
 // row of d_table once (zeros for the words that did not occur).
 //
 // The gradient of the table is summed without atomics, so the same inputs give the same bits.  The tokens are sorted by word
-// (stable radix sort on the word's bits, 9 bits at most to a pass), and the SORTED list, not the vocabulary, is cut into equal
+// (up to 8,192 tokens: every token counts the tokens before it, in one launch; more: stable radix sort on the word's bits, 9 bits at
+// most to a pass), and the SORTED list, not the vocabulary, is cut into equal
 // chunks: captions are half padding and words follow Zipf's law, so a split by word would give one workgroup half of the sum.  A
 // run of one word inside a chunk is summed in registers and written once; a run that crosses chunks leaves one fp32 partial row
 // per chunk, which the join adds in the order of the chunks.
@@ -55,14 +56,13 @@ template <typename T, int VEC> __device__ __forceinline__ void store_vec(T* p, c
 }
 
 // ---- lookup: one thread per VEC columns of a row -------------------------------------------------------------------------
-template <typename TT, typename TO, int VEC>
+template <typename TT, typename TO, int VEC, typename I>
 __global__ __launch_bounds__(256) void embed_rows_kernel(const void* __restrict__ ids, int wide, const TT* __restrict__ table, long long ld_table,
                                                          const TT* __restrict__ pos, long long ld_pos, TO* __restrict__ out, float scale,
                                                          long long n, int T, int H, int vocab) {
-    const int per_row = H / VEC;
-    const long long total = n * per_row, stride = (long long)gridDim.x * 256;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += stride) {
-        const long long r = i / per_row;
+    const I per_row = H / VEC, total = (I)n * per_row, stride = (I)gridDim.x * 256;
+    for (I i = (I)blockIdx.x * 256 + threadIdx.x; i < total; i += stride) {
+        const I r = i / per_row;
         const int c = (int)(i - r * per_row) * VEC;
         float v[VEC];
         load_vec<TT, VEC>(table + load_id(ids, wide, r, vocab) * ld_table + c, v);
@@ -70,11 +70,11 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const void* __restrict_
         for (int e = 0; e < VEC; ++e) v[e] *= scale;
         if (pos) {
             float p[VEC];
-            load_vec<TT, VEC>(pos + (r % T) * ld_pos + c, p);
+            load_vec<TT, VEC>(pos + (long long)(r % (I)T) * ld_pos + c, p);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) v[e] += p[e];
         }
-        store_vec<TO, VEC>(out + r * H + c, v);
+        store_vec<TO, VEC>(out + (long long)r * H + c, v);
     }
 }
 
@@ -109,12 +109,26 @@ __global__ __launch_bounds__(SORT_THREADS) void embed_scatter_kernel(SortArgs a)
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     // first place of every digit for this block: digits below it anywhere, then this digit in the blocks before
     unsigned before = 0, total = 0;
-    if (tid < MAX_DIGITS) {
-        for (int b = 0; b < (int)gridDim.x; ++b) {
-            const unsigned c = a.hist[b * MAX_DIGITS + tid];
+    {
+        constexpr int PARTS = SORT_THREADS / MAX_DIGITS;
+        const int dig = tid & (MAX_DIGITS - 1), blocks = gridDim.x;
+#pragma unroll 8
+        for (int b = tid / MAX_DIGITS; b < blocks; b += PARTS) {
+            const unsigned c = a.hist[b * MAX_DIGITS + dig];
             total += c;
-            if (b < (int)blockIdx.x) before += c;
+            before += b < (int)blockIdx.x ? c : 0u;
         }
+        if (tid >= MAX_DIGITS) {
+            wc[tid / MAX_DIGITS][dig] = total;
+            wc[SORT_WAVES / 2 + tid / MAX_DIGITS][dig] = before;
+        }
+        __syncthreads();
+        if (tid < MAX_DIGITS)
+#pragma unroll
+            for (int p = 1; p < PARTS; ++p) {
+                total += wc[p][tid];
+                before += wc[SORT_WAVES / 2 + p][tid];
+            }
     }
     unsigned inc = total;
 #pragma unroll
@@ -176,6 +190,7 @@ struct SumArgs {
     float *head, *tail;     // [chunks][H] partial rows of runs that began before the chunk / go on after it
     long long n;
     int H, vocab, chunk, chunks, slabs;
+    int cleared;            // the rows of words that do not occur are cleared already
     float scale;
 };
 
@@ -199,7 +214,7 @@ template <typename TG, typename TO, int VEC> __global__ __launch_bounds__(256) v
     TO* dt = (TO*)a.d_table;
     if (unit >= sums) {
         const long long v0 = (unit - sums) * 64;
-        if (v0 >= a.vocab) return;
+        if (a.cleared || v0 >= a.vocab) return;
         const int v = (int)v0 + lane;
         bool absent = false;
         if (v < a.vocab) {
@@ -221,24 +236,26 @@ template <typename TG, typename TO, int VEC> __global__ __launch_bounds__(256) v
     const int i0 = chunk * a.chunk, i1 = i0 + a.chunk < (int)a.n ? i0 + a.chunk : (int)a.n;
     const bool cont_in = i0 > 0 && a.key[i0 - 1] == a.key[i0];
     const bool cont_out = i1 < (int)a.n && a.key[i1] == a.key[i1 - 1];
+    // a chunk is at most 64 rows: lane i holds the i-th word and token
+    const int my = i0 + lane < i1 ? i0 + lane : i1 - 1, my_key = a.key[my], my_idx = a.idx[my];
     float acc[VEC] = {};
     bool first = true;  // still in the run the chunk began with
-    int word = a.key[i0];
+    int word = __builtin_amdgcn_readlane(my_key, 0);
     constexpr int U = 8;  // rows in flight
-    for (int i = i0; i < i1; i += U) {
+    const int rows = i1 - i0;
+    for (int i = 0; i < rows; i += U) {
         float v[U][VEC];
-        int w[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int j = i + u < i1 ? i + u : i1 - 1;
-            w[u] = a.key[j];
-            const long long row = a.idx[j];
+            const int j = i + u < rows ? i + u : rows - 1;
+            const long long row = __builtin_amdgcn_readlane(my_idx, j);
             if (live) load_vec<TG, VEC>(g + row * a.H + col, v[u]);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (i + u >= i1) break;
-            if (w[u] != word) {  // the run ended: the same branch for the whole wave
+            if (i + u >= rows) break;
+            const int w = __builtin_amdgcn_readlane(my_key, i + u);
+            if (w != word) {  // the run ended: the same branch for the whole wave
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) acc[e] = first && cont_in ? acc[e] : acc[e] * a.scale;
                 if (live) {
@@ -246,7 +263,7 @@ template <typename TG, typename TO, int VEC> __global__ __launch_bounds__(256) v
                     else store_vec<TO, VEC>(dt + (long long)word * a.H + col, acc);
                 }
                 first = false;
-                word = w[u];
+                word = w;
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
             }
@@ -266,64 +283,101 @@ template <typename TG, typename TO, int VEC> __global__ __launch_bounds__(256) v
     }
 }
 
-// One workgroup per chunk whose last run begins in it and goes on: adds that run's partial rows in chunk order.
-template <typename TO, int VEC> __global__ __launch_bounds__(256) void embed_join_kernel(SumArgs a) {
-    __shared__ float part[4][64 * VEC];
-    __shared__ int last_chunk;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int chunk = blockIdx.x, slab = blockIdx.y;
-    const int i0 = chunk * a.chunk, i1 = i0 + a.chunk;
-    if (i1 >= (int)a.n) return;
-    const int word = a.key[i1 - 1];
-    if (a.key[i1] != word) return;
-    if (i0 > 0 && a.key[i0] == word && a.key[i0 - 1] == word) return;  // began in an earlier chunk
-    if (threadIdx.x == 0) last_chunk = (lower_bound_key(a.key, (int)a.n, word + 1) - 1) / a.chunk;
-    __syncthreads();
-    const int m = last_chunk - chunk + 1;  // the tail of this chunk, then the heads of the following ones
-    const int col = (slab * 64 + lane) * VEC;
-    const bool live = col < a.H;
-    const int lo = (int)((long long)m * wave / 4), hi = (int)((long long)m * (wave + 1) / 4);
-    float acc[VEC] = {};
-    constexpr int U = 4;
+// Joins the partial rows of a run that crosses chunks, in the order of the chunks: the tail of the chunk it begins in (the owner),
+// then the heads of the following chunks, all of which begin with its word.  Most such runs cross one border and a wave each does
+// them; a run over more than JOIN_LONG chunks takes a workgroup of 16 waves, found by the one chunk number in JOIN_LONG that is a
+// multiple of it and the first such in the run.
+constexpr int JOIN_LONG = 32;
+
+template <int VEC> __device__ __forceinline__ void add_partials(const SumArgs& a, int owner, int lo, int hi, int col, bool live, float (&acc)[VEC]) {
+    constexpr int U = VEC == 1 ? 16 : 8;
     for (int k = lo; k < hi; k += U) {
         float v[U][VEC];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int j = k + u < hi ? k + u : hi - 1;
-            if (live) load_vec<float, VEC>((j == 0 ? a.tail : a.head) + (long long)(chunk + j) * a.H + col, v[u]);
+            if (live) load_vec<float, VEC>((j == 0 ? a.tail : a.head) + (long long)(owner + j) * a.H + col, v[u]);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int e = 0; e < VEC; ++e) acc[e] += live && k + u < hi ? v[u][e] : 0.f;
     }
+}
+
+template <typename TO, int VEC> __global__ __launch_bounds__(1024) void embed_join_kernel(SumArgs a, int long_blocks) {
+    __shared__ float part[16][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    TO* dt = (TO*)a.d_table;
+    float acc[VEC] = {};
+    if ((int)blockIdx.x >= long_blocks) {  // a wave per chunk and slab
+        const long long unit = (long long)(blockIdx.x - long_blocks) * 16 + wave;
+        const int chunk = (int)(unit / a.slabs), slab = (int)(unit - (long long)chunk * a.slabs);
+        if (chunk >= a.chunks - 1) return;
+        const int i0 = chunk * a.chunk, i1 = i0 + a.chunk, word = a.key[i1 - 1];
+        if (a.key[i1] != word) return;
+        if (i0 > 0 && a.key[i0] == word && a.key[i0 - 1] == word) return;  // began in an earlier chunk
+        const int next = chunk + 1 + lane;
+        const unsigned long long same = __ballot(next < a.chunks && a.key[(long long)(next < a.chunks ? next : chunk) * a.chunk] == word);
+        const int m = 1 + __popcll(same);
+        if (m > JOIN_LONG) return;
+        const int col = (slab * 64 + lane) * VEC;
+        const bool live = col < a.H;
+        add_partials<VEC>(a, chunk, 0, m, col, live, acc);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) part[wave][lane * VEC + e] = acc[e];
+        for (int e = 0; e < VEC; ++e) acc[e] *= a.scale;
+        if (live) store_vec<TO, VEC>(dt + (long long)word * a.H + col, acc);
+        return;
+    }
+    // 64 columns each, so that a run's partial rows are read by several compute units
+    const int slabs = (a.H + 63) / 64, at = (blockIdx.x / slabs + 1) * JOIN_LONG, slab = blockIdx.x % slabs;  // at < chunks
+    const int word = a.key[(long long)at * a.chunk];
+    {  // most runs are short: the chunks at - 32 .. at + 31 tell
+        const int near = at - 32 + lane;
+        const unsigned long long same = __ballot(near < a.chunks && a.key[(long long)(near < a.chunks ? near : at) * a.chunk] == word);
+        if (__popcll(same) < JOIN_LONG - 1) return;  // the same for every wave
+    }
+    int before = 0, after = 0;  // chunks before `at`, and from `at` on, that begin with the word
+    for (int c = at - 1;; c -= 1024) {
+        const int mine = c - (int)threadIdx.x;
+        const int more = __syncthreads_count(mine >= 0 && a.key[(long long)(mine >= 0 ? mine : 0) * a.chunk] == word);
+        before += more;
+        if (more < 1024) break;
+    }
+    for (int c = at;; c += 1024) {
+        const int mine = c + (int)threadIdx.x;
+        const int more = __syncthreads_count(mine < a.chunks && a.key[(long long)(mine < a.chunks ? mine : at) * a.chunk] == word);
+        after += more;
+        if (more < 1024) break;
+    }
+    const int begin = at - before;  // the first chunk that begins with the word; the run may begin before it
+    const int owner = begin > 0 && a.key[(long long)begin * a.chunk - 1] == word ? begin - 1 : begin;
+    const int m = at + after - owner;
+    if (m <= JOIN_LONG || at <= owner || at - JOIN_LONG > owner) return;
+    const int col = slab * 64 + lane;
+    float sum[1] = {};
+    add_partials<1>(a, owner, (int)((long long)m * wave / 16), (int)((long long)m * (wave + 1) / 16), col, col < a.H, sum);
+    part[wave][lane] = sum[0];
     __syncthreads();
-    if (wave == 0 && live) {
+    if (wave == 0 && col < a.H) {
+        float t = part[0][lane];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            float s = part[0][lane * VEC + e];
-#pragma unroll
-            for (int w = 1; w < 4; ++w) s += part[w][lane * VEC + e];
-            acc[e] = s * a.scale;
-        }
-        store_vec<TO, VEC>((TO*)a.d_table + (long long)word * a.H + col, acc);
+        for (int w = 1; w < 16; ++w) t += part[w][lane];
+        dt[(long long)word * a.H + col] = from_f32<TO>(t * a.scale);
     }
 }
 
 // ---- sum over sequences: columns of a [B][W] matrix, W = T*H; `slices` of the rows leave fp32 partial rows when there are several
 template <typename TG, typename TO, int VEC>
-__global__ __launch_bounds__(256) void embed_colsum_kernel(const TG* __restrict__ g, TO* __restrict__ out, float* __restrict__ part_out, int B,
-                                                           long long W, int slices) {
-    __shared__ float part[4][64 * VEC];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, slice = blockIdx.y;
-    const long long col = ((long long)blockIdx.x * 64 + lane) * VEC;
+__device__ __forceinline__ void colsum(float* part, const TG* __restrict__ g, TO* __restrict__ out, float* __restrict__ part_out, int B, long long W, int slices,
+                                       long long group, int slice) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long long col = (group * 64 + lane) * VEC;
     const bool live = col < W;
     const int b0 = (int)((long long)B * slice / slices), b1 = (int)((long long)B * (slice + 1) / slices), rows = b1 - b0;
-    const int lo = b0 + (int)((long long)rows * wave / 4), hi = b0 + (int)((long long)rows * (wave + 1) / 4);
+    const int lo = b0 + (int)((long long)rows * wave / 16), hi = b0 + (int)((long long)rows * (wave + 1) / 16);
     float acc[VEC] = {};
-    constexpr int U = 4;
+    constexpr int U = 8;
     for (int b = lo; b < hi; b += U) {
         float v[U][VEC];
 #pragma unroll
@@ -337,23 +391,100 @@ __global__ __launch_bounds__(256) void embed_colsum_kernel(const TG* __restrict_
             for (int e = 0; e < VEC; ++e) acc[e] += live && b + u < hi ? v[u][e] : 0.f;
     }
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) part[wave][lane * VEC + e] = acc[e];
+    for (int e = 0; e < VEC; ++e) part[wave * 64 * VEC + lane * VEC + e] = acc[e];
     __syncthreads();
-    if (wave == 0 && live) {
+    // 64 * VEC columns over 1024 threads
+    for (int c = threadIdx.x; c < 64 * VEC; c += 1024) {
+        const long long at = group * 64 * VEC + c;
+        if (at >= W) continue;
+        float s = part[c];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            float s = part[0][lane * VEC + e];
-#pragma unroll
-            for (int w = 1; w < 4; ++w) s += part[w][lane * VEC + e];
-            acc[e] = s;
-        }
-        if (slices == 1) store_vec<TO, VEC>(out + col, acc);
-        else store_vec<float, VEC>(part_out + slice * W + col, acc);
+        for (int w = 1; w < 16; ++w) s += part[w * 64 * VEC + c];
+        if (slices == 1) out[at] = from_f32<TO>(s);
+        else part_out[slice * W + at] = s;
     }
+}
+template <typename TO> __global__ __launch_bounds__(1024) void embed_colsum_join_kernel(const float* __restrict__ part_in, TO* __restrict__ out, int parts, long long W) {
+    __shared__ float part[16 * 64];
+    colsum<float, TO, 1>(part, part_in, out, nullptr, parts, W, 1, blockIdx.x, 0);
+}
+
+// ---- the first launch of the gradient: three jobs that need nothing from each other, by block number -------------------------
+//  1. sorting: up to 8,192 tokens every token's place by counting the tokens that come before it; else the first histogram
+//  2. up to 8,192 tokens: the rows of words that do not occur are cleared (with more, embed_sum_kernel does it by searching)
+//  3. the sums over sequences
+struct FirstArgs {
+    SortArgs sort;
+    const void* g;
+    void *d_table, *d_pos;
+    float* pos_part;
+    long long W;
+    int H, B, slices, rank_blocks, zero_blocks;
+    long long groups;
+};
+constexpr int RANK_MAX = 8192, RANK_TOKENS = 32, ZERO_ROWS = 128;
+constexpr int RANK_MAX_VOCAB = 1 << 18;  // word and token number share 31 bits
+
+template <typename TG, typename TO, int VEC> __global__ __launch_bounds__(1024) void embed_first_kernel(FirstArgs f) {
+    __shared__ __attribute__((aligned(16))) unsigned lds[RANK_MAX + 1024];  // 36 KiB, also the column sums' 16 x 64 x VEC floats
+    static_assert(16 * 64 * VEC <= RANK_MAX + 1024, "column sums fit");
+    const SortArgs& a = f.sort;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int block = blockIdx.x;
+    if (block < f.rank_blocks) {
+        // the place of token i is the number of (word, token) pairs below its own
+        const int n = (int)a.n, n4 = (n + 127) / 128 * 128;
+#pragma unroll 8
+        for (int i = tid; i < n4; i += 1024) lds[i] = i < n ? ((unsigned)load_id(a.ids, a.wide, i, a.vocab) << 13) | (unsigned)i : 0xffffffffu;
+        __syncthreads();
+        // 32 tokens to a workgroup (240 of them for 7,680 tokens), a half wave per thirty-second of the list
+        const int i = block * RANK_TOKENS + (lane & 31), part = tid >> 5;
+        const unsigned mine = lds[i < n ? i : n - 1];
+        unsigned count = 0;
+        const int per = n4 / 32;
+        const uint4* p = reinterpret_cast<const uint4*>(lds + part * per);
+#pragma unroll 4
+        for (int k = 0; k < per / 4; ++k) {
+            const uint4 c = p[k];
+            count += (c.x < mine) + (c.y < mine) + (c.z < mine) + (c.w < mine);
+        }
+        unsigned* counts = lds + RANK_MAX;
+        counts[tid] = count;
+        __syncthreads();
+        if (tid < RANK_TOKENS && i < n) {
+            unsigned at = 0;
+#pragma unroll
+            for (int w = 0; w < 32; ++w) at += counts[w * 32 + tid];
+            a.key_out[at] = (int)(mine >> 13);
+            a.idx_out[at] = i;
+        }
+        return;
+    }
+    block -= f.rank_blocks;
+    if (block < f.zero_blocks) {
+        const int v0 = block * ZERO_ROWS, n = (int)a.n;
+        if (tid < ZERO_ROWS) lds[tid] = 0;
+        __syncthreads();
+#pragma unroll 8
+        for (int i = tid; i < n; i += 1024) {
+            const int v = load_id(a.ids, a.wide, i, a.vocab) - v0;
+            if (v >= 0 && v < ZERO_ROWS) lds[v] = 1;
+        }
+        __syncthreads();
+        const float zero[VEC] = {};
+        for (int r = wave; r < ZERO_ROWS && v0 + r < a.vocab; r += 16) {
+            if (lds[r]) continue;
+            for (int c = lane * VEC; c < f.H; c += 64 * VEC) store_vec<TO, VEC>((TO*)f.d_table + (long long)(v0 + r) * f.H + c, zero);
+        }
+        return;
+    }
+    block -= f.zero_blocks;
+    colsum<TG, TO, VEC>(reinterpret_cast<float*>(lds), (const TG*)f.g, (TO*)f.d_pos, f.pos_part, f.B, f.W, f.slices, block % f.groups, (int)(block / f.groups));
 }
 
 // ---- the gradient's plan: everything that depends on the sizes alone -------------------------------------------------------
 struct GradPlan {
+    bool rank;              // few tokens: places by counting
     int sort_blocks, per_block, passes, bits;
     int chunk, chunks, slices;
     long long key[2], idx[2], hist, head, tail, pos, bytes;  // byte offsets into the workspace
@@ -363,6 +494,7 @@ long long up256(long long b) { return (b + 255) / 256 * 256; }
 
 GradPlan grad_plan(long long n, int T, int H, int vocab, bool want_pos) {
     GradPlan p = {};
+    p.rank = n <= RANK_MAX && vocab <= RANK_MAX_VOCAB;
     int blocks = (int)((n + SORT_THREADS - 1) / SORT_THREADS);
     blocks = blocks < 1 ? 1 : blocks > MAX_SORT_BLOCKS ? MAX_SORT_BLOCKS : blocks;
     p.per_block = (int)(((n + blocks - 1) / blocks + SORT_THREADS - 1) / SORT_THREADS * SORT_THREADS);
@@ -372,10 +504,10 @@ GradPlan grad_plan(long long n, int T, int H, int vocab, bool want_pos) {
     while (nb < 31 && (1ll << nb) < vocab) ++nb;
     p.passes = (nb + 8) / 9;
     p.bits = (nb + p.passes - 1) / p.passes;
-    // a wave per chunk and 512 columns: about 4,096 of them, 8 to 64 rows each
+    // a wave per chunk and 512 columns: about 4,096 of them, 16 to 64 rows each
     const int slabs = (H + 511) / 512;
     long long c = n * slabs / 4096;
-    p.chunk = (int)(c < 8 ? 8 : c > 64 ? 64 : c);
+    p.chunk = (int)(c < 16 ? 16 : c > 64 ? 64 : c);  // at most the 64 lanes that hold a chunk's words
     p.chunks = (int)((n + p.chunk - 1) / p.chunk);
     long long o = 0;
     for (int i = 0; i < 2; ++i) {
@@ -387,10 +519,10 @@ GradPlan grad_plan(long long n, int T, int H, int vocab, bool want_pos) {
     p.tail = o; o += up256((long long)p.chunks * H * 4);
     p.slices = 1;
     if (want_pos) {
-        // about 1,024 workgroups over the columns of [B][T*H], at least 32 sequences to a slice
+        // up to 256 workgroups over the columns of [B][T*H], at least 512 sequences to a slice
         const long long B = n / T, groups = ((long long)T * H + 511) / 512;
-        long long s = 1024 / (groups < 1 ? 1 : groups);
-        if (s > B / 32) s = B / 32;
+        long long s = 256 / (groups < 1 ? 1 : groups);
+        if (s > B / 512) s = B / 512;
         p.slices = (int)(s < 1 ? 1 : s > 512 ? 512 : s);
         p.pos = o;
         if (p.slices > 1) o += up256((long long)p.slices * T * H * 4);
@@ -407,7 +539,29 @@ int launch_grad(const GradPlan& p, const void* ids, int wide, const void* g, voi
     SortArgs a = {};
     a.wide = wide; a.vocab = vocab; a.n = n; a.per_block = p.per_block; a.bits = p.bits;
     a.hist = (unsigned*)(ws + p.hist);
-    for (int i = 0; i < p.passes && n > 0; ++i) {
+    a.ids = ids;
+    a.key_out = (int*)(ws + p.key[0]);
+    a.idx_out = (int*)(ws + p.idx[0]);
+    FirstArgs f = {};
+    f.sort = a;
+    f.g = g; f.d_table = d_table; f.d_pos = d_pos; f.H = H;
+    f.pos_part = (float*)(ws + p.pos);
+    if (p.rank) {
+        f.rank_blocks = (int)((n + RANK_TOKENS - 1) / RANK_TOKENS);
+        f.zero_blocks = (vocab + ZERO_ROWS - 1) / ZERO_ROWS;
+    }
+    if (d_pos) {
+        f.B = (int)(n / T);
+        f.W = (long long)T * H;
+        f.slices = p.slices;
+        f.groups = (f.W + 64 * VEC - 1) / (64 * VEC);
+    }
+    const long long first = f.rank_blocks + f.zero_blocks + f.groups * f.slices;
+    if (first > 0) MIC_LAUNCH((embed_first_kernel<TG, TO, VEC>), dim3((unsigned)first), dim3(1024), 0, s, f);
+    if (d_pos && p.slices > 1)
+        MIC_LAUNCH((embed_colsum_join_kernel<TO>), dim3((unsigned)((f.W + 63) / 64)), dim3(1024), 0, s, (const float*)f.pos_part, (TO*)d_pos, p.slices, f.W);
+    const int passes = p.rank ? 1 : p.passes;
+    for (int i = 0; i < passes && !p.rank; ++i) {
         a.ids = i == 0 ? ids : nullptr;
         a.key_in = (const int*)(ws + p.key[(i + 1) & 1]);
         a.idx_in = (const int*)(ws + p.idx[(i + 1) & 1]);
@@ -417,23 +571,20 @@ int launch_grad(const GradPlan& p, const void* ids, int wide, const void* g, voi
         MIC_LAUNCH(embed_hist_kernel, dim3(p.sort_blocks), dim3(SORT_THREADS), 0, s, a);
         MIC_LAUNCH(embed_scatter_kernel, dim3(p.sort_blocks), dim3(SORT_THREADS), 0, s, a);
     }
+    if (n == 0) return 0;
     SumArgs m = {};
-    m.key = (const int*)(ws + p.key[(p.passes - 1) & 1]);
-    m.idx = (const int*)(ws + p.idx[(p.passes - 1) & 1]);
+    m.key = (const int*)(ws + p.key[(passes - 1) & 1]);
+    m.idx = (const int*)(ws + p.idx[(passes - 1) & 1]);
     m.g = g; m.d_table = d_table;
     m.head = (float*)(ws + p.head); m.tail = (float*)(ws + p.tail);
-    m.n = n; m.H = H; m.vocab = vocab; m.chunk = p.chunk; m.chunks = p.chunks; m.scale = scale;
+    m.n = n; m.H = H; m.vocab = vocab; m.chunk = p.chunk; m.chunks = p.chunks; m.scale = scale; m.cleared = p.rank;
     m.slabs = (H + 64 * VEC - 1) / (64 * VEC);
-    const long long units = (long long)p.chunks * m.slabs + (vocab + 63) / 64;
+    const long long units = (long long)p.chunks * m.slabs + (p.rank ? 0 : (vocab + 63) / 64);
     MIC_LAUNCH((embed_sum_kernel<TG, TO, VEC>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, s, m);
-    if (p.chunks > 1) MIC_LAUNCH((embed_join_kernel<TO, VEC>), dim3(p.chunks, m.slabs), dim3(256), 0, s, m);
-    if (d_pos) {
-        const long long W = (long long)T * H;
-        const unsigned groups = (unsigned)((W + 64 * VEC - 1) / (64 * VEC));
-        float* part = (float*)(ws + p.pos);
-        MIC_LAUNCH((embed_colsum_kernel<TG, TO, VEC>), dim3(groups, p.slices), dim3(256), 0, s, (const TG*)g, (TO*)d_pos, part, (int)(n / T), W, p.slices);
-        if (p.slices > 1)
-            MIC_LAUNCH((embed_colsum_kernel<float, TO, VEC>), dim3(groups, 1), dim3(256), 0, s, (const float*)part, (TO*)d_pos, (float*)nullptr, p.slices, W, 1);
+    if (p.chunks > 1) {
+        const int long_blocks = (p.chunks - 1) / JOIN_LONG * ((H + 63) / 64);
+        const long long waves = (long long)(p.chunks - 1) * m.slabs;
+        MIC_LAUNCH((embed_join_kernel<TO, VEC>), dim3((unsigned)(long_blocks + (waves + 15) / 16)), dim3(1024), 0, s, m, long_blocks);
     }
     return 0;
 }
@@ -452,10 +603,16 @@ extern "C" int mic_embed_rows(const void* ids, int ids_bits, const void* table, 
     const bool vec = H % 8 == 0 && ld_table % 8 == 0 && (!pos || ld_pos % 8 == 0) && (((uintptr_t)table | (uintptr_t)out | (uintptr_t)pos) & 15) == 0;
     const long long work = n * (vec ? H / 8 : H);
     const long long blocks = (work + 255) / 256;
-    const dim3 grid((unsigned)(blocks > 65536 ? 65536 : blocks));
-#define GO(TT, TO, VEC)                                                                                                                   \
-    MIC_LAUNCH((embed_rows_kernel<TT, TO, VEC>), grid, dim3(256), 0, s, ids, ids_bits == 64, (const TT*)table, (long long)ld_table, (const TT*)pos, \
+    const dim3 grid((unsigned)(blocks > 1048576 ? 1048576 : blocks));
+    const bool small = work < (1ll << 31);  // 32-bit index arithmetic: a 64-bit division costs as much as the rest of the thread
+#define GO_I(TT, TO, VEC, I)                                                                                                                    \
+    MIC_LAUNCH((embed_rows_kernel<TT, TO, VEC, I>), grid, dim3(256), 0, s, ids, ids_bits == 64, (const TT*)table, (long long)ld_table, (const TT*)pos, \
                (long long)ld_pos, (TO*)out, scale, (long long)n, T, H, vocab)
+#define GO(TT, TO, VEC)                       \
+    do {                                      \
+        if (small) GO_I(TT, TO, VEC, unsigned); \
+        else GO_I(TT, TO, VEC, long long);    \
+    } while (0)
 #define GO_VEC(TT, TO)             \
     do {                           \
         if (vec) GO(TT, TO, 8);    \
@@ -465,6 +622,7 @@ extern "C" int mic_embed_rows(const void* ids, int ids_bits, const void* table, 
     else if (table_dtype == MIC_F32) GO_VEC(float, bf16_t);
     else if (out_dtype == MIC_F32) GO_VEC(bf16_t, float);
     else GO_VEC(bf16_t, bf16_t);
+#undef GO_I
 #undef GO
 #undef GO_VEC
     return 0;

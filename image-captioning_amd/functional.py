@@ -11,58 +11,87 @@ types, devices) or ``_lib.MicError`` (what the library refuses).
 """
 from __future__ import annotations
 
-import ctypes as C
 import math
+import struct
 from typing import Optional
 
 import torch
 
 from . import _lib as L
 
+_raw_stream = torch._C._cuda_getCurrentRawStream  # what torch.cuda.current_stream(i).cuda_stream returns, without building the object
+
 __all__ = ["embedding", "embedding_forward", "embedding_grad", "attention", "attention_forward", "attention_grad",
            "vocab_loss", "vocab_loss_forward", "vocab_loss_grad"]
 
 
-def _device(name: str, *tensors) -> torch.device:
-    """The one HIP device all given tensors (None is skipped) live on."""
-    dev = None
+# These calls are a few microseconds of host work around launches that can be as short, so the checks build their messages only
+# when they fail, and the descriptors are packed in one go instead of field by field.
+def _device(name: str, *tensors) -> int:
+    """Ordinal of the one HIP device all given tensors (None is skipped) live on."""
+    dev = -1
     for t in tensors:
         if t is None:
             continue
         if not isinstance(t, torch.Tensor):
             raise ValueError(f"{name}: expected tensors, got {type(t).__name__}")
-        if t.device.type != "cuda":
+        if not t.is_cuda:
             raise ValueError(f"{name}: tensors must be on a HIP device, got one on {t.device}")
-        if dev is not None and t.device != dev:
-            raise ValueError(f"{name}: tensors are on {dev} and {t.device}")
-        dev = t.device
+        i = t.get_device()
+        if dev != i and dev >= 0:
+            raise ValueError(f"{name}: tensors are on devices {dev} and {i}")
+        dev = i
     return dev
 
 
-def _need(ok: bool, name: str, what: str) -> None:
-    if not ok:
-        raise ValueError(f"{name}: {what}")
-
-
 def _float_code(name: str, what: str, dtype) -> int:
-    if dtype not in (torch.float32, torch.bfloat16):
-        raise ValueError(f"{name}: {what} must be float32 or bfloat16, got {dtype}")
-    return L.F32 if dtype == torch.float32 else L.BF16
+    if dtype is torch.float32:
+        return L.F32
+    if dtype is torch.bfloat16:
+        return L.BF16
+    raise ValueError(f"{name}: {what} must be float32 or bfloat16, got {dtype}")
 
 
-def _workspace(name: str, size: int, dev) -> torch.Tensor:
+def _workspace(name: str, size: int, like: torch.Tensor):
+    """`size` bytes of scratch and its address; the caller keeps the tensor until its launches are enqueued."""
     if size < 0:
-        raise ValueError(f"{name}: sizes out of range")
-    return torch.empty(size, dtype=torch.uint8, device=dev)
+        L.check(size, name)
+    if size == 0:
+        return None, 0
+    ws = torch.empty(size, dtype=torch.uint8, device=like.device)
+    return ws, ws.data_ptr()
 
 
 def _ids(name: str, what: str, t: torch.Tensor) -> torch.Tensor:
-    _need(t.dtype in (torch.int32, torch.int64), name, f"{what} must be int32 or int64, got {t.dtype}")
+    if t.dtype is not torch.int64 and t.dtype is not torch.int32:
+        raise ValueError(f"{name}: {what} must be int32 or int64, got {t.dtype}")
     return t.contiguous()
 
 
-def _stream(dev) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+def _bits(t: torch.Tensor) -> int:
+    return 64 if t.dtype is torch.int64 else 32
+
+
+def _run(what: str, fn, dev: int, *args) -> None:
+    """fn(*args, current stream of the device), with that device current."""
+    if torch.cuda.current_device() == dev:
+        rc = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev))
+    if rc != 0:
+        L.check(rc, what)
+
+
+def _ptr(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """A matrix whose rows are consecutive in memory and do not overlap (the tensor itself where it is one)."""
+    if t.stride(1) == 1 and (t.stride(0) >= t.shape[1] or t.shape[0] == 1):
+        return t
+    return t.contiguous()
 
 
 # ---- embedding --------------------------------------------------------------------------------------------------------
@@ -74,25 +103,28 @@ def embedding_forward(ids: torch.Tensor, table: torch.Tensor, pos: Optional[torc
     last dimension of ids.  Ids outside the vocabulary read its nearest row.  Returns (..., T, H)."""
     name = "embedding_forward"
     dev = _device(name, ids, table, pos)
-    _need(table.dim() == 2 and table.shape[0] > 0 and table.shape[1] > 0, name, f"table must be (vocab, H), got {tuple(table.shape)}")
-    _need(ids.dim() >= 1, name, "ids need at least one dimension")
-    H, T = table.shape[1], ids.shape[-1]
+    if table.dim() != 2 or table.numel() == 0:
+        raise ValueError(f"{name}: table must be (vocab, H), got {tuple(table.shape)}")
+    if ids.dim() < 1:
+        raise ValueError(f"{name}: ids need at least one dimension")
+    vocab, H = table.shape
+    T = ids.shape[-1]
     code = _float_code(name, "the table", table.dtype)
-    out_dtype = dtype if dtype is not None else table.dtype
+    out_dtype = table.dtype if dtype is None else dtype
     out_code = _float_code(name, "the output", out_dtype)
+    pos_ptr, ld_pos = None, 0
     if pos is not None:
-        _need(pos.dim() == 2 and pos.shape[1] == H and pos.shape[0] >= T and pos.dtype == table.dtype, name,
-              f"pos must be (>= {T}, {H}) of {table.dtype}, got {tuple(pos.shape)} of {pos.dtype}")
-        pos = pos if pos.stride(1) == 1 and pos.stride(0) >= H else pos.contiguous()
-    table = table if table.stride(1) == 1 and table.stride(0) >= H else table.contiguous()
+        if pos.dim() != 2 or pos.shape[1] != H or pos.shape[0] < T or pos.dtype is not table.dtype:
+            raise ValueError(f"{name}: pos must be (>= {T}, {H}) of {table.dtype}, got {tuple(pos.shape)} of {pos.dtype}")
+        pos = _rows(pos)
+        pos_ptr, ld_pos = pos.data_ptr(), max(pos.stride(0), H)
+    table = _rows(table)
     ids = _ids(name, "ids", ids)
-    out = torch.empty(*ids.shape, H, dtype=out_dtype, device=dev)
-    if ids.numel() == 0:
-        return out
-    with torch.cuda.device(dev):
-        L.check(L.lib.mic_embed_rows(ids.data_ptr(), 64 if ids.dtype == torch.int64 else 32, table.data_ptr(), table.stride(0), L.ptr(pos),
-                                     pos.stride(0) if pos is not None else 0, out.data_ptr(), code, out_code, scale, ids.numel(), T, H,
-                                     table.shape[0], _stream(dev)), "mic_embed_rows")
+    out = torch.empty((*ids.shape, H), dtype=out_dtype, device=table.device)
+    n = ids.numel()
+    if n:
+        _run("mic_embed_rows", L.lib.mic_embed_rows, dev, ids.data_ptr(), _bits(ids), table.data_ptr(), max(table.stride(0), H), pos_ptr, ld_pos,
+             out.data_ptr(), code, out_code, scale, n, T, H, vocab)
     return out
 
 
@@ -103,26 +135,30 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, vocab: int, *, scale: 
     Sums run in fp32 over the tokens sorted by word: the same inputs give the same bits."""
     name = "embedding_grad"
     dev = _device(name, grad, ids)
-    _need(ids.dim() >= 1 and grad.shape[:-1] == ids.shape and grad.dim() == ids.dim() + 1, name,
-          f"grad {tuple(grad.shape)} does not fit ids {tuple(ids.shape)}")
+    if ids.dim() < 1 or grad.shape[:-1] != ids.shape:
+        raise ValueError(f"{name}: grad {tuple(grad.shape)} does not fit ids {tuple(ids.shape)}")
     H, T, n = grad.shape[-1], ids.shape[-1], ids.numel()
-    _need(H > 0 and vocab > 0, name, f"bad sizes H={H} vocab={vocab}")
-    _need(positions == 0 or positions >= T, name, f"{positions} positions for sequences of {T}")
+    if H < 1 or vocab < 1:
+        raise ValueError(f"{name}: bad sizes H={H} vocab={vocab}")
+    if positions and positions < T:
+        raise ValueError(f"{name}: {positions} positions for sequences of {T}")
     code = _float_code(name, "grad", grad.dtype)
-    out_dtype = dtype if dtype is not None else grad.dtype
+    out_dtype = grad.dtype if dtype is None else dtype
     out_code = _float_code(name, "the gradients", out_dtype)
     ids, grad = _ids(name, "ids", ids), grad.contiguous()
-    d_table = torch.empty(vocab, H, dtype=out_dtype, device=dev)
+    d_table = torch.empty((vocab, H), dtype=out_dtype, device=grad.device)
     d_pos = None
     if positions:
-        d_pos = torch.empty(positions, H, dtype=out_dtype, device=dev)
+        d_pos = torch.empty((positions, H), dtype=out_dtype, device=grad.device)
         if positions > T:
             d_pos[T:].zero_()
     T = max(T, 1)
-    with torch.cuda.device(dev):
-        ws = _workspace(name, int(L.lib.mic_embed_grad_workspace_bytes(n, T, H, vocab, int(bool(positions)))), dev)
-        L.check(L.lib.mic_embed_grad(ids.data_ptr(), 64 if ids.dtype == torch.int64 else 32, grad.data_ptr(), d_table.data_ptr(), L.ptr(d_pos),
-                                     code, out_code, scale, n, T, H, vocab, ws.data_ptr(), ws.numel(), _stream(dev)), "mic_embed_grad")
+    size = L.lib.mic_embed_grad_workspace_bytes(n, T, H, vocab, 1 if positions else 0)
+    if size < 0:
+        raise ValueError(f"{name}: sizes out of range (tokens {n}, H={H}, vocab={vocab})")
+    ws, ws_ptr = _workspace(name, size, grad)
+    _run("mic_embed_grad", L.lib.mic_embed_grad, dev, ids.data_ptr(), _bits(ids), grad.data_ptr(), d_table.data_ptr(), L.ptr(d_pos), code, out_code,
+         scale, n, T, H, vocab, ws_ptr, size)
     return d_table, d_pos
 
 
@@ -148,52 +184,40 @@ def embedding(ids, table, pos=None, *, scale: float = 1.0, dtype=None) -> torch.
 
 
 # ---- attention --------------------------------------------------------------------------------------------------------
-def _heads(t: torch.Tensor) -> torch.Tensor:
-    """The tensor itself where the kernels can read it in place (columns consecutive, everything on 16-byte boundaries)."""
+_ATTN_PACK = struct.Struct("@10P16q8ifPq")  # mic_attn_seq_desc
+
+
+def _heads(t: torch.Tensor):
+    """The tensor and its strides of (batch, position, head), copied if the kernels cannot read it in place (columns consecutive,
+    everything on 16-byte boundaries).  A dimension of one entry has no stride to speak of."""
     e = 16 // t.element_size()
-    if t.data_ptr() % 16 == 0 and (t.stride(3) == 1 or t.shape[3] == 1) and all(s % e == 0 for s in _strides(t)):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+    B, T, H, D = t.shape
+    sb, st, sh, sd = t.stride()
+    sb, st, sh = sb if B > 1 else 0, st if T > 1 else 0, sh if H > 1 else 0
+    if (sd == 1 or D == 1) and not (sb % e or st % e or sh % e) and not t.data_ptr() % 16:
+        return t, sb, st, sh
+    return t.clone(memory_format=torch.contiguous_format), T * H * D, H * D, D
 
 
-def _strides(t: torch.Tensor):
-    """Strides of (batch, position, head); a dimension of one entry has none to speak of."""
-    return (C.c_int64 * 3)(*(t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)))
-
-
-def _attn_desc(name, q, k, v, causal, key_mask, scale):
+def _attn_check(name, q, k, v, key_mask):
     dev = _device(name, q, k, v, key_mask)
-    _need(q.dim() == 4 and k.dim() == 4 and v.dim() == 4, name, "q, k and v must be (batch, positions, heads, columns)")
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
+        raise ValueError(f"{name}: q, k and v must be (batch, positions, heads, columns), got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     B, Tq, Hq, D = q.shape
-    Tk, Hkv = k.shape[1], k.shape[2]
-    _need(k.shape == v.shape and k.shape[0] == B and k.shape[3] == D and Hq > 0 and Hkv > 0 and D > 0, name,
-          f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit")
-    _need(k.dtype == q.dtype and v.dtype == q.dtype, name, f"q, k and v are {q.dtype}, {k.dtype} and {v.dtype}")
-    d = L.AttnSeqDesc()
-    d.dtype = _float_code(name, "q", q.dtype)
-    q, k, v = _heads(q), _heads(k), _heads(v)
+    Bk, Tk, Hkv, Dk = k.shape
+    if Bk != B or Dk != D or Hq < 1 or Hkv < 1 or D < 1:
+        raise ValueError(f"{name}: q {tuple(q.shape)} and k {tuple(k.shape)} do not fit")
+    if k.dtype is not q.dtype or v.dtype is not q.dtype:
+        raise ValueError(f"{name}: q, k and v are {q.dtype}, {k.dtype} and {v.dtype}")
+    code = _float_code(name, "q", q.dtype)
+    mask_ptr, mask_stride = 0, 0
     if key_mask is not None:
-        _need(key_mask.dtype in (torch.bool, torch.uint8) and key_mask.shape == (B, Tk), name,
-              f"key_mask must be bool ({B}, {Tk}), got {key_mask.dtype} {tuple(key_mask.shape)}")
+        if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.shape != (B, Tk):
+            raise ValueError(f"{name}: key_mask must be bool ({B}, {Tk}), got {key_mask.dtype} {tuple(key_mask.shape)}")
         if Tk > 1 and key_mask.stride(1) != 1:
             key_mask = key_mask.contiguous()
-        d.key_mask, d.mask_stride = key_mask.data_ptr(), key_mask.stride(0)
-    d.q, d.k, d.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    d.q_stride, d.k_stride, d.v_stride = _strides(q), _strides(k), _strides(v)
-    d.B, d.Tq, d.Tk, d.Hq, d.Hkv, d.D, d.causal = B, Tq, Tk, Hq, Hkv, D, int(bool(causal))
-    d.scale = scale if scale is not None else 1.0 / math.sqrt(D)
-    return d, dev, (q, k, v, key_mask)
-
-
-def _attn_workspace(name, d, grad, dev):
-    size = int(L.lib.mic_attn_seq_workspace_bytes(C.byref(d), grad))
-    if size < 0:
-        L.check(size, name)
-    if size == 0:
-        return None
-    ws = torch.empty(size, dtype=torch.uint8, device=dev)
-    d.workspace, d.workspace_bytes = ws.data_ptr(), size
-    return ws
+        mask_ptr, mask_stride = key_mask.data_ptr(), key_mask.stride(0)
+    return dev, code, (B, Tq, Tk, Hq, Hkv, D), key_mask, mask_ptr, mask_stride
 
 
 def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool = False, key_mask: Optional[torch.Tensor] = None,
@@ -205,13 +229,22 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, caus
     be seen; what k and v hold elsewhere is never used.  A query that sees nothing gets zeros.  scale defaults to D ** -0.5.
     o (B, Tq, Hq, D) in q's dtype, lse (B, Hq, Tq) fp32.  D at most 256 and a multiple of 8 (bf16) or 4 (fp32)."""
     name = "attention_forward"
-    d, dev, keep = _attn_desc(name, q, k, v, causal, key_mask, scale)
-    o = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    lse = torch.empty(q.shape[0], q.shape[2], q.shape[1], dtype=torch.float32, device=dev)
-    d.o, d.o_stride, d.lse = o.data_ptr(), _strides(o), lse.data_ptr()
-    with torch.cuda.device(dev):
-        ws = _attn_workspace(name, d, 0, dev)  # noqa: F841  (alive until the launch is enqueued)
-        L.check(L.lib.mic_attn_seq(C.byref(d), _stream(dev)), "mic_attn_seq")
+    dev, code, (B, Tq, Tk, Hq, Hkv, D), key_mask, mask_ptr, mask_stride = _attn_check(name, q, k, v, key_mask)
+    q, *qs = _heads(q)
+    k, *ks = _heads(k)
+    v, *vs = _heads(v)
+    o = torch.empty((B, Tq, Hq, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, Hq, Tq), dtype=torch.float32, device=q.device)
+    scale = 1.0 / math.sqrt(D) if scale is None else scale
+
+    d = L.AttnSeqDesc.from_buffer_copy(_ATTN_PACK.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), mask_ptr, 0, 0, 0, 0, *qs, *ks, *vs, Tq * Hq * D, Hq * D, D, 0, 0, 0,
+        mask_stride, code, B, Tq, Tk, Hq, Hkv, D, 1 if causal else 0, scale, 0, 0))
+    size = L.lib.mic_attn_seq_workspace_bytes(d, 0)
+    ws, ws_ptr = _workspace(name, size, q)
+    if size:
+        d.workspace, d.workspace_bytes = ws_ptr, size
+    _run("mic_attn_seq", L.lib.mic_attn_seq, dev, d)
     return o, lse
 
 
@@ -220,19 +253,30 @@ def attention_grad(grad: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torc
     """Gradients ``(dq, dk, dv)`` of ``attention_forward`` for the gradient of o, from its inputs and both results.  The probabilities
     are recomputed; gradients of shared key heads are summed over their query heads in a fixed order."""
     name = "attention_grad"
-    d, dev, keep = _attn_desc(name, q, k, v, causal, key_mask, scale)
+    dev, code, (B, Tq, Tk, Hq, Hkv, D), key_mask, mask_ptr, mask_stride = _attn_check(name, q, k, v, key_mask)
     _device(name, q, grad, o, lse)
-    _need(grad.shape == q.shape and o.shape == q.shape and grad.dtype == q.dtype and o.dtype == q.dtype, name,
-          f"grad {tuple(grad.shape)} {grad.dtype} and o {tuple(o.shape)} {o.dtype} do not fit q {tuple(q.shape)} {q.dtype}")
-    _need(lse.shape == (q.shape[0], q.shape[2], q.shape[1]) and lse.dtype == torch.float32, name, f"lse {tuple(lse.shape)} {lse.dtype} does not fit q")
-    o, grad, lse = _heads(o), _heads(grad), lse.contiguous()
-    dq, dk, dv = (torch.empty(t.shape, dtype=q.dtype, device=dev) for t in (q, k, v))
-    d.o, d.o_stride, d.lse = o.data_ptr(), _strides(o), lse.data_ptr()
-    d.grad_o, d.g_stride = grad.data_ptr(), _strides(grad)
-    d.dq, d.dk, d.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-    with torch.cuda.device(dev):
-        ws = _attn_workspace(name, d, 1, dev)  # noqa: F841
-        L.check(L.lib.mic_attn_seq_grad(C.byref(d), _stream(dev)), "mic_attn_seq_grad")
+    if grad.shape != q.shape or o.shape != q.shape or grad.dtype is not q.dtype or o.dtype is not q.dtype:
+        raise ValueError(f"{name}: grad {tuple(grad.shape)} {grad.dtype} and o {tuple(o.shape)} {o.dtype} do not fit q {tuple(q.shape)} {q.dtype}")
+    if lse.shape != (B, Hq, Tq) or lse.dtype is not torch.float32:
+        raise ValueError(f"{name}: lse {tuple(lse.shape)} {lse.dtype} does not fit q {tuple(q.shape)}")
+    q, *qs = _heads(q)
+    k, *ks = _heads(k)
+    v, *vs = _heads(v)
+    o, *os = _heads(o)
+    grad, *gs = _heads(grad)
+    lse = lse.contiguous()
+    dq = torch.empty((B, Tq, Hq, D), dtype=q.dtype, device=q.device)
+    dk = torch.empty((B, Tk, Hkv, D), dtype=q.dtype, device=q.device)
+    dv = torch.empty((B, Tk, Hkv, D), dtype=q.dtype, device=q.device)
+    scale = 1.0 / math.sqrt(D) if scale is None else scale
+    d = L.AttnSeqDesc.from_buffer_copy(_ATTN_PACK.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), mask_ptr, grad.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+        *qs, *ks, *vs, *os, *gs, mask_stride, code, B, Tq, Tk, Hq, Hkv, D, 1 if causal else 0, scale, 0, 0))
+    size = L.lib.mic_attn_seq_workspace_bytes(d, 1)
+    ws, ws_ptr = _workspace(name, size, q)
+    if size:
+        d.workspace, d.workspace_bytes = ws_ptr, size
+    _run("mic_attn_seq_grad", L.lib.mic_attn_seq_grad, dev, d)
     return dq, dk, dv
 
 
@@ -258,40 +302,39 @@ def attention(q, k, v, *, causal: bool = False, key_mask=None, scale: Optional[f
 
 
 # ---- vocabulary loss ----------------------------------------------------------------------------------------------------
-def _vocab_desc(name, x, w, targets, bias, ignore):
+_VOCAB_PACK = struct.Struct("@10P2q6i4iPq")  # mic_vocab_loss_desc
+
+
+def _vocab_check(name, x, w, targets, bias, ignore):
     dev = _device(name, x, w, targets, bias)
-    _need(x.dim() == 2 and w.dim() == 2 and x.shape[1] == w.shape[1] and x.shape[1] > 0 and w.shape[0] > 0, name,
-          f"x {tuple(x.shape)} and w {tuple(w.shape)} do not fit")
-    _need(x.dtype == w.dtype, name, f"x is {x.dtype}, w {w.dtype}")
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1] or w.numel() == 0:
+        raise ValueError(f"{name}: x {tuple(x.shape)} and w {tuple(w.shape)} do not fit")
+    if x.dtype is not w.dtype:
+        raise ValueError(f"{name}: x is {x.dtype}, w {w.dtype}")
     N, H = x.shape
     V = w.shape[0]
-    _need(targets.shape == (N,), name, f"targets {tuple(targets.shape)} do not fit {N} rows")
-    d = L.VocabLossDesc()
-    d.dtype = _float_code(name, "x", x.dtype)
-    x = x if x.stride(1) == 1 and (N <= 1 or x.stride(0) >= H) else x.contiguous()
-    w = w if w.stride(1) == 1 and (V <= 1 or w.stride(0) >= H) else w.contiguous()
-    targets = _ids(name, "targets", targets)
+    if targets.shape != (N,):
+        raise ValueError(f"{name}: targets {tuple(targets.shape)} do not fit {N} rows")
+    code = _float_code(name, "x", x.dtype)
     if bias is not None:
-        _need(bias.shape == (V,) and bias.dtype == torch.float32, name, f"bias must be float32 ({V},), got {bias.dtype} {tuple(bias.shape)}")
+        if bias.shape != (V,) or bias.dtype is not torch.float32:
+            raise ValueError(f"{name}: bias must be float32 ({V},), got {bias.dtype} {tuple(bias.shape)}")
         bias = bias.contiguous()
-    ignore = tuple(int(i) for i in ignore)
-    _need(len(ignore) <= 4, name, f"{len(ignore)} ignored words (at most 4)")
-    d.x, d.w, d.bias, d.targets = x.data_ptr(), w.data_ptr(), L.ptr(bias), targets.data_ptr()
-    d.ld_x, d.ld_w = (x.stride(0) if N > 1 else H), (w.stride(0) if V > 1 else H)
-    d.N, d.H, d.V, d.target_bits, d.n_ignore = N, H, V, 64 if targets.dtype == torch.int64 else 32, len(ignore)
-    for i, v in enumerate(ignore):
-        _need(-(1 << 31) <= v < (1 << 31), name, f"ignored word {v}")
-        d.ignore[i] = v
-    return d, dev, (x, w, targets, bias)
+    ignore = tuple(ignore)
+    if len(ignore) > 4 or any(not -(1 << 31) <= i < (1 << 31) for i in ignore):
+        raise ValueError(f"{name}: at most four ignored words of 32 bits, got {ignore}")
+    return dev, code, N, H, V, _rows(x), _rows(w), _ids(name, "targets", targets), bias, ignore
 
 
-def _vocab_workspace(name, d, grad, dev):
-    size = int(L.lib.mic_vocab_loss_workspace_bytes(C.byref(d), grad))
-    if size < 0:
-        L.check(size, name)
-    ws = torch.empty(size, dtype=torch.uint8, device=dev)
-    d.workspace, d.workspace_bytes = ws.data_ptr(), size
-    return ws
+def _vocab_call(what, fn, grad, dev, code, N, H, V, x, w, targets, bias, ignore, loss, lse, grad_rows, dx, dw, db):
+    d = L.VocabLossDesc.from_buffer_copy(_VOCAB_PACK.pack(
+        x.data_ptr(), w.data_ptr(), _ptr(bias), targets.data_ptr(), _ptr(loss), lse.data_ptr(), _ptr(grad_rows), _ptr(dx), _ptr(dw), _ptr(db),
+        max(x.stride(0), H), max(w.stride(0), H), code, N, H, V, _bits(targets), len(ignore), *ignore, *(0,) * (4 - len(ignore)), 0, 0))
+    size = L.lib.mic_vocab_loss_workspace_bytes(d, grad)
+    ws, ws_ptr = _workspace(what, size, x)
+    if size:
+        d.workspace, d.workspace_bytes = ws_ptr, size
+    _run(what, fn, dev, d)
 
 
 def vocab_loss_forward(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, *, bias: Optional[torch.Tensor] = None, ignore=()):
@@ -300,14 +343,10 @@ def vocab_loss_forward(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, 
 
     targets (N,) int32 / int64; rows whose target is in ``ignore`` (at most four words, e.g. padding) or outside the vocabulary
     have loss 0.  bias (V,) fp32."""
-    name = "vocab_loss_forward"
-    d, dev, keep = _vocab_desc(name, x, w, targets, bias, ignore)
-    loss = torch.empty(x.shape[0], dtype=torch.float32, device=dev)
-    lse = torch.empty_like(loss)
-    d.loss, d.lse = loss.data_ptr(), lse.data_ptr()
-    with torch.cuda.device(dev):
-        ws = _vocab_workspace(name, d, 0, dev)  # noqa: F841  (alive until the launches are enqueued)
-        L.check(L.lib.mic_vocab_loss(C.byref(d), _stream(dev)), "mic_vocab_loss")
+    dev, code, N, H, V, x, w, targets, bias, ignore = _vocab_check("vocab_loss_forward", x, w, targets, bias, ignore)
+    loss = torch.empty(N, dtype=torch.float32, device=x.device)
+    lse = torch.empty(N, dtype=torch.float32, device=x.device)
+    _vocab_call("mic_vocab_loss", L.lib.mic_vocab_loss, 0, dev, code, N, H, V, x, w, targets, bias, ignore, loss, lse, None, None, None, None)
     return loss, lse
 
 
@@ -316,20 +355,17 @@ def vocab_loss_grad(grad: torch.Tensor, x: torch.Tensor, w: torch.Tensor, target
     """Gradients ``(dx, dw, dbias or None)`` of ``vocab_loss_forward`` for the gradient ``grad`` (N,) fp32 of its losses (a scalar tensor is
     taken for every row), from its inputs and lse.  Rows that do not count get zeros."""
     name = "vocab_loss_grad"
-    d, dev, keep = _vocab_desc(name, x, w, targets, bias, ignore)
+    dev, code, N, H, V, x, w, targets, bias, ignore = _vocab_check(name, x, w, targets, bias, ignore)
     _device(name, x, grad, lse)
-    N = x.shape[0]
-    _need(grad.dtype == torch.float32 and grad.shape in ((N,), ()), name, f"grad must be float32 ({N},), got {grad.dtype} {tuple(grad.shape)}")
-    _need(lse.dtype == torch.float32 and lse.shape == (N,), name, f"lse must be float32 ({N},), got {lse.dtype} {tuple(lse.shape)}")
+    if grad.dtype is not torch.float32 or (grad.shape != (N,) and grad.dim() != 0):
+        raise ValueError(f"{name}: grad must be float32 ({N},), got {grad.dtype} {tuple(grad.shape)}")
+    if lse.dtype is not torch.float32 or lse.shape != (N,):
+        raise ValueError(f"{name}: lse must be float32 ({N},), got {lse.dtype} {tuple(lse.shape)}")
     grad, lse = grad.expand(N).contiguous(), lse.contiguous()
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    dw = torch.empty(w.shape, dtype=w.dtype, device=dev)
-    db = None if bias is None else torch.empty(w.shape[0], dtype=torch.float32, device=dev)
-    d.grad_rows, d.lse = grad.data_ptr(), lse.data_ptr()
-    d.dx, d.dw, d.db = dx.data_ptr(), dw.data_ptr(), L.ptr(db)
-    with torch.cuda.device(dev):
-        ws = _vocab_workspace(name, d, 1, dev)  # noqa: F841
-        L.check(L.lib.mic_vocab_loss_grad(C.byref(d), _stream(dev)), "mic_vocab_loss_grad")
+    dx = torch.empty((N, H), dtype=x.dtype, device=x.device)
+    dw = torch.empty((V, H), dtype=x.dtype, device=x.device)
+    db = None if bias is None else torch.empty(V, dtype=torch.float32, device=x.device)
+    _vocab_call("mic_vocab_loss_grad", L.lib.mic_vocab_loss_grad, 1, dev, code, N, H, V, x, w, targets, bias, ignore, None, lse, grad, dx, dw, db)
     return dx, dw, db
 
 

@@ -179,3 +179,33 @@ def test_workspace_sizes_of_empty_calls(L):
     for kw in (dict(B=0), dict(Tq=0), dict(Tk=0), dict(Tq=0, Tk=0)):
         for grad in (0, 1):
             assert L.lib.mic_attn_seq_workspace_bytes(C.byref(attn_desc(L, **kw)), grad) >= 0
+
+
+def test_packed_descriptors_match_the_header(L, F):
+    """The Python layer packs the descriptors in one go: every field has to land where the header has it."""
+    import ctypes as C
+    import os
+    import subprocess
+    import tempfile
+    n = len(L.AttnSeqDesc._fields_)
+    assert F._ATTN_PACK.size == C.sizeof(L.AttnSeqDesc) and F._VOCAB_PACK.size == C.sizeof(L.VocabLossDesc) and n == 27
+    d = L.AttnSeqDesc.from_buffer_copy(F._ATTN_PACK.pack(*range(1, 35), 0.5, 35, 36))
+    assert [getattr(d, f) for f in ("q", "k", "v", "o", "lse", "key_mask", "grad_o", "dq", "dk", "dv")] == list(range(1, 11))
+    assert [x for f in ("q_stride", "k_stride", "v_stride", "o_stride", "g_stride") for x in getattr(d, f)] == list(range(11, 26))
+    assert [getattr(d, f) for f in ("mask_stride", "dtype", "B", "Tq", "Tk", "Hq", "Hkv", "D", "causal", "scale", "workspace", "workspace_bytes")] == \
+        [26, 27, 28, 29, 30, 31, 32, 33, 34, 0.5, 35, 36]
+    d = L.VocabLossDesc.from_buffer_copy(F._VOCAB_PACK.pack(*range(1, 25)))
+    assert [getattr(d, f) for f, _ in L.VocabLossDesc._fields_ if f != "ignore"] == [*range(1, 19), 23, 24] and list(d.ignore) == [19, 20, 21, 22]
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    src = """#include <stdio.h>
+#include <stddef.h>
+#include "mic_hip.h"
+int main(void) { printf("%zu %zu %zu %zu %zu %zu\\n", sizeof(mic_attn_seq_desc), offsetof(mic_attn_seq_desc, mask_stride), offsetof(mic_attn_seq_desc, workspace),
+  sizeof(mic_vocab_loss_desc), offsetof(mic_vocab_loss_desc, n_ignore), offsetof(mic_vocab_loss_desc, workspace)); return 0; }"""
+    with tempfile.TemporaryDirectory() as tmp:
+        c, exe = os.path.join(tmp, "t.c"), os.path.join(tmp, "t")
+        open(c, "w").write(src)
+        subprocess.run(["gcc", "-I", os.path.join(root, "include"), c, "-o", exe], check=True)
+        got = [int(x) for x in subprocess.run([exe], capture_output=True, text=True, check=True).stdout.split()]
+    assert got == [C.sizeof(L.AttnSeqDesc), L.AttnSeqDesc.mask_stride.offset, L.AttnSeqDesc.workspace.offset,
+                   C.sizeof(L.VocabLossDesc), L.VocabLossDesc.n_ignore.offset, L.VocabLossDesc.workspace.offset]
