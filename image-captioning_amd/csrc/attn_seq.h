@@ -190,3 +190,7 @@ template <typename T, int DP> struct KeyTile {
 int mic_attn_seq_fwd_launch(const AttnSeqArgs& a, int dtype, hipStream_t s);
 int mic_attn_seq_dq_launch(const AttnSeqArgs& a, int dtype, hipStream_t s);
 int mic_attn_seq_dkv_launch(const AttnSeqArgs& a, int dtype, hipStream_t s);
+int mic_attn_seq_dkv_join(const AttnSeqArgs& a, int dtype, hipStream_t s);  // adds the partial dK and dV of `splits` row ranges
+// up to 64 keys
+int mic_attn_seq_short_fwd_launch(const AttnSeqArgs& a, int dtype, hipStream_t s);
+int mic_attn_seq_short_grad_launch(const AttnSeqArgs& a, int dtype, hipStream_t s);

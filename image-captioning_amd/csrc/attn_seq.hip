@@ -53,6 +53,12 @@ AttnSeqArgs args_of(const mic_attn_seq_desc* d) {
     return a;
 }
 
+constexpr int SHORT_KEYS = 64;
+// One tile of keys: the kernels of attn_seq_short.hip.  Their forward reads the keys again for every 32 rows, the general one for every
+// 128, which wins from 128 rows on where there are rows enough to fill the GPU.
+bool short_grad(const AttnSeqArgs& a) { return a.Tk > 0 && a.Tk <= SHORT_KEYS; }
+bool short_fwd(const AttnSeqArgs& a) { return short_grad(a) && (a.R <= 128 || (long long)a.B * a.Hkv * a.R < 256 * 128); }
+
 // The forward shares the keys of a row tile out over workgroups when there are fewer row tiles than compute units: one tile of keys
 // per workgroup at least, 512 workgroups at most.
 void split_keys(AttnSeqArgs& a, int dtype) {
@@ -61,21 +67,21 @@ void split_keys(AttnSeqArgs& a, int dtype) {
     const int tiles = (a.Tk + BK - 1) / BK;
     a.splits = 1;
     a.tiles_per_split = tiles;
-    if (base == 0 || base >= 256 || tiles < 4) return;
+    if (short_fwd(a) || base == 0 || base >= 256 || tiles < 4) return;
     const int want = (int)((512 + base - 1) / base);
     const int s = want < tiles ? want : tiles;
     a.tiles_per_split = (tiles + s - 1) / s;
     a.splits = (tiles + a.tiles_per_split - 1) / a.tiles_per_split;
 }
-// The key gradients share the rows out in the same way, at least four tiles of 32 rows to a workgroup.
+// The key gradients share the rows out in the same way, at least four tiles of 32 rows to a workgroup (one with a single tile of keys).
 void split_rows(AttnSeqArgs& a) {
     const long long base = (long long)((a.Tk + ATTN_SEQ_BLOCK - 1) / ATTN_SEQ_BLOCK) * a.Hkv * a.B;
-    const int tiles = (a.R + 31) / 32;
+    const int tiles = (a.R + 31) / 32, least = short_grad(a) ? 1 : 4;
     a.splits = 1;
     a.tiles_per_split = tiles;
-    if (base == 0 || base >= 512 || tiles < 8) return;
+    if (base == 0 || base >= 512) return;
     const int want = (int)((512 + base - 1) / base);
-    const int s = want < tiles / 4 ? want : tiles / 4;
+    const int s = want < tiles / least ? want : tiles / least;
     if (s < 2) return;
     a.tiles_per_split = (tiles + s - 1) / s;
     a.splits = (tiles + a.tiles_per_split - 1) / a.tiles_per_split;
@@ -119,6 +125,7 @@ extern "C" int mic_attn_seq(const mic_attn_seq_desc* d, void* stream) {
         a.part = (float*)d->workspace;
         a.part_ml = (float*)((char*)d->workspace + up256(fwd_rows(a) * a.D * 4));
     }
+    if (short_fwd(a)) return mic_attn_seq_short_fwd_launch(a, d->dtype, (hipStream_t)stream);
     return mic_attn_seq_fwd_launch(a, d->dtype, (hipStream_t)stream);
 }
 
@@ -141,6 +148,7 @@ extern "C" int mic_attn_seq_grad(const mic_attn_seq_desc* d, void* stream) {
                   (long long)d->workspace_bytes, need);
     a.delta = (float*)d->workspace;
     a.part = (float*)((char*)d->workspace + delta_bytes(a));
+    if (!no_rows && short_grad(a)) return mic_attn_seq_short_grad_launch(a, d->dtype, (hipStream_t)stream);
     if (!no_rows) MIC_TRY(mic_attn_seq_dq_launch(a, d->dtype, (hipStream_t)stream));
     if (!no_keys) MIC_TRY(mic_attn_seq_dkv_launch(a, d->dtype, (hipStream_t)stream));
     return 0;

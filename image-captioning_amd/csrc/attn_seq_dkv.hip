@@ -129,12 +129,17 @@ template <typename T> __global__ __launch_bounds__(256) void attn_seq_dkv_join_k
     store4<T>(i < all ? (T*)a.dk + i : (T*)a.dv + (i - all), x[0], x[1], x[2], x[3]);
 }
 
+template <typename T> int join(const AttnSeqArgs& a, hipStream_t s) {
+    const long long quads = (long long)a.B * a.Tk * a.Hkv * a.D / 2;
+    MIC_LAUNCH((attn_seq_dkv_join_kernel<T>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s, a);
+    return 0;
+}
+
 template <typename T, int DP> int launch(const AttnSeqArgs& a, hipStream_t s) {
     const long long blocks = (long long)((a.Tk + ATTN_SEQ_BLOCK - 1) / ATTN_SEQ_BLOCK) * a.Hkv * a.B;
     if (a.splits > 1) {
         MIC_LAUNCH((attn_seq_dkv_kernel<T, DP, true>), dim3((unsigned)(blocks * a.splits)), dim3(256), 0, s, a);
-        const long long quads = (long long)a.B * a.Tk * a.Hkv * a.D / 2;
-        MIC_LAUNCH((attn_seq_dkv_join_kernel<T>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s, a);
+        return join<T>(a, s);
     } else {
         MIC_LAUNCH((attn_seq_dkv_kernel<T, DP, false>), dim3((unsigned)blocks), dim3(256), 0, s, a);
     }
@@ -149,3 +154,4 @@ template <typename T> int launch_d(const AttnSeqArgs& a, hipStream_t s) {
 int mic_attn_seq_dkv_launch(const AttnSeqArgs& a, int dtype, hipStream_t s) {
     return dtype == MIC_BF16 ? launch_d<bf16_t>(a, s) : launch_d<float>(a, s);
 }
+int mic_attn_seq_dkv_join(const AttnSeqArgs& a, int dtype, hipStream_t s) { return dtype == MIC_BF16 ? join<bf16_t>(a, s) : join<float>(a, s); }
