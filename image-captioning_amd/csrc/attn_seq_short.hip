@@ -110,8 +110,16 @@ template <typename T, int DP, int KT> __global__ __launch_bounds__(256) void att
 }
 
 // ---- gradient: a workgroup per key head (and range of rows) --------------------------------------------------------------------
-template <typename T, int DP, int KT, bool SPLIT> __global__ __launch_bounds__(256) void attn_seq_short_grad_kernel(AttnSeqArgs a) {
-    constexpr int NC = DP / 16, ND = DP / 32, HALVES = 2 / KT, NU = NC / HALVES, NDW = (ND + 3) / 4, KP = KT * 32;
+// ROWS: 0 = all row tiles, 1 = there is one row tile (its dK and dV are written column tile by column tile and need no registers
+// of their own), 2 = a range of row tiles, partial sums.  Two workgroups to a compute unit (256 registers a lane) where LDS and
+// registers allow it: one loads while the other computes.
+template <typename T, int DP, int KT, int ROWS> struct GradOccupancy {
+    static constexpr int value = (KT * 32 + 64) * DP * sizeof(T) <= 65536 && (ROWS == 1 || KT == 1) ? 2 : 1;
+};
+template <typename T, int DP, int KT, int ROWS>
+__global__ __launch_bounds__(256, (GradOccupancy<T, DP, KT, ROWS>::value)) void attn_seq_short_grad_kernel(AttnSeqArgs a) {
+    constexpr int NC = DP / 16, ND = DP / 32, HALVES = 2 / KT, NU = NC / HALVES, NDW = (ND + 3) / 4, KP = KT * 32, NDA = ROWS == 1 ? 1 : NDW;
+    constexpr bool SPLIT = ROWS == 2;
     __shared__ __attribute__((aligned(16))) T sk[KP * DP];
     __shared__ __attribute__((aligned(16))) T sq[32 * DP];
     __shared__ __attribute__((aligned(16))) T sg[32 * DP];
@@ -132,9 +140,27 @@ template <typename T, int DP, int KT, bool SPLIT> __global__ __launch_bounds__(2
     unsigned bits[KT];
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) bits[kt] = key_bits(a, b, kt * 32, lane) >> (4 * h);
-    f32x16_t dk[NDW][KT], dv[NDW][KT];
+    auto store = [&](int d, int kt, const f32x16_t& x, const f32x16_t& y) {
+        const int key = kt * 32 + (lane & 31);
+        if (key >= a.Tk) return;
+        const long long at = (((long long)b * a.Tk + key) * a.Hkv + hk) * a.D, all = (long long)a.B * a.Tk * a.Hkv * a.D;
 #pragma unroll
-    for (int n = 0; n < NDW; ++n)
+        for (int e = 0; e < 4; ++e) {
+            const int col = d * 32 + 8 * e + 4 * h;
+            if (col >= a.D) continue;
+            if (SPLIT) {
+                float* p = a.part + 2 * split * all + at + col;
+                store4<float>(p, x[4 * e] * a.scale, x[4 * e + 1] * a.scale, x[4 * e + 2] * a.scale, x[4 * e + 3] * a.scale);
+                store4<float>(p + all, y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
+            } else {
+                store4<T>((T*)a.dk + at + col, x[4 * e] * a.scale, x[4 * e + 1] * a.scale, x[4 * e + 2] * a.scale, x[4 * e + 3] * a.scale);
+                store4<T>((T*)a.dv + at + col, y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
+            }
+        }
+    };
+    f32x16_t dk[NDA][KT], dv[NDA][KT];
+#pragma unroll
+    for (int n = 0; n < NDA; ++n)
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) dk[n][kt] = dv[n][kt] = f32x16_t{};
     int t0 = 0, t1 = (a.R + 31) / 32;
@@ -152,9 +178,11 @@ template <typename T, int DP, int KT, bool SPLIT> __global__ __launch_bounds__(2
         const int r = t * 32 + (lane & 31);
         const bool row_ok = r < a.R;
         const int qi = row_ok ? r / a.group : 0, qh = hk * a.group + (row_ok ? r - qi * a.group : 0);
-        Frag8<T> uf[NU];
+        constexpr bool UREG = NU * sizeof(T) <= 32;  // else (fp32, 256 columns) the wave's operands are loaded as they are used
+        Frag8<T> uf[UREG ? NU : 1];
+        if constexpr (UREG)
 #pragma unroll
-        for (int u = 0; u < NU; ++u) uf[u] = load_frag<T>(urow, 16 * (c0 + u) + 8 * h, a.D);
+            for (int u = 0; u < NU; ++u) uf[u] = load_frag<T>(urow, 16 * (c0 + u) + 8 * h, a.D);
         float lse2 = INFINITY;
         if (row_ok) {
             const float x = a.lse[((long long)b * a.Hq + qh) * a.Tq + qi];
@@ -167,8 +195,13 @@ template <typename T, int DP, int KT, bool SPLIT> __global__ __launch_bounds__(2
         {
             f32x16_t x = f32x16_t{};
             const T* rows = utype ? sg : sq;
+            if constexpr (UREG) {
 #pragma unroll
-            for (int u = 0; u < NU; ++u) mma32(uf[u], read_row<DP>(rows, lane & 31, c0 + u, h), x);
+                for (int u = 0; u < NU; ++u) mma32(uf[u], read_row<DP>(rows, lane & 31, c0 + u, h), x);
+            } else {
+#pragma unroll 4
+                for (int u = 0; u < NU; ++u) mma32(load_frag<T>(urow, 16 * (c0 + u) + 8 * h, a.D), read_row<DP>(rows, lane & 31, c0 + u, h), x);
+            }
             give(ex, wave, lane, x);
         }
         __syncthreads();
@@ -228,41 +261,31 @@ template <typename T, int DP, int KT, bool SPLIT> __global__ __launch_bounds__(2
                     const int col = d * 32 + 8 * e + 4 * h;
                     if (col < a.D) store4<T>(dq + col, acc[4 * e] * a.scale, acc[4 * e + 1] * a.scale, acc[4 * e + 2] * a.scale, acc[4 * e + 3] * a.scale);
                 }
+            const int at = ROWS == 1 ? 0 : n;
+            if (ROWS == 1)
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) dk[0][kt] = dv[0][kt] = f32x16_t{};
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const Frag8<T> g = read_col<DP>(sg, d * 32, 16 * j, lane), q = read_col<DP>(sq, d * 32, 16 * j, lane);
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt) {
-                    mma32(g, read_col<KP>(sp, kt * 32, 16 * j, lane), dv[n][kt]);
-                    mma32(q, read_col<KP>(sd, kt * 32, 16 * j, lane), dk[n][kt]);
+                    mma32(g, read_col<KP>(sp, kt * 32, 16 * j, lane), dv[at][kt]);
+                    mma32(q, read_col<KP>(sd, kt * 32, 16 * j, lane), dk[at][kt]);
                 }
             }
+            if (ROWS == 1)
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) store(d, kt, dk[0][kt], dv[0][kt]);
         }
     }
+    if (ROWS == 1) return;
 #pragma unroll
     for (int n = 0; n < NDW; ++n) {
         const int d = n * 4 + wave;
         if (d >= ND) break;
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-            const int key = kt * 32 + (lane & 31);
-            if (key >= a.Tk) continue;
-            const long long at = (((long long)b * a.Tk + key) * a.Hkv + hk) * a.D, all = (long long)a.B * a.Tk * a.Hkv * a.D;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int col = d * 32 + 8 * e + 4 * h;
-                if (col >= a.D) continue;
-                const f32x16_t &x = dk[n][kt], &y = dv[n][kt];
-                if (SPLIT) {
-                    float* p = a.part + 2 * split * all + at + col;
-                    store4<float>(p, x[4 * e] * a.scale, x[4 * e + 1] * a.scale, x[4 * e + 2] * a.scale, x[4 * e + 3] * a.scale);
-                    store4<float>(p + all, y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
-                } else {
-                    store4<T>((T*)a.dk + at + col, x[4 * e] * a.scale, x[4 * e + 1] * a.scale, x[4 * e + 2] * a.scale, x[4 * e + 3] * a.scale);
-                    store4<T>((T*)a.dv + at + col, y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
-                }
-            }
-        }
+        for (int kt = 0; kt < KT; ++kt) store(d, kt, dk[n % NDA][kt], dv[n % NDA][kt]);
     }
 }
 
@@ -273,10 +296,11 @@ template <typename T, int DP, int KT> int launch_fwd(const AttnSeqArgs& a, hipSt
 template <typename T, int DP, int KT> int launch_grad(const AttnSeqArgs& a, hipStream_t s) {
     const long long blocks = (long long)a.Hkv * a.B;
     if (a.splits > 1) {
-        MIC_LAUNCH((attn_seq_short_grad_kernel<T, DP, KT, true>), dim3((unsigned)(blocks * a.splits)), dim3(256), 0, s, a);
+        MIC_LAUNCH((attn_seq_short_grad_kernel<T, DP, KT, 2>), dim3((unsigned)(blocks * a.splits)), dim3(256), 0, s, a);
         return mic_attn_seq_dkv_join(a, sizeof(T) == 2 ? MIC_BF16 : MIC_F32, s);
     }
-    MIC_LAUNCH((attn_seq_short_grad_kernel<T, DP, KT, false>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+    if (a.R <= 32) MIC_LAUNCH((attn_seq_short_grad_kernel<T, DP, KT, 1>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+    else MIC_LAUNCH((attn_seq_short_grad_kernel<T, DP, KT, 0>), dim3((unsigned)blocks), dim3(256), 0, s, a);
     return 0;
 }
 

@@ -11,6 +11,7 @@ types, devices) or ``_lib.MicError`` (what the library refuses).
 """
 from __future__ import annotations
 
+import functools
 import math
 import struct
 from typing import Optional
@@ -52,10 +53,8 @@ def _float_code(name: str, what: str, dtype) -> int:
     raise ValueError(f"{name}: {what} must be float32 or bfloat16, got {dtype}")
 
 
-def _workspace(name: str, size: int, like: torch.Tensor):
+def _workspace(size: int, like: torch.Tensor):
     """`size` bytes of scratch and its address; the caller keeps the tensor until its launches are enqueued."""
-    if size < 0:
-        L.check(size, name)
     if size == 0:
         return None, 0
     ws = torch.empty(size, dtype=torch.uint8, device=like.device)
@@ -128,6 +127,11 @@ def embedding_forward(ids: torch.Tensor, table: torch.Tensor, pos: Optional[torc
     return out
 
 
+@functools.lru_cache(maxsize=256)
+def _embed_workspace_bytes(n, T, H, vocab, want_pos) -> int:
+    return L.lib.mic_embed_grad_workspace_bytes(n, T, H, vocab, want_pos)
+
+
 def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, vocab: int, *, scale: float = 1.0, positions: int = 0,
                    dtype: Optional[torch.dtype] = None):
     """Gradients of ``embedding_forward``: (d_table (vocab, H), d_pos (positions, H) or None), rounded once to ``dtype`` (grad's by
@@ -153,10 +157,10 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, vocab: int, *, scale: 
         if positions > T:
             d_pos[T:].zero_()
     T = max(T, 1)
-    size = L.lib.mic_embed_grad_workspace_bytes(n, T, H, vocab, 1 if positions else 0)
+    size = _embed_workspace_bytes(n, T, H, vocab, 1 if positions else 0)
     if size < 0:
         raise ValueError(f"{name}: sizes out of range (tokens {n}, H={H}, vocab={vocab})")
-    ws, ws_ptr = _workspace(name, size, grad)
+    ws, ws_ptr = _workspace(size, grad)
     _run("mic_embed_grad", L.lib.mic_embed_grad, dev, ids.data_ptr(), _bits(ids), grad.data_ptr(), d_table.data_ptr(), L.ptr(d_pos), code, out_code,
          scale, n, T, H, vocab, ws_ptr, size)
     return d_table, d_pos
@@ -186,30 +190,46 @@ def embedding(ids, table, pos=None, *, scale: float = 1.0, dtype=None) -> torch.
 # ---- attention --------------------------------------------------------------------------------------------------------
 _ATTN_PACK = struct.Struct("@10P16q8ifPq")  # mic_attn_seq_desc
 
+@functools.lru_cache(maxsize=256)
+def _attn_workspace_bytes(code, B, Tq, Tk, Hq, Hkv, D, grad) -> int:
+    """Scratch depends on type and sizes alone."""
+    d = L.AttnSeqDesc.from_buffer_copy(_ATTN_PACK.pack(*(0,) * 26, code, B, Tq, Tk, Hq, Hkv, D, 0, 0.0, 0, 0))
+    size = L.lib.mic_attn_seq_workspace_bytes(d, grad)
+    if size < 0:
+        L.check(size, "mic_attn_seq_workspace_bytes")
+    return size
+
 
 def _heads(t: torch.Tensor):
-    """The tensor and its strides of (batch, position, head), copied if the kernels cannot read it in place (columns consecutive,
-    everything on 16-byte boundaries).  A dimension of one entry has no stride to speak of."""
+    """The tensor, its address and its strides of (batch, position, head), copied if the kernels cannot read it in place (columns
+    consecutive, everything on 16-byte boundaries).  A dimension of one entry has no stride to speak of."""
     e = 16 // t.element_size()
     B, T, H, D = t.shape
+    p = t.data_ptr()
     sb, st, sh, sd = t.stride()
-    sb, st, sh = sb if B > 1 else 0, st if T > 1 else 0, sh if H > 1 else 0
-    if (sd == 1 or D == 1) and not (sb % e or st % e or sh % e) and not t.data_ptr() % 16:
-        return t, sb, st, sh
-    return t.clone(memory_format=torch.contiguous_format), T * H * D, H * D, D
+    if B == 1:
+        sb = 0
+    if T == 1:
+        st = 0
+    if H == 1:
+        sh = 0
+    if not (sb % e or st % e or sh % e or p % 16) and (sd == 1 or D == 1):
+        return t, p, (sb, st, sh)
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.data_ptr(), (T * H * D, H * D, D)
 
 
-def _attn_check(name, q, k, v, key_mask):
-    dev = _device(name, q, k, v, key_mask)
+def _attn_check(name, dev, q, k, v, key_mask):
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
         raise ValueError(f"{name}: q, k and v must be (batch, positions, heads, columns), got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     B, Tq, Hq, D = q.shape
     Bk, Tk, Hkv, Dk = k.shape
     if Bk != B or Dk != D or Hq < 1 or Hkv < 1 or D < 1:
         raise ValueError(f"{name}: q {tuple(q.shape)} and k {tuple(k.shape)} do not fit")
-    if k.dtype is not q.dtype or v.dtype is not q.dtype:
-        raise ValueError(f"{name}: q, k and v are {q.dtype}, {k.dtype} and {v.dtype}")
-    code = _float_code(name, "q", q.dtype)
+    dtype = q.dtype
+    if k.dtype is not dtype or v.dtype is not dtype:
+        raise ValueError(f"{name}: q, k and v are {dtype}, {k.dtype} and {v.dtype}")
+    code = _float_code(name, "q", dtype)
     mask_ptr, mask_stride = 0, 0
     if key_mask is not None:
         if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.shape != (B, Tk):
@@ -217,7 +237,7 @@ def _attn_check(name, q, k, v, key_mask):
         if Tk > 1 and key_mask.stride(1) != 1:
             key_mask = key_mask.contiguous()
         mask_ptr, mask_stride = key_mask.data_ptr(), key_mask.stride(0)
-    return dev, code, (B, Tq, Tk, Hq, Hkv, D), key_mask, mask_ptr, mask_stride
+    return code, B, Tq, Tk, Hq, Hkv, D, dtype, key_mask, mask_ptr, mask_stride
 
 
 def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool = False, key_mask: Optional[torch.Tensor] = None,
@@ -229,22 +249,19 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, caus
     be seen; what k and v hold elsewhere is never used.  A query that sees nothing gets zeros.  scale defaults to D ** -0.5.
     o (B, Tq, Hq, D) in q's dtype, lse (B, Hq, Tq) fp32.  D at most 256 and a multiple of 8 (bf16) or 4 (fp32)."""
     name = "attention_forward"
-    dev, code, (B, Tq, Tk, Hq, Hkv, D), key_mask, mask_ptr, mask_stride = _attn_check(name, q, k, v, key_mask)
-    q, *qs = _heads(q)
-    k, *ks = _heads(k)
-    v, *vs = _heads(v)
-    o = torch.empty((B, Tq, Hq, D), dtype=q.dtype, device=q.device)
-    lse = torch.empty((B, Hq, Tq), dtype=torch.float32, device=q.device)
-    scale = 1.0 / math.sqrt(D) if scale is None else scale
-
-    d = L.AttnSeqDesc.from_buffer_copy(_ATTN_PACK.pack(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), mask_ptr, 0, 0, 0, 0, *qs, *ks, *vs, Tq * Hq * D, Hq * D, D, 0, 0, 0,
-        mask_stride, code, B, Tq, Tk, Hq, Hkv, D, 1 if causal else 0, scale, 0, 0))
-    size = L.lib.mic_attn_seq_workspace_bytes(d, 0)
-    ws, ws_ptr = _workspace(name, size, q)
-    if size:
-        d.workspace, d.workspace_bytes = ws_ptr, size
-    _run("mic_attn_seq", L.lib.mic_attn_seq, dev, d)
+    dev = _device(name, q, k, v, key_mask)
+    code, B, Tq, Tk, Hq, Hkv, D, dtype, key_mask, mask_ptr, mask_stride = _attn_check(name, dev, q, k, v, key_mask)
+    q, q_ptr, qs = _heads(q)
+    k, k_ptr, ks = _heads(k)
+    v, v_ptr, vs = _heads(v)
+    place = q.device
+    o = torch.empty((B, Tq, Hq, D), dtype=dtype, device=place)
+    lse = torch.empty((B, Hq, Tq), dtype=torch.float32, device=place)
+    size = _attn_workspace_bytes(code, B, Tq, Tk, Hq, Hkv, D, 0)
+    ws, ws_ptr = _workspace(size, q)
+    _run("mic_attn_seq", L.lib.mic_attn_seq, dev, L.AttnSeqDesc.from_buffer_copy(_ATTN_PACK.pack(
+        q_ptr, k_ptr, v_ptr, o.data_ptr(), lse.data_ptr(), mask_ptr, 0, 0, 0, 0, *qs, *ks, *vs, Tq * Hq * D, Hq * D, D, 0, 0, 0, mask_stride, code, B, Tq,
+        Tk, Hq, Hkv, D, 1 if causal else 0, 1.0 / math.sqrt(D) if scale is None else scale, ws_ptr, size)))
     return o, lse
 
 
@@ -253,30 +270,27 @@ def attention_grad(grad: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torc
     """Gradients ``(dq, dk, dv)`` of ``attention_forward`` for the gradient of o, from its inputs and both results.  The probabilities
     are recomputed; gradients of shared key heads are summed over their query heads in a fixed order."""
     name = "attention_grad"
-    dev, code, (B, Tq, Tk, Hq, Hkv, D), key_mask, mask_ptr, mask_stride = _attn_check(name, q, k, v, key_mask)
-    _device(name, q, grad, o, lse)
-    if grad.shape != q.shape or o.shape != q.shape or grad.dtype is not q.dtype or o.dtype is not q.dtype:
-        raise ValueError(f"{name}: grad {tuple(grad.shape)} {grad.dtype} and o {tuple(o.shape)} {o.dtype} do not fit q {tuple(q.shape)} {q.dtype}")
+    dev = _device(name, q, k, v, key_mask, grad, o, lse)
+    code, B, Tq, Tk, Hq, Hkv, D, dtype, key_mask, mask_ptr, mask_stride = _attn_check(name, dev, q, k, v, key_mask)
+    if grad.shape != q.shape or o.shape != q.shape or grad.dtype is not dtype or o.dtype is not dtype:
+        raise ValueError(f"{name}: grad {tuple(grad.shape)} {grad.dtype} and o {tuple(o.shape)} {o.dtype} do not fit q {tuple(q.shape)} {dtype}")
     if lse.shape != (B, Hq, Tq) or lse.dtype is not torch.float32:
         raise ValueError(f"{name}: lse {tuple(lse.shape)} {lse.dtype} does not fit q {tuple(q.shape)}")
-    q, *qs = _heads(q)
-    k, *ks = _heads(k)
-    v, *vs = _heads(v)
-    o, *os = _heads(o)
-    grad, *gs = _heads(grad)
+    q, q_ptr, qs = _heads(q)
+    k, k_ptr, ks = _heads(k)
+    v, v_ptr, vs = _heads(v)
+    o, o_ptr, os = _heads(o)
+    grad, g_ptr, gs = _heads(grad)
     lse = lse.contiguous()
-    dq = torch.empty((B, Tq, Hq, D), dtype=q.dtype, device=q.device)
-    dk = torch.empty((B, Tk, Hkv, D), dtype=q.dtype, device=q.device)
-    dv = torch.empty((B, Tk, Hkv, D), dtype=q.dtype, device=q.device)
-    scale = 1.0 / math.sqrt(D) if scale is None else scale
-    d = L.AttnSeqDesc.from_buffer_copy(_ATTN_PACK.pack(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), mask_ptr, grad.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-        *qs, *ks, *vs, *os, *gs, mask_stride, code, B, Tq, Tk, Hq, Hkv, D, 1 if causal else 0, scale, 0, 0))
-    size = L.lib.mic_attn_seq_workspace_bytes(d, 1)
-    ws, ws_ptr = _workspace(name, size, q)
-    if size:
-        d.workspace, d.workspace_bytes = ws_ptr, size
-    _run("mic_attn_seq_grad", L.lib.mic_attn_seq_grad, dev, d)
+    place = q.device
+    dq = torch.empty((B, Tq, Hq, D), dtype=dtype, device=place)
+    dk = torch.empty((B, Tk, Hkv, D), dtype=dtype, device=place)
+    dv = torch.empty((B, Tk, Hkv, D), dtype=dtype, device=place)
+    size = _attn_workspace_bytes(code, B, Tq, Tk, Hq, Hkv, D, 1)
+    ws, ws_ptr = _workspace(size, q)
+    _run("mic_attn_seq_grad", L.lib.mic_attn_seq_grad, dev, L.AttnSeqDesc.from_buffer_copy(_ATTN_PACK.pack(
+        q_ptr, k_ptr, v_ptr, o_ptr, lse.data_ptr(), mask_ptr, g_ptr, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *qs, *ks, *vs, *os, *gs, mask_stride,
+        code, B, Tq, Tk, Hq, Hkv, D, 1 if causal else 0, 1.0 / math.sqrt(D) if scale is None else scale, ws_ptr, size)))
     return dq, dk, dv
 
 
@@ -331,7 +345,9 @@ def _vocab_call(what, fn, grad, dev, code, N, H, V, x, w, targets, bias, ignore,
         x.data_ptr(), w.data_ptr(), _ptr(bias), targets.data_ptr(), _ptr(loss), lse.data_ptr(), _ptr(grad_rows), _ptr(dx), _ptr(dw), _ptr(db),
         max(x.stride(0), H), max(w.stride(0), H), code, N, H, V, _bits(targets), len(ignore), *ignore, *(0,) * (4 - len(ignore)), 0, 0))
     size = L.lib.mic_vocab_loss_workspace_bytes(d, grad)
-    ws, ws_ptr = _workspace(what, size, x)
+    if size < 0:
+        L.check(size, what)
+    ws, ws_ptr = _workspace(size, x)
     if size:
         d.workspace, d.workspace_bytes = ws_ptr, size
     _run(what, fn, dev, d)
