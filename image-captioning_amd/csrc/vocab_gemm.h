@@ -69,6 +69,8 @@ template <typename T, bool COL> struct OperandTile {
 
 struct GemmShape {
     Operand p, q;
+    const int* rows;  // NULL, or the number of rows to take, on the device: limits q.n (k for products over the rows)
+    int rows_are_k;
     int K, tiles_p, tiles_q, slices;
 };
 
@@ -90,6 +92,12 @@ template <typename T, bool PCOL, bool QCOL, typename Epi> __global__ __launch_bo
     id /= g.slices;
     const int tq = id % g.tiles_q, tp = id / g.tiles_q;
     const int p0 = tp * VT, q0 = tq * VT;
+    if (g.rows) {
+        const int rows = *g.rows;
+        if (g.rows_are_k) g.K = min(g.K, rows);
+        else g.q.n = min(g.q.n, rows);
+        if (q0 >= g.q.n) return;  // rows that do not count
+    }
     const int nk = (g.K + KS - 1) / KS, kb = (int)((long long)nk * slice / g.slices), ke = (int)((long long)nk * (slice + 1) / g.slices);
     f32x16_t acc[2][2];
 #pragma unroll

@@ -5,7 +5,13 @@
 // Gradient: piece by piece of the vocabulary the logits are computed again, their epilogue turns them into d (rounded to bf16 for
 // bf16 operands: both remaining products take it as a matrix-core operand; dbias is summed before the rounding), and two more
 // products use the piece.  dw's rows of a piece are complete; dx is summed over the pieces in fp32.
+// Rows that do not count (padding: half of a batch of captions) have no gradient, so the gradient's products run over the counted
+// rows alone: they are gathered first, their number stays on the device, and workgroups behind the last one end at once.
+//
+// Two kernels: 256 x 256 tiles for bf16 (vocab_gemm8.h), 128 x 128 tiles for fp32 and for products too small to fill the larger ones
+// (vocab_gemm.h).
 #include "vocab_gemm.h"
+#include "vocab_gemm8.h"
 
 namespace {
 
@@ -86,23 +92,29 @@ __global__ __launch_bounds__(256) void vocab_loss_rows_kernel(const float2* __re
 }
 
 // ---- epilogue: logits -> d --------------------------------------------------------------------------------------------------
+// What a row of the gradient needs, in the order of the gathered rows
+struct RowInfo {
+    const int* target;     // -1: the row does not count
+    const float *lse, *weight;
+};
 template <typename T> struct GradEpi {
     struct Args {
         const float* bias;
-        Targets t;
-        const float *lse, *weight;
+        RowInfo r;
         T* d;            // [N][ld], columns from v0 on
         float* part_db;  // [parts][Vc] or NULL
-        int N, V, Vc, ld, v0;
+        const int* count;  // NULL, or the rows there are
+        int N, Vc, ld, v0;
     };
-    __device__ static __forceinline__ void run(const Args& a, f32x16_t (&acc)[2][2], int p0, int q0, int lane, int, int tq, int) {
+    __device__ static __forceinline__ void run(Args a, f32x16_t (&acc)[2][2], int p0, int q0, int lane, int, int tq, int) {
+        if (a.count) a.N = min(a.N, *a.count);
         const int h = lane >> 5;
         float sum[2][16];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int row = q0 + j * 32 + (lane & 31);
-            const int t = row < a.N ? target_of(a.t, row) : -1;
-            const float w = t >= 0 ? a.weight[row] : 0.f, lse2 = t >= 0 ? a.lse[row] * ATTN_LOG2E : 0.f;
+            const int t = row < a.N ? a.r.target[row] : -1;
+            const float w = t >= 0 ? a.r.weight[row] : 0.f, lse2 = t >= 0 ? a.r.lse[row] * ATTN_LOG2E : 0.f;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -179,33 +191,256 @@ template <typename T> struct OutEpi {
     }
 };
 
-// out = the sum of `parts` fp32 matrices [rows][cols], in order
-template <typename T> __global__ __launch_bounds__(256) void vocab_sum_parts_kernel(const float* __restrict__ part, T* __restrict__ out, long long n, int parts) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (n % 4 == 0) {
-        if (i * 4 >= n) return;
-        float4 s = make_float4(0, 0, 0, 0);
-        for (int k = 0; k < parts; ++k) {
-            const float4 p = *reinterpret_cast<const float4*>(part + k * n + i * 4);
-            s.x += p.x; s.y += p.y; s.z += p.z; s.w += p.w;
-        }
-        store4<T>(out + i * 4, s.x, s.y, s.z, s.w);
-    } else {
-        for (long long e = i * 4; e < n && e < i * 4 + 4; ++e) {
+// ---- the same epilogues on the 256 x 256 tiles: a lane holds 4 consecutive p of 4 tiles for 8 rows --------------------------------
+struct StatsEpi8 {
+    typedef StatsEpi::Args Args;
+    __device__ static __forceinline__ void run(const Args& a, f32x4_t (&acc)[4][8], int p0, int q0, int lane, int wave, int tp, int, int, unsigned char*) {
+        const int pw = p0 + 64 * (wave & 3) + 4 * (lane >> 4), qw = q0 + 128 * (wave >> 2) + (lane & 15);
+        float b[4][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int v = pw + 16 * j + e;
+                b[j][e] = v < a.V ? (a.bias ? a.bias[v] : 0.f) : -INFINITY;
+            }
+        if (p0 + 64 * (wave & 3) >= a.V) return;  // its parts are not looked at
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int row = qw + 16 * i;
+            const int t = row < a.N ? target_of(a.t, row) : -1;
+            float m = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float z = acc[j][i][e] + b[j][e];
+                    if (pw + 16 * j + e == t) a.zt[row] = z;
+                    acc[j][i][e] = z;
+                    m = fmaxf(m, z);
+                }
+            m = fmaxf(m, __shfl_xor(m, 16, 64));
+            m = fmaxf(m, __shfl_xor(m, 32, 64));
+            const float m_use = m == -INFINITY ? 0.f : m;
             float s = 0.f;
-            for (int k = 0; k < parts; ++k) s += part[k * n + e];
-            out[e] = from_f32<T>(s);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f((acc[j][i][e] - m_use) * ATTN_LOG2E);
+            s += __shfl_xor(s, 16, 64);
+            s += __shfl_xor(s, 32, 64);
+            if (lane < 16 && row < a.N) a.part[(long long)row * a.parts + tp * 4 + (wave & 3)] = make_float2(m, s);
         }
+    }
+};
+
+struct GradEpi8 {
+    typedef GradEpi<bf16_t>::Args Args;
+    __device__ static __forceinline__ void run(Args a, f32x4_t (&acc)[4][8], int p0, int q0, int lane, int wave, int, int tq, int, unsigned char* smem) {
+        if (a.count) a.N = min(a.N, *a.count);
+        constexpr int LD = 256 + 8;  // staged rows of bf16
+        const int pl = 64 * (wave & 3) + 4 * (lane >> 4), ql = 128 * (wave >> 2) + (lane & 15);
+        bf16_t* st = reinterpret_cast<bf16_t*>(smem);
+        float b[4][4], sum[16];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int c = p0 + pl + 16 * j + e;
+                b[j][e] = c < a.Vc ? (a.bias ? a.bias[a.v0 + c] * ATTN_LOG2E : 0.f) : -INFINITY;  // beyond the piece: probability zero
+                sum[4 * j + e] = 0.f;
+            }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int row = q0 + ql + 16 * i;
+            const int t = row < a.N ? a.r.target[row] : -1;
+            const float w = t >= 0 ? a.r.weight[row] : 0.f, lse2 = t >= 0 ? a.r.lse[row] * ATTN_LOG2E : 0.f;
+            const int tc = t - a.v0 - p0 - pl;  // the target's column, from the lane's first
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float d[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float p = __builtin_amdgcn_exp2f(fmaf(acc[j][i][e], ATTN_LOG2E, b[j][e] - lse2));
+                    d[e] = t >= 0 ? w * (tc == 16 * j + e ? p - 1.0f : p) : 0.f;
+                    sum[4 * j + e] += d[e];
+                }
+                store4<bf16_t>(st + (ql + 16 * i) * LD + pl + 16 * j, d[0], d[1], d[2], d[3]);
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            const int x = threadIdx.x + k * 512, r = x >> 5, c = (x & 31) * 8;
+            if (q0 + r < a.N && p0 + c < a.ld) *reinterpret_cast<uint4*>(a.d + (long long)(q0 + r) * a.ld + p0 + c) = *reinterpret_cast<const uint4*>(st + r * LD + c);
+        }
+        if (a.part_db == nullptr) return;
+        // sums over 16 lanes, halving the values at every exchange: value x ends in the lane whose low four bits are x
+#pragma unroll
+        for (int d = 8; d > 0; d >>= 1) {
+            const bool up = lane & d;
+#pragma unroll
+            for (int x = 0; x < d; ++x) {
+                const float give = up ? sum[x] : sum[x + d], keep = up ? sum[x + d] : sum[x];
+                sum[x] = keep + __shfl_xor(give, d, 64);
+            }
+        }
+        const int x = lane & 15, c = p0 + pl + 16 * (x >> 2) + (x & 3);
+        if (c < a.Vc) a.part_db[(long long)(tq * 2 + (wave >> 2)) * a.Vc + c] = sum[0];
+    }
+};
+
+struct OutEpi8 {
+    typedef OutEpi<bf16_t>::Args Args;
+    __device__ static __forceinline__ void run(const Args& a, f32x4_t (&acc)[4][8], int p0, int q0, int lane, int wave, int, int, int slice, unsigned char*) {
+        const int pw = p0 + 64 * (wave & 3) + 4 * (lane >> 4), qw = q0 + 128 * (wave >> 2) + (lane & 15);
+        const bool whole = a.Np % 4 == 0 && a.ld % 4 == 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int row = qw + 16 * i;
+            if (row >= a.Nq) continue;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int c = pw + 16 * j;
+                const f32x4_t& v = acc[j][i];
+                if (a.part) {
+                    float* o = a.part + ((long long)slice * a.Nq + row) * a.Np + c;
+                    if (whole && c < a.Np) store4<float>(o, v[0], v[1], v[2], v[3]);
+                    else if (!whole)
+                        for (int e = 0; e < 4; ++e)
+                            if (c + e < a.Np) o[e] = v[e];
+                } else {
+                    bf16_t* o = a.out + (long long)row * a.ld + c;
+                    if (whole && c < a.Np) store4<bf16_t>(o, v[0], v[1], v[2], v[3]);
+                    else if (!whole)
+                        for (int e = 0; e < 4; ++e)
+                            if (c + e < a.Np) o[e] = (bf16_t)v[e];
+                }
+            }
+        }
+    }
+};
+
+// out[row] = the sum of `parts` fp32 rows at[row] (NULL: the row itself; negative: zeros), in order; parts lie `stride` elements apart
+template <typename T> __global__ __launch_bounds__(256) void vocab_sum_parts_kernel(const float* __restrict__ part, T* __restrict__ out, const int* __restrict__ at, int rows,
+                                                                                    int cols, long long stride, int parts) {
+    const int quads = (cols + 3) / 4;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    const int row = (int)(i / quads), c = (int)(i - (long long)row * quads) * 4;
+    if (row >= rows) return;
+    const int src = at ? at[row] : row;
+    float s[4] = {};
+    if (src >= 0) {
+        const float* p = part + (long long)src * cols + c;
+        if (cols % 4 == 0) {
+#pragma unroll 8
+            for (int k = 0; k < parts; ++k) {
+                const float4 x = *reinterpret_cast<const float4*>(p + k * stride);
+                s[0] += x.x; s[1] += x.y; s[2] += x.z; s[3] += x.w;
+            }
+        } else {
+            for (int e = 0; e < 4 && c + e < cols; ++e)
+                for (int k = 0; k < parts; ++k) s[e] += p[k * stride + e];
+        }
+    }
+    T* o = out + (long long)row * cols + c;
+    if (cols % 4 == 0) store4<T>(o, s[0], s[1], s[2], s[3]);
+    else
+        for (int e = 0; e < 4 && c + e < cols; ++e) o[e] = from_f32<T>(s[e]);
+}
+
+// column sums of a [parts][n] matrix: 64 columns to a workgroup, 16 waves share the rows, added in order
+__global__ __launch_bounds__(1024) void vocab_colsum_kernel(const float* __restrict__ part, float* __restrict__ out, int n, int parts, const int* __restrict__ rows, int row_tile) {
+    __shared__ float sum[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
+    if (rows) parts = min(parts, (*rows + row_tile - 1) / row_tile);  // parts of the gathered rows alone were written
+    const int lo = (int)((long long)parts * wave / 16), hi = (int)((long long)parts * (wave + 1) / 16);
+    float s = 0.f;
+#pragma unroll 8
+    for (int k = lo; k < hi; ++k) s += c < n ? part[(long long)k * n + c] : 0.f;
+    sum[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && c < n) {
+        s = sum[0][lane];
+#pragma unroll
+        for (int w = 1; w < 16; ++w) s += sum[w][lane];
+        out[c] = s;
     }
 }
 
-// rows of `cols` elements with any stride -> rows of `padded` elements, zeros behind
-template <typename T> __global__ __launch_bounds__(256) void vocab_pad_kernel(const T* __restrict__ in, long long ld, T* __restrict__ out, long long rows, int cols, int padded) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= rows * padded) return;
-    const long long r = i / padded;
-    const int c = (int)(i - r * padded);
-    out[i] = c < cols ? in[r * ld + c] : (T)0.f;
+// ---- the rows of the gradient ------------------------------------------------------------------------------------------------------
+// Every row's target, weight and lse, and with `gather` the counted rows only, in their order: `at` tells where a row went (-1: it does
+// not count), *count how many there are.  A block counts the rows before its own again (at most 64 blocks) instead of waiting for others.
+struct RowsArgs {
+    Targets t;
+    const float *weight, *lse;
+    int *target_out, *at, *count;
+    float *weight_out, *lse_out;
+    int N, per_block, gather;
+};
+__global__ __launch_bounds__(1024) void vocab_rows_kernel(RowsArgs a) {
+    __shared__ int wave_sum[16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int lo = blockIdx.x * a.per_block, hi = min(a.N, lo + a.per_block);
+    int base = 0;
+    if (a.gather) {
+        int mine = 0;
+#pragma unroll 4
+        for (int i = tid; i < lo; i += 1024) mine += target_of(a.t, i) >= 0;
+        for (int d = 32; d > 0; d >>= 1) mine += __shfl_xor(mine, d, 64);
+        if (lane == 0) wave_sum[wave] = mine;
+        __syncthreads();
+        for (int w = 0; w < 16; ++w) base += wave_sum[w];
+        __syncthreads();
+    }
+    for (int r = lo; r < hi; r += 1024) {
+        const int i = r + tid, t = i < hi ? target_of(a.t, i) : -1;
+        int to = i;
+        if (a.gather) {
+            const unsigned long long in = __ballot(t >= 0);
+            if (lane == 0) wave_sum[wave] = __popcll(in);
+            __syncthreads();
+            to = base + __popcll(in & ((1ull << lane) - 1ull));
+            int all = 0;
+            for (int w = 0; w < 16; ++w) {
+                if (w < wave) to += wave_sum[w];
+                all += wave_sum[w];
+            }
+            base += all;
+            __syncthreads();
+        }
+        if (i < hi) {
+            if (a.gather) a.at[i] = t >= 0 ? to : -1;
+            if (t >= 0 || !a.gather) {
+                a.target_out[to] = t;
+                a.weight_out[to] = t >= 0 ? a.weight[i] : 0.f;
+                a.lse_out[to] = t >= 0 ? a.lse[i] : 0.f;
+            }
+        }
+    }
+    if (a.gather && blockIdx.x == gridDim.x - 1 && tid == 0) *a.count = base;
+}
+
+// rows of `cols` elements with any stride -> rows of `padded` elements (whole 16 bytes), zeros behind; row r goes to at[r] (NULL: r;
+// negative: nowhere)
+template <typename T> __global__ __launch_bounds__(256) void vocab_pad_kernel(const T* __restrict__ in, long long ld, T* __restrict__ out, const int* __restrict__ at, long long rows,
+                                                                              int cols, int padded) {
+    constexpr int E = Vec16<T>::N;
+    const int per = padded / E;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x, r = i / per;
+    if (r >= rows) return;
+    const int c = (int)(i - r * per) * E;
+    const long long to = at ? at[r] : r;
+    if (to < 0) return;
+    const T* p = in + r * ld + c;
+    Vec16<T> v;
+    if (c + E <= cols && ((uintptr_t)p & 15) == 0) {
+        v = ld16(p);
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) v.v[e] = c + e < cols ? p[e] : (T)0.f;
+    }
+    st16(out + to * padded + c, v);
 }
 
 // ---- plan ---------------------------------------------------------------------------------------------------------------------
@@ -215,20 +450,28 @@ int tiles(long long n) { return (int)((n + VT - 1) / VT); }
 struct Plan {
     int Hp, e;              // columns of the operands the products read (H rounded up to whole 16 bytes)
     bool pad;               // x and w are copied to that width first
+    bool big;               // 256 x 256 tiles
+    bool gather;            // gradient: the counted rows alone
+    int edge;               // tile edge
     int parts;              // forward: column parts per row
     int Vc, pieces, ld;     // gradient: words per piece, row stride of d
     int sx, sw;             // slices of k of dx (per piece) and dw
-    long long xpad, wpad, part, zt, d, dx, dw, db, bytes;
+    long long xpad, wpad, part, zt, d, dx, dw, db, rows, bytes;
 };
 
-int slices(long long tiles, long long K, int ks) {
-    // k is shared out while there are fewer than 512 workgroups and every one keeps 8 steps of k
-    long long s = (512 + tiles - 1) / tiles;
-    const long long most = (K + ks - 1) / ks / 8;
+int edge_tiles(long long n, int edge) { return (int)((n + edge - 1) / edge); }
+
+// k is shared out while there are fewer than `want` workgroups and every one keeps 8 steps of k (6 of the large tiles)
+int slices(long long tiles, long long K, int ks, int want, int least) {
+    long long s = (want + tiles - 1) / tiles;
+    const long long most = (K + ks - 1) / ks / least;
     if (s > most) s = most;
     if (s > 32) s = 32;
     return (int)(s < 1 ? 1 : s);
 }
+
+// Rows kernel: the gathered targets, lse, weights, places and the count
+long long rows_bytes(long long N) { return up256(N * 4) * 4 + 256; }
 
 Plan make_plan(const mic_vocab_loss_desc* d, bool grad) {
     Plan p = {};
@@ -237,35 +480,40 @@ Plan make_plan(const mic_vocab_loss_desc* d, bool grad) {
     p.e = 16 / (int)es;
     p.Hp = (int)((H + p.e - 1) / p.e * p.e);
     p.pad = p.Hp != H || d->ld_x % p.e || d->ld_w % p.e || (((uintptr_t)d->x | (uintptr_t)d->w) & 15);
+    // the large tiles address 256 rows (64 of k) of an operand with 31 bits; below 129 rows half of one would be empty
+    p.big = d->dtype == MIC_BF16 && N > 128 && V > 128 && H >= 64 && H < (1 << 21) && d->ld_x < (1 << 21) && d->ld_w < (1 << 21);
+    p.edge = p.big ? 256 : VT;
+    p.gather = grad && N > p.edge;
     long long o = 0;
     p.xpad = o;
-    if (p.pad) o += up256(N * p.Hp * es);
+    if (p.pad || p.gather) o += up256(N * p.Hp * es);
     p.wpad = o;
     if (p.pad) o += up256(V * p.Hp * es);
     if (!grad) {
-        p.parts = tiles(V) * 2;
+        p.parts = p.big ? (int)((V + 63) / 64) : tiles(V) * 2;
         p.part = o; o += up256(N * p.parts * 8);
         p.zt = o; o += up256(N * 4);
     } else {
         // a piece of d takes at most 256 MiB (what the last-level cache holds), at least one tile of words
-        long long vc = (256ll << 20) / (es * N) / VT * VT;
-        if (vc < VT) vc = VT;
+        long long vc = (256ll << 20) / (es * N) / p.edge * p.edge;
+        if (vc < p.edge) vc = p.edge;
         if (vc > V) vc = V;
         p.pieces = (int)((V + vc - 1) / vc);
-        p.Vc = (int)(((V + p.pieces - 1) / p.pieces + VT - 1) / VT * VT);
+        p.Vc = (int)(((V + p.pieces - 1) / p.pieces + p.edge - 1) / p.edge * p.edge);
         if (p.Vc > V) p.Vc = (int)V;
         p.pieces = (int)((V + p.Vc - 1) / p.Vc);
         p.ld = (p.Vc + p.e - 1) / p.e * p.e;
-        const int ks = 128 / (int)es;
-        p.sx = slices((long long)tiles(N) * tiles(H), p.Vc, ks);
-        p.sw = slices((long long)tiles(p.Vc) * tiles(H), N, ks);
+        const int ks = 128 / (int)es, least = p.big ? 6 : 8;
+        p.sx = slices((long long)edge_tiles(N, p.edge) * edge_tiles(H, p.edge), p.Vc, ks, 512, least);
+        p.sw = slices((long long)edge_tiles(p.Vc, p.edge) * edge_tiles(H, p.edge), N, ks, p.big ? 256 : 512, least);
+        p.rows = o; o += rows_bytes(N);
         p.d = o; o += up256(N * p.ld * es);
         p.dx = o;
-        if (p.sx * p.pieces > 1) o += up256((long long)p.sx * p.pieces * N * H * 4);
+        if (p.sx * p.pieces > 1 || p.gather) o += up256((long long)p.sx * p.pieces * N * H * 4);
         p.dw = o;
         if (p.sw > 1) o += up256((long long)p.sw * p.Vc * H * 4);
         p.db = o;
-        if (d->db) o += up256((long long)tiles(N) * 2 * V * 4);
+        if (d->db) o += up256((long long)edge_tiles(N, p.edge) * 2 * p.Vc * 4);
     }
     p.bytes = o;
     return p;
@@ -292,75 +540,115 @@ Targets targets_of(const mic_vocab_loss_desc* d) {
     return t;
 }
 
-template <typename T, bool PCOL, bool QCOL, typename Epi> int gemm(const Operand& p, const Operand& q, int K, int slices, const typename Epi::Args& ea, hipStream_t s) {
-    GemmShape g = {p, q, K, tiles(p.n), tiles(q.n), slices};
+struct Rows {
+    const int* count;  // NULL: all
+    int are_k;
+};
+template <typename T, bool PCOL, bool QCOL, typename Epi> int gemm(const Operand& p, const Operand& q, const Rows& r, int K, int slices, const typename Epi::Args& ea, hipStream_t s) {
+    GemmShape g = {p, q, r.count, r.are_k, K, tiles(p.n), tiles(q.n), slices};
     MIC_LAUNCH((vocab_gemm_kernel<T, PCOL, QCOL, Epi>), dim3((unsigned)((long long)g.tiles_p * g.tiles_q * slices)), dim3(256), 0, s, g, ea);
     return 0;
 }
+template <bool PCOL, bool QCOL, typename Epi> int gemm8(const Operand& p, const Operand& q, const Rows& r, int K, int slices, const typename Epi::Args& ea, hipStream_t s) {
+    Gemm8Shape g = {{p.p, p.ld, p.n}, {q.p, q.ld, q.n}, r.count, r.are_k, K, edge_tiles(p.n, 256), edge_tiles(q.n, 256), slices};
+    MIC_LAUNCH((vocab_gemm8_kernel<PCOL, QCOL, Epi>), dim3((unsigned)((long long)g.tiles_p * g.tiles_q * slices)), dim3(512), 0, s, g, ea);
+    return 0;
+}
+// bf16 on the tiles of the plan, fp32 on the small ones
+template <typename T, bool PCOL, bool QCOL, typename Epi, typename Epi8>
+int product(const Plan& pl, const Operand& p, const Operand& q, const Rows& r, int K, int slices, const typename Epi::Args& ea, hipStream_t s) {
+    if constexpr (sizeof(T) == 2)
+        if (pl.big) return gemm8<PCOL, QCOL, Epi8>(p, q, r, K, slices, ea, s);
+    return gemm<T, PCOL, QCOL, Epi>(p, q, r, K, slices, ea, s);
+}
 
-// x and w as the products read them: in place, or copied to whole 16-byte rows
-template <typename T> int operands(const mic_vocab_loss_desc* d, const Plan& p, char* ws, Operand& x, Operand& w, hipStream_t s) {
+template <typename T> int copy_rows(const void* in, long long ld, void* out, const int* at, long long rows, int cols, int padded, hipStream_t s) {
+    const long long n = rows * (padded / Vec16<T>::N);
+    MIC_LAUNCH((vocab_pad_kernel<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, (const T*)in, ld, (T*)out, at, rows, cols, padded);
+    return 0;
+}
+// x and w as the products read them: in place, or copied to whole 16-byte rows (x: and gathered)
+template <typename T> int operands(const mic_vocab_loss_desc* d, const Plan& p, char* ws, const int* at, Operand& x, Operand& w, hipStream_t s) {
     x = {d->x, d->ld_x, d->N};
     w = {d->w, d->ld_w, d->V};
-    if (!p.pad) return 0;
-    T *xp = (T*)(ws + p.xpad), *wp = (T*)(ws + p.wpad);
-    const long long nx = (long long)d->N * p.Hp, nw = (long long)d->V * p.Hp;
-    MIC_LAUNCH((vocab_pad_kernel<T>), dim3((unsigned)((nx + 255) / 256)), dim3(256), 0, s, (const T*)d->x, (long long)d->ld_x, xp, (long long)d->N, d->H, p.Hp);
-    MIC_LAUNCH((vocab_pad_kernel<T>), dim3((unsigned)((nw + 255) / 256)), dim3(256), 0, s, (const T*)d->w, (long long)d->ld_w, wp, (long long)d->V, d->H, p.Hp);
-    x = {xp, p.Hp, d->N};
-    w = {wp, p.Hp, d->V};
+    if (p.pad || p.gather) {
+        MIC_TRY(copy_rows<T>(d->x, d->ld_x, ws + p.xpad, at, d->N, d->H, p.Hp, s));
+        x = {ws + p.xpad, p.Hp, d->N};
+    }
+    if (p.pad) {
+        MIC_TRY(copy_rows<T>(d->w, d->ld_w, ws + p.wpad, nullptr, d->V, d->H, p.Hp, s));
+        w = {ws + p.wpad, p.Hp, d->V};
+    }
     return 0;
 }
 
 template <typename T> int forward(const mic_vocab_loss_desc* d, const Plan& p, hipStream_t s) {
     char* ws = (char*)d->workspace;
     Operand x, w;
-    MIC_TRY(operands<T>(d, p, ws, x, w, s));
+    MIC_TRY(operands<T>(d, p, ws, nullptr, x, w, s));
     StatsEpi::Args ea = {};
     ea.bias = d->bias; ea.t = targets_of(d);
     ea.part = (float2*)(ws + p.part); ea.zt = (float*)(ws + p.zt);
     ea.N = d->N; ea.V = d->V; ea.parts = p.parts;
-    MIC_TRY((gemm<T, false, false, StatsEpi>(w, x, d->H, 1, ea, s)));
+    MIC_TRY((product<T, false, false, StatsEpi, StatsEpi8>(p, w, x, Rows{}, d->H, 1, ea, s)));
     MIC_LAUNCH(vocab_loss_rows_kernel, dim3((d->N + 3) / 4), dim3(256), 0, s, (const float2*)ea.part, (const float*)ea.zt, ea.t, d->loss, d->lse, d->N, p.parts);
     return 0;
 }
 
-template <typename T> int sum_parts(const float* part, void* out, long long n, int parts, hipStream_t s) {
-    MIC_LAUNCH((vocab_sum_parts_kernel<T>), dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, s, part, (T*)out, n, parts);
+template <typename T> int sum_parts(const float* part, void* out, const int* at, int rows, int cols, long long stride, int parts, hipStream_t s) {
+    const long long quads = (long long)rows * ((cols + 3) / 4);
+    MIC_LAUNCH((vocab_sum_parts_kernel<T>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s, part, (T*)out, at, rows, cols, stride, parts);
     return 0;
 }
 
 template <typename T> int gradient(const mic_vocab_loss_desc* d, const Plan& p, hipStream_t s) {
     char* ws = (char*)d->workspace;
+    const long long N = d->N, H = d->H, step = up256(N * 4);
+    RowsArgs ra = {};
+    ra.t = targets_of(d);
+    ra.weight = d->grad_rows; ra.lse = d->lse;
+    ra.target_out = (int*)(ws + p.rows);
+    ra.lse_out = (float*)(ws + p.rows + step);
+    ra.weight_out = (float*)(ws + p.rows + 2 * step);
+    ra.at = (int*)(ws + p.rows + 3 * step);
+    ra.count = (int*)(ws + p.rows + 4 * step);
+    ra.N = d->N; ra.gather = p.gather;
+    const long long share = (N + 63) / 64;
+    ra.per_block = (int)((share + 1023) / 1024 * 1024);
+    MIC_LAUNCH(vocab_rows_kernel, dim3((unsigned)((N + ra.per_block - 1) / ra.per_block)), dim3(1024), 0, s, ra);
+    const int* at = p.gather ? ra.at : nullptr;
+    const int* count = p.gather ? ra.count : nullptr;
     Operand x, w;
-    MIC_TRY(operands<T>(d, p, ws, x, w, s));
-    const long long N = d->N, H = d->H;
+    MIC_TRY(operands<T>(d, p, ws, at, x, w, s));
     T* dl = (T*)(ws + p.d);
     float *part_dx = (float*)(ws + p.dx), *part_dw = (float*)(ws + p.dw), *part_db = (float*)(ws + p.db);
+    const bool dx_parts = p.sx * p.pieces > 1 || p.gather;
     for (int i = 0; i < p.pieces; ++i) {
         const int v0 = i * p.Vc, vc = d->V - v0 < p.Vc ? d->V - v0 : p.Vc;
         const Operand wi = {(const T*)w.p + v0 * w.ld, w.ld, vc};
         typename GradEpi<T>::Args ga = {};
-        ga.bias = d->bias; ga.t = targets_of(d); ga.lse = d->lse; ga.weight = d->grad_rows;
+        ga.bias = d->bias; ga.r = {ra.target_out, ra.lse_out, ra.weight_out};
         ga.d = dl; ga.part_db = d->db ? part_db : nullptr;
-        ga.N = d->N; ga.V = d->V; ga.Vc = vc; ga.ld = p.ld; ga.v0 = v0;
-        MIC_TRY((gemm<T, false, false, GradEpi<T>>(wi, x, d->H, 1, ga, s)));
-        if (d->db) MIC_TRY(sum_parts<float>(part_db, d->db + v0, vc, tiles(N) * 2, s));
+        ga.N = d->N; ga.Vc = vc; ga.ld = p.ld; ga.v0 = v0;
+        ga.count = count;
+        MIC_TRY((product<T, false, false, GradEpi<T>, GradEpi8>(p, wi, x, Rows{count, 0}, d->H, 1, ga, s)));
+        if (d->db)
+            MIC_LAUNCH(vocab_colsum_kernel, dim3((vc + 63) / 64), dim3(1024), 0, s, (const float*)part_db, d->db + v0, vc, edge_tiles(N, p.edge) * 2, count, p.edge / 2);
         // dx += d w: k runs over the words of the piece
         typename OutEpi<T>::Args xa = {};
         xa.out = (T*)d->dx; xa.ld = H; xa.Np = d->H; xa.Nq = d->N;
-        if (p.sx * p.pieces > 1) xa.part = part_dx + (long long)i * p.sx * N * H;
+        if (dx_parts) xa.part = part_dx + (long long)i * p.sx * N * H;
         const Operand wc = {wi.p, wi.ld, d->H}, dr = {dl, p.ld, d->N};
-        MIC_TRY((gemm<T, true, false, OutEpi<T>>(wc, dr, vc, p.sx, xa, s)));
+        MIC_TRY((product<T, true, false, OutEpi<T>, OutEpi8>(p, wc, dr, Rows{count, 0}, vc, p.sx, xa, s)));
         // dw = d^T x: k runs over the rows
         typename OutEpi<T>::Args wa = {};
         wa.out = (T*)d->dw + v0 * H; wa.ld = H; wa.Np = d->H; wa.Nq = vc;
         if (p.sw > 1) wa.part = part_dw;
         const Operand xc = {x.p, x.ld, d->H}, dc = {dl, p.ld, vc};
-        MIC_TRY((gemm<T, true, true, OutEpi<T>>(xc, dc, d->N, p.sw, wa, s)));
-        if (p.sw > 1) MIC_TRY(sum_parts<T>(part_dw, wa.out, vc * H, p.sw, s));
+        MIC_TRY((product<T, true, true, OutEpi<T>, OutEpi8>(p, xc, dc, Rows{count, 1}, d->N, p.sw, wa, s)));
+        if (p.sw > 1) MIC_TRY(sum_parts<T>(part_dw, wa.out, nullptr, vc, d->H, vc * H, p.sw, s));
     }
-    if (p.sx * p.pieces > 1) MIC_TRY(sum_parts<T>(part_dx, d->dx, N * H, p.sx * p.pieces, s));
+    if (dx_parts) MIC_TRY(sum_parts<T>(part_dx, d->dx, at, d->N, d->H, N * H, p.sx * p.pieces, s));
     return 0;
 }
 

@@ -429,6 +429,9 @@ VOCAB = [
     (200, 1024, 384, False),
     (700, 128, 128, True),
     (1, 2048, 5000, False),
+    (1500, 136, 2000, True),  # gathered rows, k shared out over workgroups
+    (600, 72, 9001, False),
+    (300, 640, 257, True),
 ]
 
 
@@ -482,6 +485,17 @@ def test_vocab_loss_masks(F, dtype):
     assert not got["dw"][hide.to(DEV)].any() and got["loss"][3] == 0
     got = vocab_run(F, *on(x, w, b, torch.full_like(t, 5).int(), a), (5,))
     assert not got["loss"].any() and not got["dx"].any() and not got["dw"].any() and not got["db"].any() and torch.isfinite(got["lse"]).all()
+
+
+@pytest.mark.parametrize("counted", [0, 1, 255, 256, 257, 511, 700])
+def test_vocab_loss_counted_rows(F, counted):
+    """So many of 700 rows count, anywhere among them: those alone go through the gradient's products."""
+    x, w, b, _, a = vocab_inputs(700, 96, 600, BF16, True, seed=30)
+    t = torch.zeros(700, dtype=torch.long)
+    t[torch.randperm(700, generator=gen(31))[:counted]] = torch.randint(1, 600, (counted,), generator=gen(32))
+    got = vocab_run(F, *on(x, w, b, t, a), (0,))
+    vocab_check(got, vocab_ref(x, w, b, t, a, (0,), BF16))
+    assert not got["dx"][(t == 0).to(DEV)].any()
 
 
 def test_vocab_loss_strides_and_empty(F):
