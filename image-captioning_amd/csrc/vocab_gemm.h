@@ -82,22 +82,26 @@ template <typename T, bool PCOL, bool QCOL, typename Epi> __global__ __launch_bo
     __shared__ __attribute__((aligned(16))) T sp[2][VT * KS];
     __shared__ __attribute__((aligned(16))) T sq[2][VT * KS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wp = wave >> 1, wq = wave & 1;
-    // workgroups b and b + 8 share an XCD and its L2: every XCD takes a contiguous range of tiles
+    if (g.rows) {  // the grid is laid out for all rows: what is behind the counted ones ends here
+        const int rows = *g.rows;
+        if (g.rows_are_k) {
+            g.K = min(g.K, rows);
+        } else {
+            g.q.n = min(g.q.n, rows);
+            g.tiles_q = min(g.tiles_q, (rows + VT - 1) / VT);
+        }
+    }
+    // workgroups b and b + 8 share an XCD and its L2: every XCD takes a contiguous range of the tiles that are left
     int id;
     {
-        const int n = gridDim.x, o = blockIdx.x, per = n >> 3, rest = n & 7, xcd = o & 7;
+        const int n = g.tiles_p * g.tiles_q * g.slices, o = blockIdx.x, per = n >> 3, rest = n & 7, xcd = o & 7;
+        if (o >= n) return;
         id = (xcd < rest ? xcd * (per + 1) : rest * (per + 1) + (xcd - rest) * per) + (o >> 3);
     }
     const int slice = id % g.slices;
     id /= g.slices;
     const int tq = id % g.tiles_q, tp = id / g.tiles_q;
     const int p0 = tp * VT, q0 = tq * VT;
-    if (g.rows) {
-        const int rows = *g.rows;
-        if (g.rows_are_k) g.K = min(g.K, rows);
-        else g.q.n = min(g.q.n, rows);
-        if (q0 >= g.q.n) return;  // rows that do not count
-    }
     const int nk = (g.K + KS - 1) / KS, kb = (int)((long long)nk * slice / g.slices), ke = (int)((long long)nk * (slice + 1) / g.slices);
     f32x16_t acc[2][2];
 #pragma unroll

@@ -125,9 +125,21 @@ template <bool COL, int N> struct Read8 {
 template <bool PCOL, bool QCOL, typename Epi> __global__ __launch_bounds__(512) void vocab_gemm8_kernel(Gemm8Shape g, typename Epi::Args ea) {
     __shared__ __attribute__((aligned(16))) unsigned char smem[G8_SMEM];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wq = wave >> 2, wp = wave & 3;
+    int K = g.K;
+    if (g.rows) {  // the grid is laid out for all rows: what is behind the counted ones ends here
+        const int rows = *g.rows;
+        if (g.rows_are_k) {
+            K = min(K, rows);
+        } else {
+            g.q.n = min(g.q.n, rows);
+            g.tiles_q = min(g.tiles_q, (rows + 255) / 256);
+        }
+    }
+    // workgroups b and b + 8 share an XCD and its L2: every XCD takes a contiguous range of the tiles that are left
     int id;
     {
-        const int n = gridDim.x, o = blockIdx.x, per = n >> 3, rest = n & 7, xcd = o & 7;
+        const int n = g.tiles_p * g.tiles_q * g.slices, o = blockIdx.x, per = n >> 3, rest = n & 7, xcd = o & 7;
+        if (o >= n) return;
         id = (xcd < rest ? xcd * (per + 1) : rest * (per + 1) + (xcd - rest) * per) + (o >> 3);
     }
     const int slice = id % g.slices;
@@ -139,14 +151,7 @@ template <bool PCOL, bool QCOL, typename Epi> __global__ __launch_bounds__(512) 
         tq = band * 4 + in % left;
         tp = in / left;
     }
-    int K = g.K;
-    if (g.rows) {
-        const int rows = *g.rows;
-        if (g.rows_are_k) K = min(K, rows);
-        else g.q.n = min(g.q.n, rows);
-    }
     const int p0 = tp * 256, q0 = tq * 256;
-    if (q0 >= g.q.n) return;  // rows that do not count
     const int nk = (K + 63) / 64, t_begin = (int)((long long)slice * nk / g.slices), t_end = (int)((long long)(slice + 1) * nk / g.slices);
 
     f32x4_t acc[4][8];
