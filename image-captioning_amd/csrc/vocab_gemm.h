@@ -69,9 +69,10 @@ template <typename T, bool COL> struct OperandTile {
 
 struct GemmShape {
     Operand p, q;
-    const int* rows;  // NULL, or the number of rows to take, on the device: limits q.n (k for products over the rows)
+    const int* rows;    // NULL, or the number of rows to take, on the device: limits q.n (k for products over the rows)
+    const int* slices;  // NULL (one), or the number of ranges of k, on the device
     int rows_are_k;
-    int K, tiles_p, tiles_q, slices;
+    int K, tiles_p, tiles_q;
 };
 
 // Epi::run(args, acc, p0, q0, lane, tile_p, tile_q, wave, slice): acc[i][j] = p0 + 32 i.., q0 + 32 j..
@@ -91,18 +92,19 @@ template <typename T, bool PCOL, bool QCOL, typename Epi> __global__ __launch_bo
             g.tiles_q = min(g.tiles_q, (rows + VT - 1) / VT);
         }
     }
+    const int slices = g.slices ? *g.slices : 1;
     // workgroups b and b + 8 share an XCD and its L2: every XCD takes a contiguous range of the tiles that are left
     int id;
     {
-        const int n = g.tiles_p * g.tiles_q * g.slices, o = blockIdx.x, per = n >> 3, rest = n & 7, xcd = o & 7;
+        const int n = g.tiles_p * g.tiles_q * slices, o = blockIdx.x, per = n >> 3, rest = n & 7, xcd = o & 7;
         if (o >= n) return;
         id = (xcd < rest ? xcd * (per + 1) : rest * (per + 1) + (xcd - rest) * per) + (o >> 3);
     }
-    const int slice = id % g.slices;
-    id /= g.slices;
+    const int slice = id % slices;
+    id /= slices;
     const int tq = id % g.tiles_q, tp = id / g.tiles_q;
     const int p0 = tp * VT, q0 = tq * VT;
-    const int nk = (g.K + KS - 1) / KS, kb = (int)((long long)nk * slice / g.slices), ke = (int)((long long)nk * (slice + 1) / g.slices);
+    const int nk = (g.K + KS - 1) / KS, kb = (int)((long long)nk * slice / slices), ke = (int)((long long)nk * (slice + 1) / slices);
     f32x16_t acc[2][2];
 #pragma unroll
     for (int i = 0; i < 2; ++i)

@@ -23,9 +23,10 @@ struct Operand8 {
 };
 struct Gemm8Shape {
     Operand8 p, q;
-    const int* rows;  // NULL, or the number of rows to take, on the device: limits q.n (k for products over the rows)
+    const int* rows;    // NULL, or the number of rows to take, on the device: limits q.n (k for products over the rows)
+    const int* slices;  // NULL (one), or the number of ranges of k, on the device
     int rows_are_k;
-    int K, tiles_p, tiles_q, slices;
+    int K, tiles_p, tiles_q;
 };
 
 typedef unsigned srd_t __attribute__((ext_vector_type(4)));
@@ -135,15 +136,16 @@ template <bool PCOL, bool QCOL, typename Epi> __global__ __launch_bounds__(512) 
             g.tiles_q = min(g.tiles_q, (rows + 255) / 256);
         }
     }
+    const int slices = g.slices ? *g.slices : 1;
     // workgroups b and b + 8 share an XCD and its L2: every XCD takes a contiguous range of the tiles that are left
     int id;
     {
-        const int n = g.tiles_p * g.tiles_q * g.slices, o = blockIdx.x, per = n >> 3, rest = n & 7, xcd = o & 7;
+        const int n = g.tiles_p * g.tiles_q * slices, o = blockIdx.x, per = n >> 3, rest = n & 7, xcd = o & 7;
         if (o >= n) return;
         id = (xcd < rest ? xcd * (per + 1) : rest * (per + 1) + (xcd - rest) * per) + (o >> 3);
     }
-    const int slice = id % g.slices;
-    id /= g.slices;
+    const int slice = id % slices;
+    id /= slices;
     // 4 q tiles side by side walk the p tiles, so what runs at once on an XCD is a block of both and shares its operands in L2
     int tp, tq;
     {
@@ -152,7 +154,7 @@ template <bool PCOL, bool QCOL, typename Epi> __global__ __launch_bounds__(512) 
         tp = in / left;
     }
     const int p0 = tp * 256, q0 = tq * 256;
-    const int nk = (K + 63) / 64, t_begin = (int)((long long)slice * nk / g.slices), t_end = (int)((long long)(slice + 1) * nk / g.slices);
+    const int nk = (K + 63) / 64, t_begin = (int)((long long)slice * nk / slices), t_end = (int)((long long)(slice + 1) * nk / slices);
 
     f32x4_t acc[4][8];
 #pragma unroll

@@ -205,10 +205,12 @@ struct StatsEpi8 {
                 b[j][e] = v < a.V ? (a.bias ? a.bias[v] : 0.f) : -INFINITY;
             }
         if (p0 + 64 * (wave & 3) >= a.V) return;  // its parts are not looked at
+        int ts[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ts[i] = target_of(a.t, min(qw + 16 * i, a.N - 1));  // all in flight at once
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int row = qw + 16 * i;
-            const int t = row < a.N ? target_of(a.t, row) : -1;
+            const int row = qw + 16 * i, t = row < a.N ? ts[i] : -1;
             float m = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -250,11 +252,19 @@ struct GradEpi8 {
                 b[j][e] = c < a.Vc ? (a.bias ? a.bias[a.v0 + c] * ATTN_LOG2E : 0.f) : -INFINITY;  // beyond the piece: probability zero
                 sum[4 * j + e] = 0.f;
             }
+        int ts[8];
+        float rw[8], rl[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {  // all in flight at once
+            const int row = min(q0 + ql + 16 * i, a.N - 1);
+            ts[i] = a.r.target[row];
+            rw[i] = a.r.weight[row];
+            rl[i] = a.r.lse[row];
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int row = q0 + ql + 16 * i;
-            const int t = row < a.N ? a.r.target[row] : -1;
-            const float w = t >= 0 ? a.r.weight[row] : 0.f, lse2 = t >= 0 ? a.r.lse[row] * ATTN_LOG2E : 0.f;
+            const int t = q0 + ql + 16 * i < a.N ? ts[i] : -1;
+            const float w = t >= 0 ? rw[i] : 0.f, lse2 = t >= 0 ? rl[i] * ATTN_LOG2E : 0.f;
             const int tc = t - a.v0 - p0 - pl;  // the target's column, from the lane's first
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -321,26 +331,31 @@ struct OutEpi8 {
     }
 };
 
-// out[row] = the sum of `parts` fp32 rows at[row] (NULL: the row itself; negative: zeros), in order; parts lie `stride` elements apart
+// out[row] = the sum of fp32 rows at[row] (NULL: the row itself; negative: zeros) of the partial matrices, in order: `pieces` groups of
+// `most` matrices `stride` elements apart, of which the first *slices (of the last group: *slices_last) were written
 template <typename T> __global__ __launch_bounds__(256) void vocab_sum_parts_kernel(const float* __restrict__ part, T* __restrict__ out, const int* __restrict__ at, int rows,
-                                                                                    int cols, long long stride, int parts) {
+                                                                                    int cols, long long stride, int pieces, int most, const int* __restrict__ slices,
+                                                                                    const int* __restrict__ slices_last) {
     const int quads = (cols + 3) / 4;
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
     const int row = (int)(i / quads), c = (int)(i - (long long)row * quads) * 4;
     if (row >= rows) return;
-    const int src = at ? at[row] : row;
+    const int src = at ? at[row] : row, whole = *slices, last = *slices_last;
     float s[4] = {};
     if (src >= 0) {
-        const float* p = part + (long long)src * cols + c;
-        if (cols % 4 == 0) {
+        for (int g = 0; g < pieces; ++g) {
+            const float* p = part + (long long)g * most * stride + (long long)src * cols + c;
+            const int parts = g == pieces - 1 ? last : whole;
+            if (cols % 4 == 0) {
 #pragma unroll 8
-            for (int k = 0; k < parts; ++k) {
-                const float4 x = *reinterpret_cast<const float4*>(p + k * stride);
-                s[0] += x.x; s[1] += x.y; s[2] += x.z; s[3] += x.w;
+                for (int k = 0; k < parts; ++k) {
+                    const float4 x = *reinterpret_cast<const float4*>(p + k * stride);
+                    s[0] += x.x; s[1] += x.y; s[2] += x.z; s[3] += x.w;
+                }
+            } else {
+                for (int e = 0; e < 4 && c + e < cols; ++e)
+                    for (int k = 0; k < parts; ++k) s[e] += p[k * stride + e];
             }
-        } else {
-            for (int e = 0; e < 4 && c + e < cols; ++e)
-                for (int k = 0; k < parts; ++k) s[e] += p[k * stride + e];
         }
     }
     T* o = out + (long long)row * cols + c;
@@ -371,12 +386,39 @@ __global__ __launch_bounds__(1024) void vocab_colsum_kernel(const float* __restr
 // ---- the rows of the gradient ------------------------------------------------------------------------------------------------------
 // Every row's target, weight and lse, and with `gather` the counted rows only, in their order: `at` tells where a row went (-1: it does
 // not count), *count how many there are.  A block counts the rows before its own again (at most 64 blocks) instead of waiting for others.
+//
+// The last block also decides into how many ranges of k the products dx (of a whole piece and of the last one) and dw are cut, now that the
+// rows are known.
+struct SplitRule {
+    int capacity;           // workgroups resident at once
+    float fixed, traffic;   // in steps of k: what a workgroup costs beside its steps; what the partial tiles of a full GPU cost
+};
+struct Split {
+    int tiles, nk, most;    // tiles of the result (dx: per tile of rows), steps of k (dw: 0, by the rows), ranges allowed
+};
+__device__ __forceinline__ int choose_slices(const SplitRule& r, int tiles, int nk, int most) {
+    int best = 1;
+    float least = INFINITY;
+    for (int s = 1; s <= most; ++s) {
+        const float x = (float)tiles * s / r.capacity;
+        const float cost = ceilf(x) * (ceilf((float)nk / s) + r.fixed) + (s > 1 ? x * r.traffic : 0.f);
+        if (cost < least) {
+            least = cost;
+            best = s;
+        }
+    }
+    return best;
+}
+enum { COUNT, SX, SX_LAST, SW, SW_LAST, DECISIONS };  // what `count` points to
 struct RowsArgs {
     Targets t;
     const float *weight, *lse;
     int *target_out, *at, *count;
     float *weight_out, *lse_out;
     int N, per_block, gather;
+    SplitRule rule;
+    Split dx[2], dw[2];     // whole pieces, the last one
+    int edge, ks;
 };
 __global__ __launch_bounds__(1024) void vocab_rows_kernel(RowsArgs a) {
     __shared__ int wave_sum[16];
@@ -418,7 +460,13 @@ __global__ __launch_bounds__(1024) void vocab_rows_kernel(RowsArgs a) {
             }
         }
     }
-    if (a.gather && blockIdx.x == gridDim.x - 1 && tid == 0) *a.count = base;
+    if (blockIdx.x == gridDim.x - 1 && tid < DECISIONS) {
+        const int rows = a.gather ? base : a.N, i = (tid - 1) & 1;
+        int v = rows;
+        if (tid == SX || tid == SX_LAST) v = choose_slices(a.rule, a.dx[i].tiles * ((rows + a.edge - 1) / a.edge), a.dx[i].nk, a.dx[i].most);
+        if (tid == SW || tid == SW_LAST) v = choose_slices(a.rule, a.dw[i].tiles, (rows + a.ks - 1) / a.ks, a.dw[i].most);
+        a.count[tid] = v;
+    }
 }
 
 // rows of `cols` elements with any stride -> rows of `padded` elements (whole 16 bytes), zeros behind; row r goes to at[r] (NULL: r;
@@ -461,17 +509,14 @@ struct Plan {
 
 int edge_tiles(long long n, int edge) { return (int)((n + edge - 1) / edge); }
 
-// k is shared out while there are fewer than `want` workgroups and every one keeps 8 steps of k (6 of the large tiles)
-int slices(long long tiles, long long K, int ks, int want, int least) {
-    long long s = (want + tiles - 1) / tiles;
-    const long long most = (K + ks - 1) / ks / least;
-    if (s > most) s = most;
-    if (s > 32) s = 32;
-    return (int)(s < 1 ? 1 : s);
+// The most ranges k may be cut into: every one keeps four steps of k.  How many are used is decided when the rows are known.
+int most_slices(long long K, int ks) {
+    const long long s = (K + ks - 1) / ks / 4;
+    return (int)(s < 1 ? 1 : s > 16 ? 16 : s);
 }
 
 // Rows kernel: the gathered targets, lse, weights, places and the count
-long long rows_bytes(long long N) { return up256(N * 4) * 4 + 256; }
+long long rows_bytes(long long N) { return up256(N * 4) * 4 + 256; }  // (the decisions take five words of the last 256 bytes)
 
 Plan make_plan(const mic_vocab_loss_desc* d, bool grad) {
     Plan p = {};
@@ -503,9 +548,13 @@ Plan make_plan(const mic_vocab_loss_desc* d, bool grad) {
         if (p.Vc > V) p.Vc = (int)V;
         p.pieces = (int)((V + p.Vc - 1) / p.Vc);
         p.ld = (p.Vc + p.e - 1) / p.e * p.e;
-        const int ks = 128 / (int)es, least = p.big ? 6 : 8;
-        p.sx = slices((long long)edge_tiles(N, p.edge) * edge_tiles(H, p.edge), p.Vc, ks, 512, least);
-        p.sw = slices((long long)edge_tiles(p.Vc, p.edge) * edge_tiles(H, p.edge), N, ks, p.big ? 256 : 512, least);
+        const int ks = 128 / (int)es;
+        p.sx = most_slices(p.Vc, ks);
+        p.sw = most_slices(N, ks);
+        // never more partial tiles than would fill the GPU twice
+        const long long wide = p.big ? 512 : 1024, tx = (long long)edge_tiles(N, p.edge) * edge_tiles(H, p.edge), tw = (long long)edge_tiles(p.Vc, p.edge) * edge_tiles(H, p.edge);
+        while (p.sx > 1 && p.sx * tx > (p.gather ? 2 * wide : wide)) --p.sx;
+        while (p.sw > 1 && p.sw * tw > wide) --p.sw;
         p.rows = o; o += rows_bytes(N);
         p.d = o; o += up256(N * p.ld * es);
         p.dx = o;
@@ -541,25 +590,27 @@ Targets targets_of(const mic_vocab_loss_desc* d) {
 }
 
 struct Rows {
-    const int* count;  // NULL: all
+    const int* count;   // NULL: all
     int are_k;
+    const int* slices;  // NULL: one
+    int most;           // slices the grid is laid out for
 };
-template <typename T, bool PCOL, bool QCOL, typename Epi> int gemm(const Operand& p, const Operand& q, const Rows& r, int K, int slices, const typename Epi::Args& ea, hipStream_t s) {
-    GemmShape g = {p, q, r.count, r.are_k, K, tiles(p.n), tiles(q.n), slices};
-    MIC_LAUNCH((vocab_gemm_kernel<T, PCOL, QCOL, Epi>), dim3((unsigned)((long long)g.tiles_p * g.tiles_q * slices)), dim3(256), 0, s, g, ea);
+template <typename T, bool PCOL, bool QCOL, typename Epi> int gemm(const Operand& p, const Operand& q, const Rows& r, int K, const typename Epi::Args& ea, hipStream_t s) {
+    GemmShape g = {p, q, r.count, r.slices, r.are_k, K, tiles(p.n), tiles(q.n)};
+    MIC_LAUNCH((vocab_gemm_kernel<T, PCOL, QCOL, Epi>), dim3((unsigned)((long long)g.tiles_p * g.tiles_q * (r.slices ? r.most : 1))), dim3(256), 0, s, g, ea);
     return 0;
 }
-template <bool PCOL, bool QCOL, typename Epi> int gemm8(const Operand& p, const Operand& q, const Rows& r, int K, int slices, const typename Epi::Args& ea, hipStream_t s) {
-    Gemm8Shape g = {{p.p, p.ld, p.n}, {q.p, q.ld, q.n}, r.count, r.are_k, K, edge_tiles(p.n, 256), edge_tiles(q.n, 256), slices};
-    MIC_LAUNCH((vocab_gemm8_kernel<PCOL, QCOL, Epi>), dim3((unsigned)((long long)g.tiles_p * g.tiles_q * slices)), dim3(512), 0, s, g, ea);
+template <bool PCOL, bool QCOL, typename Epi> int gemm8(const Operand& p, const Operand& q, const Rows& r, int K, const typename Epi::Args& ea, hipStream_t s) {
+    Gemm8Shape g = {{p.p, p.ld, p.n}, {q.p, q.ld, q.n}, r.count, r.slices, r.are_k, K, edge_tiles(p.n, 256), edge_tiles(q.n, 256)};
+    MIC_LAUNCH((vocab_gemm8_kernel<PCOL, QCOL, Epi>), dim3((unsigned)((long long)g.tiles_p * g.tiles_q * (r.slices ? r.most : 1))), dim3(512), 0, s, g, ea);
     return 0;
 }
 // bf16 on the tiles of the plan, fp32 on the small ones
 template <typename T, bool PCOL, bool QCOL, typename Epi, typename Epi8>
-int product(const Plan& pl, const Operand& p, const Operand& q, const Rows& r, int K, int slices, const typename Epi::Args& ea, hipStream_t s) {
+int product(const Plan& pl, const Operand& p, const Operand& q, const Rows& r, int K, const typename Epi::Args& ea, hipStream_t s) {
     if constexpr (sizeof(T) == 2)
-        if (pl.big) return gemm8<PCOL, QCOL, Epi8>(p, q, r, K, slices, ea, s);
-    return gemm<T, PCOL, QCOL, Epi>(p, q, r, K, slices, ea, s);
+        if (pl.big) return gemm8<PCOL, QCOL, Epi8>(p, q, r, K, ea, s);
+    return gemm<T, PCOL, QCOL, Epi>(p, q, r, K, ea, s);
 }
 
 template <typename T> int copy_rows(const void* in, long long ld, void* out, const int* at, long long rows, int cols, int padded, hipStream_t s) {
@@ -590,14 +641,8 @@ template <typename T> int forward(const mic_vocab_loss_desc* d, const Plan& p, h
     ea.bias = d->bias; ea.t = targets_of(d);
     ea.part = (float2*)(ws + p.part); ea.zt = (float*)(ws + p.zt);
     ea.N = d->N; ea.V = d->V; ea.parts = p.parts;
-    MIC_TRY((product<T, false, false, StatsEpi, StatsEpi8>(p, w, x, Rows{}, d->H, 1, ea, s)));
+    MIC_TRY((product<T, false, false, StatsEpi, StatsEpi8>(p, w, x, Rows{}, d->H, ea, s)));
     MIC_LAUNCH(vocab_loss_rows_kernel, dim3((d->N + 3) / 4), dim3(256), 0, s, (const float2*)ea.part, (const float*)ea.zt, ea.t, d->loss, d->lse, d->N, p.parts);
-    return 0;
-}
-
-template <typename T> int sum_parts(const float* part, void* out, const int* at, int rows, int cols, long long stride, int parts, hipStream_t s) {
-    const long long quads = (long long)rows * ((cols + 3) / 4);
-    MIC_LAUNCH((vocab_sum_parts_kernel<T>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s, part, (T*)out, at, rows, cols, stride, parts);
     return 0;
 }
 
@@ -615,6 +660,16 @@ template <typename T> int gradient(const mic_vocab_loss_desc* d, const Plan& p, 
     ra.N = d->N; ra.gather = p.gather;
     const long long share = (N + 63) / 64;
     ra.per_block = (int)((share + 1023) / 1024 * 1024);
+    // measured on 256 x 256 tiles: a step of 64 k is 1.7 us, a workgroup's start and end 4 steps, writing and reading again the partial
+    // tiles of all compute units 16; on 128 x 128 tiles (two workgroups to a compute unit) 2 and 7
+    ra.rule = p.big ? SplitRule{256, 4.f, 16.f} : SplitRule{512, 2.f, 7.f};
+    ra.edge = p.edge;
+    ra.ks = 128 / (int)sizeof(T);
+    const int last = d->V - (p.pieces - 1) * p.Vc, th = edge_tiles(H, p.edge);
+    ra.dx[0] = {th, (p.Vc + ra.ks - 1) / ra.ks, p.sx};
+    ra.dx[1] = {th, (last + ra.ks - 1) / ra.ks, p.sx};
+    ra.dw[0] = {th * edge_tiles(p.Vc, p.edge), 0, p.sw};
+    ra.dw[1] = {th * edge_tiles(last, p.edge), 0, p.sw};
     MIC_LAUNCH(vocab_rows_kernel, dim3((unsigned)((N + ra.per_block - 1) / ra.per_block)), dim3(1024), 0, s, ra);
     const int* at = p.gather ? ra.at : nullptr;
     const int* count = p.gather ? ra.count : nullptr;
@@ -623,15 +678,22 @@ template <typename T> int gradient(const mic_vocab_loss_desc* d, const Plan& p, 
     T* dl = (T*)(ws + p.d);
     float *part_dx = (float*)(ws + p.dx), *part_dw = (float*)(ws + p.dw), *part_db = (float*)(ws + p.db);
     const bool dx_parts = p.sx * p.pieces > 1 || p.gather;
+    auto sum_parts = [&](const float* part, T* out, const int* where, int rows, long long stride, int pieces, int most, int whole, int end) -> int {
+        const long long quads = (long long)rows * ((H + 3) / 4);
+        MIC_LAUNCH((vocab_sum_parts_kernel<T>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s, part, out, where, rows, d->H, stride, pieces, most,
+                   (const int*)ra.count + whole, (const int*)ra.count + end);
+        return 0;
+    };
     for (int i = 0; i < p.pieces; ++i) {
-        const int v0 = i * p.Vc, vc = d->V - v0 < p.Vc ? d->V - v0 : p.Vc;
+        const bool end = i == p.pieces - 1;
+        const int v0 = i * p.Vc, vc = end ? last : p.Vc;
         const Operand wi = {(const T*)w.p + v0 * w.ld, w.ld, vc};
         typename GradEpi<T>::Args ga = {};
         ga.bias = d->bias; ga.r = {ra.target_out, ra.lse_out, ra.weight_out};
         ga.d = dl; ga.part_db = d->db ? part_db : nullptr;
         ga.N = d->N; ga.Vc = vc; ga.ld = p.ld; ga.v0 = v0;
         ga.count = count;
-        MIC_TRY((product<T, false, false, GradEpi<T>, GradEpi8>(p, wi, x, Rows{count, 0}, d->H, 1, ga, s)));
+        MIC_TRY((product<T, false, false, GradEpi<T>, GradEpi8>(p, wi, x, Rows{count, 0, nullptr, 1}, d->H, ga, s)));
         if (d->db)
             MIC_LAUNCH(vocab_colsum_kernel, dim3((vc + 63) / 64), dim3(1024), 0, s, (const float*)part_db, d->db + v0, vc, edge_tiles(N, p.edge) * 2, count, p.edge / 2);
         // dx += d w: k runs over the words of the piece
@@ -639,16 +701,18 @@ template <typename T> int gradient(const mic_vocab_loss_desc* d, const Plan& p, 
         xa.out = (T*)d->dx; xa.ld = H; xa.Np = d->H; xa.Nq = d->N;
         if (dx_parts) xa.part = part_dx + (long long)i * p.sx * N * H;
         const Operand wc = {wi.p, wi.ld, d->H}, dr = {dl, p.ld, d->N};
-        MIC_TRY((product<T, true, false, OutEpi<T>, OutEpi8>(p, wc, dr, Rows{count, 0}, vc, p.sx, xa, s)));
+        const Rows rx = {count, 0, p.sx > 1 ? ra.count + (end ? SX_LAST : SX) : nullptr, p.sx};
+        MIC_TRY((product<T, true, false, OutEpi<T>, OutEpi8>(p, wc, dr, rx, vc, xa, s)));
         // dw = d^T x: k runs over the rows
         typename OutEpi<T>::Args wa = {};
         wa.out = (T*)d->dw + v0 * H; wa.ld = H; wa.Np = d->H; wa.Nq = vc;
         if (p.sw > 1) wa.part = part_dw;
         const Operand xc = {x.p, x.ld, d->H}, dc = {dl, p.ld, vc};
-        MIC_TRY((product<T, true, true, OutEpi<T>, OutEpi8>(p, xc, dc, Rows{count, 1}, d->N, p.sw, wa, s)));
-        if (p.sw > 1) MIC_TRY(sum_parts<T>(part_dw, wa.out, nullptr, vc, d->H, vc * H, p.sw, s));
+        const Rows rw = {count, 1, p.sw > 1 ? ra.count + (end ? SW_LAST : SW) : nullptr, p.sw};
+        MIC_TRY((product<T, true, true, OutEpi<T>, OutEpi8>(p, xc, dc, rw, d->N, wa, s)));
+        if (p.sw > 1) MIC_TRY(sum_parts(part_dw, wa.out, nullptr, vc, vc * H, 1, p.sw, SW, end ? SW_LAST : SW));
     }
-    if (dx_parts) MIC_TRY(sum_parts<T>(part_dx, d->dx, at, d->N, d->H, N * H, p.sx * p.pieces, s));
+    if (dx_parts) MIC_TRY(sum_parts(part_dx, (T*)d->dx, at, d->N, N * H, p.pieces, p.sx, SX, SX_LAST));
     return 0;
 }
 
