@@ -26,6 +26,7 @@ struct AttnSeqArgs {
     int causal, off;                // query i sees keys up to i + off
     float scale, scale_log2;
     int splits, tiles_per_split;
+    unsigned group_magic;           // ceil(2^32 / group) where a small x / group is the high half of x times it, else 0
 };
 
 namespace {
@@ -158,6 +159,48 @@ template <typename T, int DP, int ROWS, int THREADS, typename P> __device__ __fo
     }
 }
 
+// ---- tiles straight to LDS -----------------------------------------------------------------------------------------------------
+// One buffer load per 1 KiB of a tile: a wave's 64 lanes fetch 16 bytes each from their own offsets and the result lands linearly in
+// LDS, so the tile image's swizzle is applied to the chunk a lane fetches.  The buffer's base is the tile's, its length 2 GiB: an
+// offset with bit 31 set (a row that is hidden or does not exist, a chunk past the head's columns) returns zeros without touching
+// memory.  The loads are inline assembly because the compiler would drain the memory counter before the next LDS read if it saw
+// them; the kernels wait for it themselves (s_waitcnt vmcnt(0), then a barrier, before a tile is read).
+typedef unsigned srd_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ srd_t make_srd(const void* p) {
+    const unsigned long long a = (unsigned long long)p;
+    return srd_t{(unsigned)a, (unsigned)(a >> 32) & 0xffffu, 0x80000000u, 0x00020000u};
+}
+__device__ __forceinline__ void request16(unsigned voff, const srd_t& srd, unsigned lds) {
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep)
+                 : "v"(voff), "s"(lds), "s"(srd)
+                 : "memory");
+}
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
+__device__ __forceinline__ unsigned lds_address(const void* p) { return __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(lds_ptr_t)p); }
+// every request of this wave has landed and every wave is here: the tile requested last may be read, the other one written
+__device__ __forceinline__ void tile_landed() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// ROWS rows of a tile by four waves; offset(row) is the row's byte offset from the base, or bit 31
+template <typename T, int DP, int ROWS, typename F> __device__ __forceinline__ void request_tile(const T* base, unsigned lds, int D, int wave, int lane, F offset) {
+    using L = Tile<T, DP>;
+    constexpr int ROWB = DP * (int)sizeof(T), PIECES = ROWS * ROWB / 1024, PER = (PIECES + 3) / 4;
+    const srd_t srd = make_srd(base);
+#pragma unroll
+    for (int n = 0; n < PER; ++n) {
+        const int piece = n * 4 + wave;
+        if (PIECES % 4 != 0 && piece >= PIECES) break;
+        const int at = piece * 1024 + lane * 16, row = at / ROWB, c = (at % ROWB / 16) ^ L::swizzle(row);
+        const unsigned off = c * L::E < D ? offset(row) + c * 16u : 0x80000000u;
+        request16(off, srd, lds + piece * 1024);
+    }
+}
+
 // four consecutive columns of a result, rounded once
 template <typename T> __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
     if constexpr (sizeof(T) == 2) {
@@ -175,6 +218,8 @@ __device__ __forceinline__ unsigned key_bits(const AttnSeqArgs& a, int b, int k0
     if (ok && a.mask) ok = a.mask[b * a.mask_sb + key] != 0;
     return (unsigned)__ballot(ok);
 }
+// x / group for x < group + 64
+__device__ __forceinline__ unsigned by_group(const AttnSeqArgs& a, unsigned x) { return a.group == 1 ? x : a.group_magic ? __umulhi(x, a.group_magic) : x / (unsigned)a.group; }
 __device__ __forceinline__ bool key_seen(const AttnSeqArgs& a, int b, int key) { return key < a.Tk && (!a.mask || a.mask[b * a.mask_sb + key] != 0); }
 
 }  // namespace

@@ -4,16 +4,20 @@
 namespace {
 
 constexpr long long MAX_STRIDE = 1ll << 40;
+// A tile's rows are addressed by 31-bit byte offsets from its first: up to 64 positions and the heads of one position
+constexpr long long MAX_TILE_BYTES = 1ll << 30;
 
 int head_columns(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
-int check_tensor(const char* who, const char* name, const void* p, const int64_t st[3], int dtype, bool empty) {
+int check_tensor(const char* who, const char* name, const void* p, const int64_t st[3], int heads, int dtype, bool empty) {
     if (empty) return 0;
     MIC_ARG_CHECK(p, "%s: %s is a null pointer", who, name);
     const int e = 16 / (int)mic_dtype_size(dtype);
     MIC_ARG_CHECK(((uintptr_t)p & 15) == 0, "%s: %s is not 16-byte aligned", who, name);
     for (int i = 0; i < 3; ++i)
         MIC_ARG_CHECK(st[i] >= 0 && st[i] < MAX_STRIDE && st[i] % e == 0, "%s: stride %lld of %s is not a multiple of 16 bytes", who, (long long)st[i], name);
+    MIC_ARG_CHECK(64 * st[1] * (16 / e) <= MAX_TILE_BYTES && heads * st[2] * (16 / e) <= MAX_TILE_BYTES, "%s: strides %lld, %lld of %s are too large", who, (long long)st[1],
+                  (long long)st[2], name);
     return 0;
 }
 
@@ -50,6 +54,7 @@ AttnSeqArgs args_of(const mic_attn_seq_desc* d) {
     a.scale = d->scale;
     a.scale_log2 = d->scale * ATTN_LOG2E;
     a.splits = 1;
+    a.group_magic = a.group > 1 && a.group <= 1024 ? (unsigned)(((1ull << 32) + a.group - 1) / a.group) : 0;
     return a;
 }
 
@@ -112,10 +117,10 @@ extern "C" int mic_attn_seq(const mic_attn_seq_desc* d, void* stream) {
     AttnSeqArgs a = args_of(d);
     const bool no_rows = d->B == 0 || d->Tq == 0, no_keys = d->B == 0 || d->Tk == 0;
     if (no_rows) return 0;
-    MIC_TRY(check_tensor(who, "q", d->q, d->q_stride, d->dtype, false));
-    MIC_TRY(check_tensor(who, "k", d->k, d->k_stride, d->dtype, no_keys));
-    MIC_TRY(check_tensor(who, "v", d->v, d->v_stride, d->dtype, no_keys));
-    MIC_TRY(check_tensor(who, "o", d->o, d->o_stride, d->dtype, false));
+    MIC_TRY(check_tensor(who, "q", d->q, d->q_stride, d->Hq, d->dtype, false));
+    MIC_TRY(check_tensor(who, "k", d->k, d->k_stride, d->Hkv, d->dtype, no_keys));
+    MIC_TRY(check_tensor(who, "v", d->v, d->v_stride, d->Hkv, d->dtype, no_keys));
+    MIC_TRY(check_tensor(who, "o", d->o, d->o_stride, d->Hq, d->dtype, false));
     MIC_ARG_CHECK(d->lse, "%s: lse is a null pointer", who);
     split_keys(a, d->dtype);
     const long long need = fwd_bytes(a);
@@ -134,11 +139,11 @@ extern "C" int mic_attn_seq_grad(const mic_attn_seq_desc* d, void* stream) {
     MIC_TRY(check_sizes(who, d));
     AttnSeqArgs a = args_of(d);
     const bool no_rows = d->B == 0 || d->Tq == 0, no_keys = d->B == 0 || d->Tk == 0;
-    MIC_TRY(check_tensor(who, "q", d->q, d->q_stride, d->dtype, no_rows));
-    MIC_TRY(check_tensor(who, "k", d->k, d->k_stride, d->dtype, no_keys));
-    MIC_TRY(check_tensor(who, "v", d->v, d->v_stride, d->dtype, no_keys));
-    MIC_TRY(check_tensor(who, "o", d->o, d->o_stride, d->dtype, no_rows));
-    MIC_TRY(check_tensor(who, "grad_o", d->grad_o, d->g_stride, d->dtype, no_rows));
+    MIC_TRY(check_tensor(who, "q", d->q, d->q_stride, d->Hq, d->dtype, no_rows));
+    MIC_TRY(check_tensor(who, "k", d->k, d->k_stride, d->Hkv, d->dtype, no_keys));
+    MIC_TRY(check_tensor(who, "v", d->v, d->v_stride, d->Hkv, d->dtype, no_keys));
+    MIC_TRY(check_tensor(who, "o", d->o, d->o_stride, d->Hq, d->dtype, no_rows));
+    MIC_TRY(check_tensor(who, "grad_o", d->grad_o, d->g_stride, d->Hq, d->dtype, no_rows));
     MIC_ARG_CHECK(no_rows || (d->lse && d->dq), "%s: lse or dq is a null pointer", who);
     MIC_ARG_CHECK(no_keys || (d->dk && d->dv), "%s: dk or dv is a null pointer", who);
     MIC_ARG_CHECK((((uintptr_t)d->dq | (uintptr_t)d->dk | (uintptr_t)d->dv) & 15) == 0, "%s: a gradient is not 16-byte aligned", who);

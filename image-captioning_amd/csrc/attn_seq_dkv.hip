@@ -7,17 +7,17 @@
 
 namespace {
 
-template <typename T, int DP, bool SPLIT> __global__ __launch_bounds__(256) void attn_seq_dkv_kernel(AttnSeqArgs a) {
-    constexpr int NC = DP / 16, ND = DP / 32, NR = InRegs<T, DP>::value ? NC : 1;
-    __shared__ __attribute__((aligned(16))) T sq[32 * DP];
-    __shared__ __attribute__((aligned(16))) T sg[32 * DP];
-    __shared__ float s_lse[32], s_delta[32];
+template <typename T, int DP, bool SPLIT> __global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void attn_seq_dkv_kernel(AttnSeqArgs a) {
+    constexpr int NC = DP / 16, ND = DP / 32, NR = InRegs<T, DP>::value ? NC : 1, ES = sizeof(T);
+    __shared__ __attribute__((aligned(16))) T sq[2][32 * DP];
+    __shared__ __attribute__((aligned(16))) T sg[2][32 * DP];
+    __shared__ __attribute__((aligned(16))) float s_lse[2][32], s_delta[2][32];
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int tiles_k = (a.Tk + ATTN_SEQ_BLOCK - 1) / ATTN_SEQ_BLOCK;
+    const int heads = a.Hkv * a.B;
     int id = blockIdx.x;
     const int split = SPLIT ? id % a.splits : 0;
     if (SPLIT) id /= a.splits;
-    const int kt = id % tiles_k, hk = id / tiles_k % a.Hkv, b = id / tiles_k / a.Hkv;  // the first keys, which the most rows see, first
+    const int kt = id / heads, hk = id % heads % a.Hkv, b = id % heads / a.Hkv;  // the first keys, which the most rows see, first
     const int k0 = kt * ATTN_SEQ_BLOCK + wave * 32, key = k0 + (lane & 31);
     const bool seen = key_seen(a, b, key);
     const T* krow = seen ? (const T*)a.k + b * a.k_sb + hk * a.k_sh + (long long)key * a.k_st : nullptr;
@@ -30,72 +30,104 @@ template <typename T, int DP, bool SPLIT> __global__ __launch_bounds__(256) void
             vf[c] = load_frag<T>(vrow, 16 * c + 8 * h, a.D);
         }
     }
-    // rows below `first` see no key of the workgroup (of the wave: w_first)
+    // rows below `first` see no key of the workgroup, below w_first none of the wave; from w_all on they see every key of the wave
     const int first = a.causal ? max(0, kt * ATTN_SEQ_BLOCK - a.off) * a.group : 0, w_first = a.causal ? max(0, k0 - a.off) * a.group : 0;
+    const int w_all = a.causal ? max(0, k0 + 31 - a.off) * a.group : 0;
+    const bool all_seen = (unsigned)__ballot(seen) == 0xffffffffu;
+    // a row sees this lane's key from row (key - off) * group on
+    const int from = !seen ? 0x7fffffff : a.causal ? max(0, key - a.off) * a.group : 0;
     int t0 = min(first, a.R) / 32, t1 = (a.R + 31) / 32;
-    if (SPLIT) {
-        t0 = max(t0, split * a.tiles_per_split);
-        t1 = min(t1, (split + 1) * a.tiles_per_split);
+    if (SPLIT) {  // an even share of the tiles that see anything
+        const int n = t1 - t0;
+        t1 = t0 + (int)((long long)n * (split + 1) / a.splits);
+        t0 = t0 + (int)((long long)n * split / a.splits);
     }
+    const unsigned q_row = (unsigned)(a.q_st * ES), q_head = (unsigned)(a.q_sh * ES), g_row = (unsigned)(a.g_st * ES), g_head = (unsigned)(a.g_sh * ES);
+    const unsigned lds_q = lds_address(sq), lds_g = lds_address(sg);
+    const T* qb = (const T*)a.q + b * a.q_sb + hk * a.group * a.q_sh;
+    const T* gb = (const T*)a.g + b * a.g_sb + hk * a.group * a.g_sh;
+    auto request = [&](int t, int buf) {
+        const int r0 = t * 32, i0 = r0 / a.group, rest = r0 - i0 * a.group;
+        auto row = [&](unsigned per_row, unsigned per_head) {
+            return [&, per_row, per_head](int x) {
+                const unsigned y = rest + x, i = by_group(a, y);
+                return r0 + x < a.R ? i * per_row + (y - i * a.group) * per_head : 0x80000000u;
+            };
+        };
+        request_tile<T, DP, 32>(qb + (long long)i0 * a.q_st, lds_q + buf * 32 * DP * ES, a.D, wave, lane, row(q_row, q_head));
+        request_tile<T, DP, 32>(gb + (long long)i0 * a.g_st, lds_g + buf * 32 * DP * ES, a.D, wave, lane, row(g_row, g_head));
+    };
+    // lse and delta of a tile's rows: 32 threads, loaded a tile ahead
+    float lse2 = INFINITY, delta = 0.f;
+    auto load_stats = [&](int t) {
+        lse2 = INFINITY;
+        delta = 0.f;
+        const int r = t * 32 + threadIdx.x;
+        if (threadIdx.x < 32 && r < a.R) {
+            const int qi = r / a.group;
+            const long long at = ((long long)b * a.Hq + hk * a.group + r - qi * a.group) * a.Tq + qi;
+            lse2 = a.lse[at];
+            delta = a.delta[at];
+        }
+    };
+    auto put_stats = [&](int buf) {
+        if (threadIdx.x < 32) {
+            s_lse[buf][threadIdx.x] = lse2 == -INFINITY ? INFINITY : lse2 * ATTN_LOG2E;  // no key seen: every probability is zero
+            s_delta[buf][threadIdx.x] = delta;
+        }
+    };
     f32x16_t dk[ND], dv[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) dk[d] = dv[d] = f32x16_t{};
+    if (t0 < t1) {
+        request(t0, 0);
+        load_stats(t0);
+        put_stats(0);
+    }
     for (int t = t0; t < t1; ++t) {
-        const int r0 = t * 32;
-        auto row_of = [&](const void* p, long long sb, long long st, long long sh, int x) -> const T* {
-            const int r = r0 + x;
-            if (r >= a.R) return nullptr;
-            const int qi = r / a.group;
-            return (const T*)p + b * sb + qi * st + (hk * a.group + r - qi * a.group) * sh;
-        };
-        __syncthreads();
-        stage<T, DP, 32, 256>(sq, a.D, [&](int x) { return row_of(a.q, a.q_sb, a.q_st, a.q_sh, x); });
-        stage<T, DP, 32, 256>(sg, a.D, [&](int x) { return row_of(a.g, a.g_sb, a.g_st, a.g_sh, x); });
-        if (threadIdx.x < 32) {
-            const int r = r0 + threadIdx.x;
-            float lse2 = INFINITY, delta = 0.f;
-            if (r < a.R) {
-                const int qi = r / a.group;
-                const long long at = ((long long)b * a.Hq + hk * a.group + r - qi * a.group) * a.Tq + qi;
-                const float x = a.lse[at];
-                lse2 = x == -INFINITY ? INFINITY : x * ATTN_LOG2E;
-                delta = a.delta[at];
+        const int r0 = t * 32, cur = (t - t0) & 1;
+        tile_landed();
+        if (t + 1 < t1) {
+            request(t + 1, cur ^ 1);
+            load_stats(t + 1);
+        }
+        if (k0 < a.Tk && r0 + 31 >= w_first) {
+            f32x16_t s = f32x16_t{}, dp = f32x16_t{};
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                if constexpr (InRegs<T, DP>::value) {
+                    mma32(read_row<DP>(sq[cur], lane & 31, c, h), kf[c], s);
+                    mma32(read_row<DP>(sg[cur], lane & 31, c, h), vf[c], dp);
+                } else {
+                    mma32(read_row<DP>(sq[cur], lane & 31, c, h), load_frag<T>(krow, 16 * c + 8 * h, a.D), s);
+                    mma32(read_row<DP>(sg[cur], lane & 31, c, h), load_frag<T>(vrow, 16 * c + 8 * h, a.D), dp);
+                }
             }
-            s_lse[threadIdx.x] = lse2;
-            s_delta[threadIdx.x] = delta;
-        }
-        __syncthreads();
-        if (k0 >= a.Tk || r0 + 31 < w_first) continue;
-        f32x16_t s = f32x16_t{}, dp = f32x16_t{};
+            const bool whole = all_seen && r0 >= w_all;  // nothing hidden: the common case
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            if constexpr (InRegs<T, DP>::value) {
-                mma32(read_row<DP>(sq, lane & 31, c, h), kf[c], s);
-                mma32(read_row<DP>(sg, lane & 31, c, h), vf[c], dp);
-            } else {
-                mma32(read_row<DP>(sq, lane & 31, c, h), load_frag<T>(krow, 16 * c + 8 * h, a.D), s);
-                mma32(read_row<DP>(sg, lane & 31, c, h), load_frag<T>(vrow, 16 * c + 8 * h, a.D), dp);
+            for (int e4 = 0; e4 < 4; ++e4) {
+                const float4 l4 = *reinterpret_cast<const float4*>(&s_lse[cur][8 * e4 + 4 * h]), d4 = *reinterpret_cast<const float4*>(&s_delta[cur][8 * e4 + 4 * h]);
+                const float ls[4] = {l4.x, l4.y, l4.z, l4.w}, ds[4] = {d4.x, d4.y, d4.z, d4.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int e = 4 * e4 + i;
+                    const bool ok = whole || r0 + 8 * e4 + 4 * h + i >= from;
+                    const float p = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2, -ls[i]));
+                    s[e] = ok ? p : 0.f;
+                    dp[e] = ok ? p * (dp[e] - ds[i]) : 0.f;
+                }
             }
-        }
-        // a query sees this lane's key from row (key - off) * group on
-        const int from = !seen ? 0x7fffffff : a.causal ? max(0, key - a.off) * a.group : 0;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const int x = 8 * (e >> 2) + 4 * h + (e & 3);
-            const bool ok = r0 + x >= from;
-            const float p = ok ? __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2, -s_lse[x])) : 0.f;
-            s[e] = p;
-            dp[e] = ok ? p * (dp[e] - s_delta[x]) : 0.f;
-        }
+            for (int j = 0; j < 2; ++j) {
+                const Frag8<T> p = frag_of<T>(s, j), ds = frag_of<T>(dp, j);  // bf16: rounded for the products
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const Frag8<T> p = frag_of<T>(s, j), ds = frag_of<T>(dp, j);  // bf16: rounded for the products
-#pragma unroll
-            for (int d = 0; d < ND; ++d) {
-                mma32(read_col<DP>(sg, d * 32, 16 * j, lane), p, dv[d]);
-                mma32(read_col<DP>(sq, d * 32, 16 * j, lane), ds, dk[d]);
+                for (int d = 0; d < ND; ++d) {
+                    mma32(read_col<DP>(sg[cur], d * 32, 16 * j, lane), p, dv[d]);
+                    mma32(read_col<DP>(sq[cur], d * 32, 16 * j, lane), ds, dk[d]);
+                }
             }
         }
+        if (t + 1 < t1) put_stats(cur ^ 1);
     }
     if (key >= a.Tk) return;
     const long long at = (((long long)b * a.Tk + key) * a.Hkv + hk) * a.D, all = (long long)a.B * a.Tk * a.Hkv * a.D;

@@ -8,17 +8,17 @@
 
 namespace {
 
-template <typename T, int DP, int BK, bool SPLIT> __global__ __launch_bounds__(256) void attn_seq_fwd_kernel(AttnSeqArgs a) {
-    constexpr int NC = DP / 16, ND = DP / 32, KT = BK / 32, NR = InRegs<T, DP>::value ? NC : 1;
-    __shared__ __attribute__((aligned(16))) T sk[BK * DP];
-    __shared__ __attribute__((aligned(16))) T sv[BK * DP];
+template <typename T, int DP, int BK, bool SPLIT> __global__ __launch_bounds__(256, (DP * sizeof(T) <= 512 ? 2 : 1)) void attn_seq_fwd_kernel(AttnSeqArgs a) {
+    constexpr int NC = DP / 16, ND = DP / 32, KT = BK / 32, NR = InRegs<T, DP>::value ? NC : 1, ES = sizeof(T);
+    __shared__ __attribute__((aligned(16))) T sk[2][BK * DP];
+    __shared__ __attribute__((aligned(16))) T sv[2][BK * DP];
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int tiles_r = (a.R + ATTN_SEQ_BLOCK - 1) / ATTN_SEQ_BLOCK;
+    const int tiles_r = (a.R + ATTN_SEQ_BLOCK - 1) / ATTN_SEQ_BLOCK, heads = a.Hkv * a.B;
     int id = blockIdx.x;
     const int split = SPLIT ? id % a.splits : 0;
     if (SPLIT) id /= a.splits;
     // the last rows, which see the most keys, first
-    const int rt = tiles_r - 1 - id % tiles_r, hk = id / tiles_r % a.Hkv, b = id / tiles_r / a.Hkv;
+    const int rt = tiles_r - 1 - id / heads, hk = id % heads % a.Hkv, b = id % heads / a.Hkv;
     const int r0 = rt * ATTN_SEQ_BLOCK + wave * 32, r = r0 + (lane & 31);
     const bool row_ok = r < a.R;
     const int qi = row_ok ? r / a.group : 0, qh = hk * a.group + (row_ok ? r - qi * a.group : 0);
@@ -29,9 +29,10 @@ template <typename T, int DP, int BK, bool SPLIT> __global__ __launch_bounds__(2
 
     const int last = min(rt * ATTN_SEQ_BLOCK + ATTN_SEQ_BLOCK, a.R) - 1;
     const int k_end = a.causal ? min(a.Tk, last / a.group + a.off + 1) : a.Tk;  // keys any row of the workgroup may see
-    const int w_last = min(r0 + 31, a.R - 1);
+    const int w_first = min(r0, a.R - 1), w_last = min(r0 + 31, a.R - 1);
     const int w_end = r0 < a.R ? (a.causal ? min(a.Tk, w_last / a.group + a.off + 1) : a.Tk) : 0;  // any row of the wave
-    const int lim = a.causal ? qi + a.off : a.Tk - 1;  // last key this lane's row sees
+    const int w_all = a.causal ? w_first / a.group + a.off : a.Tk - 1;                             // last key every row of the wave sees
+    const int lim = a.causal ? qi + a.off : a.Tk - 1;                                              // last key this lane's row sees
     int t0 = 0, t1 = k_end > 0 ? (k_end + BK - 1) / BK : 0;
     if (SPLIT) {
         t0 = split * a.tiles_per_split;
@@ -43,59 +44,89 @@ template <typename T, int DP, int BK, bool SPLIT> __global__ __launch_bounds__(2
     float m = -INFINITY, l = 0.f;
     const T* kb = (const T*)a.k + b * a.k_sb + hk * a.k_sh;
     const T* vb = (const T*)a.v + b * a.v_sb + hk * a.v_sh;
+    const unsigned k_row = (unsigned)(a.k_st * ES), v_row = (unsigned)(a.v_st * ES), lds_k = lds_address(sk), lds_v = lds_address(sv);
+    // rows no query may see are zeros: whatever they hold, infinities and NaN included, stays out of the products
+    auto request = [&](int t, int buf, const unsigned (&seen)[KT]) {
+        auto row = [&](unsigned stride) {
+            return [&, stride](int x) { return (seen[x >> 5] >> (x & 31)) & 1 ? x * stride : 0x80000000u; };
+        };
+        request_tile<T, DP, BK>(kb + (long long)t * BK * a.k_st, lds_k + buf * BK * DP * ES, a.D, wave, lane, row(k_row));
+        request_tile<T, DP, BK>(vb + (long long)t * BK * a.v_st, lds_v + buf * BK * DP * ES, a.D, wave, lane, row(v_row));
+    };
+    unsigned bits[KT], next[KT];
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+        bits[kt] = key_bits(a, b, t0 * BK + kt * 32, lane);
+        next[kt] = key_bits(a, b, (t0 + 1) * BK + kt * 32, lane);
+    }
+    if (t0 < t1) request(t0, 0, bits);
     for (int t = t0; t < t1; ++t) {
-        const int k0 = t * BK;
-        __syncthreads();
-        // rows no query may see are zeros: whatever they hold, infinities and NaN included, stays out of the products
-        stage<T, DP, BK, 256>(sk, a.D, [&](int x) { return key_seen(a, b, k0 + x) ? kb + (long long)(k0 + x) * a.k_st : nullptr; });
-        stage<T, DP, BK, 256>(sv, a.D, [&](int x) { return key_seen(a, b, k0 + x) ? vb + (long long)(k0 + x) * a.v_st : nullptr; });
-        __syncthreads();
-        f32x16_t s[KT];
-        float top = -INFINITY;
+        const int k0 = t * BK, cur = (t - t0) & 1;
+        tile_landed();
+        if (t + 1 < t1) request(t + 1, cur ^ 1, next);
+        bool ok[KT];  // the tile after the next
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-            s[kt] = f32x16_t{};
-            if (k0 + kt * 32 >= w_end) continue;
+        for (int kt = 0; kt < KT; ++kt) ok[kt] = key_seen(a, b, k0 + 2 * BK + kt * 32 + (lane & 31));
+        if (k0 < w_end) {
+            f32x16_t s[KT];
+            float top = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < NC; ++c)
-                mma32(read_row<DP>(sk, kt * 32 + (lane & 31), c, h), InRegs<T, DP>::value ? qf[c % NR] : load_frag<T>(qrow, 16 * c + 8 * h, a.D), s[kt]);
-            const unsigned bits = key_bits(a, b, k0 + kt * 32, lane) >> (4 * h);
+            for (int kt = 0; kt < KT; ++kt) {
+                s[kt] = f32x16_t{};
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int j = 8 * (e >> 2) + (e & 3);
-                const bool seen = ((bits >> j) & 1) && k0 + kt * 32 + 4 * h + j <= lim;
-                s[kt][e] = seen ? s[kt][e] * a.scale_log2 : -INFINITY;
-                top = fmaxf(top, s[kt][e]);
+                for (int c = 0; c < NC; ++c)
+                    mma32(read_row<DP>(sk[cur], kt * 32 + (lane & 31), c, h), InRegs<T, DP>::value ? qf[c % NR] : load_frag<T>(qrow, 16 * c + 8 * h, a.D), s[kt]);
+                if (bits[kt] == 0xffffffffu && k0 + kt * 32 + 31 <= w_all) {  // nothing hidden: the common case
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        s[kt][e] *= a.scale_log2;
+                        top = fmaxf(top, s[kt][e]);
+                    }
+                } else {
+                    const unsigned mine = bits[kt] >> (4 * h);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int j = 8 * (e >> 2) + (e & 3);
+                        const bool seen = ((mine >> j) & 1) && k0 + kt * 32 + 4 * h + j <= lim;
+                        s[kt][e] = seen ? s[kt][e] * a.scale_log2 : -INFINITY;
+                        top = fmaxf(top, s[kt][e]);
+                    }
+                }
             }
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float m_new = fmaxf(m, top), m_use = m_new == -INFINITY ? 0.f : m_new;
+            float sum = 0.f;
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    s[kt][e] = __builtin_amdgcn_exp2f(s[kt][e] - m_use);
+                    sum += s[kt][e];
+                }
+            sum += __shfl_xor(sum, 32, 64);
+            if (__any(m_new > m)) {  // some row's maximum rose
+                const float alpha = __builtin_amdgcn_exp2f(m - m_use);
+                l *= alpha;
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) acc[d][e] *= alpha;
+            }
+            m = m_new;
+            l += sum;
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const Frag8<T> p = frag_of<T>(s[kt], j);  // bf16: the probabilities are rounded for the product, the sum l is not
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) mma32(read_col<DP>(sv[cur], d * 32, kt * 32 + 16 * j, lane), p, acc[d]);
+                }
         }
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float m_new = fmaxf(m, top), m_use = m_new == -INFINITY ? 0.f : m_new;
-        const float alpha = __builtin_amdgcn_exp2f(m - m_use);
-        m = m_new;
-        float sum = 0.f;
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) {
-            if (k0 + kt * 32 >= w_end) continue;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                s[kt][e] = __builtin_amdgcn_exp2f(s[kt][e] - m_use);
-                sum += s[kt][e];
-            }
-        }
-        l = l * alpha + sum + __shfl_xor(sum, 32, 64);
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[d][e] *= alpha;
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-            if (k0 + kt * 32 >= w_end) continue;
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const Frag8<T> p = frag_of<T>(s[kt], j);  // bf16: the probabilities are rounded for the product, the sum l is not
-#pragma unroll
-                for (int d = 0; d < ND; ++d) mma32(read_col<DP>(sv, d * 32, kt * 32 + 16 * j, lane), p, acc[d]);
-            }
+            bits[kt] = next[kt];
+            next[kt] = (unsigned)__ballot(ok[kt]);
         }
     }
     if (!row_ok) return;

@@ -10,6 +10,7 @@
 // operand is too long; an index outside the operand or a k past the end is bit 31 of the offset, which returns zeros without
 // touching memory.
 #pragma once
+#include "attn_seq.h"
 #include "igemm_shared.h"
 
 namespace {
@@ -28,15 +29,6 @@ struct Gemm8Shape {
     int rows_are_k;
     int K, tiles_p, tiles_q;
 };
-
-typedef unsigned srd_t __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ void request16(unsigned voff, const srd_t& srd, unsigned lds) {
-    unsigned keep;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
-                 : "=&s"(keep)
-                 : "v"(voff), "s"(lds), "s"(srd)
-                 : "memory");
-}
 
 constexpr unsigned G8_HALF = 16384, G8_TILE = 4 * G8_HALF, G8_DEAD = 0x80000000u;
 constexpr unsigned G8_Q0 = 0, G8_P0 = G8_HALF, G8_P1 = 2 * G8_HALF, G8_Q1 = 3 * G8_HALF;
