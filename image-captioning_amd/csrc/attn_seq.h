@@ -114,6 +114,78 @@ template <int DP> __device__ __forceinline__ Frag8<float> read_col(const float* 
     return f;
 }
 
+// The same reads with a lane's addresses computed once.  The swizzle mixes a few low bits of the chunk number with bits of the row
+// that depend on the lane alone, so a handful of registers serve every step, column tile and row tile: what differs otherwise is
+// a constant, which the instruction carries.  `tile` is the tile's byte offset in `smem`, a constant too.
+typedef __attribute__((address_space(3))) const unsigned char* lds_bytes_t;
+template <typename T, int DP> struct TileReader;
+template <int DP> struct TileReader<bf16_t, DP> {
+    static constexpr int NR = DP / 16 < 8 ? DP / 16 : 8, NCOL = DP / 32 < 4 ? DP / 32 : 4;
+    unsigned row[NR], col[NCOL][2];
+    __device__ __forceinline__ void init(int lane) {
+        const int h = lane >> 5, j = lane & 15;
+#pragma unroll
+        for (int c = 0; c < NR; ++c) row[c] = (unsigned)Tile<bf16_t, DP>::at(lane & 31, 2 * c + h) * 2u;
+#pragma unroll
+        for (int d = 0; d < NCOL; ++d)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const int c = d * 32 + ((lane >> 4) & 1) * 16 + (j & 3) * 4;
+                col[d][s] = (unsigned)(Tile<bf16_t, DP>::at(4 * h + (j >> 2) + 8 * s, c >> 3) + (c & 7)) * 2u;
+            }
+    }
+    __device__ __forceinline__ Frag8<bf16_t> rows(lds_bytes_t smem, int tile, int c) const {
+        typedef __attribute__((address_space(3))) const bf16x8_t* p_t;
+        Frag8<bf16_t> f;
+        f.v = *(p_t)(smem + row[c % NR] + (tile + c / NR * 256));
+        return f;
+    }
+    __device__ __forceinline__ Frag8<bf16_t> cols(lds_bytes_t smem, int tile, int d, int r0) const {
+        typedef __attribute__((address_space(3))) v4i16_t* p_t;
+        const int k = tile + r0 * DP * 2 + d / NCOL * 256;
+        const v4i16_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p_t)(smem + col[d % NCOL][0] + k));
+        const v4i16_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p_t)(smem + col[d % NCOL][1] + k));
+        typedef short v8i16_t __attribute__((ext_vector_type(8)));
+        Frag8<bf16_t> f;
+        f.v = __builtin_bit_cast(bf16x8_t, (v8i16_t)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        return f;
+    }
+};
+template <int DP> struct TileReader<float, DP> {
+    static constexpr int NR = DP / 16 < 4 ? DP / 16 : 4, NCOL = DP / 32 < 2 ? DP / 32 : 2;
+    unsigned row[NR][2], col[NCOL][8];
+    __device__ __forceinline__ void init(int lane) {
+        const int h = lane >> 5;
+#pragma unroll
+        for (int c = 0; c < NR; ++c)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) row[c][k] = (unsigned)Tile<float, DP>::at(lane & 31, 4 * c + 2 * h + k) * 4u;
+#pragma unroll
+        for (int d = 0; d < NCOL; ++d)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int c = d * 32 + (lane & 31);
+                col[d][e] = (unsigned)(Tile<float, DP>::at(4 * h + (e & 3) + (e >> 2) * 8, c >> 2) + (c & 3)) * 4u;
+            }
+    }
+    __device__ __forceinline__ Frag8<float> rows(lds_bytes_t smem, int tile, int c) const {
+        Frag8<float> f;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const f32x4_t x = *(__attribute__((address_space(3))) const f32x4_t*)(smem + row[c % NR][k] + (tile + c / NR * 256));
+            f.v[4 * k] = x[0]; f.v[4 * k + 1] = x[1]; f.v[4 * k + 2] = x[2]; f.v[4 * k + 3] = x[3];
+        }
+        return f;
+    }
+    __device__ __forceinline__ Frag8<float> cols(lds_bytes_t smem, int tile, int d, int r0) const {
+        typedef __attribute__((address_space(3))) const float* p_t;
+        Frag8<float> f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f.v[e] = *(p_t)(smem + col[d % NCOL][e] + (tile + r0 * DP * 4 + d / NCOL * 256));
+        return f;
+    }
+};
+
 // fp32 with more than 128 columns: the wave's own operands do not fit the registers next to the sums, they are read again for
 // every tile
 template <typename T, int DP> struct InRegs {

@@ -64,7 +64,7 @@ constexpr int SHORT_KEYS = 64;
 bool short_grad(const AttnSeqArgs& a) { return a.Tk > 0 && a.Tk <= SHORT_KEYS; }
 bool short_fwd(const AttnSeqArgs& a) { return short_grad(a) && (a.R <= 128 || (long long)a.B * a.Hkv * a.R < 256 * 128); }
 
-// The forward shares the keys of a row tile out over workgroups when there are fewer row tiles than compute units: one tile of keys
+// The forward shares the keys of a row tile out over workgroups when row tiles leave a third of the compute units idle: one tile of keys
 // per workgroup at least, 512 workgroups at most.
 void split_keys(AttnSeqArgs& a, int dtype) {
     const int BK = head_columns(a.D) * (int)mic_dtype_size(dtype) <= 256 ? 64 : 32;
@@ -72,8 +72,8 @@ void split_keys(AttnSeqArgs& a, int dtype) {
     const int tiles = (a.Tk + BK - 1) / BK;
     a.splits = 1;
     a.tiles_per_split = tiles;
-    if (short_fwd(a) || base == 0 || base >= 256 || tiles < 4) return;
-    const int want = (int)((512 + base - 1) / base);
+    if (short_fwd(a) || base == 0 || base >= 160 || tiles < 4) return;
+    const int want = (int)((512 + base - 1) / base);  // at most 512: the join's table
     const int s = want < tiles ? want : tiles;
     a.tiles_per_split = (tiles + s - 1) / s;
     a.splits = (tiles + a.tiles_per_split - 1) / a.tiles_per_split;

@@ -1,17 +1,22 @@
 // Whole-sequence attention, gradients of the keys and values:
 //   dv = P^T g     dk = scale * dS^T q     over all rows (queries of every head of the group) that see the key
-// A wave owns 32 keys: their k and v stay in registers as B operands, S = Q K^T and dP = G V^T come out with a lane per key, and P
-// and dS are the B operands of dV^T = G^T P and dK^T = Q^T dS.  The workgroup's four waves walk the same tiles of 32 rows.
+// A wave owns 32 keys: their k stay in registers as B operands and their v in LDS (the registers are full with dK and dV), S = Q K^T
+// and dP = G V^T come out with a lane per key, and P and dS are the B operands of dV^T = G^T P and dK^T = Q^T dS.  The workgroup's
+// four waves walk the same tiles of 32 rows.
 // With `splits` the rows are shared out over several workgroups, which leave fp32 partial sums that a second launch adds in order.
 #include "attn_seq.h"
+
+#include <type_traits>
 
 namespace {
 
 template <typename T, int DP, bool SPLIT> __global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void attn_seq_dkv_kernel(AttnSeqArgs a) {
-    constexpr int NC = DP / 16, ND = DP / 32, NR = InRegs<T, DP>::value ? NC : 1, ES = sizeof(T);
-    __shared__ __attribute__((aligned(16))) T sq[2][32 * DP];
-    __shared__ __attribute__((aligned(16))) T sg[2][32 * DP];
+    constexpr int NC = DP / 16, ND = DP / 32, ES = sizeof(T);
+    constexpr bool KEEP = InRegs<T, DP>::value;  // else k and v are read from memory for every tile
+    constexpr int TILE = 32 * DP * ES, OFF_Q = 0, OFF_G = 2 * TILE, OFF_V = 4 * TILE;  // two tiles of q, two of g, the four waves' v
+    __shared__ __attribute__((aligned(16))) unsigned char smem[4 * TILE + (KEEP ? 4 * TILE : 0)];
     __shared__ __attribute__((aligned(16))) float s_lse[2][32], s_delta[2][32];
+    const lds_bytes_t lds = (lds_bytes_t)smem;
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int heads = a.Hkv * a.B;
     int id = blockIdx.x;
@@ -22,12 +27,24 @@ template <typename T, int DP, bool SPLIT> __global__ __launch_bounds__(256, (DP 
     const bool seen = key_seen(a, b, key);
     const T* krow = seen ? (const T*)a.k + b * a.k_sb + hk * a.k_sh + (long long)key * a.k_st : nullptr;
     const T* vrow = seen ? (const T*)a.v + b * a.v_sb + hk * a.v_sh + (long long)key * a.v_st : nullptr;
-    Frag8<T> kf[NR], vf[NR];
-    if constexpr (InRegs<T, DP>::value) {
+    TileReader<T, DP> read;
+    read.init(lane);
+    Frag8<T> kf[KEEP ? NC : 1];
+    if constexpr (KEEP) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) kf[c] = load_frag<T>(krow, 16 * c + 8 * h, a.D);
+        T* sv = reinterpret_cast<T*>(smem + OFF_V) + wave * 32 * DP;  // rows hidden keys would have are zeros
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            kf[c] = load_frag<T>(krow, 16 * c + 8 * h, a.D);
-            vf[c] = load_frag<T>(vrow, 16 * c + 8 * h, a.D);
+            const Frag8<T> v = load_frag<T>(vrow, 16 * c + 8 * h, a.D);
+            constexpr int E = Tile<T, DP>::E;
+#pragma unroll
+            for (int k = 0; k < 8 / E; ++k) {
+                Vec16<T> x;
+#pragma unroll
+                for (int e = 0; e < E; ++e) x.v[e] = v.v[k * E + e];
+                st16(sv + Tile<T, DP>::at(lane & 31, (16 * c + 8 * h) / E + k), x);
+            }
         }
     }
     // rows below `first` see no key of the workgroup, below w_first none of the wave; from w_all on they see every key of the wave
@@ -43,7 +60,7 @@ template <typename T, int DP, bool SPLIT> __global__ __launch_bounds__(256, (DP 
         t0 = t0 + (int)((long long)n * split / a.splits);
     }
     const unsigned q_row = (unsigned)(a.q_st * ES), q_head = (unsigned)(a.q_sh * ES), g_row = (unsigned)(a.g_st * ES), g_head = (unsigned)(a.g_sh * ES);
-    const unsigned lds_q = lds_address(sq), lds_g = lds_address(sg);
+    const unsigned lds0 = lds_address(smem);
     const T* qb = (const T*)a.q + b * a.q_sb + hk * a.group * a.q_sh;
     const T* gb = (const T*)a.g + b * a.g_sb + hk * a.group * a.g_sh;
     auto request = [&](int t, int buf) {
@@ -54,8 +71,8 @@ template <typename T, int DP, bool SPLIT> __global__ __launch_bounds__(256, (DP 
                 return r0 + x < a.R ? i * per_row + (y - i * a.group) * per_head : 0x80000000u;
             };
         };
-        request_tile<T, DP, 32>(qb + (long long)i0 * a.q_st, lds_q + buf * 32 * DP * ES, a.D, wave, lane, row(q_row, q_head));
-        request_tile<T, DP, 32>(gb + (long long)i0 * a.g_st, lds_g + buf * 32 * DP * ES, a.D, wave, lane, row(g_row, g_head));
+        request_tile<T, DP, 32>(qb + (long long)i0 * a.q_st, lds0 + OFF_Q + buf * TILE, a.D, wave, lane, row(q_row, q_head));
+        request_tile<T, DP, 32>(gb + (long long)i0 * a.g_st, lds0 + OFF_G + buf * TILE, a.D, wave, lane, row(g_row, g_head));
     };
     // lse and delta of a tile's rows: 32 threads, loaded a tile ahead
     float lse2 = INFINITY, delta = 0.f;
@@ -84,29 +101,32 @@ template <typename T, int DP, bool SPLIT> __global__ __launch_bounds__(256, (DP 
         load_stats(t0);
         put_stats(0);
     }
-    for (int t = t0; t < t1; ++t) {
-        const int r0 = t * 32, cur = (t - t0) & 1;
+    // one tile out of buffer CUR
+    auto step = [&](auto which, int t) {
+        constexpr int CUR = decltype(which)::value;
+        const int r0 = t * 32;
         tile_landed();
         if (t + 1 < t1) {
-            request(t + 1, cur ^ 1);
+            request(t + 1, CUR ^ 1);
             load_stats(t + 1);
         }
         if (k0 < a.Tk && r0 + 31 >= w_first) {
             f32x16_t s = f32x16_t{}, dp = f32x16_t{};
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-                if constexpr (InRegs<T, DP>::value) {
-                    mma32(read_row<DP>(sq[cur], lane & 31, c, h), kf[c], s);
-                    mma32(read_row<DP>(sg[cur], lane & 31, c, h), vf[c], dp);
+                const Frag8<T> q = read.rows(lds, OFF_Q + CUR * TILE, c), g = read.rows(lds, OFF_G + CUR * TILE, c);
+                if constexpr (KEEP) {
+                    mma32(q, kf[c], s);
+                    mma32(g, read.rows(lds + wave * TILE, OFF_V, c), dp);
                 } else {
-                    mma32(read_row<DP>(sq[cur], lane & 31, c, h), load_frag<T>(krow, 16 * c + 8 * h, a.D), s);
-                    mma32(read_row<DP>(sg[cur], lane & 31, c, h), load_frag<T>(vrow, 16 * c + 8 * h, a.D), dp);
+                    mma32(q, load_frag<T>(krow, 16 * c + 8 * h, a.D), s);
+                    mma32(g, load_frag<T>(vrow, 16 * c + 8 * h, a.D), dp);
                 }
             }
             const bool whole = all_seen && r0 >= w_all;  // nothing hidden: the common case
 #pragma unroll
             for (int e4 = 0; e4 < 4; ++e4) {
-                const float4 l4 = *reinterpret_cast<const float4*>(&s_lse[cur][8 * e4 + 4 * h]), d4 = *reinterpret_cast<const float4*>(&s_delta[cur][8 * e4 + 4 * h]);
+                const float4 l4 = *reinterpret_cast<const float4*>(&s_lse[CUR][8 * e4 + 4 * h]), d4 = *reinterpret_cast<const float4*>(&s_delta[CUR][8 * e4 + 4 * h]);
                 const float ls[4] = {l4.x, l4.y, l4.z, l4.w}, ds[4] = {d4.x, d4.y, d4.z, d4.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -117,17 +137,25 @@ template <typename T, int DP, bool SPLIT> __global__ __launch_bounds__(256, (DP 
                     dp[e] = ok ? p * (dp[e] - ds[i]) : 0.f;
                 }
             }
+            Frag8<T> p[2], ds[2];  // bf16: rounded for the products
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const Frag8<T> p = frag_of<T>(s, j), ds = frag_of<T>(dp, j);  // bf16: rounded for the products
+                p[j] = frag_of<T>(s, j);
+                ds[j] = frag_of<T>(dp, j);
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
-                    mma32(read_col<DP>(sg[cur], d * 32, 16 * j, lane), p, dv[d]);
-                    mma32(read_col<DP>(sq[cur], d * 32, 16 * j, lane), ds, dk[d]);
+                    mma32(read.cols(lds, OFF_G + CUR * TILE, d, 16 * j), p[j], dv[d]);
+                    mma32(read.cols(lds, OFF_Q + CUR * TILE, d, 16 * j), ds[j], dk[d]);
                 }
-            }
         }
-        if (t + 1 < t1) put_stats(cur ^ 1);
+        if (t + 1 < t1) put_stats(CUR ^ 1);
+    };
+    for (int t = t0; t < t1; t += 2) {
+        step(std::integral_constant<int, 0>{}, t);
+        if (t + 1 < t1) step(std::integral_constant<int, 1>{}, t + 1);
     }
     if (key >= a.Tk) return;
     const long long at = (((long long)b * a.Tk + key) * a.Hkv + hk) * a.D, all = (long long)a.B * a.Tk * a.Hkv * a.D;

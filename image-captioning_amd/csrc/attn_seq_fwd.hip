@@ -158,28 +158,43 @@ template <typename T, int DP, int BK, bool SPLIT> __global__ __launch_bounds__(2
     if (h == 0) a.lse[((long long)b * a.Hq + qh) * a.Tq + qi] = l == 0.f ? -INFINITY : (m + log2f(l)) * ATTN_LN2;
 }
 
-// joins the key ranges of a row: one wave per row
+// Joins the key ranges of a row: a workgroup per row.  The weight of every range first (a lane each), then each wave adds a quarter of the
+// ranges, all of whose loads are independent, and the waves' sums are added in order.
 template <typename T> __global__ __launch_bounds__(256) void attn_seq_join_kernel(AttnSeqArgs a) {
-    const int lane = threadIdx.x & 63;
-    const long long rows = (long long)a.B * a.Hkv * a.R, row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= rows) return;
-    float m = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[2 * (s * rows + row)]);
+    __shared__ float weight[512], part[4][256];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long long rows = (long long)a.B * a.Hkv * a.R, row = blockIdx.x;
+    float m = -INFINITY;  // every wave looks at all ranges
+    for (int s = lane; s < a.splits; s += 64) m = fmaxf(m, a.part_ml[2 * (s * rows + row)]);
+    m = wave_max(m);
     const float m_use = m == -INFINITY ? 0.f : m;
-    float l = 0.f, acc[4] = {};
-    const int col = lane * 4;
-    for (int s = 0; s < a.splits; ++s) {
+    float l = 0.f;
+    for (int s = lane; s < a.splits; s += 64) {
         const float w = __builtin_amdgcn_exp2f(a.part_ml[2 * (s * rows + row)] - m_use);
+        if (wave == 0) weight[s] = w;
         l += w * a.part_ml[2 * (s * rows + row) + 1];
-        if (col < a.D) {
+    }
+    l = wave_sum(l);
+    __syncthreads();
+    const int col = lane * 4, s0 = a.splits * wave / 4, s1 = a.splits * (wave + 1) / 4;
+    float acc[4] = {};
+    if (col < a.D)
+#pragma unroll 8
+        for (int s = s0; s < s1; ++s) {
             const float4 x = *reinterpret_cast<const float4*>(a.part + (s * rows + row) * a.D + col);
+            const float w = weight[s];
             acc[0] += w * x.x; acc[1] += w * x.y; acc[2] += w * x.z; acc[3] += w * x.w;
         }
-    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) part[wave][col + e] = acc[e];
+    __syncthreads();
+    if (wave) return;
     const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] = ((part[0][col + e] + part[1][col + e]) + part[2][col + e] + part[3][col + e]) * inv;
     const int r = (int)(row % a.R), hk = (int)(row / a.R % a.Hkv), qi = r / a.group, qh = hk * a.group + r - qi * a.group;
     const long long b = row / a.R / a.Hkv;
-    if (col < a.D) store4<T>((T*)a.o + b * a.o_sb + qi * a.o_st + qh * a.o_sh + col, acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+    if (col < a.D) store4<T>((T*)a.o + b * a.o_sb + qi * a.o_st + qh * a.o_sh + col, acc[0], acc[1], acc[2], acc[3]);
     if (lane == 0) a.lse[(b * a.Hq + qh) * a.Tq + qi] = l == 0.f ? -INFINITY : (m + log2f(l)) * ATTN_LN2;
 }
 
@@ -189,7 +204,7 @@ template <typename T, int DP> int launch(const AttnSeqArgs& a, hipStream_t s) {
     if (a.splits > 1) {
         MIC_LAUNCH((attn_seq_fwd_kernel<T, DP, BK, true>), dim3((unsigned)(blocks * a.splits)), dim3(256), 0, s, a);
         const long long rows = (long long)a.B * a.Hkv * a.R;
-        MIC_LAUNCH((attn_seq_join_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
+        MIC_LAUNCH((attn_seq_join_kernel<T>), dim3((unsigned)rows), dim3(256), 0, s, a);
     } else {
         MIC_LAUNCH((attn_seq_fwd_kernel<T, DP, BK, false>), dim3((unsigned)blocks), dim3(256), 0, s, a);
     }

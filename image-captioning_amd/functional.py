@@ -202,7 +202,8 @@ def _attn_workspace_bytes(code, B, Tq, Tk, Hq, Hkv, D, grad) -> int:
 
 def _heads(t: torch.Tensor):
     """The tensor, its address and its strides of (batch, position, head), copied if the kernels cannot read it in place (columns
-    consecutive, everything on 16-byte boundaries).  A dimension of one entry has no stride to speak of."""
+    consecutive, everything on 16-byte boundaries, 64 positions and the heads of one within 1 GiB).  A dimension of one entry has no
+    stride to speak of."""
     e = 16 // t.element_size()
     B, T, H, D = t.shape
     p = t.data_ptr()
@@ -213,7 +214,7 @@ def _heads(t: torch.Tensor):
         st = 0
     if H == 1:
         sh = 0
-    if not (sb % e or st % e or sh % e or p % 16) and (sd == 1 or D == 1):
+    if not (sb % e or st % e or sh % e or p % 16) and (sd == 1 or D == 1) and st <= e << 20 and sh * H <= e << 26:
         return t, p, (sb, st, sh)
     t = t.clone(memory_format=torch.contiguous_format)
     return t, t.data_ptr(), (T * H * D, H * D, D)

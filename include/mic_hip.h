@@ -525,7 +525,7 @@ int mic_embed_grad(const void* ids, int ids_bits, const void* g, void* d_table, 
  * whatever k and v hold there (infinities and NaN included); k and v of every other key must be finite, also where causality
  * hides them from some rows.
  * q, o, grad_o [B][Tq][Hq][D], k, v [B][Tk][Hkv][D] of dtype, addressed by element strides (batch, position, head), the D columns of
- * a head consecutive; pointers and strides multiples of 16 bytes.  lse fp32 [B][Hq][Tq]; key_mask bytes [B][mask_stride].  The
+ * a head consecutive; pointers and strides multiples of 16 bytes, 64 positions and the heads of one position within 1 GiB.  lse fp32 [B][Hq][Tq]; key_mask bytes [B][mask_stride].  The
  * gradients dq [B][Tq][Hq][D], dk, dv [B][Tk][Hkv][D] are written whole and contiguous.  D <= 256, D * element size a multiple of 16 bytes.
  * bf16: scores, statistics and sums in fp32; probabilities and their gradients are rounded to bf16 for the second products only.
  * Sizes of zero are allowed.  mic_attn_seq_workspace_bytes(d, grad) looks at dtype and sizes alone (an argument error is negative). */

@@ -113,6 +113,10 @@ def test_attn_seq_refuses(L):
             refused(L, f(C.byref(d), None), b"stride")
             getattr(d, s)[1] = -64
             refused(L, f(C.byref(d), None), b"stride")
+        for i, far in ((1, (1 << 23) + 8), (2, 1 << 29)):  # 64 positions, the heads of one, beyond 1 GiB
+            d = attn_desc(L)
+            d.k_stride[i] = far if i == 1 else far + 8
+            refused(L, f(C.byref(d), None), b"too large")
     for n in ("dq", "dk", "dv"):
         refused(L, L.lib.mic_attn_seq_grad(C.byref(attn_desc(L, **{n: None})), None), b"null pointer")
     refused(L, L.lib.mic_attn_seq_grad(C.byref(attn_desc(L, dv=P + 4)), None), b"aligned")
