@@ -240,7 +240,8 @@ template <typename T, int DP, int ROWS, int THREADS, typename P> __device__ __fo
 typedef unsigned srd_t __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ srd_t make_srd(const void* p) {
     const unsigned long long a = (unsigned long long)p;
-    return srd_t{(unsigned)a, (unsigned)(a >> 32) & 0xffffu, 0x80000000u, 0x00020000u};
+    // the same in every lane, but perhaps computed in vector registers
+    return srd_t{(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)a), (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(a >> 32)) & 0xffffu, 0x80000000u, 0x00020000u};
 }
 __device__ __forceinline__ void request16(unsigned voff, const srd_t& srd, unsigned lds) {
     unsigned keep;

@@ -63,12 +63,15 @@ template <typename T, int DP, bool SPLIT> __global__ __launch_bounds__(256, (DP 
     const unsigned lds0 = lds_address(smem);
     const T* qb = (const T*)a.q + b * a.q_sb + hk * a.group * a.q_sh;
     const T* gb = (const T*)a.g + b * a.g_sb + hk * a.group * a.g_sh;
+    const bool even = 32 % a.group == 0;  // every tile then begins with a query's first head, and a lane's offsets never change
+    const int step_i = 32 / a.group;
     auto request = [&](int t, int buf) {
-        const int r0 = t * 32, i0 = r0 / a.group, rest = r0 - i0 * a.group;
+        const int r0 = t * 32, i0 = even ? t * step_i : r0 / a.group, rest = even ? 0 : r0 - i0 * a.group;
+        const bool whole = r0 + 32 <= a.R;
         auto row = [&](unsigned per_row, unsigned per_head) {
             return [&, per_row, per_head](int x) {
                 const unsigned y = rest + x, i = by_group(a, y);
-                return r0 + x < a.R ? i * per_row + (y - i * a.group) * per_head : 0x80000000u;
+                return whole || r0 + x < a.R ? i * per_row + (y - i * a.group) * per_head : 0x80000000u;
             };
         };
         request_tile<T, DP, 32>(qb + (long long)i0 * a.q_st, lds0 + OFF_Q + buf * TILE, a.D, wave, lane, row(q_row, q_head));
@@ -123,7 +126,6 @@ template <typename T, int DP, bool SPLIT> __global__ __launch_bounds__(256, (DP 
                     mma32(g, load_frag<T>(vrow, 16 * c + 8 * h, a.D), dp);
                 }
             }
-            const bool whole = all_seen && r0 >= w_all;  // nothing hidden: the common case
 #pragma unroll
             for (int e4 = 0; e4 < 4; ++e4) {
                 const float4 l4 = *reinterpret_cast<const float4*>(&s_lse[CUR][8 * e4 + 4 * h]), d4 = *reinterpret_cast<const float4*>(&s_delta[CUR][8 * e4 + 4 * h]);
@@ -131,12 +133,17 @@ template <typename T, int DP, bool SPLIT> __global__ __launch_bounds__(256, (DP 
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int e = 4 * e4 + i;
-                    const bool ok = whole || r0 + 8 * e4 + 4 * h + i >= from;
-                    const float p = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2, -ls[i]));
-                    s[e] = ok ? p : 0.f;
-                    dp[e] = ok ? p * (dp[e] - ds[i]) : 0.f;
+                    s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2, -ls[i]));
+                    dp[e] = s[e] * (dp[e] - ds[i]);
                 }
             }
+            if (!(all_seen && r0 >= w_all))  // something is hidden
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const bool ok = r0 + 8 * (e >> 2) + 4 * h + (e & 3) >= from;
+                    s[e] = ok ? s[e] : 0.f;
+                    dp[e] = ok ? dp[e] : 0.f;
+                }
             Frag8<T> p[2], ds[2];  // bf16: rounded for the products
 #pragma unroll
             for (int j = 0; j < 2; ++j) {

@@ -133,10 +133,19 @@ template <typename T, bool PCOL, bool QCOL, typename Epi> __global__ __launch_bo
                 a[i] = TP::frag(sp[cur], wp * 64 + i * 32, s, lane);
                 b[i] = TQ::frag(sq[cur], wq * 64 + i * 32, s, lane);
             }
+            if constexpr (sizeof(T) == 4) {  // the four sums in turn: no product waits for the one before
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+                for (int e = 0; e < 8; ++e)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) mma32(a[i], b[j], acc[i][j]);
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i].v[e], b[j].v[e], acc[i][j], 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) mma32(a[i], b[j], acc[i][j]);
+            }
         }
         if (t + 1 < ke) {
             fp.put(sp[cur ^ 1]);
