@@ -247,7 +247,7 @@ __device__ __forceinline__ void request16(unsigned voff, const srd_t& srd, unsig
     unsigned keep;
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
                  : "=&s"(keep)
-                 : "v"(voff), "s"(lds), "s"(srd)
+                 : "v"(voff), "s"(__builtin_amdgcn_readfirstlane((int)lds)), "s"(srd)
                  : "memory");
 }
 typedef __attribute__((address_space(3))) void* lds_ptr_t;

@@ -6,6 +6,9 @@
 //  * row operand (k consecutive in memory): two planes of 128 rows x 64 bytes, read with ds_read_b128, as in igemm8.hip;
 //  * column operand (index consecutive): 64 rows of k x 256 bytes, read with transposing reads.  16-byte chunk c of row k is stored at
 //    chunk c ^ 2f, f = (k & 3) | (k >> 3 & 1) << 2: the 8 rows x 2 chunks that half a wave reads at once are 16 different chunks.
+// A workgroup stays and takes every 256th tile: the next tile's first requests are under way while the epilogue of the last one
+// computes (epilogues leave LDS alone; what they need of bias and rows is put into a small side buffer beforehand).  With H = 512 a
+// tile is 13 us of products, and its start and end used to cost 17 us more.
 // Requests go straight to LDS through a buffer descriptor whose base is the K-tile's, so a lane's offset never changes and no
 // operand is too long; an index outside the operand or a k past the end is bit 31 of the offset, which returns zeros without
 // touching memory.
@@ -32,8 +35,7 @@ struct Gemm8Shape {
 
 constexpr unsigned G8_HALF = 16384, G8_TILE = 4 * G8_HALF, G8_DEAD = 0x80000000u;
 constexpr unsigned G8_Q0 = 0, G8_P0 = G8_HALF, G8_P1 = 2 * G8_HALF, G8_Q1 = 3 * G8_HALF;
-constexpr int G8_SMEM = 256 * (256 + 8) * 2;  // the epilogue's staged tile of 256 rows, a little more than two K-tiles
-static_assert(G8_SMEM >= 2 * (int)G8_TILE, "two K-tiles fit");
+constexpr int G8_SIDE = 4 * 256;  // per tile: four values for each of its 256 columns or rows
 
 // What one wave requests of an operand.  IS_Q: indices of a half-tile are 2 x 64 (wave rows), else 4 x 32 (wave columns).
 template <bool COL, bool IS_Q> struct Request8 {
@@ -73,7 +75,7 @@ template <bool COL, bool IS_Q> struct Request8 {
         k[0] = k[1] = k0;
     }
     __device__ __forceinline__ void issue(int h, unsigned lds, int K) {
-        const srd_t srd = {(unsigned)base[h], (unsigned)(base[h] >> 32) & 0xffffu, 0x80000000u, 0x00020000u};
+        const srd_t srd = make_srd((const void*)base[h]);
         const unsigned d0 = k[h] + k_lane >= K ? G8_DEAD : 0u, d1 = k[h] + k_lane + k_step >= K ? G8_DEAD : 0u;
         request16(off[h] | d0, srd, lds);
         request16((off[h] + step) | d1, srd, lds + (COL ? 1024u : 8192u));
@@ -114,13 +116,15 @@ template <bool COL, int N> struct Read8 {
     }
 };
 
-// Epi::run(args, acc, p0, q0, lane, wave, tile_p, tile_q, slice, smem): acc[j][i] = p0 + 64 (wave & 3) + 16 j.., q0 + 128 (wave >> 2) + 16 i..
+// Epi::side(args, p0, q0, thread, side) fills the side buffer; Epi::run(args, acc, p0, q0, lane, wave, tile_p, tile_q, slice, side):
+// acc[j][i] = p0 + 64 (wave & 3) + 16 j.., q0 + 128 (wave >> 2) + 16 i..
 template <bool PCOL, bool QCOL, typename Epi> __global__ __launch_bounds__(512) void vocab_gemm8_kernel(Gemm8Shape g, typename Epi::Args ea) {
-    __shared__ __attribute__((aligned(16))) unsigned char smem[G8_SMEM];
+    __shared__ __attribute__((aligned(16))) unsigned char smem[2 * G8_TILE];
+    __shared__ __attribute__((aligned(16))) float side[2][G8_SIDE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wq = wave >> 2, wp = wave & 3;
     int K = g.K;
     if (g.rows) {  // the grid is laid out for all rows: what is behind the counted ones ends here
-        const int rows = *g.rows;
+        const int rows = __builtin_amdgcn_readfirstlane(*g.rows);
         if (g.rows_are_k) {
             K = min(K, rows);
         } else {
@@ -128,35 +132,37 @@ template <bool PCOL, bool QCOL, typename Epi> __global__ __launch_bounds__(512) 
             g.tiles_q = min(g.tiles_q, (rows + 255) / 256);
         }
     }
-    const int slices = g.slices ? *g.slices : 1;
-    // workgroups b and b + 8 share an XCD and its L2: every XCD takes a contiguous range of the tiles that are left
-    int id;
-    {
-        const int n = g.tiles_p * g.tiles_q * slices, o = blockIdx.x, per = n >> 3, rest = n & 7, xcd = o & 7;
-        if (o >= n) return;
-        id = (xcd < rest ? xcd * (per + 1) : rest * (per + 1) + (xcd - rest) * per) + (o >> 3);
-    }
-    const int slice = id % slices;
-    id /= slices;
-    // 4 q tiles side by side walk the p tiles, so what runs at once on an XCD is a block of both and shares its operands in L2
-    int tp, tq;
-    {
-        const int band = id / (4 * g.tiles_p), left = min(4, g.tiles_q - band * 4), in = id - band * 4 * g.tiles_p;
-        tq = band * 4 + in % left;
-        tp = in / left;
-    }
-    const int p0 = tp * 256, q0 = tq * 256;
-    const int nk = (K + 63) / 64, t_begin = (int)((long long)slice * nk / slices), t_end = (int)((long long)(slice + 1) * nk / slices);
+    const int slices = g.slices ? __builtin_amdgcn_readfirstlane(*g.slices) : 1, total = g.tiles_p * g.tiles_q * slices, nk = (K + 63) / 64;
+    int order = blockIdx.x;
+    if (order >= total) return;
 
-    f32x4_t acc[4][8];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) acc[j][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    struct Place {
+        int tp, tq, slice, t_begin, t_end;
+    };
+    auto place = [&](int o) {
+        // tiles o and o + 8 share an XCD and its L2: every XCD takes a contiguous range
+        const int per = total >> 3, rest = total & 7, xcd = o & 7;
+        int id = (xcd < rest ? xcd * (per + 1) : rest * (per + 1) + (xcd - rest) * per) + (o >> 3);
+        Place x;
+        x.slice = id % slices;
+        id /= slices;
+        // 4 q tiles side by side walk the p tiles, so what runs at once on an XCD is a block of both and shares its operands in L2
+        const int band = id / (4 * g.tiles_p), left = min(4, g.tiles_q - band * 4), in = id - band * 4 * g.tiles_p;
+        x.tq = band * 4 + in % left;
+        x.tp = in / left;
+        x.t_begin = (int)((long long)x.slice * nk / slices);
+        x.t_end = (int)((long long)(x.slice + 1) * nk / slices);
+        // the same in every lane, computed in vector registers: the buffers' bases are built from them
+        x.tp = __builtin_amdgcn_readfirstlane(x.tp);
+        x.tq = __builtin_amdgcn_readfirstlane(x.tq);
+        x.slice = __builtin_amdgcn_readfirstlane(x.slice);
+        x.t_begin = __builtin_amdgcn_readfirstlane(x.t_begin);
+        x.t_end = __builtin_amdgcn_readfirstlane(x.t_end);
+        return x;
+    };
+
     Request8<QCOL, true> rq;
     Request8<PCOL, false> rp;
-    rq.init(g.q, q0, t_begin * 64, wave, lane);
-    rp.init(g.p, p0, t_begin * 64, wave, lane);
     Read8<QCOL, 4> fq;
     Read8<PCOL, 2> fp;
     fq.init(wq * 64, lane);
@@ -164,7 +170,22 @@ template <bool PCOL, bool QCOL, typename Epi> __global__ __launch_bounds__(512) 
     const unsigned lds0 = (unsigned)(uintptr_t)(lptr_t)smem;
     const unsigned piece_q = __builtin_amdgcn_readfirstlane(lds0 + Request8<QCOL, true>::piece(wave));
     const unsigned piece_p = __builtin_amdgcn_readfirstlane(lds0 + Request8<PCOL, false>::piece(wave));
+    // a tile's side buffer, its first K-tile and three half-tiles of the second
+    auto begin = [&](const Place& x, int parity) {
+        Epi::side(ea, x.tp * 256, x.tq * 256, threadIdx.x, side[parity]);
+        if (x.t_begin >= x.t_end) return;
+        rq.init(g.q, x.tq * 256, x.t_begin * 64, wave, lane);
+        rp.init(g.p, x.tp * 256, x.t_begin * 64, wave, lane);
+        rq.issue(0, piece_q + G8_Q0, K);
+        rp.issue(0, piece_p + G8_P0, K);
+        rp.issue(1, piece_p + G8_P1, K);
+        rq.issue(1, piece_q + G8_Q1, K);
+        rq.issue(0, piece_q + G8_TILE + G8_Q0, K);
+        rp.issue(0, piece_p + G8_TILE + G8_P0, K);
+        rp.issue(1, piece_p + G8_TILE + G8_P1, K);
+    };
 
+    f32x4_t acc[4][8];
     uint4 xa[4][2] = {}, wb0[2][2] = {}, wb1[2][2] = {};
     auto ldq = [&](unsigned off) {
 #pragma unroll
@@ -220,27 +241,37 @@ template <bool PCOL, bool QCOL, typename Epi> __global__ __launch_bounds__(512) 
         VG_BARRIER();
         quadrant(wb0, 1, 0);
     };
-    if (t_begin < t_end) {
-        rq.issue(0, piece_q + G8_Q0, K);
-        rp.issue(0, piece_p + G8_P0, K);
-        rp.issue(1, piece_p + G8_P1, K);
-        rq.issue(1, piece_q + G8_Q1, K);
-        rq.issue(0, piece_q + G8_TILE + G8_Q0, K);
-        rp.issue(0, piece_p + G8_TILE + G8_P0, K);
-        rp.issue(1, piece_p + G8_TILE + G8_P1, K);
-        asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
-        VG_BARRIER();
-        if (wq == 1) VG_BARRIER();
-        unsigned cur = 0;
-        for (int t = t_begin; t < t_end; ++t) {
-            tile(cur, G8_TILE - cur);
-            cur = G8_TILE - cur;
+
+    Place at = place(order);
+    begin(at, 0);
+    for (int parity = 0;; parity ^= 1) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[j][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        if (at.t_begin < at.t_end) {
+            // all but the last three half-tiles (an epilogue's stores, issued since, only make the wait longer)
+            asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+            VG_BARRIER();
+            if (wq == 1) VG_BARRIER();
+            unsigned cur = 0;
+            for (int t = at.t_begin; t < at.t_end; ++t) {
+                tile(cur, G8_TILE - cur);
+                cur = G8_TILE - cur;
+            }
+            if (wq == 0) VG_BARRIER();
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // requests past the end are still landing
         }
-        if (wq == 0) VG_BARRIER();
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // requests past the end are still landing
+        __syncthreads();  // nobody reads the tile any more, the side buffer is whole
+        const Place done = at;
+        order += gridDim.x;
+        if (order < total) {
+            at = place(order);
+            begin(at, parity ^ 1);
+        }
+        Epi::run(ea, acc, done.tp * 256, done.tq * 256, lane, wave, done.tp, done.tq, done.slice, side[parity]);
+        if (order >= total) return;
     }
-    __syncthreads();
-    Epi::run(ea, acc, p0, q0, lane, wave, tp, tq, slice, smem);
 }
 
 }  // namespace

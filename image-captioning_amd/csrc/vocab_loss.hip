@@ -35,7 +35,7 @@ struct StatsEpi {
     struct Args {
         const float* bias;
         Targets t;
-        float2* part;  // [N][parts]
+        float2* part;  // [parts][N]
         float* zt;     // [N] logit of the target
         int N, V, parts;
     };
@@ -66,25 +66,37 @@ struct StatsEpi {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s += __builtin_amdgcn_exp2f((acc[i][j][e] - m_use) * ATTN_LOG2E);
             s += __shfl_xor(s, 32, 64);
-            if (h == 0 && row < a.N) a.part[(long long)row * a.parts + tp] = make_float2(m, s);
+            if (h == 0 && row < a.N) a.part[(long long)tp * a.N + row] = make_float2(m, s);
         }
     }
 };
 
-// one wave per row
-__global__ __launch_bounds__(256) void vocab_loss_rows_kernel(const float2* __restrict__ part, const float* __restrict__ zt, Targets t, float* __restrict__ loss,
-                                                              float* __restrict__ lse, int N, int parts) {
-    const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= N) return;
-    const float2* p = part + (long long)row * parts;
-    float m = -INFINITY;
-    for (int i = lane; i < parts; i += 64) m = fmaxf(m, p[i].x);
-    m = wave_max(m);
-    const float m_use = m == -INFINITY ? 0.f : m;
-    float s = 0.f;
-    for (int i = lane; i < parts; i += 64) s += p[i].y * __builtin_amdgcn_exp2f((p[i].x - m_use) * ATTN_LOG2E);
-    s = wave_sum(s);
-    if (lane == 0) {
+// joins the parts of a row: 16 rows to a workgroup, 64 threads share a row's parts
+__global__ __launch_bounds__(1024) void vocab_loss_rows_kernel(const float2* __restrict__ part, const float* __restrict__ zt, Targets t, float* __restrict__ loss,
+                                                               float* __restrict__ lse, int N, int parts) {
+    __shared__ float2 sum[64][16];
+    const int lane = threadIdx.x & 15, share = threadIdx.x >> 4, row = blockIdx.x * 16 + lane;
+    float m = -INFINITY, s = 0.f;
+    if (row < N)
+#pragma unroll 4
+        for (int i = share; i < parts; i += 64) {
+            const float2 p = part[(long long)i * N + row];
+            const float top = fmaxf(m, p.x), use = top == -INFINITY ? 0.f : top;
+            s = s * __builtin_amdgcn_exp2f((m - use) * ATTN_LOG2E) + p.y * __builtin_amdgcn_exp2f((p.x - use) * ATTN_LOG2E);
+            m = top;
+        }
+    sum[share][lane] = make_float2(m, s);
+    for (int d = 32; d > 0; d >>= 1) {
+        __syncthreads();
+        if (share < d) {
+            const float2 o = sum[share + d][lane];
+            const float top = fmaxf(m, o.x), use = top == -INFINITY ? 0.f : top;
+            s = s * __builtin_amdgcn_exp2f((m - use) * ATTN_LOG2E) + o.y * __builtin_amdgcn_exp2f((o.x - use) * ATTN_LOG2E);
+            m = top;
+            sum[share][lane] = make_float2(m, s);
+        }
+    }
+    if (share == 0 && row < N) {
         const float l = m + logf(s);
         lse[row] = l;
         loss[row] = target_of(t, row) >= 0 ? l - zt[row] : 0.f;
@@ -192,97 +204,116 @@ template <typename T> struct OutEpi {
 };
 
 // ---- the same epilogues on the 256 x 256 tiles: a lane holds 4 consecutive p of 4 tiles for 8 rows --------------------------------
+// side buffer: [0] bias of the tile's 256 columns (-infinity past the last word), [1] targets of its 256 rows, [2] weights, [3] lse
 struct StatsEpi8 {
     typedef StatsEpi::Args Args;
-    __device__ static __forceinline__ void run(const Args& a, f32x4_t (&acc)[4][8], int p0, int q0, int lane, int wave, int tp, int, int, unsigned char*) {
-        const int pw = p0 + 64 * (wave & 3) + 4 * (lane >> 4), qw = q0 + 128 * (wave >> 2) + (lane & 15);
-        float b[4][4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int v = pw + 16 * j + e;
-                b[j][e] = v < a.V ? (a.bias ? a.bias[v] : 0.f) : -INFINITY;
-            }
+    __device__ static __forceinline__ void side(const Args& a, int p0, int q0, int tid, float* side) {
+        const int i = tid & 255;
+        if (tid < 256) {
+            side[i] = p0 + i < a.V ? (a.bias ? a.bias[p0 + i] : 0.f) : -INFINITY;
+        } else {
+            reinterpret_cast<int*>(side)[256 + i] = q0 + i < a.N ? target_of(a.t, q0 + i) : -1;
+        }
+    }
+    __device__ static __forceinline__ void run(const Args& a, f32x4_t (&acc)[4][8], int p0, int q0, int lane, int wave, int tp, int, int, const float* side) {
+        const int pl = 64 * (wave & 3) + 4 * (lane >> 4), ql = 128 * (wave >> 2) + (lane & 15);
         if (p0 + 64 * (wave & 3) >= a.V) return;  // its parts are not looked at
-        int ts[8];
+        float m[8], s[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ts[i] = target_of(a.t, min(qw + 16 * i, a.N - 1));  // all in flight at once
+        for (int i = 0; i < 8; ++i) m[i] = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const f32x4_t b = *reinterpret_cast<const f32x4_t*>(side + pl + 16 * j);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                acc[j][i] += b;
+                m[i] = fmaxf(m[i], fmaxf(fmaxf(acc[j][i][0], acc[j][i][1]), fmaxf(acc[j][i][2], acc[j][i][3])));
+            }
+        }
+        // the four lanes of a row, all rows at once: an exchange's latency is paid four times, not 32
+#pragma unroll
+        for (int d = 16; d < 64; d <<= 1) {
+            float o[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[i] = __shfl_xor(m[i], d, 64);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m[i] = fmaxf(m[i], o[i]);
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int row = qw + 16 * i, t = row < a.N ? ts[i] : -1;
-            float m = -INFINITY;
+            const int tc = reinterpret_cast<const int*>(side)[256 + ql + 16 * i] - p0 - pl;  // the target's column, from the lane's first
+            const float m2 = (m[i] == -INFINITY ? 0.f : m[i]) * ATTN_LOG2E;
+            s[i] = 0.f;
+            if ((unsigned)tc < 64u)  // in this wave's columns, but perhaps in another lane's
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (tc == 16 * j + e) a.zt[q0 + ql + 16 * i] = acc[j][i][e];
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float z = acc[j][i][e] + b[j][e];
-                    if (pw + 16 * j + e == t) a.zt[row] = z;
-                    acc[j][i][e] = z;
-                    m = fmaxf(m, z);
-                }
-            m = fmaxf(m, __shfl_xor(m, 16, 64));
-            m = fmaxf(m, __shfl_xor(m, 32, 64));
-            const float m_use = m == -INFINITY ? 0.f : m;
-            float s = 0.f;
+                for (int e = 0; e < 4; ++e) s[i] += __builtin_amdgcn_exp2f(fmaf(acc[j][i][e], ATTN_LOG2E, -m2));
+        }
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+        for (int d = 16; d < 64; d <<= 1) {
+            float o[8];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f((acc[j][i][e] - m_use) * ATTN_LOG2E);
-            s += __shfl_xor(s, 16, 64);
-            s += __shfl_xor(s, 32, 64);
-            if (lane < 16 && row < a.N) a.part[(long long)row * a.parts + tp * 4 + (wave & 3)] = make_float2(m, s);
+            for (int i = 0; i < 8; ++i) o[i] = __shfl_xor(s[i], d, 64);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i] += o[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int row = q0 + ql + 16 * i;
+            if (lane < 16 && row < a.N) a.part[(long long)(tp * 4 + (wave & 3)) * a.N + row] = make_float2(m[i], s[i]);
         }
     }
 };
 
 struct GradEpi8 {
     typedef GradEpi<bf16_t>::Args Args;
-    __device__ static __forceinline__ void run(Args a, f32x4_t (&acc)[4][8], int p0, int q0, int lane, int wave, int, int tq, int, unsigned char* smem) {
-        if (a.count) a.N = min(a.N, *a.count);
-        constexpr int LD = 256 + 8;  // staged rows of bf16
-        const int pl = 64 * (wave & 3) + 4 * (lane >> 4), ql = 128 * (wave >> 2) + (lane & 15);
-        bf16_t* st = reinterpret_cast<bf16_t*>(smem);
-        float b[4][4], sum[16];
+    __device__ static __forceinline__ int rows(const Args& a) { return a.count ? min(a.N, *a.count) : a.N; }
+    __device__ static __forceinline__ void side(const Args& a, int p0, int q0, int tid, float* side) {
+        const int i = tid & 255;
+        if (tid < 256) {
+            side[i] = p0 + i < a.Vc ? (a.bias ? a.bias[a.v0 + p0 + i] * ATTN_LOG2E : 0.f) : -INFINITY;  // beyond the piece: probability zero
+        } else {
+            const int row = q0 + i;
+            const int t = row < rows(a) ? a.r.target[row] : -1;
+            reinterpret_cast<int*>(side)[256 + i] = t < 0 ? -(1 << 30) : t - a.v0 - p0;  // column of the tile, anything outside it for none
+            side[512 + i] = t < 0 ? 0.f : a.r.weight[row];
+            side[768 + i] = t < 0 ? 0.f : a.r.lse[row] * ATTN_LOG2E;
+        }
+    }
+    __device__ static __forceinline__ void run(const Args& a, f32x4_t (&acc)[4][8], int p0, int q0, int lane, int wave, int, int tq, int, const float* side) {
+        const int pl = 64 * (wave & 3) + 4 * (lane >> 4), ql = 128 * (wave >> 2) + (lane & 15), n = rows(a);
+        f32x4_t b[4];
+        float sum[16];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 4; ++j) {
+            b[j] = *reinterpret_cast<const f32x4_t*>(side + pl + 16 * j);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int c = p0 + pl + 16 * j + e;
-                b[j][e] = c < a.Vc ? (a.bias ? a.bias[a.v0 + c] * ATTN_LOG2E : 0.f) : -INFINITY;  // beyond the piece: probability zero
-                sum[4 * j + e] = 0.f;
-            }
-        int ts[8];
-        float rw[8], rl[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {  // all in flight at once
-            const int row = min(q0 + ql + 16 * i, a.N - 1);
-            ts[i] = a.r.target[row];
-            rw[i] = a.r.weight[row];
-            rl[i] = a.r.lse[row];
+            for (int e = 0; e < 4; ++e) sum[4 * j + e] = 0.f;
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int t = q0 + ql + 16 * i < a.N ? ts[i] : -1;
-            const float w = t >= 0 ? rw[i] : 0.f, lse2 = t >= 0 ? rl[i] * ATTN_LOG2E : 0.f;
-            const int tc = t - a.v0 - p0 - pl;  // the target's column, from the lane's first
+            const int row = q0 + ql + 16 * i;
+            const int tc = reinterpret_cast<const int*>(side)[256 + ql + 16 * i] - pl;
+            const float w = side[512 + ql + 16 * i], lse2 = side[768 + ql + 16 * i];
+            const bool counts = tc > -(1 << 29);
+            bf16_t* out = a.d + (long long)row * a.ld + p0 + pl;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 float d[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float p = __builtin_amdgcn_exp2f(fmaf(acc[j][i][e], ATTN_LOG2E, b[j][e] - lse2));
-                    d[e] = t >= 0 ? w * (tc == 16 * j + e ? p - 1.0f : p) : 0.f;
+                    d[e] = counts ? w * (tc == 16 * j + e ? p - 1.0f : p) : 0.f;  // a row that does not count stays zero whatever its logits are
                     sum[4 * j + e] += d[e];
                 }
-                store4<bf16_t>(st + (ql + 16 * i) * LD + pl + 16 * j, d[0], d[1], d[2], d[3]);
+                if (row < n && p0 + pl + 16 * j < a.ld) store4<bf16_t>(out + 16 * j, d[0], d[1], d[2], d[3]);
             }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-            const int x = threadIdx.x + k * 512, r = x >> 5, c = (x & 31) * 8;
-            if (q0 + r < a.N && p0 + c < a.ld) *reinterpret_cast<uint4*>(a.d + (long long)(q0 + r) * a.ld + p0 + c) = *reinterpret_cast<const uint4*>(st + r * LD + c);
         }
         if (a.part_db == nullptr) return;
         // sums over 16 lanes, halving the values at every exchange: value x ends in the lane whose low four bits are x
@@ -302,7 +333,8 @@ struct GradEpi8 {
 
 struct OutEpi8 {
     typedef OutEpi<bf16_t>::Args Args;
-    __device__ static __forceinline__ void run(const Args& a, f32x4_t (&acc)[4][8], int p0, int q0, int lane, int wave, int, int, int slice, unsigned char*) {
+    __device__ static __forceinline__ void side(const Args&, int, int, int, float*) {}
+    __device__ static __forceinline__ void run(const Args& a, f32x4_t (&acc)[4][8], int p0, int q0, int lane, int wave, int, int, int slice, const float*) {
         const int pw = p0 + 64 * (wave & 3) + 4 * (lane >> 4), qw = q0 + 128 * (wave >> 2) + (lane & 15);
         const bool whole = a.Np % 4 == 0 && a.ld % 4 == 0;
 #pragma unroll
@@ -602,7 +634,8 @@ template <typename T, bool PCOL, bool QCOL, typename Epi> int gemm(const Operand
 }
 template <bool PCOL, bool QCOL, typename Epi> int gemm8(const Operand& p, const Operand& q, const Rows& r, int K, const typename Epi::Args& ea, hipStream_t s) {
     Gemm8Shape g = {{p.p, p.ld, p.n}, {q.p, q.ld, q.n}, r.count, r.slices, r.are_k, K, edge_tiles(p.n, 256), edge_tiles(q.n, 256)};
-    MIC_LAUNCH((vocab_gemm8_kernel<PCOL, QCOL, Epi>), dim3((unsigned)((long long)g.tiles_p * g.tiles_q * (r.slices ? r.most : 1))), dim3(512), 0, s, g, ea);
+    const long long all = (long long)g.tiles_p * g.tiles_q * (r.slices ? r.most : 1);
+    MIC_LAUNCH((vocab_gemm8_kernel<PCOL, QCOL, Epi>), dim3((unsigned)(all < 256 ? all : 256)), dim3(512), 0, s, g, ea);  // one to a compute unit
     return 0;
 }
 // bf16 on the tiles of the plan, fp32 on the small ones
@@ -642,7 +675,7 @@ template <typename T> int forward(const mic_vocab_loss_desc* d, const Plan& p, h
     ea.part = (float2*)(ws + p.part); ea.zt = (float*)(ws + p.zt);
     ea.N = d->N; ea.V = d->V; ea.parts = p.parts;
     MIC_TRY((product<T, false, false, StatsEpi, StatsEpi8>(p, w, x, Rows{}, d->H, ea, s)));
-    MIC_LAUNCH(vocab_loss_rows_kernel, dim3((d->N + 3) / 4), dim3(256), 0, s, (const float2*)ea.part, (const float*)ea.zt, ea.t, d->loss, d->lse, d->N, p.parts);
+    MIC_LAUNCH(vocab_loss_rows_kernel, dim3((d->N + 15) / 16), dim3(1024), 0, s, (const float2*)ea.part, (const float*)ea.zt, ea.t, d->loss, d->lse, d->N, p.parts);
     return 0;
 }
 
