@@ -1,4 +1,5 @@
-// Tiled matrix product of the vocabulary loss:  out[q][p] = sum_k Q(q, k) P(p, k), 128 x 128 tiles, four waves of 64 x 64.
+// Tiled matrix product of the vocabulary loss:  out[q][p] = sum_k Q(q, k) P(p, k), tiles of 128 x 128 or 64 x 64 (S = 2, 1), four
+// waves of half that edge.
 //
 // Each operand lies in memory either with k consecutive (a row per index: "row" operand) or with its index consecutive (a row per
 // k: "column" operand), and goes to LDS as it lies; a column operand is read from LDS by a transposing read (bf16) or scalar
@@ -29,16 +30,14 @@ template <int DP> __device__ __forceinline__ Frag8<float> read_col_k(const float
     return f;
 }
 
-constexpr int VT = 128;  // tile edge
-
 struct Operand {
     const void* p;
     long long ld;  // elements between rows in memory
     int n;         // how many indices there are
 };
 
-// One operand's tile of 128 indices x KS steps of k: fetched to registers, later stored to LDS.
-template <typename T, bool COL> struct OperandTile {
+// One operand's tile of VT indices x KS steps of k: fetched to registers, later stored to LDS.
+template <typename T, bool COL, int VT> struct OperandTile {
     static constexpr int KS = 128 / (int)sizeof(T);
     static constexpr int DP = COL ? VT : KS;
     using L = Tile<T, DP>;
@@ -75,10 +74,11 @@ struct GemmShape {
     int K, tiles_p, tiles_q;
 };
 
-// Epi::run(args, acc, p0, q0, lane, tile_p, tile_q, wave, slice): acc[i][j] = p0 + 32 i.., q0 + 32 j..
-template <typename T, bool PCOL, bool QCOL, typename Epi> __global__ __launch_bounds__(256) void vocab_gemm_kernel(GemmShape g, typename Epi::Args ea) {
-    using TP = OperandTile<T, PCOL>;
-    using TQ = OperandTile<T, QCOL>;
+// Epi::run(args, acc, p0, q0, lane, part_p, part_q, slice): acc[i][j] = p0 + 32 i.., q0 + 32 j..; parts number the waves' columns and rows
+template <typename T, int S, bool PCOL, bool QCOL, typename Epi> __global__ __launch_bounds__(256) void vocab_gemm_kernel(GemmShape g, typename Epi::Args ea) {
+    constexpr int VT = 64 * S, WAVE = 32 * S;
+    using TP = OperandTile<T, PCOL, VT>;
+    using TQ = OperandTile<T, QCOL, VT>;
     constexpr int KS = TP::KS;
     __shared__ __attribute__((aligned(16))) T sp[2][VT * KS];
     __shared__ __attribute__((aligned(16))) T sq[2][VT * KS];
@@ -105,11 +105,11 @@ template <typename T, bool PCOL, bool QCOL, typename Epi> __global__ __launch_bo
     const int tq = id % g.tiles_q, tp = id / g.tiles_q;
     const int p0 = tp * VT, q0 = tq * VT;
     const int nk = (g.K + KS - 1) / KS, kb = (int)((long long)nk * slice / slices), ke = (int)((long long)nk * (slice + 1) / slices);
-    f32x16_t acc[2][2];
+    f32x16_t acc[S][S];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < S; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = f32x16_t{};
+        for (int j = 0; j < S; ++j) acc[i][j] = f32x16_t{};
     TP fp;
     TQ fq;
     if (kb < ke) {
@@ -127,24 +127,24 @@ template <typename T, bool PCOL, bool QCOL, typename Epi> __global__ __launch_bo
         }
 #pragma unroll
         for (int s = 0; s < KS / 16; ++s) {
-            Frag8<T> a[2], b[2];
+            Frag8<T> a[S], b[S];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                a[i] = TP::frag(sp[cur], wp * 64 + i * 32, s, lane);
-                b[i] = TQ::frag(sq[cur], wq * 64 + i * 32, s, lane);
+            for (int i = 0; i < S; ++i) {
+                a[i] = TP::frag(sp[cur], wp * WAVE + i * 32, s, lane);
+                b[i] = TQ::frag(sq[cur], wq * WAVE + i * 32, s, lane);
             }
-            if constexpr (sizeof(T) == 4) {  // the four sums in turn: no product waits for the one before
+            if constexpr (sizeof(T) == 4) {  // the sums in turn: no product waits for the one before
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
+                    for (int i = 0; i < S; ++i)
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i].v[e], b[j].v[e], acc[i][j], 0, 0, 0);
+                        for (int j = 0; j < S; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i].v[e], b[j].v[e], acc[i][j], 0, 0, 0);
             } else {
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
+                for (int i = 0; i < S; ++i)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) mma32(a[i], b[j], acc[i][j]);
+                    for (int j = 0; j < S; ++j) mma32(a[i], b[j], acc[i][j]);
             }
         }
         if (t + 1 < ke) {
@@ -152,7 +152,7 @@ template <typename T, bool PCOL, bool QCOL, typename Epi> __global__ __launch_bo
             fq.put(sq[cur ^ 1]);
         }
     }
-    Epi::run(ea, acc, p0 + wp * 64, q0 + wq * 64, lane, tp * 2 + wp, tq * 2 + wq, slice);
+    Epi::run(ea, acc, p0 + wp * WAVE, q0 + wq * WAVE, lane, tp * 2 + wp, tq * 2 + wq, slice);
 }
 
 }  // namespace

@@ -8,8 +8,8 @@
 // Rows that do not count (padding: half of a batch of captions) have no gradient, so the gradient's products run over the counted
 // rows alone: they are gathered first, their number stays on the device, and workgroups behind the last one end at once.
 //
-// Two kernels: 256 x 256 tiles for bf16 (vocab_gemm8.h), 128 x 128 tiles for fp32 and for products too small to fill the larger ones
-// (vocab_gemm.h).
+// Two kernels: 256 x 256 tiles for bf16 (vocab_gemm8.h), 128 x 128 and 64 x 64 tiles for fp32 and for products too small to fill the
+// larger ones (vocab_gemm.h).
 #include "vocab_gemm.h"
 #include "vocab_gemm8.h"
 
@@ -39,15 +39,15 @@ struct StatsEpi {
         float* zt;     // [N] logit of the target
         int N, V, parts;
     };
-    __device__ static __forceinline__ void run(const Args& a, f32x16_t (&acc)[2][2], int p0, int q0, int lane, int tp, int, int) {
+    template <int S> __device__ static __forceinline__ void run(const Args& a, f32x16_t (&acc)[S][S], int p0, int q0, int lane, int tp, int, int) {
         const int h = lane >> 5;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < S; ++j) {
             const int row = q0 + j * 32 + (lane & 31);
             const int t = row < a.N ? target_of(a.t, row) : -1;
             float m = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < S; ++i)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const int v = p0 + i * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
@@ -62,7 +62,7 @@ struct StatsEpi {
             const float m_use = m == -INFINITY ? 0.f : m;
             float s = 0.f;
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < S; ++i)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s += __builtin_amdgcn_exp2f((acc[i][j][e] - m_use) * ATTN_LOG2E);
             s += __shfl_xor(s, 32, 64);
@@ -118,17 +118,17 @@ template <typename T> struct GradEpi {
         const int* count;  // NULL, or the rows there are
         int N, Vc, ld, v0;
     };
-    __device__ static __forceinline__ void run(Args a, f32x16_t (&acc)[2][2], int p0, int q0, int lane, int, int tq, int) {
-        if (a.count) a.N = min(a.N, *a.count);
+    template <int S> __device__ static __forceinline__ void run(const Args& a, f32x16_t (&acc)[S][S], int p0, int q0, int lane, int, int tq, int) {
+        const int n = a.count ? min(a.N, *a.count) : a.N;
         const int h = lane >> 5;
-        float sum[2][16];
+        float sum[S][16];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < S; ++j) {
             const int row = q0 + j * 32 + (lane & 31);
-            const int t = row < a.N ? a.r.target[row] : -1;
+            const int t = row < n ? a.r.target[row] : -1;
             const float w = t >= 0 ? a.r.weight[row] : 0.f, lse2 = t >= 0 ? a.r.lse[row] * ATTN_LOG2E : 0.f;
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < S; ++i)
 #pragma unroll
                 for (int e4 = 0; e4 < 4; ++e4) {
                     const int c = p0 + i * 32 + 8 * e4 + 4 * h;  // column of the piece
@@ -142,16 +142,17 @@ template <typename T> struct GradEpi {
                         d[e] = t >= 0 && c + e < a.Vc ? w * (v == t ? p - 1.0f : p) : 0.f;
                         sum[i][4 * e4 + e] = (j ? sum[i][4 * e4 + e] : 0.f) + d[e];
                     }
-                    if (row < a.N && c < a.ld) store4<T>(a.d + (long long)row * a.ld + c, d[0], d[1], d[2], d[3]);
+                    if (row < n && c < a.ld) store4<T>(a.d + (long long)row * a.ld + c, d[0], d[1], d[2], d[3]);
                 }
         }
         if (a.part_db == nullptr) return;
-        // sums over the 32 lanes of a half: every exchange halves the values a lane carries; value x ends in the lane whose low five bits are x
-        float v[32];
+        // sums over the 32 lanes of a half: every exchange halves the values a lane carries; value x ends in the lanes whose low bits are x
+        constexpr int N = 16 * S;
+        float v[N];
 #pragma unroll
-        for (int x = 0; x < 32; ++x) v[x] = sum[x >> 4][x & 15];
+        for (int x = 0; x < N; ++x) v[x] = sum[x >> 4][x & 15];
 #pragma unroll
-        for (int d = 16; d > 0; d >>= 1) {
+        for (int d = N / 2; d > 0; d >>= 1) {
             const bool up = lane & d;
 #pragma unroll
             for (int x = 0; x < d; ++x) {
@@ -159,7 +160,8 @@ template <typename T> struct GradEpi {
                 v[x] = keep + __shfl_xor(give, d, 64);
             }
         }
-        const int x = lane & 31, c = p0 + (x >> 4) * 32 + 8 * ((x & 15) >> 2) + 4 * h + (x & 3);
+        if (S == 1) v[0] += __shfl_xor(v[0], 16, 64);
+        const int x = lane & (N - 1), c = p0 + (x >> 4) * 32 + 8 * ((x & 15) >> 2) + 4 * h + (x & 3);
         if (c < a.Vc) a.part_db[(long long)tq * a.Vc + c] = v[0];
     }
 };
@@ -172,15 +174,15 @@ template <typename T> struct OutEpi {
         long long ld;
         int Np, Nq;
     };
-    __device__ static __forceinline__ void run(const Args& a, f32x16_t (&acc)[2][2], int p0, int q0, int lane, int, int, int slice) {
+    template <int S> __device__ static __forceinline__ void run(const Args& a, f32x16_t (&acc)[S][S], int p0, int q0, int lane, int, int, int slice) {
         const int h = lane >> 5;
         const bool whole = a.Np % 4 == 0 && a.ld % 4 == 0;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < S; ++j) {
             const int row = q0 + j * 32 + (lane & 31);
             if (row >= a.Nq) continue;
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < S; ++i)
 #pragma unroll
                 for (int e4 = 0; e4 < 4; ++e4) {
                     const int c = p0 + i * 32 + 8 * e4 + 4 * h;
@@ -525,7 +527,8 @@ template <typename T> __global__ __launch_bounds__(256) void vocab_pad_kernel(co
 
 // ---- plan ---------------------------------------------------------------------------------------------------------------------
 long long up256(long long b) { return (b + 255) / 256 * 256; }
-int tiles(long long n) { return (int)((n + VT - 1) / VT); }
+
+int edge_tiles(long long n, int edge) { return (int)((n + edge - 1) / edge); }
 
 struct Plan {
     int Hp, e;              // columns of the operands the products read (H rounded up to whole 16 bytes)
@@ -539,7 +542,6 @@ struct Plan {
     long long xpad, wpad, part, zt, d, dx, dw, db, rows, bytes;
 };
 
-int edge_tiles(long long n, int edge) { return (int)((n + edge - 1) / edge); }
 
 // The most ranges k may be cut into: every one keeps four steps of k.  How many are used is decided when the rows are known.
 int most_slices(long long K, int ks) {
@@ -559,7 +561,8 @@ Plan make_plan(const mic_vocab_loss_desc* d, bool grad) {
     p.pad = p.Hp != H || d->ld_x % p.e || d->ld_w % p.e || (((uintptr_t)d->x | (uintptr_t)d->w) & 15);
     // the large tiles address 256 rows (64 of k) of an operand with 31 bits; below 129 rows half of one would be empty
     p.big = d->dtype == MIC_BF16 && N > 128 && V > 128 && H >= 64 && H < (1 << 21) && d->ld_x < (1 << 21) && d->ld_w < (1 << 21);
-    p.edge = p.big ? 256 : VT;
+    // 64 x 64 tiles where 128 x 128 ones would leave compute units idle
+    p.edge = p.big ? 256 : (long long)edge_tiles(N, 128) * edge_tiles(V, 128) < 512 ? 64 : 128;
     p.gather = grad && N > p.edge;
     long long o = 0;
     p.xpad = o;
@@ -567,7 +570,7 @@ Plan make_plan(const mic_vocab_loss_desc* d, bool grad) {
     p.wpad = o;
     if (p.pad) o += up256(V * p.Hp * es);
     if (!grad) {
-        p.parts = p.big ? (int)((V + 63) / 64) : tiles(V) * 2;
+        p.parts = p.big ? (int)((V + 63) / 64) : edge_tiles(V, p.edge) * 2;
         p.part = o; o += up256(N * p.parts * 8);
         p.zt = o; o += up256(N * 4);
     } else {
@@ -584,7 +587,7 @@ Plan make_plan(const mic_vocab_loss_desc* d, bool grad) {
         p.sx = most_slices(p.Vc, ks);
         p.sw = most_slices(N, ks);
         // never more partial tiles than would fill the GPU twice
-        const long long wide = p.big ? 512 : 1024, tx = (long long)edge_tiles(N, p.edge) * edge_tiles(H, p.edge), tw = (long long)edge_tiles(p.Vc, p.edge) * edge_tiles(H, p.edge);
+        const long long wide = p.big ? 512 : p.edge == 128 ? 1024 : 2048, tx = (long long)edge_tiles(N, p.edge) * edge_tiles(H, p.edge), tw = (long long)edge_tiles(p.Vc, p.edge) * edge_tiles(H, p.edge);
         while (p.sx > 1 && p.sx * tx > (p.gather ? 2 * wide : wide)) --p.sx;
         while (p.sw > 1 && p.sw * tw > wide) --p.sw;
         p.rows = o; o += rows_bytes(N);
@@ -605,8 +608,8 @@ int check_desc(const char* who, const mic_vocab_loss_desc* d) {
     MIC_ARG_CHECK(d->dtype == MIC_F32 || d->dtype == MIC_BF16, "%s: bad dtype %d", who, d->dtype);
     MIC_ARG_CHECK(d->N >= 0 && d->H > 0 && d->V > 0, "%s: bad sizes N=%d H=%d V=%d", who, d->N, d->H, d->V);
     const long long lim = 1ll << 30;
-    MIC_ARG_CHECK(d->N < lim && d->H < lim && d->V < lim && (long long)(tiles(d->N) + 1) * (tiles(d->V) + 1) < lim / 32 && (long long)(tiles(d->N) + 1) * (tiles(d->H) + 1) < lim / 32 &&
-                      (long long)(tiles(d->V) + 1) * (tiles(d->H) + 1) < lim / 32,
+    MIC_ARG_CHECK(d->N < lim && d->H < lim && d->V < lim && (d->N / 64 + 2ll) * (d->V / 64 + 2ll) < lim / 32 && (d->N / 64 + 2ll) * (d->H / 64 + 2ll) < lim / 32 &&
+                      (d->V / 64 + 2ll) * (d->H / 64 + 2ll) < lim / 32,
                   "%s: sizes out of range N=%d H=%d V=%d", who, d->N, d->H, d->V);
     MIC_ARG_CHECK(d->target_bits == 32 || d->target_bits == 64, "%s: targets of %d bits", who, d->target_bits);
     MIC_ARG_CHECK(d->n_ignore >= 0 && d->n_ignore <= MAX_IGNORE, "%s: %d ignored words (at most %d)", who, d->n_ignore, MAX_IGNORE);
@@ -627,9 +630,10 @@ struct Rows {
     const int* slices;  // NULL: one
     int most;           // slices the grid is laid out for
 };
-template <typename T, bool PCOL, bool QCOL, typename Epi> int gemm(const Operand& p, const Operand& q, const Rows& r, int K, const typename Epi::Args& ea, hipStream_t s) {
-    GemmShape g = {p, q, r.count, r.slices, r.are_k, K, tiles(p.n), tiles(q.n)};
-    MIC_LAUNCH((vocab_gemm_kernel<T, PCOL, QCOL, Epi>), dim3((unsigned)((long long)g.tiles_p * g.tiles_q * (r.slices ? r.most : 1))), dim3(256), 0, s, g, ea);
+template <typename T, int S, bool PCOL, bool QCOL, typename Epi>
+int gemm(const Operand& p, const Operand& q, const Rows& r, int K, const typename Epi::Args& ea, hipStream_t s) {
+    GemmShape g = {p, q, r.count, r.slices, r.are_k, K, edge_tiles(p.n, 64 * S), edge_tiles(q.n, 64 * S)};
+    MIC_LAUNCH((vocab_gemm_kernel<T, S, PCOL, QCOL, Epi>), dim3((unsigned)((long long)g.tiles_p * g.tiles_q * (r.slices ? r.most : 1))), dim3(256), 0, s, g, ea);
     return 0;
 }
 template <bool PCOL, bool QCOL, typename Epi> int gemm8(const Operand& p, const Operand& q, const Rows& r, int K, const typename Epi::Args& ea, hipStream_t s) {
@@ -643,7 +647,8 @@ template <typename T, bool PCOL, bool QCOL, typename Epi, typename Epi8>
 int product(const Plan& pl, const Operand& p, const Operand& q, const Rows& r, int K, const typename Epi::Args& ea, hipStream_t s) {
     if constexpr (sizeof(T) == 2)
         if (pl.big) return gemm8<PCOL, QCOL, Epi8>(p, q, r, K, ea, s);
-    return gemm<T, PCOL, QCOL, Epi>(p, q, r, K, ea, s);
+    if (pl.edge == 64) return gemm<T, 1, PCOL, QCOL, Epi>(p, q, r, K, ea, s);
+    return gemm<T, 2, PCOL, QCOL, Epi>(p, q, r, K, ea, s);
 }
 
 template <typename T> int copy_rows(const void* in, long long ld, void* out, const int* at, long long rows, int cols, int padded, hipStream_t s) {
@@ -695,7 +700,7 @@ template <typename T> int gradient(const mic_vocab_loss_desc* d, const Plan& p, 
     ra.per_block = (int)((share + 1023) / 1024 * 1024);
     // measured on 256 x 256 tiles: a step of 64 k is 1.7 us, a workgroup's start and end 4 steps, writing and reading again the partial
     // tiles of all compute units 16; on 128 x 128 tiles (two workgroups to a compute unit) 2 and 7
-    ra.rule = p.big ? SplitRule{256, 4.f, 16.f} : SplitRule{512, 2.f, 7.f};
+    ra.rule = p.big ? SplitRule{256, 4.f, 16.f} : p.edge == 128 ? SplitRule{512, 2.f, 7.f} : SplitRule{1024, 3.f, 7.f};
     ra.edge = p.edge;
     ra.ks = 128 / (int)sizeof(T);
     const int last = d->V - (p.pieces - 1) * p.Vc, th = edge_tiles(H, p.edge);
