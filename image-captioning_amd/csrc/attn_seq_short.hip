@@ -114,7 +114,7 @@ template <typename T, int DP, int KT> __global__ __launch_bounds__(256) void att
 // of their own), 2 = a range of row tiles, partial sums.  Two workgroups to a compute unit (256 registers a lane) where LDS and
 // registers allow it: one loads while the other computes.
 template <typename T, int DP, int KT, int ROWS> struct GradOccupancy {
-    static constexpr int value = (KT * 32 + 64) * DP * sizeof(T) <= 65536 && (ROWS == 1 || KT == 1) ? 2 : 1;
+    static constexpr int value = (KT * 32 + 64) * DP * sizeof(T) <= 65536 && (ROWS == 1 || KT == 1 || (sizeof(T) == 2 && DP <= 128)) ? 2 : 1;
 };
 template <typename T, int DP, int KT, int ROWS>
 __global__ __launch_bounds__(256, (GradOccupancy<T, DP, KT, ROWS>::value)) void attn_seq_short_grad_kernel(AttnSeqArgs a) {

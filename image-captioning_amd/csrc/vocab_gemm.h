@@ -75,7 +75,7 @@ struct GemmShape {
 };
 
 // Epi::run(args, acc, p0, q0, lane, part_p, part_q, slice): acc[i][j] = p0 + 32 i.., q0 + 32 j..; parts number the waves' columns and rows
-template <typename T, int S, bool PCOL, bool QCOL, typename Epi> __global__ __launch_bounds__(256) void vocab_gemm_kernel(GemmShape g, typename Epi::Args ea) {
+template <typename T, int S, bool PCOL, bool QCOL, typename Epi> __global__ __launch_bounds__(256, 2) void vocab_gemm_kernel(GemmShape g, typename Epi::Args ea) {
     constexpr int VT = 64 * S, WAVE = 32 * S;
     using TP = OperandTile<T, PCOL, VT>;
     using TQ = OperandTile<T, QCOL, VT>;
@@ -125,26 +125,31 @@ template <typename T, int S, bool PCOL, bool QCOL, typename Epi> __global__ __la
             fp.fetch(g.p, p0, (t + 1) * KS, g.K);
             fq.fetch(g.q, q0, (t + 1) * KS, g.K);
         }
-#pragma unroll
-        for (int s = 0; s < KS / 16; ++s) {
-            Frag8<T> a[S], b[S];
+        // the next step's operands are on their way from LDS while a step's products run
+        Frag8<T> a[2][S], b[2][S];
+        auto load = [&](int s) {
 #pragma unroll
             for (int i = 0; i < S; ++i) {
-                a[i] = TP::frag(sp[cur], wp * WAVE + i * 32, s, lane);
-                b[i] = TQ::frag(sq[cur], wq * WAVE + i * 32, s, lane);
+                a[s & 1][i] = TP::frag(sp[cur], wp * WAVE + i * 32, s, lane);
+                b[s & 1][i] = TQ::frag(sq[cur], wq * WAVE + i * 32, s, lane);
             }
+        };
+        load(0);
+#pragma unroll
+        for (int s = 0; s < KS / 16; ++s) {
+            if (s + 1 < KS / 16) load(s + 1);
             if constexpr (sizeof(T) == 4) {  // the sums in turn: no product waits for the one before
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
 #pragma unroll
                     for (int i = 0; i < S; ++i)
 #pragma unroll
-                        for (int j = 0; j < S; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i].v[e], b[j].v[e], acc[i][j], 0, 0, 0);
+                        for (int j = 0; j < S; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[s & 1][i].v[e], b[s & 1][j].v[e], acc[i][j], 0, 0, 0);
             } else {
 #pragma unroll
                 for (int i = 0; i < S; ++i)
 #pragma unroll
-                    for (int j = 0; j < S; ++j) mma32(a[i], b[j], acc[i][j]);
+                    for (int j = 0; j < S; ++j) mma32(a[s & 1][i], b[s & 1][j], acc[i][j]);
             }
         }
         if (t + 1 < ke) {
