@@ -26,6 +26,7 @@ struct AttnSeqArgs {
     int causal, off;                // query i sees keys up to i + off
     float scale, scale_log2;
     int splits, tiles_per_split;
+    int dq_splits;                  // key ranges of the query gradients
     unsigned group_magic;           // ceil(2^32 / group) where a small x / group is the high half of x times it, else 0
 };
 

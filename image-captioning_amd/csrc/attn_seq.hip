@@ -53,7 +53,7 @@ AttnSeqArgs args_of(const mic_attn_seq_desc* d) {
     a.off = d->Tk - d->Tq;
     a.scale = d->scale;
     a.scale_log2 = d->scale * ATTN_LOG2E;
-    a.splits = 1;
+    a.splits = a.dq_splits = 1;
     a.group_magic = a.group > 1 && a.group <= 1024 ? (unsigned)(((1ull << 32) + a.group - 1) / a.group) : 0;
     return a;
 }
@@ -79,7 +79,9 @@ void split_keys(AttnSeqArgs& a, int dtype) {
     a.splits = (tiles + a.tiles_per_split - 1) / a.tiles_per_split;
 }
 // The key gradients share the rows out in the same way, at least four tiles of 32 rows to a workgroup (one with a single tile of keys).
-void split_rows(AttnSeqArgs& a) {
+void split_rows(AttnSeqArgs& a, int dtype) {
+    split_keys(a, dtype);  // the query gradients' rule is the forward's, whichever kernel takes the forward
+    a.dq_splits = short_grad(a) ? 1 : a.splits;
     const long long base = (long long)((a.Tk + ATTN_SEQ_BLOCK - 1) / ATTN_SEQ_BLOCK) * a.Hkv * a.B;
     const int tiles = (a.R + 31) / 32, least = short_grad(a) ? 1 : 4;
     a.splits = 1;
@@ -96,7 +98,12 @@ long long up256(long long b) { return (b + 255) / 256 * 256; }
 long long fwd_rows(const AttnSeqArgs& a) { return (long long)a.splits * a.B * a.Hkv * a.R; }
 long long fwd_bytes(const AttnSeqArgs& a) { return a.splits > 1 ? up256(fwd_rows(a) * a.D * 4) + up256(fwd_rows(a) * 8) : 0; }
 long long delta_bytes(const AttnSeqArgs& a) { return up256((long long)a.B * a.Hq * a.Tq * 4); }
-long long grad_bytes(const AttnSeqArgs& a) { return delta_bytes(a) + (a.splits > 1 ? up256(2ll * a.splits * a.B * a.Tk * a.Hkv * a.D * 4) : 0); }
+// the partial sums of dQ and, after them, of dK and dV lie in the same place
+long long grad_bytes(const AttnSeqArgs& a) {
+    const long long q = a.dq_splits > 1 ? up256((long long)a.dq_splits * a.B * a.Tq * a.Hq * a.D * 4) : 0;
+    const long long kv = a.splits > 1 ? up256(2ll * a.splits * a.B * a.Tk * a.Hkv * a.D * 4) : 0;
+    return delta_bytes(a) + (q > kv ? q : kv);
+}
 
 }  // namespace
 
@@ -104,7 +111,7 @@ extern "C" int64_t mic_attn_seq_workspace_bytes(const mic_attn_seq_desc* d, int 
     MIC_TRY(check_sizes("mic_attn_seq_workspace_bytes", d));
     AttnSeqArgs a = args_of(d);
     if (grad) {
-        split_rows(a);
+        split_rows(a, d->dtype);
         return grad_bytes(a);
     }
     split_keys(a, d->dtype);
@@ -147,7 +154,7 @@ extern "C" int mic_attn_seq_grad(const mic_attn_seq_desc* d, void* stream) {
     MIC_ARG_CHECK(no_rows || (d->lse && d->dq), "%s: lse or dq is a null pointer", who);
     MIC_ARG_CHECK(no_keys || (d->dk && d->dv), "%s: dk or dv is a null pointer", who);
     MIC_ARG_CHECK((((uintptr_t)d->dq | (uintptr_t)d->dk | (uintptr_t)d->dv) & 15) == 0, "%s: a gradient is not 16-byte aligned", who);
-    split_rows(a);
+    split_rows(a, d->dtype);
     const long long need = grad_bytes(a);
     MIC_ARG_CHECK(need == 0 || (d->workspace && d->workspace_bytes >= need && ((uintptr_t)d->workspace & 15) == 0), "%s: workspace of %lld bytes, %lld needed", who,
                   (long long)d->workspace_bytes, need);

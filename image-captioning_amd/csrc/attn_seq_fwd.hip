@@ -6,12 +6,15 @@
 // the lane 32 away.  P^T then is the B operand of O^T = V^T P^T.
 #include "attn_seq.h"
 
+#include <type_traits>
+
 namespace {
 
 template <typename T, int DP, int BK, bool SPLIT> __global__ __launch_bounds__(256, (DP * sizeof(T) <= 512 ? 2 : 1)) void attn_seq_fwd_kernel(AttnSeqArgs a) {
     constexpr int NC = DP / 16, ND = DP / 32, KT = BK / 32, NR = InRegs<T, DP>::value ? NC : 1, ES = sizeof(T);
-    __shared__ __attribute__((aligned(16))) T sk[2][BK * DP];
-    __shared__ __attribute__((aligned(16))) T sv[2][BK * DP];
+    constexpr int TILE = BK * DP * ES, OFF_K = 0, OFF_V = 2 * TILE;  // two tiles of k, two of v
+    __shared__ __attribute__((aligned(16))) unsigned char smem[4 * TILE];
+    const lds_bytes_t lds = (lds_bytes_t)smem;
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tiles_r = (a.R + ATTN_SEQ_BLOCK - 1) / ATTN_SEQ_BLOCK, heads = a.Hkv * a.B;
     int id = blockIdx.x;
@@ -44,14 +47,16 @@ template <typename T, int DP, int BK, bool SPLIT> __global__ __launch_bounds__(2
     float m = -INFINITY, l = 0.f;
     const T* kb = (const T*)a.k + b * a.k_sb + hk * a.k_sh;
     const T* vb = (const T*)a.v + b * a.v_sb + hk * a.v_sh;
-    const unsigned k_row = (unsigned)(a.k_st * ES), v_row = (unsigned)(a.v_st * ES), lds_k = lds_address(sk), lds_v = lds_address(sv);
+    const unsigned k_row = (unsigned)(a.k_st * ES), v_row = (unsigned)(a.v_st * ES), lds0 = lds_address(smem);
+    TileReader<T, DP> read;
+    read.init(lane);
     // rows no query may see are zeros: whatever they hold, infinities and NaN included, stays out of the products
     auto request = [&](int t, int buf, const unsigned (&seen)[KT]) {
         auto row = [&](unsigned stride) {
             return [&, stride](int x) { return (seen[x >> 5] >> (x & 31)) & 1 ? x * stride : 0x80000000u; };
         };
-        request_tile<T, DP, BK>(kb + (long long)t * BK * a.k_st, lds_k + buf * BK * DP * ES, a.D, wave, lane, row(k_row));
-        request_tile<T, DP, BK>(vb + (long long)t * BK * a.v_st, lds_v + buf * BK * DP * ES, a.D, wave, lane, row(v_row));
+        request_tile<T, DP, BK>(kb + (long long)t * BK * a.k_st, lds0 + OFF_K + buf * TILE, a.D, wave, lane, row(k_row));
+        request_tile<T, DP, BK>(vb + (long long)t * BK * a.v_st, lds0 + OFF_V + buf * TILE, a.D, wave, lane, row(v_row));
     };
     unsigned bits[KT], next[KT];
 #pragma unroll
@@ -60,10 +65,12 @@ template <typename T, int DP, int BK, bool SPLIT> __global__ __launch_bounds__(2
         next[kt] = key_bits(a, b, (t0 + 1) * BK + kt * 32, lane);
     }
     if (t0 < t1) request(t0, 0, bits);
-    for (int t = t0; t < t1; ++t) {
-        const int k0 = t * BK, cur = (t - t0) & 1;
+    // one tile out of buffer CUR
+    auto step = [&](auto which, int t) {
+        constexpr int CUR = decltype(which)::value;
+        const int k0 = t * BK;
         tile_landed();
-        if (t + 1 < t1) request(t + 1, cur ^ 1, next);
+        if (t + 1 < t1) request(t + 1, CUR ^ 1, next);
         bool ok[KT];  // the tile after the next
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) ok[kt] = key_seen(a, b, k0 + 2 * BK + kt * 32 + (lane & 31));
@@ -75,7 +82,7 @@ template <typename T, int DP, int BK, bool SPLIT> __global__ __launch_bounds__(2
                 s[kt] = f32x16_t{};
 #pragma unroll
                 for (int c = 0; c < NC; ++c)
-                    mma32(read_row<DP>(sk[cur], kt * 32 + (lane & 31), c, h), InRegs<T, DP>::value ? qf[c % NR] : load_frag<T>(qrow, 16 * c + 8 * h, a.D), s[kt]);
+                    mma32(read.rows(lds, OFF_K + CUR * TILE + kt * 32 * DP * ES, c), InRegs<T, DP>::value ? qf[c % NR] : load_frag<T>(qrow, 16 * c + 8 * h, a.D), s[kt]);
                 if (bits[kt] == 0xffffffffu && k0 + kt * 32 + 31 <= w_all) {  // nothing hidden: the common case
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
@@ -120,7 +127,7 @@ template <typename T, int DP, int BK, bool SPLIT> __global__ __launch_bounds__(2
                 for (int j = 0; j < 2; ++j) {
                     const Frag8<T> p = frag_of<T>(s[kt], j);  // bf16: the probabilities are rounded for the product, the sum l is not
 #pragma unroll
-                    for (int d = 0; d < ND; ++d) mma32(read_col<DP>(sv[cur], d * 32, kt * 32 + 16 * j, lane), p, acc[d]);
+                    for (int d = 0; d < ND; ++d) mma32(read.cols(lds, OFF_V + CUR * TILE, d, kt * 32 + 16 * j), p, acc[d]);
                 }
         }
 #pragma unroll
@@ -128,6 +135,10 @@ template <typename T, int DP, int BK, bool SPLIT> __global__ __launch_bounds__(2
             bits[kt] = next[kt];
             next[kt] = (unsigned)__ballot(ok[kt]);
         }
+    };
+    for (int t = t0; t < t1; t += 2) {
+        step(std::integral_constant<int, 0>{}, t);
+        if (t + 1 < t1) step(std::integral_constant<int, 1>{}, t + 1);
     }
     if (!row_ok) return;
     if (SPLIT) {
