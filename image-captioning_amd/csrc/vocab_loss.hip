@@ -365,56 +365,76 @@ struct OutEpi8 {
     }
 };
 
+// ---- the sums of partial results, by block number in one launch ---------------------------------------------------------------------
 // out[row] = the sum of fp32 rows at[row] (NULL: the row itself; negative: zeros) of the partial matrices, in order: `pieces` groups of
 // `most` matrices `stride` elements apart, of which the first *slices (of the last group: *slices_last) were written
-template <typename T> __global__ __launch_bounds__(256) void vocab_sum_parts_kernel(const float* __restrict__ part, T* __restrict__ out, const int* __restrict__ at, int rows,
-                                                                                    int cols, long long stride, int pieces, int most, const int* __restrict__ slices,
-                                                                                    const int* __restrict__ slices_last) {
-    const int quads = (cols + 3) / 4;
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+struct SumParts {
+    const float* part;
+    void* out;
+    const int *at, *slices, *slices_last;
+    long long stride;
+    int rows, cols, pieces, most;
+    unsigned blocks;  // 0: nothing to do
+};
+template <typename T> __device__ __forceinline__ void sum_parts(const SumParts& a, unsigned block) {
+    const int quads = (a.cols + 3) / 4;
+    const long long i = (long long)block * 256 + threadIdx.x;
     const int row = (int)(i / quads), c = (int)(i - (long long)row * quads) * 4;
-    if (row >= rows) return;
-    const int src = at ? at[row] : row, whole = *slices, last = *slices_last;
+    if (row >= a.rows) return;
+    const int src = a.at ? a.at[row] : row, whole = *a.slices, last = *a.slices_last;
     float s[4] = {};
     if (src >= 0) {
-        for (int g = 0; g < pieces; ++g) {
-            const float* p = part + (long long)g * most * stride + (long long)src * cols + c;
-            const int parts = g == pieces - 1 ? last : whole;
-            if (cols % 4 == 0) {
+        for (int g = 0; g < a.pieces; ++g) {
+            const float* p = a.part + (long long)g * a.most * a.stride + (long long)src * a.cols + c;
+            const int parts = g == a.pieces - 1 ? last : whole;
+            if (a.cols % 4 == 0) {
 #pragma unroll 8
                 for (int k = 0; k < parts; ++k) {
-                    const float4 x = *reinterpret_cast<const float4*>(p + k * stride);
+                    const float4 x = *reinterpret_cast<const float4*>(p + k * a.stride);
                     s[0] += x.x; s[1] += x.y; s[2] += x.z; s[3] += x.w;
                 }
             } else {
-                for (int e = 0; e < 4 && c + e < cols; ++e)
-                    for (int k = 0; k < parts; ++k) s[e] += p[k * stride + e];
+                for (int e = 0; e < 4 && c + e < a.cols; ++e)
+                    for (int k = 0; k < parts; ++k) s[e] += p[k * a.stride + e];
             }
         }
     }
-    T* o = out + (long long)row * cols + c;
-    if (cols % 4 == 0) store4<T>(o, s[0], s[1], s[2], s[3]);
+    T* o = (T*)a.out + (long long)row * a.cols + c;
+    if (a.cols % 4 == 0) store4<T>(o, s[0], s[1], s[2], s[3]);
     else
-        for (int e = 0; e < 4 && c + e < cols; ++e) o[e] = from_f32<T>(s[e]);
+        for (int e = 0; e < 4 && c + e < a.cols; ++e) o[e] = from_f32<T>(s[e]);
 }
-
-// column sums of a [parts][n] matrix: 64 columns to a workgroup, 16 waves share the rows, added in order
-__global__ __launch_bounds__(1024) void vocab_colsum_kernel(const float* __restrict__ part, float* __restrict__ out, int n, int parts, const int* __restrict__ rows, int row_tile) {
-    __shared__ float sum[16][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
-    if (rows) parts = min(parts, (*rows + row_tile - 1) / row_tile);  // parts of the gathered rows alone were written
-    const int lo = (int)((long long)parts * wave / 16), hi = (int)((long long)parts * (wave + 1) / 16);
+// column sums of a [parts][n] matrix: 16 columns to a workgroup, 16 groups of threads share the rows, added in order
+struct ColSum {
+    const float* part;
+    float* out;
+    const int* rows;  // NULL, or the gathered rows there are: parts of row_tile rows beyond them were not written
+    int n, parts, row_tile;
+    unsigned blocks;
+};
+__device__ __forceinline__ void column_sums(const ColSum& a, unsigned block) {
+    __shared__ float sum[16][17];
+    const int lane = threadIdx.x & 15, group = threadIdx.x >> 4, c = block * 16 + lane;
+    const int parts = a.rows ? min(a.parts, (*a.rows + a.row_tile - 1) / a.row_tile) : a.parts;
+    const int lo = (int)((long long)parts * group / 16), hi = (int)((long long)parts * (group + 1) / 16);
     float s = 0.f;
 #pragma unroll 8
-    for (int k = lo; k < hi; ++k) s += c < n ? part[(long long)k * n + c] : 0.f;
-    sum[wave][lane] = s;
+    for (int k = lo; k < hi; ++k) s += c < a.n ? a.part[(long long)k * a.n + c] : 0.f;
+    sum[group][lane] = s;
     __syncthreads();
-    if (wave == 0 && c < n) {
+    if (group == 0 && c < a.n) {
         s = sum[0][lane];
 #pragma unroll
         for (int w = 1; w < 16; ++w) s += sum[w][lane];
-        out[c] = s;
+        a.out[c] = s;
     }
+}
+template <typename T> __global__ __launch_bounds__(256) void vocab_finish_kernel(SumParts x, SumParts y, ColSum b) {
+    unsigned block = blockIdx.x;
+    if (block < b.blocks) return column_sums(b, block);
+    block -= b.blocks;
+    if (block < x.blocks) return sum_parts<T>(x, block);
+    sum_parts<T>(y, block - x.blocks);
 }
 
 // ---- the rows of the gradient ------------------------------------------------------------------------------------------------------
@@ -430,18 +450,21 @@ struct SplitRule {
 struct Split {
     int tiles, nk, most;    // tiles of the result (dx: per tile of rows), steps of k (dw: 0, by the rows), ranges allowed
 };
-__device__ __forceinline__ int choose_slices(const SplitRule& r, int tiles, int nk, int most) {
-    int best = 1;
-    float least = INFINITY;
-    for (int s = 1; s <= most; ++s) {
-        const float x = (float)tiles * s / r.capacity;
-        const float cost = ceilf(x) * (ceilf((float)nk / s) + r.fixed) + (s > 1 ? x * r.traffic : 0.f);
-        if (cost < least) {
-            least = cost;
-            best = s;
+// 16 lanes to a decision, lane i looks at i + 1 ranges; the cheapest, the smaller number where two cost the same, ends in all of them
+__device__ __forceinline__ int choose_slices(const SplitRule& r, int tiles, int nk, int most, int lane) {
+    int s = (lane & 15) + 1;
+    const float x = (float)tiles * s / r.capacity;
+    float cost = s <= most ? ceilf(x) * (ceilf((float)nk / s) + r.fixed) + (s > 1 ? x * r.traffic : 0.f) : INFINITY;
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1) {
+        const float c = __shfl_xor(cost, d, 64);
+        const int o = __shfl_xor(s, d, 64);
+        if (c < cost || (c == cost && o < s)) {
+            cost = c;
+            s = o;
         }
     }
-    return best;
+    return s;
 }
 enum { COUNT, SX, SX_LAST, SW, SW_LAST, DECISIONS };  // what `count` points to
 struct RowsArgs {
@@ -494,12 +517,13 @@ __global__ __launch_bounds__(1024) void vocab_rows_kernel(RowsArgs a) {
             }
         }
     }
-    if (blockIdx.x == gridDim.x - 1 && tid < DECISIONS) {
-        const int rows = a.gather ? base : a.N, i = (tid - 1) & 1;
-        int v = rows;
-        if (tid == SX || tid == SX_LAST) v = choose_slices(a.rule, a.dx[i].tiles * ((rows + a.edge - 1) / a.edge), a.dx[i].nk, a.dx[i].most);
-        if (tid == SW || tid == SW_LAST) v = choose_slices(a.rule, a.dw[i].tiles, (rows + a.ks - 1) / a.ks, a.dw[i].most);
-        a.count[tid] = v;
+    if (blockIdx.x == gridDim.x - 1 && wave == 0) {
+        const int rows = a.gather ? base : a.N, i = (lane >> 4) & 1;  // dx, dx last, dw, dw last
+        const bool is_dw = lane >= 32;
+        const int s = choose_slices(a.rule, is_dw ? a.dw[i].tiles : a.dx[i].tiles * ((rows + a.edge - 1) / a.edge), is_dw ? (rows + a.ks - 1) / a.ks : a.dx[i].nk,
+                                    is_dw ? a.dw[i].most : a.dx[i].most, lane);
+        if ((lane & 15) == 0) a.count[SX + (lane >> 4)] = s;
+        if (lane == 0) a.count[COUNT] = rows;
     }
 }
 
@@ -717,10 +741,13 @@ template <typename T> int gradient(const mic_vocab_loss_desc* d, const Plan& p, 
     T* dl = (T*)(ws + p.d);
     float *part_dx = (float*)(ws + p.dx), *part_dw = (float*)(ws + p.dw), *part_db = (float*)(ws + p.db);
     const bool dx_parts = p.sx * p.pieces > 1 || p.gather;
-    auto sum_parts = [&](const float* part, T* out, const int* where, int rows, long long stride, int pieces, int most, int whole, int end) -> int {
+    auto parts_of = [&](const float* part, T* out, const int* where, int rows, long long stride, int pieces, int most, int whole, int end) {
         const long long quads = (long long)rows * ((H + 3) / 4);
-        MIC_LAUNCH((vocab_sum_parts_kernel<T>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s, part, out, where, rows, d->H, stride, pieces, most,
-                   (const int*)ra.count + whole, (const int*)ra.count + end);
+        return SumParts{part, out, where, ra.count + whole, ra.count + end, stride, rows, d->H, pieces, most, (unsigned)((quads + 255) / 256)};
+    };
+    auto finish = [&](const SumParts& x1, const SumParts& x2, const ColSum& c) -> int {
+        const unsigned blocks = x1.blocks + x2.blocks + c.blocks;
+        if (blocks) MIC_LAUNCH((vocab_finish_kernel<T>), dim3(blocks), dim3(256), 0, s, x1, x2, c);
         return 0;
     };
     for (int i = 0; i < p.pieces; ++i) {
@@ -733,8 +760,6 @@ template <typename T> int gradient(const mic_vocab_loss_desc* d, const Plan& p, 
         ga.N = d->N; ga.Vc = vc; ga.ld = p.ld; ga.v0 = v0;
         ga.count = count;
         MIC_TRY((product<T, false, false, GradEpi<T>, GradEpi8>(p, wi, x, Rows{count, 0, nullptr, 1}, d->H, ga, s)));
-        if (d->db)
-            MIC_LAUNCH(vocab_colsum_kernel, dim3((vc + 63) / 64), dim3(1024), 0, s, (const float*)part_db, d->db + v0, vc, edge_tiles(N, p.edge) * 2, count, p.edge / 2);
         // dx += d w: k runs over the words of the piece
         typename OutEpi<T>::Args xa = {};
         xa.out = (T*)d->dx; xa.ld = H; xa.Np = d->H; xa.Nq = d->N;
@@ -749,9 +774,13 @@ template <typename T> int gradient(const mic_vocab_loss_desc* d, const Plan& p, 
         const Operand xc = {x.p, x.ld, d->H}, dc = {dl, p.ld, vc};
         const Rows rw = {count, 1, p.sw > 1 ? ra.count + (end ? SW_LAST : SW) : nullptr, p.sw};
         MIC_TRY((product<T, true, true, OutEpi<T>, OutEpi8>(p, xc, dc, rw, d->N, wa, s)));
-        if (p.sw > 1) MIC_TRY(sum_parts(part_dw, wa.out, nullptr, vc, vc * H, 1, p.sw, SW, end ? SW_LAST : SW));
+        SumParts sw = {}, sx = {};
+        ColSum sb = {};
+        if (p.sw > 1) sw = parts_of(part_dw, wa.out, nullptr, vc, vc * H, 1, p.sw, SW, end ? SW_LAST : SW);
+        if (d->db) sb = {part_db, d->db + v0, count, vc, edge_tiles(N, p.edge) * 2, p.edge / 2, (unsigned)((vc + 15) / 16)};
+        if (end && dx_parts) sx = parts_of(part_dx, (T*)d->dx, at, d->N, N * H, p.pieces, p.sx, SX, SX_LAST);
+        MIC_TRY(finish(sx, sw, sb));
     }
-    if (dx_parts) MIC_TRY(sum_parts(part_dx, (T*)d->dx, at, d->N, N * H, p.pieces, p.sx, SX, SX_LAST));
     return 0;
 }
 
