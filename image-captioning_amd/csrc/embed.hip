@@ -26,55 +26,78 @@ __device__ __forceinline__ int load_id(const void* ids, int wide, long long i, i
     return v < 0 ? 0 : (v >= vocab ? vocab - 1 : (int)v);  // never index outside the table
 }
 
-// VEC consecutive elements as fp32: one 16-byte access (two for 8 floats) where VEC > 1
-template <typename T, int VEC> __device__ __forceinline__ void load_vec(const T* p, float (&v)[VEC]) {
-    if constexpr (VEC == 1) {
-        v[0] = to_f32<T>(*p);
-    } else {
-        constexpr int E = Vec16<T>::N;
+// Eight columns at a time, whatever H and the alignment are: A = rows are whole 16-byte pieces on 16-byte boundaries; else only the first n of
+// the eight belong to the row, and the vector access takes any address (HSA devices run with unaligned access on).
+constexpr int VEC = 8;
+template <typename T, bool A> __device__ __forceinline__ void load8(const T* p, int n, float (&v)[VEC]) {
+    if (A || n >= VEC) {
+        T x[VEC];
+        if constexpr (A) {
 #pragma unroll
-        for (int c = 0; c < VEC / E; ++c) {
-            const Vec16<T> x = ld16(p + c * E);
+            for (int c = 0; c < VEC / Vec16<T>::N; ++c) {
+                const Vec16<T> y = ld16(p + c * Vec16<T>::N);
 #pragma unroll
-            for (int e = 0; e < E; ++e) v[c * E + e] = to_f32<T>(x.v[e]);
+                for (int e = 0; e < Vec16<T>::N; ++e) x[c * Vec16<T>::N + e] = y.v[e];
+            }
+        } else {
+            __builtin_memcpy(x, p, sizeof(x));
         }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = to_f32<T>(x[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = e < n ? to_f32<T>(p[e]) : 0.f;
     }
 }
-template <typename T, int VEC> __device__ __forceinline__ void store_vec(T* p, const float (&v)[VEC]) {
-    if constexpr (VEC == 1) {
-        *p = from_f32<T>(v[0]);
-    } else {
-        constexpr int E = Vec16<T>::N;
+// The same from a row of a matrix that ends at `end`: what follows the row is the next one, so the vector access is safe for all but
+// the last columns of the matrix, and the columns past n are never stored.
+template <typename T, bool A> __device__ __forceinline__ void load8_before(const T* p, const T* end, int n, float (&v)[VEC]) {
+    load8<T, A>(p, A || p + VEC <= end ? VEC : n, v);
+}
+template <typename T, bool A> __device__ __forceinline__ void store8(T* p, int n, const float (&v)[VEC]) {
+    if (A || n >= VEC) {
+        if constexpr (A) {
 #pragma unroll
-        for (int c = 0; c < VEC / E; ++c) {
-            Vec16<T> x;
+            for (int c = 0; c < VEC / Vec16<T>::N; ++c) {
+                Vec16<T> y;
 #pragma unroll
-            for (int e = 0; e < E; ++e) x.v[e] = from_f32<T>(v[c * E + e]);
-            st16(p + c * E, x);
+                for (int e = 0; e < Vec16<T>::N; ++e) y.v[e] = from_f32<T>(v[c * Vec16<T>::N + e]);
+                st16(p + c * Vec16<T>::N, y);
+            }
+        } else {
+            T x[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) x[e] = from_f32<T>(v[e]);
+            __builtin_memcpy(p, x, sizeof(x));
         }
+    } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+            if (e < n) p[e] = from_f32<T>(v[e]);
     }
 }
 
-// ---- lookup: one thread per VEC columns of a row -------------------------------------------------------------------------
-template <typename TT, typename TO, int VEC, typename I>
+// ---- lookup: one thread per eight columns of a row ---------------------------------------------------------------------------
+template <typename TT, typename TO, bool A, typename I>
 __global__ __launch_bounds__(256) void embed_rows_kernel(const void* __restrict__ ids, int wide, const TT* __restrict__ table, long long ld_table,
                                                          const TT* __restrict__ pos, long long ld_pos, TO* __restrict__ out, float scale,
                                                          long long n, int T, int H, int vocab) {
-    const I per_row = H / VEC, total = (I)n * per_row, stride = (I)gridDim.x * 256;
+    const I per_row = (H + VEC - 1) / VEC, total = (I)n * per_row, stride = (I)gridDim.x * 256;
+    const TT *table_end = table + (vocab - 1) * ld_table + H, *pos_end = pos ? pos + (T - 1) * ld_pos + H : nullptr;
     for (I i = (I)blockIdx.x * 256 + threadIdx.x; i < total; i += stride) {
         const I r = i / per_row;
-        const int c = (int)(i - r * per_row) * VEC;
+        const int c = (int)(i - r * per_row) * VEC, m = H - c;
         float v[VEC];
-        load_vec<TT, VEC>(table + load_id(ids, wide, r, vocab) * ld_table + c, v);
+        load8_before<TT, A>(table + load_id(ids, wide, r, vocab) * ld_table + c, table_end, m, v);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) v[e] *= scale;
         if (pos) {
             float p[VEC];
-            load_vec<TT, VEC>(pos + (long long)(r % (I)T) * ld_pos + c, p);
+            load8_before<TT, A>(pos + (long long)(r % (I)T) * ld_pos + c, pos_end, m, p);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) v[e] += p[e];
         }
-        store_vec<TO, VEC>(out + (long long)r * H + c, v);
+        store8<TO, A>(out + (long long)r * H + c, m, v);
     }
 }
 
@@ -187,9 +210,9 @@ struct SumArgs {
     const int *key, *idx;   // sorted words and the tokens they stand for
     const void* g;
     void* d_table;
-    float *head, *tail;     // [chunks][H] partial rows of runs that began before the chunk / go on after it
+    float *head, *tail;     // [chunks][Hs] partial rows of runs that began before the chunk / go on after it
     long long n;
-    int H, vocab, chunk, chunks, slabs;
+    int H, Hs, vocab, chunk, chunks, slabs;  // Hs: H rounded up to eight columns
     int cleared;            // the rows of words that do not occur are cleared already
     float scale;
 };
@@ -207,10 +230,10 @@ __device__ __forceinline__ int lower_bound_key(const int* key, int n, int v) {
 
 // A wave takes one chunk of the sorted list and one slab of 64*VEC columns; the waves behind those clear the rows of words that
 // do not occur, 64 rows each.
-template <typename TG, typename TO, int VEC> __global__ __launch_bounds__(256) void embed_sum_kernel(SumArgs a) {
+template <typename TG, typename TO, bool A> __global__ __launch_bounds__(256) void embed_sum_kernel(SumArgs a) {
     const int lane = threadIdx.x & 63;
     const long long unit = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), sums = (long long)a.chunks * a.slabs;
-    const TG* g = (const TG*)a.g;
+    const TG *g = (const TG*)a.g, *g_end = g + a.n * a.H;
     TO* dt = (TO*)a.d_table;
     if (unit >= sums) {
         const long long v0 = (unit - sums) * 64;
@@ -226,13 +249,13 @@ template <typename TG, typename TO, int VEC> __global__ __launch_bounds__(256) v
         while (todo) {
             const int r = __ffsll((unsigned long long)todo) - 1;
             todo &= todo - 1;
-            for (int c = lane * VEC; c < a.H; c += 64 * VEC) store_vec<TO, VEC>(dt + (v0 + r) * a.H + c, zero);
+            for (int c = lane * VEC; c < a.H; c += 64 * VEC) store8<TO, A>(dt + (v0 + r) * a.H + c, a.H - c, zero);
         }
         return;
     }
     const int chunk = (int)(unit / a.slabs), slab = (int)(unit - (long long)chunk * a.slabs);
-    const int col = (slab * 64 + lane) * VEC;
-    const bool live = col < a.H;
+    const int col = (slab * 64 + lane) * VEC, m = a.H - col;
+    const bool live = m > 0;
     const int i0 = chunk * a.chunk, i1 = i0 + a.chunk < (int)a.n ? i0 + a.chunk : (int)a.n;
     const bool cont_in = i0 > 0 && a.key[i0 - 1] == a.key[i0];
     const bool cont_out = i1 < (int)a.n && a.key[i1] == a.key[i1 - 1];
@@ -249,7 +272,7 @@ template <typename TG, typename TO, int VEC> __global__ __launch_bounds__(256) v
         for (int u = 0; u < U; ++u) {
             const int j = i + u < rows ? i + u : rows - 1;
             const long long row = __builtin_amdgcn_readlane(my_idx, j);
-            if (live) load_vec<TG, VEC>(g + row * a.H + col, v[u]);
+            if (live) load8_before<TG, A>(g + row * a.H + col, g_end, m, v[u]);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -259,8 +282,8 @@ template <typename TG, typename TO, int VEC> __global__ __launch_bounds__(256) v
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) acc[e] = first && cont_in ? acc[e] : acc[e] * a.scale;
                 if (live) {
-                    if (first && cont_in) store_vec<float, VEC>(a.head + (long long)chunk * a.H + col, acc);
-                    else store_vec<TO, VEC>(dt + (long long)word * a.H + col, acc);
+                    if (first && cont_in) store8<float, true>(a.head + (long long)chunk * a.Hs + col, m, acc);
+                    else store8<TO, A>(dt + (long long)word * a.H + col, m, acc);
                 }
                 first = false;
                 word = w;
@@ -273,13 +296,13 @@ template <typename TG, typename TO, int VEC> __global__ __launch_bounds__(256) v
     }
     if (!live) return;
     if (first && cont_in) {
-        store_vec<float, VEC>(a.head + (long long)chunk * a.H + col, acc);
+        store8<float, true>(a.head + (long long)chunk * a.Hs + col, m, acc);
     } else if (cont_out) {
-        store_vec<float, VEC>(a.tail + (long long)chunk * a.H + col, acc);
+        store8<float, true>(a.tail + (long long)chunk * a.Hs + col, m, acc);
     } else {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) acc[e] *= a.scale;
-        store_vec<TO, VEC>(dt + (long long)word * a.H + col, acc);
+        store8<TO, A>(dt + (long long)word * a.H + col, m, acc);
     }
 }
 
@@ -289,23 +312,27 @@ template <typename TG, typename TO, int VEC> __global__ __launch_bounds__(256) v
 // multiple of it and the first such in the run.
 constexpr int JOIN_LONG = 32;
 
-template <int VEC> __device__ __forceinline__ void add_partials(const SumArgs& a, int owner, int lo, int hi, int col, bool live, float (&acc)[VEC]) {
-    constexpr int U = VEC == 1 ? 16 : 8;
+// W columns of a lane (8, or 1 where a run is long)
+template <int W> __device__ __forceinline__ void add_partials(const SumArgs& a, int owner, int lo, int hi, int col, bool live, float (&acc)[W]) {
+    constexpr int U = W == 1 ? 16 : 8;
     for (int k = lo; k < hi; k += U) {
-        float v[U][VEC];
+        float v[U][W];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int j = k + u < hi ? k + u : hi - 1;
-            if (live) load_vec<float, VEC>((j == 0 ? a.tail : a.head) + (long long)(owner + j) * a.H + col, v[u]);
+            if (!live) continue;
+            const float* p = (j == 0 ? a.tail : a.head) + (long long)(owner + j) * a.Hs + col;
+            if constexpr (W == 1) v[u][0] = *p;
+            else load8<float, true>(p, W, v[u]);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) acc[e] += live && k + u < hi ? v[u][e] : 0.f;
+            for (int e = 0; e < W; ++e) acc[e] += live && k + u < hi ? v[u][e] : 0.f;
     }
 }
 
-template <typename TO, int VEC> __global__ __launch_bounds__(1024) void embed_join_kernel(SumArgs a, int long_blocks) {
+template <typename TO, bool A> __global__ __launch_bounds__(1024) void embed_join_kernel(SumArgs a, int long_blocks) {
     __shared__ float part[16][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     TO* dt = (TO*)a.d_table;
@@ -326,7 +353,7 @@ template <typename TO, int VEC> __global__ __launch_bounds__(1024) void embed_jo
         add_partials<VEC>(a, chunk, 0, m, col, live, acc);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) acc[e] *= a.scale;
-        if (live) store_vec<TO, VEC>(dt + (long long)word * a.H + col, acc);
+        if (live) store8<TO, A>(dt + (long long)word * a.H + col, a.H - col, acc);
         return;
     }
     // 64 columns each, so that a run's partial rows are read by several compute units
@@ -368,45 +395,49 @@ template <typename TO, int VEC> __global__ __launch_bounds__(1024) void embed_jo
 }
 
 // ---- sum over sequences: columns of a [B][W] matrix, W = T*H; `slices` of the rows leave fp32 partial rows when there are several
-template <typename TG, typename TO, int VEC>
+// (N columns to a lane: 8, or 1)
+template <typename TG, typename TO, int N, bool A>
 __device__ __forceinline__ void colsum(float* part, const TG* __restrict__ g, TO* __restrict__ out, float* __restrict__ part_out, int B, long long W, int slices,
                                        long long group, int slice) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long long col = (group * 64 + lane) * VEC;
+    const long long col = (group * 64 + lane) * N;
     const bool live = col < W;
+    const int m = W - col < N ? (int)(W - col) : N;
     const int b0 = (int)((long long)B * slice / slices), b1 = (int)((long long)B * (slice + 1) / slices), rows = b1 - b0;
     const int lo = b0 + (int)((long long)rows * wave / 16), hi = b0 + (int)((long long)rows * (wave + 1) / 16);
-    float acc[VEC] = {};
+    float acc[N] = {};
     constexpr int U = 8;
     for (int b = lo; b < hi; b += U) {
-        float v[U][VEC];
+        float v[U][N];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int j = b + u < hi ? b + u : hi - 1;
-            if (live) load_vec<TG, VEC>(g + j * W + col, v[u]);
+            if (!live) continue;
+            if constexpr (N == 1) v[u][0] = to_f32<TG>(g[j * W + col]);
+            else load8<TG, A>(g + j * W + col, m, v[u]);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) acc[e] += live && b + u < hi ? v[u][e] : 0.f;
+            for (int e = 0; e < N; ++e) acc[e] += live && b + u < hi ? v[u][e] : 0.f;
     }
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) part[wave * 64 * VEC + lane * VEC + e] = acc[e];
+    for (int e = 0; e < N; ++e) part[wave * 64 * N + lane * N + e] = acc[e];
     __syncthreads();
-    // 64 * VEC columns over 1024 threads
-    for (int c = threadIdx.x; c < 64 * VEC; c += 1024) {
-        const long long at = group * 64 * VEC + c;
+    // 64 * N columns over 1024 threads
+    for (int c = threadIdx.x; c < 64 * N; c += 1024) {
+        const long long at = group * 64 * N + c;
         if (at >= W) continue;
         float s = part[c];
 #pragma unroll
-        for (int w = 1; w < 16; ++w) s += part[w * 64 * VEC + c];
+        for (int w = 1; w < 16; ++w) s += part[w * 64 * N + c];
         if (slices == 1) out[at] = from_f32<TO>(s);
         else part_out[slice * W + at] = s;
     }
 }
 template <typename TO> __global__ __launch_bounds__(1024) void embed_colsum_join_kernel(const float* __restrict__ part_in, TO* __restrict__ out, int parts, long long W) {
     __shared__ float part[16 * 64];
-    colsum<float, TO, 1>(part, part_in, out, nullptr, parts, W, 1, blockIdx.x, 0);
+    colsum<float, TO, 1, true>(part, part_in, out, nullptr, parts, W, 1, blockIdx.x, 0);
 }
 
 // ---- the first launch of the gradient: three jobs that need nothing from each other, by block number -------------------------
@@ -425,7 +456,7 @@ struct FirstArgs {
 constexpr int RANK_MAX = 8192, RANK_TOKENS = 32, ZERO_ROWS = 128;
 constexpr int RANK_MAX_VOCAB = 1 << 18;  // word and token number share 31 bits
 
-template <typename TG, typename TO, int VEC> __global__ __launch_bounds__(1024) void embed_first_kernel(FirstArgs f) {
+template <typename TG, typename TO, bool A> __global__ __launch_bounds__(1024) void embed_first_kernel(FirstArgs f) {
     __shared__ __attribute__((aligned(16))) unsigned lds[RANK_MAX + 1024];  // 36 KiB, also the column sums' 16 x 64 x VEC floats
     static_assert(16 * 64 * VEC <= RANK_MAX + 1024, "column sums fit");
     const SortArgs& a = f.sort;
@@ -474,12 +505,12 @@ template <typename TG, typename TO, int VEC> __global__ __launch_bounds__(1024) 
         const float zero[VEC] = {};
         for (int r = wave; r < ZERO_ROWS && v0 + r < a.vocab; r += 16) {
             if (lds[r]) continue;
-            for (int c = lane * VEC; c < f.H; c += 64 * VEC) store_vec<TO, VEC>((TO*)f.d_table + (long long)(v0 + r) * f.H + c, zero);
+            for (int c = lane * VEC; c < f.H; c += 64 * VEC) store8<TO, A>((TO*)f.d_table + (long long)(v0 + r) * f.H + c, f.H - c, zero);
         }
         return;
     }
     block -= f.zero_blocks;
-    colsum<TG, TO, VEC>(reinterpret_cast<float*>(lds), (const TG*)f.g, (TO*)f.d_pos, f.pos_part, f.B, f.W, f.slices, block % f.groups, (int)(block / f.groups));
+    colsum<TG, TO, VEC, A>(reinterpret_cast<float*>(lds), (const TG*)f.g, (TO*)f.d_pos, f.pos_part, f.B, f.W, f.slices, block % f.groups, (int)(block / f.groups));
 }
 
 // ---- the gradient's plan: everything that depends on the sizes alone -------------------------------------------------------
@@ -515,8 +546,9 @@ GradPlan grad_plan(long long n, int T, int H, int vocab, bool want_pos) {
         p.idx[i] = o; o += up256(n * 4);
     }
     p.hist = o; o += up256((long long)p.sort_blocks * MAX_DIGITS * 4);
-    p.head = o; o += up256((long long)p.chunks * H * 4);
-    p.tail = o; o += up256((long long)p.chunks * H * 4);
+    const long long row = (H + VEC - 1) / VEC * VEC * 4;
+    p.head = o; o += up256(p.chunks * row);
+    p.tail = o; o += up256(p.chunks * row);
     p.slices = 1;
     if (want_pos) {
         // up to 256 workgroups over the columns of [B][T*H], at least 512 sequences to a slice
@@ -533,7 +565,7 @@ GradPlan grad_plan(long long n, int T, int H, int vocab, bool want_pos) {
 
 bool ok_dtype(int d) { return d == MIC_F32 || d == MIC_BF16; }
 
-template <typename TG, typename TO, int VEC>
+template <typename TG, typename TO, bool A>
 int launch_grad(const GradPlan& p, const void* ids, int wide, const void* g, void* d_table, void* d_pos, float scale, long long n, int T, int H, int vocab,
                 char* ws, hipStream_t s) {
     SortArgs a = {};
@@ -557,7 +589,7 @@ int launch_grad(const GradPlan& p, const void* ids, int wide, const void* g, voi
         f.groups = (f.W + 64 * VEC - 1) / (64 * VEC);
     }
     const long long first = f.rank_blocks + f.zero_blocks + f.groups * f.slices;
-    if (first > 0) MIC_LAUNCH((embed_first_kernel<TG, TO, VEC>), dim3((unsigned)first), dim3(1024), 0, s, f);
+    if (first > 0) MIC_LAUNCH((embed_first_kernel<TG, TO, A>), dim3((unsigned)first), dim3(1024), 0, s, f);
     if (d_pos && p.slices > 1)
         MIC_LAUNCH((embed_colsum_join_kernel<TO>), dim3((unsigned)((f.W + 63) / 64)), dim3(1024), 0, s, (const float*)f.pos_part, (TO*)d_pos, p.slices, f.W);
     const int passes = p.rank ? 1 : p.passes;
@@ -577,14 +609,14 @@ int launch_grad(const GradPlan& p, const void* ids, int wide, const void* g, voi
     m.idx = (const int*)(ws + p.idx[(passes - 1) & 1]);
     m.g = g; m.d_table = d_table;
     m.head = (float*)(ws + p.head); m.tail = (float*)(ws + p.tail);
-    m.n = n; m.H = H; m.vocab = vocab; m.chunk = p.chunk; m.chunks = p.chunks; m.scale = scale; m.cleared = p.rank;
+    m.n = n; m.H = H; m.Hs = (H + VEC - 1) / VEC * VEC; m.vocab = vocab; m.chunk = p.chunk; m.chunks = p.chunks; m.scale = scale; m.cleared = p.rank;
     m.slabs = (H + 64 * VEC - 1) / (64 * VEC);
     const long long units = (long long)p.chunks * m.slabs + (p.rank ? 0 : (vocab + 63) / 64);
-    MIC_LAUNCH((embed_sum_kernel<TG, TO, VEC>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, s, m);
+    MIC_LAUNCH((embed_sum_kernel<TG, TO, A>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, s, m);
     if (p.chunks > 1) {
         const int long_blocks = (p.chunks - 1) / JOIN_LONG * ((H + 63) / 64);
         const long long waves = (long long)(p.chunks - 1) * m.slabs;
-        MIC_LAUNCH((embed_join_kernel<TO, VEC>), dim3((unsigned)(long_blocks + (waves + 15) / 16)), dim3(1024), 0, s, m, long_blocks);
+        MIC_LAUNCH((embed_join_kernel<TO, A>), dim3((unsigned)(long_blocks + (waves + 15) / 16)), dim3(1024), 0, s, m, long_blocks);
     }
     return 0;
 }
@@ -601,22 +633,22 @@ extern "C" int mic_embed_rows(const void* ids, int ids_bits, const void* table, 
     MIC_ARG_CHECK(ids && table && out, "mic_embed_rows: null pointer");
     hipStream_t s = (hipStream_t)stream;
     const bool vec = H % 8 == 0 && ld_table % 8 == 0 && (!pos || ld_pos % 8 == 0) && (((uintptr_t)table | (uintptr_t)out | (uintptr_t)pos) & 15) == 0;
-    const long long work = n * (vec ? H / 8 : H);
+    const long long work = n * ((H + VEC - 1) / VEC);
     const long long blocks = (work + 255) / 256;
     const dim3 grid((unsigned)(blocks > 1048576 ? 1048576 : blocks));
     const bool small = work < (1ll << 31);  // 32-bit index arithmetic: a 64-bit division costs as much as the rest of the thread
-#define GO_I(TT, TO, VEC, I)                                                                                                                    \
-    MIC_LAUNCH((embed_rows_kernel<TT, TO, VEC, I>), grid, dim3(256), 0, s, ids, ids_bits == 64, (const TT*)table, (long long)ld_table, (const TT*)pos, \
+#define GO_I(TT, TO, A, I)                                                                                                                     \
+    MIC_LAUNCH((embed_rows_kernel<TT, TO, A, I>), grid, dim3(256), 0, s, ids, ids_bits == 64, (const TT*)table, (long long)ld_table, (const TT*)pos, \
                (long long)ld_pos, (TO*)out, scale, (long long)n, T, H, vocab)
-#define GO(TT, TO, VEC)                       \
-    do {                                      \
-        if (small) GO_I(TT, TO, VEC, unsigned); \
-        else GO_I(TT, TO, VEC, long long);    \
+#define GO(TT, TO, A)                       \
+    do {                                    \
+        if (small) GO_I(TT, TO, A, unsigned); \
+        else GO_I(TT, TO, A, long long);    \
     } while (0)
 #define GO_VEC(TT, TO)             \
     do {                           \
-        if (vec) GO(TT, TO, 8);    \
-        else GO(TT, TO, 1);        \
+        if (vec) GO(TT, TO, true);    \
+        else GO(TT, TO, false);        \
     } while (0)
     if (table_dtype == MIC_F32 && out_dtype == MIC_F32) GO_VEC(float, float);
     else if (table_dtype == MIC_F32) GO_VEC(float, bf16_t);
@@ -645,11 +677,11 @@ extern "C" int mic_embed_grad(const void* ids, int ids_bits, const void* g, void
     MIC_ARG_CHECK(((uintptr_t)workspace & 15) == 0, "mic_embed_grad: workspace is not 16-byte aligned");
     hipStream_t s = (hipStream_t)stream;
     const bool vec = H % 8 == 0 && (((uintptr_t)g | (uintptr_t)d_table | (uintptr_t)d_pos) & 15) == 0;
-#define GO(TG, TO, VEC) return launch_grad<TG, TO, VEC>(p, ids, ids_bits == 64, g, d_table, d_pos, scale, n, T, H, vocab, (char*)workspace, s)
+#define GO(TG, TO, A) return launch_grad<TG, TO, A>(p, ids, ids_bits == 64, g, d_table, d_pos, scale, n, T, H, vocab, (char*)workspace, s)
 #define GO_VEC(TG, TO)             \
     do {                           \
-        if (vec) GO(TG, TO, 8);    \
-        else GO(TG, TO, 1);        \
+        if (vec) GO(TG, TO, true);    \
+        else GO(TG, TO, false);        \
     } while (0)
     if (g_dtype == MIC_F32 && out_dtype == MIC_F32) GO_VEC(float, float);
     else if (g_dtype == MIC_F32) GO_VEC(float, bf16_t);
