@@ -20,9 +20,11 @@ template <typename T, int DP, bool SPLIT> __global__ __launch_bounds__(256, (DP 
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int heads = a.Hkv * a.B;
     int id = blockIdx.x;
+    const int hk = id % heads % a.Hkv, b = id % heads / a.Hkv;
+    id /= heads;
     const int split = SPLIT ? id % a.splits : 0;
     if (SPLIT) id /= a.splits;
-    const int kt = id / heads, hk = id % heads % a.Hkv, b = id % heads / a.Hkv;  // the first keys, which the most rows see, first
+    const int kt = id;  // the first keys, which the most rows see, first
     const int k0 = kt * ATTN_SEQ_BLOCK + wave * 32, key = k0 + (lane & 31);
     const bool seen = key_seen(a, b, key);
     const T* krow = seen ? (const T*)a.k + b * a.k_sb + hk * a.k_sh + (long long)key * a.k_st : nullptr;
@@ -54,10 +56,10 @@ template <typename T, int DP, bool SPLIT> __global__ __launch_bounds__(256, (DP 
     // a row sees this lane's key from row (key - off) * group on
     const int from = !seen ? 0x7fffffff : a.causal ? max(0, key - a.off) * a.group : 0;
     int t0 = min(first, a.R) / 32, t1 = (a.R + 31) / 32;
-    if (SPLIT) {  // an even share of the tiles that see anything
-        const int n = t1 - t0;
-        t1 = t0 + (int)((long long)n * (split + 1) / a.splits);
-        t0 = t0 + (int)((long long)n * split / a.splits);
+    if (SPLIT) {
+        t0 += split * a.tiles_per_split;
+        if (split > 0 && t0 >= t1) return;  // this key tile needs fewer workgroups
+        t1 = min(t1, t0 + a.tiles_per_split);
     }
     const unsigned q_row = (unsigned)(a.q_st * ES), q_head = (unsigned)(a.q_sh * ES), g_row = (unsigned)(a.g_st * ES), g_head = (unsigned)(a.g_sh * ES);
     const unsigned lds0 = lds_address(smem);
@@ -184,21 +186,28 @@ template <typename T, int DP, bool SPLIT> __global__ __launch_bounds__(256, (DP 
         }
 }
 
-// adds the partial sums of all row ranges, four elements per thread
-template <typename T> __global__ __launch_bounds__(256) void attn_seq_dkv_join_kernel(AttnSeqArgs a) {
+// adds the partial sums of all row ranges of a key, four elements per thread
+template <typename T> __global__ __launch_bounds__(256) void attn_seq_dkv_join_kernel(AttnSeqArgs a, int general) {
     const long long all = (long long)a.B * a.Tk * a.Hkv * a.D, i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
     if (i >= 2 * all) return;
+    int ranges = a.splits;
+    if (general && a.causal) {  // as many as the key's tile has
+        const int key = (int)((i < all ? i : i - all) / ((long long)a.Hkv * a.D) % a.Tk), kt = key / ATTN_SEQ_BLOCK;
+        const int first = max(0, kt * ATTN_SEQ_BLOCK - a.off) * a.group, n = (a.R + 31) / 32 - min(first, a.R) / 32;
+        ranges = max(1, (n + a.tiles_per_split - 1) / a.tiles_per_split);
+    }
     float x[4] = {};
-    for (int s = 0; s < a.splits; ++s) {
+#pragma unroll 4
+    for (int s = 0; s < ranges; ++s) {
         const float4 p = *reinterpret_cast<const float4*>(a.part + 2 * s * all + i);
         x[0] += p.x; x[1] += p.y; x[2] += p.z; x[3] += p.w;
     }
     store4<T>(i < all ? (T*)a.dk + i : (T*)a.dv + (i - all), x[0], x[1], x[2], x[3]);
 }
 
-template <typename T> int join(const AttnSeqArgs& a, hipStream_t s) {
+template <typename T> int join(const AttnSeqArgs& a, int general, hipStream_t s) {
     const long long quads = (long long)a.B * a.Tk * a.Hkv * a.D / 2;
-    MIC_LAUNCH((attn_seq_dkv_join_kernel<T>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s, a);
+    MIC_LAUNCH((attn_seq_dkv_join_kernel<T>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s, a, general);
     return 0;
 }
 
@@ -206,7 +215,7 @@ template <typename T, int DP> int launch(const AttnSeqArgs& a, hipStream_t s) {
     const long long blocks = (long long)((a.Tk + ATTN_SEQ_BLOCK - 1) / ATTN_SEQ_BLOCK) * a.Hkv * a.B;
     if (a.splits > 1) {
         MIC_LAUNCH((attn_seq_dkv_kernel<T, DP, true>), dim3((unsigned)(blocks * a.splits)), dim3(256), 0, s, a);
-        return join<T>(a, s);
+        return join<T>(a, 1, s);
     } else {
         MIC_LAUNCH((attn_seq_dkv_kernel<T, DP, false>), dim3((unsigned)blocks), dim3(256), 0, s, a);
     }
@@ -221,4 +230,4 @@ template <typename T> int launch_d(const AttnSeqArgs& a, hipStream_t s) {
 int mic_attn_seq_dkv_launch(const AttnSeqArgs& a, int dtype, hipStream_t s) {
     return dtype == MIC_BF16 ? launch_d<bf16_t>(a, s) : launch_d<float>(a, s);
 }
-int mic_attn_seq_dkv_join(const AttnSeqArgs& a, int dtype, hipStream_t s) { return dtype == MIC_BF16 ? join<bf16_t>(a, s) : join<float>(a, s); }
+int mic_attn_seq_dkv_join(const AttnSeqArgs& a, int dtype, hipStream_t s) { return dtype == MIC_BF16 ? join<bf16_t>(a, 0, s) : join<float>(a, 0, s); }

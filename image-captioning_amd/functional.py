@@ -191,9 +191,9 @@ def embedding(ids, table, pos=None, *, scale: float = 1.0, dtype=None) -> torch.
 _ATTN_PACK = struct.Struct("@10P16q8ifPq")  # mic_attn_seq_desc
 
 @functools.lru_cache(maxsize=256)
-def _attn_workspace_bytes(code, B, Tq, Tk, Hq, Hkv, D, grad) -> int:
-    """Scratch depends on type and sizes alone."""
-    d = L.AttnSeqDesc.from_buffer_copy(_ATTN_PACK.pack(*(0,) * 26, code, B, Tq, Tk, Hq, Hkv, D, 0, 0.0, 0, 0))
+def _attn_workspace_bytes(code, B, Tq, Tk, Hq, Hkv, D, causal, grad) -> int:
+    """Scratch depends on type, sizes and causality alone."""
+    d = L.AttnSeqDesc.from_buffer_copy(_ATTN_PACK.pack(*(0,) * 26, code, B, Tq, Tk, Hq, Hkv, D, causal, 0.0, 0, 0))
     size = L.lib.mic_attn_seq_workspace_bytes(d, grad)
     if size < 0:
         L.check(size, "mic_attn_seq_workspace_bytes")
@@ -258,11 +258,12 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, caus
     place = q.device
     o = torch.empty((B, Tq, Hq, D), dtype=dtype, device=place)
     lse = torch.empty((B, Hq, Tq), dtype=torch.float32, device=place)
-    size = _attn_workspace_bytes(code, B, Tq, Tk, Hq, Hkv, D, 0)
+    causal = 1 if causal else 0
+    size = _attn_workspace_bytes(code, B, Tq, Tk, Hq, Hkv, D, causal, 0)
     ws, ws_ptr = _workspace(size, q)
     _run("mic_attn_seq", L.lib.mic_attn_seq, dev, L.AttnSeqDesc.from_buffer_copy(_ATTN_PACK.pack(
         q_ptr, k_ptr, v_ptr, o.data_ptr(), lse.data_ptr(), mask_ptr, 0, 0, 0, 0, *qs, *ks, *vs, Tq * Hq * D, Hq * D, D, 0, 0, 0, mask_stride, code, B, Tq,
-        Tk, Hq, Hkv, D, 1 if causal else 0, 1.0 / math.sqrt(D) if scale is None else scale, ws_ptr, size)))
+        Tk, Hq, Hkv, D, causal, 1.0 / math.sqrt(D) if scale is None else scale, ws_ptr, size)))
     return o, lse
 
 
@@ -287,11 +288,12 @@ def attention_grad(grad: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torc
     dq = torch.empty((B, Tq, Hq, D), dtype=dtype, device=place)
     dk = torch.empty((B, Tk, Hkv, D), dtype=dtype, device=place)
     dv = torch.empty((B, Tk, Hkv, D), dtype=dtype, device=place)
-    size = _attn_workspace_bytes(code, B, Tq, Tk, Hq, Hkv, D, 1)
+    causal = 1 if causal else 0
+    size = _attn_workspace_bytes(code, B, Tq, Tk, Hq, Hkv, D, causal, 1)
     ws, ws_ptr = _workspace(size, q)
     _run("mic_attn_seq_grad", L.lib.mic_attn_seq_grad, dev, L.AttnSeqDesc.from_buffer_copy(_ATTN_PACK.pack(
         q_ptr, k_ptr, v_ptr, o_ptr, lse.data_ptr(), mask_ptr, g_ptr, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *qs, *ks, *vs, *os, *gs, mask_stride,
-        code, B, Tq, Tk, Hq, Hkv, D, 1 if causal else 0, 1.0 / math.sqrt(D) if scale is None else scale, ws_ptr, size)))
+        code, B, Tq, Tk, Hq, Hkv, D, causal, 1.0 / math.sqrt(D) if scale is None else scale, ws_ptr, size)))
     return dq, dk, dv
 
 

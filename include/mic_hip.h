@@ -528,7 +528,7 @@ int mic_embed_grad(const void* ids, int ids_bits, const void* g, void* d_table, 
  * a head consecutive; pointers and strides multiples of 16 bytes, 64 positions and the heads of one position within 1 GiB.  lse fp32 [B][Hq][Tq]; key_mask bytes [B][mask_stride].  The
  * gradients dq [B][Tq][Hq][D], dk, dv [B][Tk][Hkv][D] are written whole and contiguous.  D <= 256, D * element size a multiple of 16 bytes.
  * bf16: scores, statistics and sums in fp32; probabilities and their gradients are rounded to bf16 for the second products only.
- * Sizes of zero are allowed.  mic_attn_seq_workspace_bytes(d, grad) looks at dtype and sizes alone (an argument error is negative). */
+ * Sizes of zero are allowed.  mic_attn_seq_workspace_bytes(d, grad) looks at dtype, sizes and causal alone (an argument error is negative). */
 typedef struct mic_attn_seq_desc {
     const void *q, *k, *v;
     void* o;              /* written by mic_attn_seq, read by mic_attn_seq_grad */
