@@ -6,7 +6,8 @@
 // bf16 operands: both remaining products take it as a matrix-core operand; dbias is summed before the rounding), and two more
 // products use the piece.  dw's rows of a piece are complete; dx is summed over the pieces in fp32.
 // Rows that do not count (padding: half of a batch of captions) have no gradient, so the gradient's products run over the counted
-// rows alone: they are gathered first, their number stays on the device, and workgroups behind the last one end at once.
+// rows alone, whatever the others hold: they are gathered first, their number stays on the device, and workgroups behind the last one
+// end at once.
 //
 // Two kernels: 256 x 256 tiles for bf16 (vocab_gemm8.h), 128 x 128 and 64 x 64 tiles for fp32 and for products too small to fill the
 // larger ones (vocab_gemm.h).
@@ -106,7 +107,7 @@ __global__ __launch_bounds__(1024) void vocab_loss_rows_kernel(const float2* __r
 // ---- epilogue: logits -> d --------------------------------------------------------------------------------------------------
 // What a row of the gradient needs, in the order of the gathered rows
 struct RowInfo {
-    const int* target;     // -1: the row does not count
+    const int* target;
     const float *lse, *weight;
 };
 template <typename T> struct GradEpi {
@@ -115,11 +116,11 @@ template <typename T> struct GradEpi {
         RowInfo r;
         T* d;            // [N][ld], columns from v0 on
         float* part_db;  // [parts][Vc] or NULL
-        const int* count;  // NULL, or the rows there are
-        int N, Vc, ld, v0;
+        const int* count;  // the rows there are
+        int Vc, ld, v0;
     };
     template <int S> __device__ static __forceinline__ void run(const Args& a, f32x16_t (&acc)[S][S], int p0, int q0, int lane, int, int tq, int) {
-        const int n = a.count ? min(a.N, *a.count) : a.N;
+        const int n = *a.count;
         const int h = lane >> 5;
         float sum[S][16];
 #pragma unroll
@@ -275,7 +276,7 @@ struct StatsEpi8 {
 
 struct GradEpi8 {
     typedef GradEpi<bf16_t>::Args Args;
-    __device__ static __forceinline__ int rows(const Args& a) { return a.count ? min(a.N, *a.count) : a.N; }
+    __device__ static __forceinline__ int rows(const Args& a) { return *a.count; }
     __device__ static __forceinline__ void side(const Args& a, int p0, int q0, int tid, float* side) {
         const int i = tid & 255;
         if (tid < 256) {
@@ -408,14 +409,14 @@ template <typename T> __device__ __forceinline__ void sum_parts(const SumParts& 
 struct ColSum {
     const float* part;
     float* out;
-    const int* rows;  // NULL, or the gathered rows there are: parts of row_tile rows beyond them were not written
+    const int* rows;  // the gathered rows there are: parts of row_tile rows beyond them were not written
     int n, parts, row_tile;
     unsigned blocks;
 };
 __device__ __forceinline__ void column_sums(const ColSum& a, unsigned block) {
     __shared__ float sum[16][17];
     const int lane = threadIdx.x & 15, group = threadIdx.x >> 4, c = block * 16 + lane;
-    const int parts = a.rows ? min(a.parts, (*a.rows + a.row_tile - 1) / a.row_tile) : a.parts;
+    const int parts = min(a.parts, (*a.rows + a.row_tile - 1) / a.row_tile);
     const int lo = (int)((long long)parts * group / 16), hi = (int)((long long)parts * (group + 1) / 16);
     float s = 0.f;
 #pragma unroll 8
@@ -438,8 +439,8 @@ template <typename T> __global__ __launch_bounds__(256) void vocab_finish_kernel
 }
 
 // ---- the rows of the gradient ------------------------------------------------------------------------------------------------------
-// Every row's target, weight and lse, and with `gather` the counted rows only, in their order: `at` tells where a row went (-1: it does
-// not count), *count how many there are.  A block counts the rows before its own again (at most 64 blocks) instead of waiting for others.
+// Target, weight and lse of the counted rows, in their order: `at` tells where a row went (-1: it does not count), *count how many there
+// are.  A block counts the rows before its own again (at most 64 blocks) instead of waiting for others.
 //
 // The last block also decides into how many ranges of k the products dx (of a whole piece and of the last one) and dw are cut, now that the
 // rows are known.
@@ -472,7 +473,7 @@ struct RowsArgs {
     const float *weight, *lse;
     int *target_out, *at, *count;
     float *weight_out, *lse_out;
-    int N, per_block, gather;
+    int N, per_block;
     SplitRule rule;
     Split dx[2], dw[2];     // whole pieces, the last one
     int edge, ks;
@@ -481,44 +482,35 @@ __global__ __launch_bounds__(1024) void vocab_rows_kernel(RowsArgs a) {
     __shared__ int wave_sum[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int lo = blockIdx.x * a.per_block, hi = min(a.N, lo + a.per_block);
-    int base = 0;
-    if (a.gather) {
-        int mine = 0;
+    int base = 0, mine = 0;
 #pragma unroll 4
-        for (int i = tid; i < lo; i += 1024) mine += target_of(a.t, i) >= 0;
-        for (int d = 32; d > 0; d >>= 1) mine += __shfl_xor(mine, d, 64);
-        if (lane == 0) wave_sum[wave] = mine;
-        __syncthreads();
-        for (int w = 0; w < 16; ++w) base += wave_sum[w];
-        __syncthreads();
-    }
+    for (int i = tid; i < lo; i += 1024) mine += target_of(a.t, i) >= 0;
+    for (int d = 32; d > 0; d >>= 1) mine += __shfl_xor(mine, d, 64);
+    if (lane == 0) wave_sum[wave] = mine;
+    __syncthreads();
+    for (int w = 0; w < 16; ++w) base += wave_sum[w];
+    __syncthreads();
     for (int r = lo; r < hi; r += 1024) {
         const int i = r + tid, t = i < hi ? target_of(a.t, i) : -1;
-        int to = i;
-        if (a.gather) {
-            const unsigned long long in = __ballot(t >= 0);
-            if (lane == 0) wave_sum[wave] = __popcll(in);
-            __syncthreads();
-            to = base + __popcll(in & ((1ull << lane) - 1ull));
-            int all = 0;
-            for (int w = 0; w < 16; ++w) {
-                if (w < wave) to += wave_sum[w];
-                all += wave_sum[w];
-            }
-            base += all;
-            __syncthreads();
+        const unsigned long long in = __ballot(t >= 0);
+        if (lane == 0) wave_sum[wave] = __popcll(in);
+        __syncthreads();
+        int to = base + __popcll(in & ((1ull << lane) - 1ull)), all = 0;
+        for (int w = 0; w < 16; ++w) {
+            if (w < wave) to += wave_sum[w];
+            all += wave_sum[w];
         }
-        if (i < hi) {
-            if (a.gather) a.at[i] = t >= 0 ? to : -1;
-            if (t >= 0 || !a.gather) {
-                a.target_out[to] = t;
-                a.weight_out[to] = t >= 0 ? a.weight[i] : 0.f;
-                a.lse_out[to] = t >= 0 ? a.lse[i] : 0.f;
-            }
+        base += all;
+        __syncthreads();
+        if (i < hi) a.at[i] = t >= 0 ? to : -1;
+        if (t >= 0) {
+            a.target_out[to] = t;
+            a.weight_out[to] = a.weight[i];
+            a.lse_out[to] = a.lse[i];
         }
     }
     if (blockIdx.x == gridDim.x - 1 && wave == 0) {
-        const int rows = a.gather ? base : a.N, i = (lane >> 4) & 1;  // dx, dx last, dw, dw last
+        const int rows = base, i = (lane >> 4) & 1;  // dx, dx last, dw, dw last
         const bool is_dw = lane >= 32;
         const int s = choose_slices(a.rule, is_dw ? a.dw[i].tiles : a.dx[i].tiles * ((rows + a.edge - 1) / a.edge), is_dw ? (rows + a.ks - 1) / a.ks : a.dx[i].nk,
                                     is_dw ? a.dw[i].most : a.dx[i].most, lane);
@@ -558,7 +550,7 @@ struct Plan {
     int Hp, e;              // columns of the operands the products read (H rounded up to whole 16 bytes)
     bool pad;               // x and w are copied to that width first
     bool big;               // 256 x 256 tiles
-    bool gather;            // gradient: the counted rows alone
+    bool copy_x;            // x is copied: to that width, or (gradient) its counted rows alone
     int edge;               // tile edge
     int parts;              // forward: column parts per row
     int Vc, pieces, ld;     // gradient: words per piece, row stride of d
@@ -588,10 +580,10 @@ Plan make_plan(const mic_vocab_loss_desc* d, bool grad) {
     p.big = d->dtype == MIC_BF16 && (long long)edge_tiles(N, 256) * edge_tiles(V, 256) >= 128 && H >= 64 && H < (1 << 21) && d->ld_x < (1 << 21) && d->ld_w < (1 << 21);
     // 64 x 64 tiles where 128 x 128 ones would leave compute units idle
     p.edge = p.big ? 256 : (long long)edge_tiles(N, 128) * edge_tiles(V, 128) < 512 ? 64 : 128;
-    p.gather = grad && N > p.edge;
+    p.copy_x = p.pad || grad;
     long long o = 0;
     p.xpad = o;
-    if (p.pad || p.gather) o += up256(N * p.Hp * es);
+    if (p.copy_x) o += up256(N * p.Hp * es);
     p.wpad = o;
     if (p.pad) o += up256(V * p.Hp * es);
     if (!grad) {
@@ -599,8 +591,11 @@ Plan make_plan(const mic_vocab_loss_desc* d, bool grad) {
         p.part = o; o += up256(N * p.parts * 8);
         p.zt = o; o += up256(N * 4);
     } else {
-        // a piece of d takes at most 256 MiB (what the last-level cache holds), at least one tile of words
-        long long vc = (256ll << 20) / (es * N) / p.edge * p.edge;
+        // a piece of d takes at most 256 MiB (what the last-level cache holds), but with many rows it is that wide that d and the
+        // partial sums of dx, N * H * 4 bytes per piece, take the same space: es * Vc = 4 H V / Vc (and 31 bits address 256 of its rows)
+        long long vc = (256ll << 20) / (es * N), even = (long long)sqrt(4.0 * H * V / es);
+        if (even > 1 << 20) even = 1 << 20;
+        vc = (vc > even ? vc : even) / p.edge * p.edge;
         if (vc < p.edge) vc = p.edge;
         if (vc > V) vc = V;
         p.pieces = (int)((V + vc - 1) / vc);
@@ -613,12 +608,12 @@ Plan make_plan(const mic_vocab_loss_desc* d, bool grad) {
         p.sw = most_slices(N, ks);
         // never more partial tiles than would fill the GPU twice
         const long long wide = p.big ? 512 : p.edge == 128 ? 1024 : 2048, tx = (long long)edge_tiles(N, p.edge) * edge_tiles(H, p.edge), tw = (long long)edge_tiles(p.Vc, p.edge) * edge_tiles(H, p.edge);
-        while (p.sx > 1 && p.sx * tx > (p.gather ? 2 * wide : wide)) --p.sx;
+        while (p.sx > 1 && p.sx * tx > 2 * wide) --p.sx;
         while (p.sw > 1 && p.sw * tw > wide) --p.sw;
         p.rows = o; o += rows_bytes(N);
         p.d = o; o += up256(N * p.ld * es);
         p.dx = o;
-        if (p.sx * p.pieces > 1 || p.gather) o += up256((long long)p.sx * p.pieces * N * H * 4);
+        o += up256((long long)p.sx * p.pieces * N * H * 4);
         p.dw = o;
         if (p.sw > 1) o += up256((long long)p.sw * p.Vc * H * 4);
         p.db = o;
@@ -632,10 +627,10 @@ int check_desc(const char* who, const mic_vocab_loss_desc* d) {
     MIC_ARG_CHECK(d, "%s: null descriptor", who);
     MIC_ARG_CHECK(d->dtype == MIC_F32 || d->dtype == MIC_BF16, "%s: bad dtype %d", who, d->dtype);
     MIC_ARG_CHECK(d->N >= 0 && d->H > 0 && d->V > 0, "%s: bad sizes N=%d H=%d V=%d", who, d->N, d->H, d->V);
-    const long long lim = 1ll << 30;
-    MIC_ARG_CHECK(d->N < lim && d->H < lim && d->V < lim && (d->N / 64 + 2ll) * (d->V / 64 + 2ll) < lim / 32 && (d->N / 64 + 2ll) * (d->H / 64 + 2ll) < lim / 32 &&
-                      (d->V / 64 + 2ll) * (d->H / 64 + 2ll) < lim / 32,
-                  "%s: sizes out of range N=%d H=%d V=%d", who, d->N, d->H, d->V);
+    // launches and tile numbers have 32 bits: at most 2^37 logits, 2^33 elements of x or w
+    const long long N = d->N / 64 + 2ll, H = d->H / 64 + 2ll, V = d->V / 64 + 2ll;
+    MIC_ARG_CHECK(N <= 1 << 19 && H <= 1 << 21 && V <= 1 << 21 && N * V < 1 << 25 && N * H < 1 << 21 && V * H < 1 << 21, "%s: sizes out of range N=%d H=%d V=%d", who, d->N,
+                  d->H, d->V);
     MIC_ARG_CHECK(d->target_bits == 32 || d->target_bits == 64, "%s: targets of %d bits", who, d->target_bits);
     MIC_ARG_CHECK(d->n_ignore >= 0 && d->n_ignore <= MAX_IGNORE, "%s: %d ignored words (at most %d)", who, d->n_ignore, MAX_IGNORE);
     MIC_ARG_CHECK(d->ld_x >= d->H && d->ld_w >= d->H, "%s: row stride below H=%d", who, d->H);
@@ -685,7 +680,7 @@ template <typename T> int copy_rows(const void* in, long long ld, void* out, con
 template <typename T> int operands(const mic_vocab_loss_desc* d, const Plan& p, char* ws, const int* at, Operand& x, Operand& w, hipStream_t s) {
     x = {d->x, d->ld_x, d->N};
     w = {d->w, d->ld_w, d->V};
-    if (p.pad || p.gather) {
+    if (p.copy_x) {
         MIC_TRY(copy_rows<T>(d->x, d->ld_x, ws + p.xpad, at, d->N, d->H, p.Hp, s));
         x = {ws + p.xpad, p.Hp, d->N};
     }
@@ -720,7 +715,7 @@ template <typename T> int gradient(const mic_vocab_loss_desc* d, const Plan& p, 
     ra.weight_out = (float*)(ws + p.rows + 2 * step);
     ra.at = (int*)(ws + p.rows + 3 * step);
     ra.count = (int*)(ws + p.rows + 4 * step);
-    ra.N = d->N; ra.gather = p.gather;
+    ra.N = d->N;
     const long long share = (N + 63) / 64;
     ra.per_block = (int)((share + 1023) / 1024 * 1024);
     // measured on 256 x 256 tiles: a step of 64 k is 1.7 us, a workgroup's start and end 4 steps, writing and reading again the partial
@@ -734,13 +729,11 @@ template <typename T> int gradient(const mic_vocab_loss_desc* d, const Plan& p, 
     ra.dw[0] = {th * edge_tiles(p.Vc, p.edge), 0, p.sw};
     ra.dw[1] = {th * edge_tiles(last, p.edge), 0, p.sw};
     MIC_LAUNCH(vocab_rows_kernel, dim3((unsigned)((N + ra.per_block - 1) / ra.per_block)), dim3(1024), 0, s, ra);
-    const int* at = p.gather ? ra.at : nullptr;
-    const int* count = p.gather ? ra.count : nullptr;
+    const int *at = ra.at, *count = ra.count;
     Operand x, w;
     MIC_TRY(operands<T>(d, p, ws, at, x, w, s));
     T* dl = (T*)(ws + p.d);
     float *part_dx = (float*)(ws + p.dx), *part_dw = (float*)(ws + p.dw), *part_db = (float*)(ws + p.db);
-    const bool dx_parts = p.sx * p.pieces > 1 || p.gather;
     auto parts_of = [&](const float* part, T* out, const int* where, int rows, long long stride, int pieces, int most, int whole, int end) {
         const long long quads = (long long)rows * ((H + 3) / 4);
         return SumParts{part, out, where, ra.count + whole, ra.count + end, stride, rows, d->H, pieces, most, (unsigned)((quads + 255) / 256)};
@@ -757,13 +750,13 @@ template <typename T> int gradient(const mic_vocab_loss_desc* d, const Plan& p, 
         typename GradEpi<T>::Args ga = {};
         ga.bias = d->bias; ga.r = {ra.target_out, ra.lse_out, ra.weight_out};
         ga.d = dl; ga.part_db = d->db ? part_db : nullptr;
-        ga.N = d->N; ga.Vc = vc; ga.ld = p.ld; ga.v0 = v0;
+        ga.Vc = vc; ga.ld = p.ld; ga.v0 = v0;
         ga.count = count;
         MIC_TRY((product<T, false, false, GradEpi<T>, GradEpi8>(p, wi, x, Rows{count, 0, nullptr, 1}, d->H, ga, s)));
         // dx += d w: k runs over the words of the piece
         typename OutEpi<T>::Args xa = {};
-        xa.out = (T*)d->dx; xa.ld = H; xa.Np = d->H; xa.Nq = d->N;
-        if (dx_parts) xa.part = part_dx + (long long)i * p.sx * N * H;
+        xa.ld = H; xa.Np = d->H; xa.Nq = d->N;
+        xa.part = part_dx + (long long)i * p.sx * N * H;  // rows of the gathered order
         const Operand wc = {wi.p, wi.ld, d->H}, dr = {dl, p.ld, d->N};
         const Rows rx = {count, 0, p.sx > 1 ? ra.count + (end ? SX_LAST : SX) : nullptr, p.sx};
         MIC_TRY((product<T, true, false, OutEpi<T>, OutEpi8>(p, wc, dr, rx, vc, xa, s)));
@@ -778,15 +771,14 @@ template <typename T> int gradient(const mic_vocab_loss_desc* d, const Plan& p, 
         ColSum sb = {};
         if (p.sw > 1) sw = parts_of(part_dw, wa.out, nullptr, vc, vc * H, 1, p.sw, SW, end ? SW_LAST : SW);
         if (d->db) sb = {part_db, d->db + v0, count, vc, edge_tiles(N, p.edge) * 2, p.edge / 2, (unsigned)((vc + 15) / 16)};
-        if (end && dx_parts) sx = parts_of(part_dx, (T*)d->dx, at, d->N, N * H, p.pieces, p.sx, SX, SX_LAST);
+        if (end) sx = parts_of(part_dx, (T*)d->dx, at, d->N, N * H, p.pieces, p.sx, SX, SX_LAST);
         MIC_TRY(finish(sx, sw, sb));
     }
     return 0;
 }
 
 __global__ __launch_bounds__(256) void vocab_clear_kernel(uint16_t* p, long long n) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i < n) p[i] = 0;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) p[i] = 0;
 }
 
 }  // namespace
@@ -823,8 +815,13 @@ extern "C" int mic_vocab_loss_grad(const mic_vocab_loss_desc* d, void* stream) {
     hipStream_t s = (hipStream_t)stream;
     if (d->N == 0) {  // no rows: the sums over them are zero
         const long long n = (long long)d->V * d->H * (long long)mic_dtype_size(d->dtype) / 2;
-        MIC_LAUNCH(vocab_clear_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, (uint16_t*)d->dw, n);
-        if (d->db) MIC_LAUNCH(vocab_clear_kernel, dim3((unsigned)((2ll * d->V + 255) / 256)), dim3(256), 0, s, (uint16_t*)d->db, 2ll * d->V);
+        auto clear = [&](void* p, long long halves) -> int {
+            const long long blocks = (halves + 255) / 256;
+            MIC_LAUNCH(vocab_clear_kernel, dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, s, (uint16_t*)p, halves);
+            return 0;
+        };
+        MIC_TRY(clear(d->dw, n));
+        if (d->db) MIC_TRY(clear(d->db, 2ll * d->V));
         return 0;
     }
     return d->dtype == MIC_BF16 ? gradient<bf16_t>(d, p, s) : gradient<float>(d, p, s);
