@@ -28,9 +28,10 @@ int check_sizes(const char* who, const mic_attn_seq_desc* d) {
                   d->Tk, d->Hq, d->Hkv, d->D);
     MIC_ARG_CHECK(d->Hq % d->Hkv == 0, "%s: %d query heads do not share %d key heads evenly", who, d->Hq, d->Hkv);
     MIC_ARG_CHECK(d->D <= 256 && d->D % (16 / (int)mic_dtype_size(d->dtype)) == 0, "%s: heads of %d columns (at most 256, whole 16 bytes)", who, d->D);
-    const long long lim = 1ll << 30;  // row and key numbers are 32-bit, grids as well
+    // row and key numbers have 32 bits, and a launch has fewer than 2^32 threads (the short forward four workgroups of 256 to 128 rows)
+    const long long lim = 1ll << 30, tiles = 1ll << 22;
     const long long group = d->Hq / d->Hkv, R = d->Tq * group;
-    MIC_ARG_CHECK(R < lim && d->Tk < lim && ((R + 127) / 128 + 1) * d->Hkv * (long long)d->B < lim && (((long long)d->Tk + 127) / 128 + 1) * d->Hkv * (long long)d->B < lim,
+    MIC_ARG_CHECK(d->Hq <= 1 << 20 && R < lim && d->Tk < lim && ((R + 127) / 128) * d->Hkv * (long long)d->B < tiles && (((long long)d->Tk + 127) / 128) * d->Hkv * (long long)d->B < tiles,
                   "%s: too many rows (B=%d Tq=%d Tk=%d Hq=%d)", who, d->B, d->Tq, d->Tk, d->Hq);
     return 0;
 }

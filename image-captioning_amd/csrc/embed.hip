@@ -570,6 +570,10 @@ GradPlan grad_plan(long long n, int T, int H, int vocab, bool want_pos) {
     return p;
 }
 
+// columns of a row, and elements of d_pos (a launch has fewer than 2^32 threads)
+constexpr int MAX_H = 1 << 20;
+constexpr long long MAX_POS = 1ll << 31;
+
 bool ok_dtype(int d) { return d == MIC_F32 || d == MIC_BF16; }
 
 template <typename TG, typename TO, bool A>
@@ -632,7 +636,7 @@ int launch_grad(const GradPlan& p, const void* ids, int wide, const void* g, voi
 
 extern "C" int mic_embed_rows(const void* ids, int ids_bits, const void* table, int64_t ld_table, const void* pos, int64_t ld_pos, void* out,
                               int table_dtype, int out_dtype, float scale, int64_t n, int T, int H, int vocab, void* stream) {
-    MIC_ARG_CHECK(n >= 0 && n < (1ll << 31) && T > 0 && H > 0 && vocab > 0, "mic_embed_rows: bad sizes n=%lld T=%d H=%d vocab=%d", (long long)n, T, H, vocab);
+    MIC_ARG_CHECK(n >= 0 && n < (1ll << 31) && T > 0 && H > 0 && H <= MAX_H && vocab > 0, "mic_embed_rows: bad sizes n=%lld T=%d H=%d vocab=%d", (long long)n, T, H, vocab);
     MIC_ARG_CHECK(ids_bits == 32 || ids_bits == 64, "mic_embed_rows: token ids of %d bits", ids_bits);
     MIC_ARG_CHECK(ok_dtype(table_dtype) && ok_dtype(out_dtype), "mic_embed_rows: bad dtype %d / %d", table_dtype, out_dtype);
     MIC_ARG_CHECK(ld_table >= H && (!pos || ld_pos >= H), "mic_embed_rows: row stride below H=%d", H);
@@ -668,13 +672,14 @@ extern "C" int mic_embed_rows(const void* ids, int ids_bits, const void* table, 
 }
 
 extern "C" int64_t mic_embed_grad_workspace_bytes(int64_t n, int T, int H, int vocab, int want_pos) {
-    if (n < 0 || n >= (1ll << 30) || T <= 0 || H <= 0 || vocab <= 0 || (want_pos && n % T != 0)) return MIC_ERR_ARG;
+    if (n < 0 || n >= (1ll << 30) || T <= 0 || H <= 0 || H > MAX_H || vocab <= 0 || (want_pos && (n % T != 0 || (long long)T * H >= MAX_POS))) return MIC_ERR_ARG;
     return grad_plan(n, T, H, vocab, want_pos != 0).bytes;
 }
 
 extern "C" int mic_embed_grad(const void* ids, int ids_bits, const void* g, void* d_table, void* d_pos, int g_dtype, int out_dtype, float scale,
                               int64_t n, int T, int H, int vocab, void* workspace, int64_t workspace_bytes, void* stream) {
-    MIC_ARG_CHECK(n >= 0 && n < (1ll << 30) && T > 0 && H > 0 && vocab > 0, "mic_embed_grad: bad sizes n=%lld T=%d H=%d vocab=%d", (long long)n, T, H, vocab);
+    MIC_ARG_CHECK(n >= 0 && n < (1ll << 30) && T > 0 && H > 0 && H <= MAX_H && vocab > 0 && (!d_pos || (long long)T * H < MAX_POS),
+                  "mic_embed_grad: bad sizes n=%lld T=%d H=%d vocab=%d", (long long)n, T, H, vocab);
     MIC_ARG_CHECK(ids_bits == 32 || ids_bits == 64, "mic_embed_grad: token ids of %d bits", ids_bits);
     MIC_ARG_CHECK(ok_dtype(g_dtype) && ok_dtype(out_dtype), "mic_embed_grad: bad dtype %d / %d", g_dtype, out_dtype);
     MIC_ARG_CHECK(!d_pos || n % T == 0, "mic_embed_grad: %lld tokens are not whole sequences of %d", (long long)n, T);

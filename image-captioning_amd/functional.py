@@ -6,8 +6,9 @@ kernels on the current stream of the tensors' device and return new tensors, and
 ``torch.autograd`` built on the pair: ``embedding``, ``attention``, ``vocab_loss``.
 
 Tensors live on one HIP device, fp32 or bf16.  Nothing synchronises; every call may be captured into a HIP graph (workspaces
-come from torch's allocator, which gives a captured graph a pool of its own).  Refused arguments raise ``ValueError`` (shapes,
-types, devices) or ``_lib.MicError`` (what the library refuses).
+come from torch's allocator, which gives a captured graph a pool of its own).  Capture the plain calls, or ``torch.autograd.grad``
+of the differentiable ones: a captured ``.backward()`` into leaves that an eager graph still holds ends the process inside torch.
+Refused arguments raise ``ValueError`` (shapes, types, devices) or ``_lib.MicError`` (what the library refuses).
 """
 from __future__ import annotations
 
@@ -67,6 +68,12 @@ def _ids(name: str, what: str, t: torch.Tensor) -> torch.Tensor:
     return t.contiguous()
 
 
+def _small(name: str, *sizes) -> None:
+    """The library takes sizes of 32 bits."""
+    if max(sizes) >= 1 << 31:
+        raise ValueError(f"{name}: sizes out of range {sizes}")
+
+
 def _bits(t: torch.Tensor) -> int:
     return 64 if t.dtype is torch.int64 else 32
 
@@ -108,6 +115,7 @@ def embedding_forward(ids: torch.Tensor, table: torch.Tensor, pos: Optional[torc
         raise ValueError(f"{name}: ids need at least one dimension")
     vocab, H = table.shape
     T = ids.shape[-1]
+    _small(name, vocab, H, T)
     code = _float_code(name, "the table", table.dtype)
     out_dtype = table.dtype if dtype is None else dtype
     out_code = _float_code(name, "the output", out_dtype)
@@ -144,6 +152,7 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, vocab: int, *, scale: 
     H, T, n = grad.shape[-1], ids.shape[-1], ids.numel()
     if H < 1 or vocab < 1:
         raise ValueError(f"{name}: bad sizes H={H} vocab={vocab}")
+    _small(name, vocab, H, T, positions)
     if positions and positions < T:
         raise ValueError(f"{name}: {positions} positions for sequences of {T}")
     code = _float_code(name, "grad", grad.dtype)
@@ -227,6 +236,7 @@ def _attn_check(name, dev, q, k, v, key_mask):
     Bk, Tk, Hkv, Dk = k.shape
     if Bk != B or Dk != D or Hq < 1 or Hkv < 1 or D < 1:
         raise ValueError(f"{name}: q {tuple(q.shape)} and k {tuple(k.shape)} do not fit")
+    _small(name, B, Tq, Tk, Hq, Hkv)
     dtype = q.dtype
     if k.dtype is not dtype or v.dtype is not dtype:
         raise ValueError(f"{name}: q, k and v are {dtype}, {k.dtype} and {v.dtype}")
@@ -247,7 +257,8 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, caus
 
     q (B, Tq, Hq, D); k, v (B, Tk, Hkv, D), Hq a multiple of Hkv (query head h reads key head h // (Hq // Hkv)); any strides, e.g.
     slices of one packed projection.  ``causal``: query i sees keys up to i + Tk - Tq.  key_mask (B, Tk) bool: True where a key may
-    be seen; what k and v hold elsewhere is never used.  A query that sees nothing gets zeros.  scale defaults to D ** -0.5.
+    be seen; what k and v hold elsewhere is never used.  (A key hidden from a query by causality alone takes part in its products with
+    weight zero, so it has to be finite.)  A query that sees nothing gets zeros.  scale defaults to D ** -0.5.
     o (B, Tq, Hq, D) in q's dtype, lse (B, Hq, Tq) fp32.  D at most 256 and a multiple of 8 (bf16) or 4 (fp32)."""
     name = "attention_forward"
     dev = _device(name, q, k, v, key_mask)
@@ -330,6 +341,7 @@ def _vocab_check(name, x, w, targets, bias, ignore):
         raise ValueError(f"{name}: x is {x.dtype}, w {w.dtype}")
     N, H = x.shape
     V = w.shape[0]
+    _small(name, N, H, V)
     if targets.shape != (N,):
         raise ValueError(f"{name}: targets {tuple(targets.shape)} do not fit {N} rows")
     code = _float_code(name, "x", x.dtype)

@@ -213,3 +213,22 @@ int main(void) { printf("%zu %zu %zu %zu %zu %zu\\n", sizeof(mic_attn_seq_desc),
         got = [int(x) for x in subprocess.run([exe], capture_output=True, text=True, check=True).stdout.split()]
     assert got == [C.sizeof(L.AttnSeqDesc), L.AttnSeqDesc.mask_stride.offset, L.AttnSeqDesc.workspace.offset,
                    C.sizeof(L.VocabLossDesc), L.VocabLossDesc.n_ignore.offset, L.VocabLossDesc.workspace.offset]
+
+
+def test_sizes_beyond_a_launch_are_refused(L):
+    """What would need 2^32 threads or more in one launch, or more scratch than 64 bits of bytes tell."""
+    import ctypes as C
+    assert L.lib.mic_embed_grad_workspace_bytes(1 << 16, 1 << 16, 1 << 14, 100, 1) >= 0
+    assert L.lib.mic_embed_grad_workspace_bytes(1 << 16, 1 << 16, 1 << 15, 100, 1) < 0
+    assert L.lib.mic_embed_grad_workspace_bytes(8, 8, (1 << 20) + 8, 100, 0) < 0
+    d = attn_desc(L, B=1, Tq=1, Hq=(1 << 20) + 2, Hkv=1)
+    refused(L, L.lib.mic_attn_seq(C.byref(d), None), b"too many rows")
+    d = attn_desc(L, B=1 << 22, Tq=1)
+    refused(L, L.lib.mic_attn_seq(C.byref(d), None), b"too many rows")
+    for N, H, V in ((1 << 26, 8, 8), (8, 1 << 28, 8), (8, 8, 1 << 28), (1 << 24, 1 << 10, 8), (8, 1 << 10, 1 << 24), (1 << 20, 8, 1 << 20)):
+        v = L.VocabLossDesc()
+        v.dtype, v.N, v.H, v.V, v.target_bits, v.ld_x, v.ld_w = L.BF16, N, H, V, 32, H, H
+        for grad in (0, 1):
+            assert L.lib.mic_vocab_loss_workspace_bytes(C.byref(v), grad) == -1 and b"sizes out of range" in L.lib.mic_last_error()
+    v.N, v.H, v.V, v.ld_x, v.ld_w = 1 << 17, 1 << 10, 1 << 17, 1 << 10, 1 << 10
+    assert L.lib.mic_vocab_loss_workspace_bytes(C.byref(v), 1) < 16 << 30  # d and the partial dx share a few GiB
