@@ -31,7 +31,7 @@ int check_sizes(const char* who, const mic_attn_seq_desc* d) {
     // row and key numbers have 32 bits, and a launch has fewer than 2^32 threads (the short forward four workgroups of 256 to 128 rows)
     const long long lim = 1ll << 30, tiles = 1ll << 22;
     const long long group = d->Hq / d->Hkv, R = d->Tq * group;
-    MIC_ARG_CHECK(d->Hq <= 1 << 20 && R < lim && d->Tk < lim && ((R + 127) / 128) * d->Hkv * (long long)d->B < tiles && (((long long)d->Tk + 127) / 128) * d->Hkv * (long long)d->B < tiles,
+    MIC_ARG_CHECK(d->Hq <= 1 << 15 && R < lim && d->Tk < lim && ((R + 127) / 128) * d->Hkv * (long long)d->B < tiles && (((long long)d->Tk + 127) / 128) * d->Hkv * (long long)d->B < tiles,
                   "%s: too many rows (B=%d Tq=%d Tk=%d Hq=%d)", who, d->B, d->Tq, d->Tk, d->Hq);
     return 0;
 }
@@ -55,7 +55,7 @@ AttnSeqArgs args_of(const mic_attn_seq_desc* d) {
     a.scale = d->scale;
     a.scale_log2 = d->scale * ATTN_LOG2E;
     a.splits = a.dq_splits = 1;
-    a.group_magic = a.group > 1 && a.group <= 1024 ? (unsigned)(((1ull << 32) + a.group - 1) / a.group) : 0;
+    a.group_magic = a.group > 1 ? (unsigned)(((1ull << 32) + a.group - 1) / a.group) : 0;
     return a;
 }
 
@@ -87,7 +87,9 @@ int row_tiles_of(const AttnSeqArgs& a, int kt) {
 // The key gradients share the rows out where key tiles alone leave compute units idle: every workgroup takes `tiles_per_split` row tiles
 // of a key tile, as many as make 512 workgroups (two to a compute unit), at least four (one with a single tile of keys).  Under
 // causality the first keys are seen by the most rows and get the most workgroups: 2 x 4096 queries of 16 heads, a fixed number of
-// ranges per key tile took 518 us, ranges of equal length 400 us.
+// ranges per key tile took 518 us, ranges of equal length 400 us.  Without it 1024 workgroups: a mask leaves some with little to do
+// (9 x 333 queries, 391 keys, 8 heads of 64, padded, fp32: 45 us where 512 took 56; 1024 under causality: the same, and a join of 24 us
+// instead of 13).
 void split_rows(AttnSeqArgs& a, int dtype) {
     split_keys(a, dtype);  // the query gradients' rule is the forward's, whichever kernel takes the forward
     a.dq_splits = short_grad(a) ? 1 : a.splits;
@@ -106,12 +108,12 @@ void split_rows(AttnSeqArgs& a, int dtype) {
     }
     work *= (long long)a.Hkv * a.B;
     // every key tile's last range is half empty on average
-    const long long room = short_grad(a) ? 512 : 512 - base / 2;
+    const long long room = short_grad(a) ? 512 : (a.causal ? 512 : 1024) - base / 2;
     long long per = (work + room - 1) / room;
     if (per < least) per = least;
     if (per >= longest) return;
-    a.tiles_per_split = (int)per;
     a.splits = (int)((longest + per - 1) / per);
+    a.tiles_per_split = a.causal ? (int)per : (longest + a.splits - 1) / a.splits;  // all key tiles alike: even ranges
 }
 
 long long up256(long long b) { return (b + 255) / 256 * 256; }

@@ -52,7 +52,11 @@ template <typename T, int DP, bool SPLIT> __global__ __launch_bounds__(256, (DP 
     // rows below `first` see no key of the workgroup, below w_first none of the wave; from w_all on they see every key of the wave
     const int first = a.causal ? max(0, kt * ATTN_SEQ_BLOCK - a.off) * a.group : 0, w_first = a.causal ? max(0, k0 - a.off) * a.group : 0;
     const int w_all = a.causal ? max(0, k0 + 31 - a.off) * a.group : 0;
-    const bool all_seen = (unsigned)__ballot(seen) == 0xffffffffu;
+    const unsigned w_seen = (unsigned)__ballot(seen);
+    const bool all_seen = w_seen == 0xffffffffu;
+    unsigned b_seen = w_seen;  // does any wave of the workgroup have a key to work for?
+#pragma unroll
+    for (int w = 1; w < 4; ++w) b_seen |= key_bits(a, b, kt * ATTN_SEQ_BLOCK + (wave + w) % 4 * 32, lane);
     // a row sees this lane's key from row (key - off) * group on
     const int from = !seen ? 0x7fffffff : a.causal ? max(0, key - a.off) * a.group : 0;
     int t0 = min(first, a.R) / 32, t1 = (a.R + 31) / 32;
@@ -61,35 +65,40 @@ template <typename T, int DP, bool SPLIT> __global__ __launch_bounds__(256, (DP 
         if (split > 0 && t0 >= t1) return;  // this key tile needs fewer workgroups
         t1 = min(t1, t0 + a.tiles_per_split);
     }
+    if (b_seen == 0) t1 = t0;
     const unsigned q_row = (unsigned)(a.q_st * ES), q_head = (unsigned)(a.q_sh * ES), g_row = (unsigned)(a.g_st * ES), g_head = (unsigned)(a.g_sh * ES);
     const unsigned lds0 = lds_address(smem);
+    TileOffsets<T, DP, 32> at_q, at_g;
     const T* qb = (const T*)a.q + b * a.q_sb + hk * a.group * a.q_sh;
     const T* gb = (const T*)a.g + b * a.g_sb + hk * a.group * a.g_sh;
     const bool even = 32 % a.group == 0;  // every tile then begins with a query's first head, and a lane's offsets never change
-    const int step_i = 32 / a.group;
-    auto request = [&](int t, int buf) {
-        const int r0 = t * 32, i0 = even ? t * step_i : r0 / a.group, rest = even ? 0 : r0 - i0 * a.group;
-        const bool whole = r0 + 32 <= a.R;
+    const int step_i = even ? 32 / a.group : 0;
+    long long at_stats;  // lse and delta of the lane's row: 32 threads, loaded a tile ahead
+    // row x of a tile: query (rest + x) / group from the tile's first on, of `rows` that there are
+    auto places = [&](int rest, int rows) {
         auto row = [&](unsigned per_row, unsigned per_head) {
             return [&, per_row, per_head](int x) {
-                const unsigned y = rest + x, i = by_group(a, y);
-                return whole || r0 + x < a.R ? i * per_row + (y - i * a.group) * per_head : 0x80000000u;
+                const unsigned y = rest + x, i = a.group == 1 ? y : by_group(a, y);
+                return x < rows ? i * per_row + (y - i * a.group) * per_head : 0x80000000u;
             };
         };
-        request_tile<T, DP, 32>(qb + (long long)i0 * a.q_st, lds0 + OFF_Q + buf * TILE, a.D, wave, lane, row(q_row, q_head));
-        request_tile<T, DP, 32>(gb + (long long)i0 * a.g_st, lds0 + OFF_G + buf * TILE, a.D, wave, lane, row(g_row, g_head));
+        at_q.set(a.D, wave, lane, row(q_row, q_head));
+        at_g.set(a.D, wave, lane, row(g_row, g_head));
+        const unsigned y = rest + (lane & 31), i = a.group == 1 ? y : by_group(a, y);
+        at_stats = ((long long)b * a.Hq + hk * a.group + (y - i * a.group)) * a.Tq + i;
     };
-    // lse and delta of a tile's rows: 32 threads, loaded a tile ahead
+    if (even) places(0, 32);
     float lse2 = INFINITY, delta = 0.f;
-    auto load_stats = [&](int t) {
+    auto request = [&](int t, int buf) {
+        const int r0 = t * 32, i0 = even ? t * step_i : r0 / a.group;
+        if (!even || r0 + 32 > a.R) places(even ? 0 : r0 - i0 * a.group, a.R - r0);
+        at_q.request(qb + (long long)i0 * a.q_st, lds0 + OFF_Q + buf * TILE, wave);
+        at_g.request(gb + (long long)i0 * a.g_st, lds0 + OFF_G + buf * TILE, wave);
         lse2 = INFINITY;
         delta = 0.f;
-        const int r = t * 32 + threadIdx.x;
-        if (threadIdx.x < 32 && r < a.R) {
-            const int qi = r / a.group;
-            const long long at = ((long long)b * a.Hq + hk * a.group + r - qi * a.group) * a.Tq + qi;
-            lse2 = a.lse[at];
-            delta = a.delta[at];
+        if (threadIdx.x < 32 && r0 + (int)threadIdx.x < a.R) {
+            lse2 = a.lse[at_stats + i0];
+            delta = a.delta[at_stats + i0];
         }
     };
     auto put_stats = [&](int buf) {
@@ -103,7 +112,6 @@ template <typename T, int DP, bool SPLIT> __global__ __launch_bounds__(256, (DP 
     for (int d = 0; d < ND; ++d) dk[d] = dv[d] = f32x16_t{};
     if (t0 < t1) {
         request(t0, 0);
-        load_stats(t0);
         put_stats(0);
     }
     // one tile out of buffer CUR
@@ -111,12 +119,11 @@ template <typename T, int DP, bool SPLIT> __global__ __launch_bounds__(256, (DP 
         constexpr int CUR = decltype(which)::value;
         const int r0 = t * 32;
         tile_landed();
-        if (t + 1 < t1) {
-            request(t + 1, CUR ^ 1);
-            load_stats(t + 1);
-        }
-        if (k0 < a.Tk && r0 + 31 >= w_first) {
+        if (t + 1 < t1) request(t + 1, CUR ^ 1);
+        if (w_seen != 0 && r0 + 31 >= w_first) {
             f32x16_t s = f32x16_t{}, dp = f32x16_t{};
+            if constexpr (sizeof(T) == 2) asm volatile("" : "+v"(read.row));  // recomputed in every step: the registers are needed for reads ahead
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 const Frag8<T> q = read.rows(lds, OFF_Q + CUR * TILE, c), g = read.rows(lds, OFF_G + CUR * TILE, c);
@@ -128,6 +135,8 @@ template <typename T, int DP, bool SPLIT> __global__ __launch_bounds__(256, (DP 
                     mma32(g, load_frag<T>(vrow, 16 * c + 8 * h, a.D), dp);
                 }
             }
+            if constexpr (sizeof(T) == 2) reads_ahead<3, 2, NC>();
+            __builtin_amdgcn_s_setprio(0);
 #pragma unroll
             for (int e4 = 0; e4 < 4; ++e4) {
                 const float4 l4 = *reinterpret_cast<const float4*>(&s_lse[CUR][8 * e4 + 4 * h]), d4 = *reinterpret_cast<const float4*>(&s_delta[CUR][8 * e4 + 4 * h]);
@@ -152,6 +161,7 @@ template <typename T, int DP, bool SPLIT> __global__ __launch_bounds__(256, (DP 
                 p[j] = frag_of<T>(s, j);
                 ds[j] = frag_of<T>(dp, j);
             }
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -159,7 +169,9 @@ template <typename T, int DP, bool SPLIT> __global__ __launch_bounds__(256, (DP 
                     mma32(read.cols(lds, OFF_G + CUR * TILE, d, 16 * j), p[j], dv[d]);
                     mma32(read.cols(lds, OFF_Q + CUR * TILE, d, 16 * j), ds[j], dk[d]);
                 }
+            if constexpr (sizeof(T) == 2) reads_ahead<4, 2, 2 * ND>();
         }
+        __builtin_amdgcn_s_setprio(0);
         if (t + 1 < t1) put_stats(CUR ^ 1);
     };
     for (int t = t0; t < t1; t += 2) {

@@ -62,18 +62,29 @@ template <typename T, int DP, int BK, bool SPLIT> __global__ __launch_bounds__(2
     const T* kb = (const T*)a.k + b * a.k_sb + hk * a.k_sh;
     const T* vb = (const T*)a.v + b * a.v_sb + hk * a.v_sh;
     const unsigned k_row = (unsigned)(a.k_st * ES), v_row = (unsigned)(a.v_st * ES), lds0 = lds_address(smem);
+    TileOffsets<T, DP, BK> at_k, at_v;  // of a tile whose keys are all seen
+    at_k.set(a.D, wave, lane, [&](int x) { return x * k_row; });
+    at_v.set(a.D, wave, lane, [&](int x) { return x * v_row; });
     auto request = [&](int t, int buf, const unsigned (&seen)[KT]) {
+        const T *kt0 = kb + (long long)t * BK * a.k_st, *vt0 = vb + (long long)t * BK * a.v_st;
+        if ((seen[0] | seen[KT - 1]) == 0) return;  // a tile whose keys are all hidden is passed over
+        if ((seen[0] & seen[KT - 1]) == 0xffffffffu) {
+            at_k.request(kt0, lds0 + OFF_K + buf * TILE, wave);
+            at_v.request(vt0, lds0 + OFF_V + buf * TILE, wave);
+            return;
+        }
         auto row = [&](unsigned stride) {
             return [&, stride](int x) { return (seen[x >> 5] >> (x & 31)) & 1 ? x * stride : 0x80000000u; };
         };
-        request_tile<T, DP, BK>(kb + (long long)t * BK * a.k_st, lds0 + OFF_K + buf * TILE, a.D, wave, lane, row(k_row));
-        request_tile<T, DP, BK>(vb + (long long)t * BK * a.v_st, lds0 + OFF_V + buf * TILE, a.D, wave, lane, row(v_row));
+        request_tile<T, DP, BK>(kt0, lds0 + OFF_K + buf * TILE, a.D, wave, lane, row(k_row));
+        request_tile<T, DP, BK>(vt0, lds0 + OFF_V + buf * TILE, a.D, wave, lane, row(v_row));
     };
     int t0 = 0, t1 = k_end > 0 ? (k_end + BK - 1) / BK : 0;
     if (SPLIT) {  // an even share of the tiles that are seen
         t0 = (int)((long long)t1 * split / a.dq_splits);
         t1 = (int)((long long)t1 * (split + 1) / a.dq_splits);
     }
+    const unsigned char* mask = a.mask ? a.mask + b * a.mask_sb : nullptr;
     unsigned bits[KT], next[KT];
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
@@ -86,14 +97,18 @@ template <typename T, int DP, int BK, bool SPLIT> __global__ __launch_bounds__(2
         constexpr int CUR = decltype(which)::value;
         const int k0 = t * BK;
         tile_landed();
-        if (t + 1 < t1) request(t + 1, CUR ^ 1, next);
-        bool ok[KT];  // the tile after the next
+        unsigned ok[KT];  // the tile after the next: loaded now, waited for when this one is done
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) ok[kt] = key_seen(a, b, k0 + 2 * BK + kt * 32 + (lane & 31));
+        for (int kt = 0; kt < KT; ++kt) ok[kt] = 1;
+        if (mask)
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) ok[kt] = mask[min(k0 + 2 * BK + kt * 32 + (lane & 31), a.Tk - 1)];
+        if (t + 1 < t1) request(t + 1, CUR ^ 1, next);
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) {
-            if (k0 + kt * 32 >= w_end) continue;
+            if (k0 + kt * 32 >= w_end || bits[kt] == 0) continue;
             f32x16_t s = f32x16_t{}, dp = f32x16_t{};
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 const int at = kt * 32 * DP * ES;
@@ -109,6 +124,8 @@ template <typename T, int DP, int BK, bool SPLIT> __global__ __launch_bounds__(2
                     mma32(v, load_frag<T>(grow, 16 * c + 8 * h, a.D), dp);
                 }
             }
+            if constexpr (sizeof(T) == 2) reads_ahead<(GLDS ? 3 : 2), 2, NC>();
+            __builtin_amdgcn_s_setprio(0);
             if (bits[kt] == 0xffffffffu && k0 + kt * 32 + 31 <= w_all) {  // nothing hidden: the common case
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2, -lse2)) * (dp[e] - delta);
@@ -122,17 +139,21 @@ template <typename T, int DP, int BK, bool SPLIT> __global__ __launch_bounds__(2
                     s[e] = seen ? p * (dp[e] - delta) : 0.f;
                 }
             }
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const Frag8<T> ds = frag_of<T>(s, j);  // bf16: rounded for the product
 #pragma unroll
                 for (int d = 0; d < ND; ++d) mma32(read.cols(lds, OFF_K + CUR * TILE, d, kt * 32 + 16 * j), ds, acc[d]);
             }
+            if constexpr (sizeof(T) == 2) reads_ahead<4, 2, ND>();
+            __builtin_amdgcn_s_setprio(0);
         }
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) {
             bits[kt] = next[kt];
-            next[kt] = (unsigned)__ballot(ok[kt]);
+            asm volatile("" : "+v"(ok[kt]));  // (else the comparison, and its wait, moves up to the load)
+            next[kt] = (unsigned)__ballot(ok[kt] != 0 && k0 + 2 * BK + kt * 32 + (lane & 31) < a.Tk);
         }
     };
     for (int t = t0; t < t1; t += 2) {

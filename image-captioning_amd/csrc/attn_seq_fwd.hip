@@ -51,13 +51,24 @@ template <typename T, int DP, int BK, bool SPLIT> __global__ __launch_bounds__(2
     TileReader<T, DP> read;
     read.init(lane);
     // rows no query may see are zeros: whatever they hold, infinities and NaN included, stays out of the products
+    TileOffsets<T, DP, BK> at_k, at_v;  // of a tile whose keys are all seen
+    at_k.set(a.D, wave, lane, [&](int x) { return x * k_row; });
+    at_v.set(a.D, wave, lane, [&](int x) { return x * v_row; });
     auto request = [&](int t, int buf, const unsigned (&seen)[KT]) {
+        const T *kt0 = kb + (long long)t * BK * a.k_st, *vt0 = vb + (long long)t * BK * a.v_st;
+        if ((seen[0] | seen[KT - 1]) == 0) return;  // a tile whose keys are all hidden is passed over
+        if ((seen[0] & seen[KT - 1]) == 0xffffffffu) {
+            at_k.request(kt0, lds0 + OFF_K + buf * TILE, wave);
+            at_v.request(vt0, lds0 + OFF_V + buf * TILE, wave);
+            return;
+        }
         auto row = [&](unsigned stride) {
             return [&, stride](int x) { return (seen[x >> 5] >> (x & 31)) & 1 ? x * stride : 0x80000000u; };
         };
-        request_tile<T, DP, BK>(kb + (long long)t * BK * a.k_st, lds0 + OFF_K + buf * TILE, a.D, wave, lane, row(k_row));
-        request_tile<T, DP, BK>(vb + (long long)t * BK * a.v_st, lds0 + OFF_V + buf * TILE, a.D, wave, lane, row(v_row));
+        request_tile<T, DP, BK>(kt0, lds0 + OFF_K + buf * TILE, a.D, wave, lane, row(k_row));
+        request_tile<T, DP, BK>(vt0, lds0 + OFF_V + buf * TILE, a.D, wave, lane, row(v_row));
     };
+    const unsigned char* mask = a.mask ? a.mask + b * a.mask_sb : nullptr;
     unsigned bits[KT], next[KT];
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
@@ -70,19 +81,28 @@ template <typename T, int DP, int BK, bool SPLIT> __global__ __launch_bounds__(2
         constexpr int CUR = decltype(which)::value;
         const int k0 = t * BK;
         tile_landed();
-        if (t + 1 < t1) request(t + 1, CUR ^ 1, next);
-        bool ok[KT];  // the tile after the next
+        unsigned ok[KT];  // the tile after the next: loaded now, waited for when this one is done
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) ok[kt] = key_seen(a, b, k0 + 2 * BK + kt * 32 + (lane & 31));
-        if (k0 < w_end) {
+        for (int kt = 0; kt < KT; ++kt) ok[kt] = 1;
+        if (mask)
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) ok[kt] = mask[min(k0 + 2 * BK + kt * 32 + (lane & 31), a.Tk - 1)];
+        if (t + 1 < t1) request(t + 1, CUR ^ 1, next);
+        if (k0 < w_end && (bits[0] | bits[KT - 1]) != 0) {
             f32x16_t s[KT];
             float top = -INFINITY;
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt) {
-                s[kt] = f32x16_t{};
+            for (int kt = 0; kt < KT; ++kt) s[kt] = f32x16_t{};
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-                for (int c = 0; c < NC; ++c)
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
                     mma32(read.rows(lds, OFF_K + CUR * TILE + kt * 32 * DP * ES, c), InRegs<T, DP>::value ? qf[c % NR] : load_frag<T>(qrow, 16 * c + 8 * h, a.D), s[kt]);
+            if constexpr (sizeof(T) == 2) reads_ahead<KT, KT, NC>();
+            __builtin_amdgcn_s_setprio(0);
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
                 if (bits[kt] == 0xffffffffu && k0 + kt * 32 + 31 <= w_all) {  // nothing hidden: the common case
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
@@ -121,6 +141,7 @@ template <typename T, int DP, int BK, bool SPLIT> __global__ __launch_bounds__(2
             }
             m = m_new;
             l += sum;
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -129,11 +150,14 @@ template <typename T, int DP, int BK, bool SPLIT> __global__ __launch_bounds__(2
 #pragma unroll
                     for (int d = 0; d < ND; ++d) mma32(read.cols(lds, OFF_V + CUR * TILE, d, kt * 32 + 16 * j), p, acc[d]);
                 }
+            if constexpr (sizeof(T) == 2) reads_ahead<4, 2, KT * ND>();
+            __builtin_amdgcn_s_setprio(0);
         }
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) {
             bits[kt] = next[kt];
-            next[kt] = (unsigned)__ballot(ok[kt]);
+            asm volatile("" : "+v"(ok[kt]));  // (else the comparison, and its wait, moves up to the load)
+            next[kt] = (unsigned)__ballot(ok[kt] != 0 && k0 + 2 * BK + kt * 32 + (lane & 31) < a.Tk);
         }
     };
     for (int t = t0; t < t1; t += 2) {
