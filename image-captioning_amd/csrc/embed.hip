@@ -402,18 +402,21 @@ template <typename TO, bool A> __global__ __launch_bounds__(1024) void embed_joi
 }
 
 // ---- sum over sequences: columns of a [B][W] matrix, W = T*H; `slices` of the rows leave fp32 partial rows when there are several
-// (N columns to a lane: 8, or 1)
-template <typename TG, typename TO, int N, bool A>
-__device__ __forceinline__ void colsum(float* part, const TG* __restrict__ g, TO* __restrict__ out, float* __restrict__ part_out, int B, long long W, int slices,
+// A workgroup takes L * N columns, N to a lane; its 1024 / L groups of L lanes share the rows.  With L = 16 and N = 8 a batch of 256 captions
+// of 30 x 512 columns is 120 workgroups with one round of loads each, two to a compute unit: the first launch of the gradient takes 8.6 us, with L = 64 and one
+// workgroup to a compute unit it took 13.9 us.
+template <typename TG, typename TO, int L, int N, bool A>
+__device__ __forceinline__ void colsum(float* lds, const TG* __restrict__ g, TO* __restrict__ out, float* __restrict__ part_out, int B, long long W, int slices,
                                        long long group, int slice) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long long col = (group * 64 + lane) * N;
+    constexpr int C = L * N, SHARES = 1024 / L, PARTS = 1024 / C, U = 4;
+    static_assert(SHARES % PARTS == 0, "whole shares");
+    const int lane = threadIdx.x % L, share = threadIdx.x / L;
+    const long long col = group * C + lane * N;
     const bool live = col < W;
     const int m = W - col < N ? (int)(W - col) : N;
     const int b0 = (int)((long long)B * slice / slices), b1 = (int)((long long)B * (slice + 1) / slices), rows = b1 - b0;
-    const int lo = b0 + (int)((long long)rows * wave / 16), hi = b0 + (int)((long long)rows * (wave + 1) / 16);
+    const int lo = b0 + (int)((long long)rows * share / SHARES), hi = b0 + (int)((long long)rows * (share + 1) / SHARES);
     float acc[N] = {};
-    constexpr int U = 8;
     for (int b = lo; b < hi; b += U) {
         float v[U][N];
 #pragma unroll
@@ -429,22 +432,26 @@ __device__ __forceinline__ void colsum(float* part, const TG* __restrict__ g, TO
             for (int e = 0; e < N; ++e) acc[e] += live && b + u < hi ? v[u][e] : 0.f;
     }
 #pragma unroll
-    for (int e = 0; e < N; ++e) part[wave * 64 * N + lane * N + e] = acc[e];
+    for (int e = 0; e < N; ++e) lds[share * C + lane * N + e] = acc[e];
     __syncthreads();
-    // 64 * N columns over 1024 threads
-    for (int c = threadIdx.x; c < 64 * N; c += 1024) {
-        const long long at = group * 64 * N + c;
-        if (at >= W) continue;
-        float s = part[c];
+    // the shares of a column in order: PARTS threads take some each, one adds what they leave
+    const int c = threadIdx.x % C, part = threadIdx.x / C;
+    float t = lds[part * (SHARES / PARTS) * C + c];
 #pragma unroll
-        for (int w = 1; w < 16; ++w) s += part[w * 64 * N + c];
-        if (slices == 1) out[at] = from_f32<TO>(s);
-        else part_out[slice * W + at] = s;
-    }
+    for (int k = 1; k < SHARES / PARTS; ++k) t += lds[(part * (SHARES / PARTS) + k) * C + c];
+    __syncthreads();
+    lds[threadIdx.x] = t;
+    __syncthreads();
+    const long long at = group * C + c;
+    if (part > 0 || at >= W) return;
+#pragma unroll
+    for (int k = 1; k < PARTS; ++k) t += lds[k * C + c];
+    if (slices == 1) out[at] = from_f32<TO>(t);
+    else part_out[slice * W + at] = t;
 }
 template <typename TO> __global__ __launch_bounds__(1024) void embed_colsum_join_kernel(const float* __restrict__ part_in, TO* __restrict__ out, int parts, long long W) {
-    __shared__ float part[16 * 64];
-    colsum<float, TO, 1, true>(part, part_in, out, nullptr, parts, W, 1, blockIdx.x, 0);
+    __shared__ float lds[1024];
+    colsum<float, TO, 64, 1, true>(lds, part_in, out, nullptr, parts, W, 1, blockIdx.x, 0);
 }
 
 // ---- the first launch of the gradient: three jobs that need nothing from each other, by block number -------------------------
@@ -460,12 +467,13 @@ struct FirstArgs {
     int H, B, slices, rank_blocks, zero_blocks;
     long long groups;
 };
+constexpr int SUM_COLUMNS = 16 * VEC;
 constexpr int RANK_MAX = 8192, RANK_TOKENS = 32, ZERO_ROWS = 128;
 constexpr int RANK_MAX_VOCAB = 1 << 18;  // word and token number share 31 bits
 
-template <typename TG, typename TO, bool A> __global__ __launch_bounds__(1024) void embed_first_kernel(FirstArgs f) {
-    __shared__ __attribute__((aligned(16))) unsigned lds[RANK_MAX + 1024];  // 36 KiB, also the column sums' 16 x 64 x VEC floats
-    static_assert(16 * 64 * VEC <= RANK_MAX + 1024, "column sums fit");
+template <typename TG, typename TO, bool A> __global__ __launch_bounds__(1024, 8) void embed_first_kernel(FirstArgs f) {  // two workgroups to a compute unit
+    __shared__ __attribute__((aligned(16))) unsigned lds[RANK_MAX + 1024];  // 36 KiB, also the column sums' 1024 x VEC floats
+    static_assert(1024 * VEC <= RANK_MAX + 1024, "column sums fit");
     const SortArgs& a = f.sort;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int block = blockIdx.x;
@@ -517,7 +525,7 @@ template <typename TG, typename TO, bool A> __global__ __launch_bounds__(1024) v
         return;
     }
     block -= f.zero_blocks;
-    colsum<TG, TO, VEC, A>(reinterpret_cast<float*>(lds), (const TG*)f.g, (TO*)f.d_pos, f.pos_part, f.B, f.W, f.slices, block % f.groups, (int)(block / f.groups));
+    colsum<TG, TO, 16, VEC, A>(reinterpret_cast<float*>(lds), (const TG*)f.g, (TO*)f.d_pos, f.pos_part, f.B, f.W, f.slices, block % f.groups, (int)(block / f.groups));
 }
 
 // ---- the gradient's plan: everything that depends on the sizes alone -------------------------------------------------------
@@ -558,10 +566,10 @@ GradPlan grad_plan(long long n, int T, int H, int vocab, bool want_pos) {
     p.tail = o; o += up256(p.chunks * row);
     p.slices = 1;
     if (want_pos) {
-        // up to 256 workgroups over the columns of [B][T*H], at least 512 sequences to a slice
-        const long long B = n / T, groups = ((long long)T * H + 511) / 512;
+        // up to 256 workgroups over the columns of [B][T*H], at least 256 sequences (a round of loads) to a slice
+        const long long B = n / T, groups = ((long long)T * H + SUM_COLUMNS - 1) / SUM_COLUMNS;
         long long s = 256 / (groups < 1 ? 1 : groups);
-        if (s > B / 512) s = B / 512;
+        if (s > B / 256) s = B / 256;
         p.slices = (int)(s < 1 ? 1 : s > 512 ? 512 : s);
         p.pos = o;
         if (p.slices > 1) o += up256((long long)p.slices * T * H * 4);
@@ -597,7 +605,7 @@ int launch_grad(const GradPlan& p, const void* ids, int wide, const void* g, voi
         f.B = (int)(n / T);
         f.W = (long long)T * H;
         f.slices = p.slices;
-        f.groups = (f.W + 64 * VEC - 1) / (64 * VEC);
+        f.groups = (f.W + SUM_COLUMNS - 1) / SUM_COLUMNS;
     }
     const long long first = f.rank_blocks + f.zero_blocks + f.groups * f.slices;
     if (first > 0) MIC_LAUNCH((embed_first_kernel<TG, TO, A>), dim3((unsigned)first), dim3(1024), 0, s, f);
