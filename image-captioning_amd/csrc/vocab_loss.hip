@@ -546,6 +546,9 @@ long long up256(long long b) { return (b + 255) / 256 * 256; }
 
 int edge_tiles(long long n, int edge) { return (int)((n + edge - 1) / edge); }
 
+// the share of the rounds of `slots` workgroups that `tiles` keep busy
+double filled(long long tiles, int slots) { return (double)tiles / ((tiles + slots - 1) / slots * slots); }
+
 struct Plan {
     int Hp, e;              // columns of the operands the products read (H rounded up to whole 16 bytes)
     bool pad;               // x and w are copied to that width first
@@ -578,8 +581,11 @@ Plan make_plan(const mic_vocab_loss_desc* d, bool grad) {
     // The large tiles from half a tile per compute unit on.  V = 3500, H = 512, forward and gradient: 2,400 rows (140 large tiles) 120 us
     // on large tiles and 145 us on small ones, 1,200 rows (70) 106 and 92 us.  They address 256 rows (64 of k) with 31 bits.
     p.big = d->dtype == MIC_BF16 && (long long)edge_tiles(N, 256) * edge_tiles(V, 256) >= 128 && H >= 64 && H < (1 << 21) && d->ld_x < (1 << 21) && d->ld_w < (1 << 21);
-    // 64 x 64 tiles where 128 x 128 ones would leave compute units idle
-    p.edge = p.big ? 256 : (long long)edge_tiles(N, 128) * edge_tiles(V, 128) < 512 ? 64 : 128;
+    // 64 x 64 tiles where 128 x 128 ones would leave compute units idle, half of each tile (H = 64: 20,000 x 3500 forward and gradient 533
+    // us, on the larger 746), and in fp32 also the last round of them: a small tile costs 8 % more there (4096 x 512 x 16384: 2663 and
+    // 2443 us), 1111 x 300 x 10007 is 1.4 rounds of large tiles and 2.8 of small ones (266 and 302 us)
+    const long long large = (long long)edge_tiles(N, 128) * edge_tiles(V, 128), small = (long long)edge_tiles(N, 64) * edge_tiles(V, 64);
+    p.edge = p.big ? 256 : large < 512 || H <= 64 || (d->dtype == MIC_F32 && 1.08 * filled(large, 512) < filled(small, 1024)) ? 64 : 128;
     p.copy_x = p.pad || grad;
     long long o = 0;
     p.xpad = o;
