@@ -75,13 +75,13 @@ struct GemmShape {
 };
 
 // Epi::run(args, acc, p0, q0, lane, part_p, part_q, slice): acc[i][j] = p0 + 32 i.., q0 + 32 j..; parts number the waves' columns and rows
-template <typename T, int S, bool PCOL, bool QCOL, typename Epi> __global__ __launch_bounds__(256, 2) void vocab_gemm_kernel(GemmShape g, typename Epi::Args ea) {
+template <typename T, int S> using GemmLds = T[2][64 * S * 128 / (int)sizeof(T)];  // two tiles of an operand
+// the tile of workgroup `order` of the product
+template <typename T, int S, bool PCOL, bool QCOL, typename Epi> __device__ __forceinline__ void vocab_gemm_tile(GemmShape g, const typename Epi::Args& ea, int order, GemmLds<T, S>& sp, GemmLds<T, S>& sq) {
     constexpr int VT = 64 * S, WAVE = 32 * S;
     using TP = OperandTile<T, PCOL, VT>;
     using TQ = OperandTile<T, QCOL, VT>;
     constexpr int KS = TP::KS;
-    __shared__ __attribute__((aligned(16))) T sp[2][VT * KS];
-    __shared__ __attribute__((aligned(16))) T sq[2][VT * KS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wp = wave >> 1, wq = wave & 1;
     if (g.rows) {  // the grid is laid out for all rows: what is behind the counted ones ends here
         const int rows = *g.rows;
@@ -96,7 +96,7 @@ template <typename T, int S, bool PCOL, bool QCOL, typename Epi> __global__ __la
     // workgroups b and b + 8 share an XCD and its L2: every XCD takes a contiguous range of the tiles that are left
     int id;
     {
-        const int n = g.tiles_p * g.tiles_q * slices, o = blockIdx.x, per = n >> 3, rest = n & 7, xcd = o & 7;
+        const int n = g.tiles_p * g.tiles_q * slices, o = order, per = n >> 3, rest = n & 7, xcd = o & 7;
         if (o >= n) return;
         id = (xcd < rest ? xcd * (per + 1) : rest * (per + 1) + (xcd - rest) * per) + (o >> 3);
     }
@@ -158,6 +158,20 @@ template <typename T, int S, bool PCOL, bool QCOL, typename Epi> __global__ __la
         }
     }
     Epi::run(ea, acc, p0 + wp * WAVE, q0 + wq * WAVE, lane, tp * 2 + wp, tq * 2 + wq, slice);
+}
+template <typename T, int S, typename Epi> __global__ __launch_bounds__(256, 2) void vocab_gemm_kernel(GemmShape g, typename Epi::Args ea) {
+    __shared__ __attribute__((aligned(16))) GemmLds<T, S> sp;
+    __shared__ __attribute__((aligned(16))) GemmLds<T, S> sq;
+    vocab_gemm_tile<T, S, false, false, Epi>(g, ea, blockIdx.x, sp, sq);
+}
+// Two products in one launch, both of whose P lie with their index consecutive: the second one's workgroups from `first` on (a multiple of
+// 8), its Q likewise.
+template <typename T, int S, typename Epi>
+__global__ __launch_bounds__(256, 2) void vocab_gemm_pair_kernel(GemmShape x, typename Epi::Args xa, GemmShape w, typename Epi::Args wa, int first) {
+    __shared__ __attribute__((aligned(16))) GemmLds<T, S> sp;
+    __shared__ __attribute__((aligned(16))) GemmLds<T, S> sq;
+    if ((int)blockIdx.x < first) vocab_gemm_tile<T, S, true, false, Epi>(x, xa, blockIdx.x, sp, sq);
+    else vocab_gemm_tile<T, S, true, true, Epi>(w, wa, (int)blockIdx.x - first, sp, sq);
 }
 
 }  // namespace

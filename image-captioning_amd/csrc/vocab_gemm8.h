@@ -27,8 +27,8 @@ struct Operand8 {
 };
 struct Gemm8Shape {
     Operand8 p, q;
-    const int* rows;    // NULL, or the number of rows to take, on the device: limits q.n (k for products over the rows)
-    const int* slices;  // NULL (one), or the number of ranges of k, on the device
+    const int* rows;    // the number of rows to take, on the device: limits q.n (k for products over the rows)
+    const int* slices;  // the number of ranges of k, on the device
     int rows_are_k;
     int K, tiles_p, tiles_q;
 };
@@ -118,23 +118,26 @@ template <bool COL, int N> struct Read8 {
 
 // Epi::side(args, p0, q0, thread, side) fills the side buffer; Epi::run(args, acc, p0, q0, lane, wave, tile_p, tile_q, slice, side):
 // acc[j][i] = p0 + 64 (wave & 3) + 16 j.., q0 + 128 (wave >> 2) + 16 i..
-template <bool PCOL, bool QCOL, typename Epi> __global__ __launch_bounds__(512) void vocab_gemm8_kernel(Gemm8Shape g, typename Epi::Args ea) {
-    __shared__ __attribute__((aligned(16))) unsigned char smem[2 * G8_TILE];
-    __shared__ __attribute__((aligned(16))) float side[2][G8_SIDE];
+// The tiles of a product from `order` on, gridDim.x apart; returns how many there are.  COUNTED, SLICED: whether the shape has rows and slices
+// (what it has not costs scalar registers).
+template <bool PCOL, bool QCOL, bool COUNTED, bool SLICED, typename Epi>
+__device__ __forceinline__ int vocab_gemm8_tiles(const Gemm8Shape& shape, const typename Epi::Args& ea, int order, unsigned char (&smem)[2 * G8_TILE], float (&side)[2][G8_SIDE]) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wq = wave >> 2, wp = wave & 3;
-    int K = g.K;
-    if (g.rows) {  // the grid is laid out for all rows: what is behind the counted ones ends here
-        const int rows = __builtin_amdgcn_readfirstlane(*g.rows);
-        if (g.rows_are_k) {
+    const Operand8 &gp = shape.p;
+    Operand8 gq = shape.q;
+    int K = shape.K, tiles_q = shape.tiles_q;
+    const int tiles_p = shape.tiles_p;
+    if (COUNTED) {  // the grid is laid out for all rows: what is behind the counted ones ends here
+        const int rows = __builtin_amdgcn_readfirstlane(*shape.rows);
+        if (shape.rows_are_k) {
             K = min(K, rows);
         } else {
-            g.q.n = min(g.q.n, rows);
-            g.tiles_q = min(g.tiles_q, (rows + 255) / 256);
+            gq.n = min(gq.n, rows);
+            tiles_q = min(tiles_q, (rows + 255) / 256);
         }
     }
-    const int slices = g.slices ? __builtin_amdgcn_readfirstlane(*g.slices) : 1, total = g.tiles_p * g.tiles_q * slices, nk = (K + 63) / 64;
-    int order = blockIdx.x;
-    if (order >= total) return;
+    const int slices = SLICED ? __builtin_amdgcn_readfirstlane(*shape.slices) : 1, total = tiles_p * tiles_q * slices, nk = (K + 63) / 64;
+    if (order >= total) return total;
 
     struct Place {
         int tp, tq, slice, t_begin, t_end;
@@ -144,14 +147,17 @@ template <bool PCOL, bool QCOL, typename Epi> __global__ __launch_bounds__(512) 
         const int per = total >> 3, rest = total & 7, xcd = o & 7;
         int id = (xcd < rest ? xcd * (per + 1) : rest * (per + 1) + (xcd - rest) * per) + (o >> 3);
         Place x;
-        x.slice = id % slices;
-        id /= slices;
+        x.slice = 0;
+        if (SLICED) {
+            x.slice = id % slices;
+            id /= slices;
+        }
         // 4 q tiles side by side walk the p tiles, so what runs at once on an XCD is a block of both and shares its operands in L2
-        const int band = id / (4 * g.tiles_p), left = min(4, g.tiles_q - band * 4), in = id - band * 4 * g.tiles_p;
+        const int band = id / (4 * tiles_p), left = min(4, tiles_q - band * 4), in = id - band * 4 * tiles_p;
         x.tq = band * 4 + in % left;
         x.tp = in / left;
-        x.t_begin = (int)((long long)x.slice * nk / slices);
-        x.t_end = (int)((long long)(x.slice + 1) * nk / slices);
+        x.t_begin = SLICED ? (int)((long long)x.slice * nk / slices) : 0;
+        x.t_end = SLICED ? (int)((long long)(x.slice + 1) * nk / slices) : nk;
         // the same in every lane, computed in vector registers: the buffers' bases are built from them
         x.tp = __builtin_amdgcn_readfirstlane(x.tp);
         x.tq = __builtin_amdgcn_readfirstlane(x.tq);
@@ -174,8 +180,8 @@ template <bool PCOL, bool QCOL, typename Epi> __global__ __launch_bounds__(512) 
     auto begin = [&](const Place& x, int parity) {
         Epi::side(ea, x.tp * 256, x.tq * 256, threadIdx.x, side[parity]);
         if (x.t_begin >= x.t_end) return;
-        rq.init(g.q, x.tq * 256, x.t_begin * 64, wave, lane);
-        rp.init(g.p, x.tp * 256, x.t_begin * 64, wave, lane);
+        rq.init(gq, x.tq * 256, x.t_begin * 64, wave, lane);
+        rp.init(gp, x.tp * 256, x.t_begin * 64, wave, lane);
         rq.issue(0, piece_q + G8_Q0, K);
         rp.issue(0, piece_p + G8_P0, K);
         rp.issue(1, piece_p + G8_P1, K);
@@ -270,8 +276,22 @@ template <bool PCOL, bool QCOL, typename Epi> __global__ __launch_bounds__(512) 
             begin(at, parity ^ 1);
         }
         Epi::run(ea, acc, done.tp * 256, done.tq * 256, lane, wave, done.tp, done.tq, done.slice, side[parity]);
-        if (order >= total) return;
+        if (order >= total) return total;
     }
+}
+template <typename Epi> __global__ __launch_bounds__(512) void vocab_gemm8_kernel(Gemm8Shape g, typename Epi::Args ea) {
+    __shared__ __attribute__((aligned(16))) unsigned char smem[2 * G8_TILE];
+    __shared__ __attribute__((aligned(16))) float side[2][G8_SIDE];
+    vocab_gemm8_tiles<false, false, Epi::COUNTED, false, Epi>(g, ea, blockIdx.x, smem, side);
+}
+// Two products in one launch, both of whose P lie with their index consecutive, and the second one's Q: their tiles are dealt out in turn,
+// the second one's from the next multiple of 8 on.  An epilogue without a side buffer leaves LDS alone, so a workgroup goes from
+// one product to the other like from tile to tile.
+template <typename Epi> __global__ __launch_bounds__(512) void vocab_gemm8_pair_kernel(Gemm8Shape x, typename Epi::Args xa, Gemm8Shape w, typename Epi::Args wa) {
+    __shared__ __attribute__((aligned(16))) unsigned char smem[2 * G8_TILE];
+    __shared__ __attribute__((aligned(16))) float side[2][G8_SIDE];
+    const int n = (vocab_gemm8_tiles<true, false, true, true, Epi>(x, xa, blockIdx.x, smem, side) + 7) & ~7, grid = gridDim.x, block = blockIdx.x;
+    vocab_gemm8_tiles<true, true, true, true, Epi>(w, wa, block >= n ? block - n : (n - block + grid - 1) / grid * grid + block - n, smem, side);
 }
 
 }  // namespace

@@ -210,6 +210,7 @@ template <typename T> struct OutEpi {
 // side buffer: [0] bias of the tile's 256 columns (-infinity past the last word), [1] targets of its 256 rows, [2] weights, [3] lse
 struct StatsEpi8 {
     typedef StatsEpi::Args Args;
+    static constexpr bool COUNTED = false;
     __device__ static __forceinline__ void side(const Args& a, int p0, int q0, int tid, float* side) {
         const int i = tid & 255;
         if (tid < 256) {
@@ -247,12 +248,14 @@ struct StatsEpi8 {
             const int tc = reinterpret_cast<const int*>(side)[256 + ql + 16 * i] - p0 - pl;  // the target's column, from the lane's first
             const float m2 = (m[i] == -INFINITY ? 0.f : m[i]) * ATTN_LOG2E;
             s[i] = 0.f;
-            if ((unsigned)tc < 64u)  // in this wave's columns, but perhaps in another lane's
+            if ((unsigned)tc < 64u && (tc & 12) == 0) {  // in this lane's columns
+                float z = 0.f;
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (tc == 16 * j + e) a.zt[q0 + ql + 16 * i] = acc[j][i][e];
+                    for (int e = 0; e < 4; ++e) z = tc == 16 * j + e ? acc[j][i][e] : z;
+                a.zt[q0 + ql + 16 * i] = z;
+            }
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -276,6 +279,7 @@ struct StatsEpi8 {
 
 struct GradEpi8 {
     typedef GradEpi<bf16_t>::Args Args;
+    static constexpr bool COUNTED = true;
     __device__ static __forceinline__ int rows(const Args& a) { return *a.count; }
     __device__ static __forceinline__ void side(const Args& a, int p0, int q0, int tid, float* side) {
         const int i = tid & 255;
@@ -442,30 +446,43 @@ template <typename T> __global__ __launch_bounds__(256) void vocab_finish_kernel
 // Target, weight and lse of the counted rows, in their order: `at` tells where a row went (-1: it does not count), *count how many there
 // are.  A block counts the rows before its own again (at most 64 blocks) instead of waiting for others.
 //
-// The last block also decides into how many ranges of k the products dx (of a whole piece and of the last one) and dw are cut, now that the
+// The last block also decides into how many ranges of k the products dx and dw are cut (of a whole piece and of the last one), now that the
 // rows are known.
 struct SplitRule {
-    int capacity;           // workgroups resident at once
+    float capacity;         // workgroups resident at once
     float fixed, traffic;   // in steps of k: what a workgroup costs beside its steps; what the partial tiles of a full GPU cost
 };
 struct Split {
     int tiles, nk, most;    // tiles of the result (dx: per tile of rows), steps of k (dw: 0, by the rows), ranges allowed
 };
-// 16 lanes to a decision, lane i looks at i + 1 ranges; the cheapest, the smaller number where two cost the same, ends in all of them
-__device__ __forceinline__ int choose_slices(const SplitRule& r, int tiles, int nk, int most, int lane) {
-    int s = (lane & 15) + 1;
-    const float x = (float)tiles * s / r.capacity;
-    float cost = s <= most ? ceilf(x) * (ceilf((float)nk / s) + r.fixed) + (s > 1 ? x * r.traffic : 0.f) : INFINITY;
+// The pair of numbers that costs least, up to 16 each: a lane looks at one number for x and four for w.  Both products are one launch, whose
+// tiles are dealt out in turn: the first workgroups have one tile of x more, or the ones behind them one of w.
+__device__ __forceinline__ int2 choose_slices(const SplitRule& r, int tiles_x, int nk_x, int most_x, int tiles_w, int nk_w, int most_w, int lane) {
+    const int sx = (lane & 15) + 1;
+    const float all_x = (float)(tiles_x * sx) / r.capacity, some = floorf(all_x), up = ceilf(all_x), kx = ceilf((float)nk_x / sx) + r.fixed;
+    float best = INFINITY;
+    int at = 0;
 #pragma unroll
-    for (int d = 8; d > 0; d >>= 1) {
-        const float c = __shfl_xor(cost, d, 64);
-        const int o = __shfl_xor(s, d, 64);
-        if (c < cost || (c == cost && o < s)) {
-            cost = c;
-            s = o;
+    for (int i = 0; i < 4; ++i) {
+        const int sw = (lane >> 4) * 4 + i + 1;
+        const float all_w = (float)(tiles_w * sw) / r.capacity, rounds = ceilf(all_x + all_w), kw = ceilf((float)nk_w / sw) + r.fixed;
+        float cost = fmaxf(up * kx + (rounds - up) * kw, some * kx + (rounds - some) * kw) + (all_x + (sw > 1 ? all_w : 0.f)) * r.traffic;
+        if (sx > most_x || sw > most_w) cost = INFINITY;
+        if (cost < best) {
+            best = cost;
+            at = sw * 32 + sx;
         }
     }
-    return s;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+        const float c = __shfl_xor(best, d, 64);
+        const int o = __shfl_xor(at, d, 64);
+        if (c < best || (c == best && o < at)) {
+            best = c;
+            at = o;
+        }
+    }
+    return make_int2(at & 31, at >> 5);
 }
 enum { COUNT, SX, SX_LAST, SW, SW_LAST, DECISIONS };  // what `count` points to
 struct RowsArgs {
@@ -509,13 +526,14 @@ __global__ __launch_bounds__(1024) void vocab_rows_kernel(RowsArgs a) {
             a.lse_out[to] = a.lse[i];
         }
     }
-    if (blockIdx.x == gridDim.x - 1 && wave == 0) {
-        const int rows = base, i = (lane >> 4) & 1;  // dx, dx last, dw, dw last
-        const bool is_dw = lane >= 32;
-        const int s = choose_slices(a.rule, is_dw ? a.dw[i].tiles : a.dx[i].tiles * ((rows + a.edge - 1) / a.edge), is_dw ? (rows + a.ks - 1) / a.ks : a.dx[i].nk,
-                                    is_dw ? a.dw[i].most : a.dx[i].most, lane);
-        if ((lane & 15) == 0) a.count[SX + (lane >> 4)] = s;
-        if (lane == 0) a.count[COUNT] = rows;
+    if (blockIdx.x == gridDim.x - 1 && wave < 2) {  // whole pieces, the last one
+        const int rows = base, i = wave;
+        const int2 n = choose_slices(a.rule, a.dx[i].tiles * ((rows + a.edge - 1) / a.edge), a.dx[i].nk, a.dx[i].most, a.dw[i].tiles, (rows + a.ks - 1) / a.ks, a.dw[i].most, lane);
+        if (lane == 0) {
+            a.count[i ? SX_LAST : SX] = n.x;
+            a.count[i ? SW_LAST : SW] = n.y;
+            if (i == 0) a.count[COUNT] = rows;
+        }
     }
 }
 
@@ -656,25 +674,50 @@ struct Rows {
     const int* slices;  // NULL: one
     int most;           // slices the grid is laid out for
 };
-template <typename T, int S, bool PCOL, bool QCOL, typename Epi>
-int gemm(const Operand& p, const Operand& q, const Rows& r, int K, const typename Epi::Args& ea, hipStream_t s) {
-    GemmShape g = {p, q, r.count, r.slices, r.are_k, K, edge_tiles(p.n, 64 * S), edge_tiles(q.n, 64 * S)};
-    MIC_LAUNCH((vocab_gemm_kernel<T, S, PCOL, QCOL, Epi>), dim3((unsigned)((long long)g.tiles_p * g.tiles_q * (r.slices ? r.most : 1))), dim3(256), 0, s, g, ea);
-    return 0;
+int grid_tiles(const GemmShape& g, int most) { return g.tiles_p * g.tiles_q * most; }
+template <typename T, int S> GemmShape shape_of(const Operand& p, const Operand& q, const Rows& r, int K) {
+    return {p, q, r.count, r.slices, r.are_k, K, edge_tiles(p.n, 64 * S), edge_tiles(q.n, 64 * S)};
 }
-template <bool PCOL, bool QCOL, typename Epi> int gemm8(const Operand& p, const Operand& q, const Rows& r, int K, const typename Epi::Args& ea, hipStream_t s) {
-    Gemm8Shape g = {{p.p, p.ld, p.n}, {q.p, q.ld, q.n}, r.count, r.slices, r.are_k, K, edge_tiles(p.n, 256), edge_tiles(q.n, 256)};
-    const long long all = (long long)g.tiles_p * g.tiles_q * (r.slices ? r.most : 1);
-    MIC_LAUNCH((vocab_gemm8_kernel<PCOL, QCOL, Epi>), dim3((unsigned)(all < 256 ? all : 256)), dim3(512), 0, s, g, ea);  // one to a compute unit
-    return 0;
+Gemm8Shape shape8_of(const Operand& p, const Operand& q, const Rows& r, int K) {
+    return {{p.p, p.ld, p.n}, {q.p, q.ld, q.n}, r.count, r.slices, r.are_k, K, edge_tiles(p.n, 256), edge_tiles(q.n, 256)};
 }
 // bf16 on the tiles of the plan, fp32 on the small ones
-template <typename T, bool PCOL, bool QCOL, typename Epi, typename Epi8>
-int product(const Plan& pl, const Operand& p, const Operand& q, const Rows& r, int K, const typename Epi::Args& ea, hipStream_t s) {
+template <typename T, typename Epi, typename Epi8> int product(const Plan& pl, const Operand& p, const Operand& q, const Rows& r, int K, const typename Epi::Args& ea, hipStream_t s) {
     if constexpr (sizeof(T) == 2)
-        if (pl.big) return gemm8<PCOL, QCOL, Epi8>(p, q, r, K, ea, s);
-    if (pl.edge == 64) return gemm<T, 1, PCOL, QCOL, Epi>(p, q, r, K, ea, s);
-    return gemm<T, 2, PCOL, QCOL, Epi>(p, q, r, K, ea, s);
+        if (pl.big) {
+            const Gemm8Shape g = shape8_of(p, q, r, K);
+            const long long all = (long long)g.tiles_p * g.tiles_q;
+            MIC_LAUNCH((vocab_gemm8_kernel<Epi8>), dim3((unsigned)(all < 256 ? all : 256)), dim3(512), 0, s, g, ea);  // one to a compute unit
+            return 0;
+        }
+    if (pl.edge == 64) {
+        const GemmShape g = shape_of<T, 1>(p, q, r, K);
+        MIC_LAUNCH((vocab_gemm_kernel<T, 1, Epi>), dim3((unsigned)grid_tiles(g, 1)), dim3(256), 0, s, g, ea);
+    } else {
+        const GemmShape g = shape_of<T, 2>(p, q, r, K);
+        MIC_LAUNCH((vocab_gemm_kernel<T, 2, Epi>), dim3((unsigned)grid_tiles(g, 1)), dim3(256), 0, s, g, ea);
+    }
+    return 0;
+}
+struct OutProduct {
+    Operand p, q;
+    Rows r;
+    int K;
+};
+template <typename T, int S> int pair_of(const OutProduct& x, const typename OutEpi<T>::Args& xa, const OutProduct& w, const typename OutEpi<T>::Args& wa, hipStream_t s) {
+    const GemmShape gx = shape_of<T, S>(x.p, x.q, x.r, x.K), gw = shape_of<T, S>(w.p, w.q, w.r, w.K);
+    const int first = (grid_tiles(gx, x.r.most) + 7) / 8 * 8;
+    MIC_LAUNCH((vocab_gemm_pair_kernel<T, S, OutEpi<T>>), dim3((unsigned)(first + grid_tiles(gw, w.r.most))), dim3(256), 0, s, gx, xa, gw, wa, first);
+    return 0;
+}
+// dx and dw of a piece: two launches would each end with half of the GPU idle
+template <typename T> int products(const Plan& pl, const OutProduct& x, const typename OutEpi<T>::Args& xa, const OutProduct& w, const typename OutEpi<T>::Args& wa, hipStream_t s) {
+    if constexpr (sizeof(T) == 2)
+        if (pl.big) {
+            MIC_LAUNCH((vocab_gemm8_pair_kernel<OutEpi8>), dim3(256), dim3(512), 0, s, shape8_of(x.p, x.q, x.r, x.K), xa, shape8_of(w.p, w.q, w.r, w.K), wa);
+            return 0;
+        }
+    return pl.edge == 64 ? pair_of<T, 1>(x, xa, w, wa, s) : pair_of<T, 2>(x, xa, w, wa, s);
 }
 
 template <typename T> int copy_rows(const void* in, long long ld, void* out, const int* at, long long rows, int cols, int padded, hipStream_t s) {
@@ -705,7 +748,7 @@ template <typename T> int forward(const mic_vocab_loss_desc* d, const Plan& p, h
     ea.bias = d->bias; ea.t = targets_of(d);
     ea.part = (float2*)(ws + p.part); ea.zt = (float*)(ws + p.zt);
     ea.N = d->N; ea.V = d->V; ea.parts = p.parts;
-    MIC_TRY((product<T, false, false, StatsEpi, StatsEpi8>(p, w, x, Rows{}, d->H, ea, s)));
+    MIC_TRY((product<T, StatsEpi, StatsEpi8>(p, w, x, Rows{}, d->H, ea, s)));
     MIC_LAUNCH(vocab_loss_rows_kernel, dim3((d->N + 15) / 16), dim3(1024), 0, s, (const float2*)ea.part, (const float*)ea.zt, ea.t, d->loss, d->lse, d->N, p.parts);
     return 0;
 }
@@ -726,7 +769,7 @@ template <typename T> int gradient(const mic_vocab_loss_desc* d, const Plan& p, 
     ra.per_block = (int)((share + 1023) / 1024 * 1024);
     // measured on 256 x 256 tiles: a step of 64 k is 1.7 us, a workgroup's start and end 4 steps, writing and reading again the partial
     // tiles of all compute units 16; on 128 x 128 tiles (two workgroups to a compute unit) 2 and 7
-    ra.rule = p.big ? SplitRule{256, 4.f, 16.f} : p.edge == 128 ? SplitRule{512, 2.f, 7.f} : SplitRule{1024, 3.f, 7.f};
+    ra.rule = p.big ? SplitRule{256.f, 4.f, 16.f} : p.edge == 128 ? SplitRule{512.f, 2.f, 7.f} : SplitRule{1024.f, 3.f, 7.f};
     ra.edge = p.edge;
     ra.ks = 128 / (int)sizeof(T);
     const int last = d->V - (p.pieces - 1) * p.Vc, th = edge_tiles(H, p.edge);
@@ -758,21 +801,20 @@ template <typename T> int gradient(const mic_vocab_loss_desc* d, const Plan& p, 
         ga.d = dl; ga.part_db = d->db ? part_db : nullptr;
         ga.Vc = vc; ga.ld = p.ld; ga.v0 = v0;
         ga.count = count;
-        MIC_TRY((product<T, false, false, GradEpi<T>, GradEpi8>(p, wi, x, Rows{count, 0, nullptr, 1}, d->H, ga, s)));
+        MIC_TRY((product<T, GradEpi<T>, GradEpi8>(p, wi, x, Rows{count, 0, nullptr, 1}, d->H, ga, s)));
         // dx += d w: k runs over the words of the piece
         typename OutEpi<T>::Args xa = {};
         xa.ld = H; xa.Np = d->H; xa.Nq = d->N;
         xa.part = part_dx + (long long)i * p.sx * N * H;  // rows of the gathered order
         const Operand wc = {wi.p, wi.ld, d->H}, dr = {dl, p.ld, d->N};
-        const Rows rx = {count, 0, p.sx > 1 ? ra.count + (end ? SX_LAST : SX) : nullptr, p.sx};
-        MIC_TRY((product<T, true, false, OutEpi<T>, OutEpi8>(p, wc, dr, rx, vc, xa, s)));
+        const Rows rx = {count, 0, ra.count + (end ? SX_LAST : SX), p.sx};
         // dw = d^T x: k runs over the rows
         typename OutEpi<T>::Args wa = {};
         wa.out = (T*)d->dw + v0 * H; wa.ld = H; wa.Np = d->H; wa.Nq = vc;
         if (p.sw > 1) wa.part = part_dw;
         const Operand xc = {x.p, x.ld, d->H}, dc = {dl, p.ld, vc};
-        const Rows rw = {count, 1, p.sw > 1 ? ra.count + (end ? SW_LAST : SW) : nullptr, p.sw};
-        MIC_TRY((product<T, true, true, OutEpi<T>, OutEpi8>(p, xc, dc, rw, d->N, wa, s)));
+        const Rows rw = {count, 1, ra.count + (end ? SW_LAST : SW), p.sw};
+        MIC_TRY((products<T>(p, {wc, dr, rx, vc}, xa, {xc, dc, rw, d->N}, wa, s)));
         SumParts sw = {}, sx = {};
         ColSum sb = {};
         if (p.sw > 1) sw = parts_of(part_dw, wa.out, nullptr, vc, vc * H, 1, p.sw, SW, end ? SW_LAST : SW);
