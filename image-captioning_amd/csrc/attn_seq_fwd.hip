@@ -4,6 +4,10 @@
 // A workgroup of four waves takes 128 rows of one key head; a wave keeps 32 rows' queries as B operands in registers and computes
 // S^T = K Q^T, so a lane owns one row (query) and the statistics of a row are 16 registers of one lane and one exchange with
 // the lane 32 away.  P^T then is the B operand of O^T = V^T P^T.
+//
+// 2 x 4096 causal queries of 16 heads (2 key heads) of 128 columns, bf16: 190 us, 720 TFLOP/s; matrix and vector instructions (32 exponentials
+// and some 150 others beside 32 products per wave and tile) together fill the time.  One query, 4093 keys, 8 x 8 heads on 2 key
+// heads: 9.9 us for 33.5 MB and 3.9 us to join 64 ranges of keys.  9 x 333 queries, 391 padded keys, 8 heads of 64, fp32: 30 us.
 #include "attn_seq.h"
 
 #include <type_traits>

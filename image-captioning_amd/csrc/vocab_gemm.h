@@ -6,6 +6,7 @@
 // reads (fp32).  So logits (x w^T), dx (d w) and dw (d^T x) run on the same tiles without a transposed copy of anything.
 // The result tile holds a lane per q and eight-row groups of p in registers: a row of the output (a token's logits) belongs to
 // two lanes, whose statistics need one exchange.
+// 24 x 512 x 32000, bf16: 10.5 us, 33 MB of w read once at 3.1 TB/s.  1111 x 300 x 10007, fp32: 81 us, 82 TFLOP/s; 4096 x 1024 x 32000: 122.
 #pragma once
 #include "attn_seq.h"
 

@@ -503,13 +503,14 @@ int mic_sample_update(const float* val, const int32_t* idx, int32_t* tokens, int
 /* out[n, :] = scale * table[ids[n], :] + pos[n mod T, :], rounded once to out_dtype (SeqEmbedding.forward over a whole caption,
  * models/transformer.py:44-50; nn.Embedding at models/basic.py:43, models/intermediate.py:59).  ids: ids_bits 32 or 64; ids
  * outside [0, vocab) read the nearest row of the table, as in mic_embed_pos.  table [vocab][ld_table], pos [T][ld_pos] or NULL,
- * both table_dtype; out [n][H] out_dtype.  n < 2^31. */
+ * both table_dtype; out [n][H] out_dtype.  n < 2^31, H <= 2^20. */
 int mic_embed_rows(const void* ids, int ids_bits, const void* table, int64_t ld_table, const void* pos, int64_t ld_pos, void* out,
                    int table_dtype, int out_dtype, float scale, int64_t n, int T, int H, int vocab, void* stream);
 
 /* Gradient of mic_embed_rows: d_table [vocab][H] = scale * the sum of g's rows [n][H] per word (zero rows for words that do not
  * occur), and d_pos [T][H] = the sum over sequences (NULL = not wanted; n must then be a multiple of T).  g is g_dtype, both
- * outputs out_dtype.  The tokens are sorted by word, so no row is summed by atomics.  n < 2^30; n = 0 clears the outputs.
+ * outputs out_dtype.  The tokens are sorted by word, so no row is summed by atomics.  n < 2^30, T * H < 2^31 with d_pos; n = 0
+ * clears the outputs.
  * mic_embed_grad_workspace_bytes returns MIC_ERR_ARG for sizes the gradient would refuse. */
 int64_t mic_embed_grad_workspace_bytes(int64_t n, int T, int H, int vocab, int want_pos);
 int mic_embed_grad(const void* ids, int ids_bits, const void* g, void* d_table, void* d_pos, int g_dtype, int out_dtype, float scale,
@@ -528,7 +529,8 @@ int mic_embed_grad(const void* ids, int ids_bits, const void* g, void* d_table, 
  * a head consecutive; pointers and strides multiples of 16 bytes, 64 positions and the heads of one position within 1 GiB.  lse fp32 [B][Hq][Tq]; key_mask bytes [B][mask_stride].  The
  * gradients dq [B][Tq][Hq][D], dk, dv [B][Tk][Hkv][D] are written whole and contiguous.  D <= 256, D * element size a multiple of 16 bytes.
  * bf16: scores, statistics and sums in fp32; probabilities and their gradients are rounded to bf16 for the second products only.
- * Sizes of zero are allowed.  mic_attn_seq_workspace_bytes(d, grad) looks at dtype, sizes and causal alone (an argument error is negative). */
+ * Sizes of zero are allowed; Hq <= 32768, Tq * Hq / Hkv < 2^30, and at most 2^29 rows (or keys) over all heads and batches in tiles of 128.
+ * mic_attn_seq_workspace_bytes(d, grad) looks at dtype, sizes and causal alone (an argument error is negative). */
 typedef struct mic_attn_seq_desc {
     const void *q, *k, *v;
     void* o;              /* written by mic_attn_seq, read by mic_attn_seq_grad */
@@ -551,11 +553,13 @@ int mic_attn_seq_grad(const mic_attn_seq_desc* d, void* stream);
  * train.py:318-354; with row weights the reward-weighted loss of train.py:209-262):
  *     z = x w^T + bias,   lse[n] = log sum_v exp z[n, v],   loss[n] = lse[n] - z[n, targets[n]]
  * and, for row weights a = grad_rows, d = a[n] (exp(z - lse) - onehot(target)):   dx = d w,  dw = d^T x,  db = column sums of d.
- * A row whose target is one of the `ignore` words or outside [0, V) has loss 0 and no gradient; its lse is computed all the same.
+ * A row whose target is one of the `ignore` words or outside [0, V) has loss 0 and no gradient, whatever x and grad_rows hold there; its
+ * lse is computed all the same.
  * x [N][ld_x], w [V][ld_w] of dtype, bias fp32 [V] or NULL, targets int32 / int64; loss, lse, grad_rows fp32 [N]; dx [N][H] and
  * dw [V][H] of dtype, db fp32 [V] or NULL (not wanted), written whole.  A bias may hide words with -infinity.  The gradient takes
  * x, w, targets, bias and ignore as the loss did, and its lse; it computes the logits again, a piece of the vocabulary at a time
- * (a piece of d takes up to 256 MiB of the workspace).  bf16: products and sums in fp32, d rounded to bf16 for the products with w and x,
+ * (a piece of d takes up to 256 MiB of the workspace, more where the partial sums of dx, N * H * 4 bytes a piece, would outgrow it).  At
+ * most 2^25 rows, 2^37 logits, 2^33 elements of x or w.  bf16: products and sums in fp32, d rounded to bf16 for the products with w and x,
  * db summed before that.  H of any size; x and w whose rows are not whole 16 bytes on 16-byte boundaries are copied into
  * the workspace first.  mic_vocab_loss_workspace_bytes(d, grad) looks at dtype, sizes, strides and the alignment of x, w and
  * whether db is NULL (an argument error is negative). */
