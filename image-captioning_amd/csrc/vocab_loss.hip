@@ -596,14 +596,15 @@ Plan make_plan(const mic_vocab_loss_desc* d, bool grad) {
     p.e = 16 / (int)es;
     p.Hp = (int)((H + p.e - 1) / p.e * p.e);
     p.pad = p.Hp != H || d->ld_x % p.e || d->ld_w % p.e || (((uintptr_t)d->x | (uintptr_t)d->w) & 15);
-    // The large tiles from half a tile per compute unit on.  V = 3500, H = 512, forward and gradient: 2,400 rows (140 large tiles) 120 us
-    // on large tiles and 145 us on small ones, 1,200 rows (70) 106 and 92 us.  They address 256 rows (64 of k) with 31 bits.
-    p.big = d->dtype == MIC_BF16 && (long long)edge_tiles(N, 256) * edge_tiles(V, 256) >= 128 && H >= 64 && H < (1 << 21) && d->ld_x < (1 << 21) && d->ld_w < (1 << 21);
+    // The large tiles from 128 rows and as many logits as 96 full tiles on.  V = 3500, H = 512, all rows counted, forward and gradient: 2,400
+    // rows 97 us on large tiles and 121 us on small ones, 1,800 rows 92 and 99, 1,200 rows 88 and 80; 100 rows, H = 1024, V = 70000: 273 and
+    // 217.  They address 256 rows (64 of k) with 31 bits.
+    p.big = d->dtype == MIC_BF16 && N >= 128 && N * V >= 96ll << 16 && H >= 64 && H < (1 << 21) && d->ld_x < (1 << 21) && d->ld_w < (1 << 21);
     // 64 x 64 tiles where 128 x 128 ones would leave compute units idle, half of each tile (H = 64: 20,000 x 3500 forward and gradient 533
     // us, on the larger 746), and in fp32 also the last round of them: a small tile costs 8 % more there (4096 x 512 x 16384: 2663 and
     // 2443 us), 1111 x 300 x 10007 is 1.4 rounds of large tiles and 2.8 of small ones (266 and 302 us)
     const long long large = (long long)edge_tiles(N, 128) * edge_tiles(V, 128), small = (long long)edge_tiles(N, 64) * edge_tiles(V, 64);
-    p.edge = p.big ? 256 : large < 512 || H <= 64 || (d->dtype == MIC_F32 && 1.08 * filled(large, 512) < filled(small, 1024)) ? 64 : 128;
+    p.edge = p.big ? 256 : large < 512 || H <= 64 || N <= 64 || (d->dtype == MIC_F32 && 1.08 * filled(large, 512) < filled(small, 1024)) ? 64 : 128;
     p.copy_x = p.pad || grad;
     long long o = 0;
     p.xpad = o;

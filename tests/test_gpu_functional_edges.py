@@ -191,3 +191,10 @@ def test_gradients_of_the_differentiable_calls_in_a_graph(F):  # noqa: F811
         torch.cuda.synchronize()
         for a, b in zip(out, eager):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("N,H,V,bias", [(130, 100, 50021, True), (2100, 136, 3119, False), (257, 70, 26001, True), (60, 96, 9001, True), (127, 64, 52000, False)])
+def test_vocab_loss_around_the_large_tiles(F, poisoned, N, H, V, bias):  # noqa: F811
+    """bf16 on both sides of the rule for the large tiles, edges of every kind."""
+    x, w, b, t, a = vocab_inputs(N, H, V, BF16, bias, seed=67)
+    vocab_check(vocab_run(F, *on(x, w, b, t, a), (0,)), vocab_ref(x, w, b, t, a, (0,), BF16))
