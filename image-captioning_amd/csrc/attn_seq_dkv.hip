@@ -14,7 +14,7 @@ namespace {
 
 template <typename T, int DP, bool SPLIT> __global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void attn_seq_dkv_kernel(AttnSeqArgs a) {
     constexpr int NC = DP / 16, ND = DP / 32, ES = sizeof(T);
-    constexpr bool KEEP = InRegs<T, DP>::value;  // else k and v are read from memory for every tile
+    constexpr bool KEEP = InRegs<T, DP>::value;  // else v is read from memory for every tile
     constexpr int TILE = 32 * DP * ES, OFF_Q = 0, OFF_G = 2 * TILE, OFF_V = 4 * TILE;  // two tiles of q, two of g, the four waves' v
     __shared__ __attribute__((aligned(16))) unsigned char smem[4 * TILE + (KEEP ? 4 * TILE : 0)];
     __shared__ __attribute__((aligned(16))) float s_lse[2][32], s_delta[2][32];
@@ -33,10 +33,10 @@ template <typename T, int DP, bool SPLIT> __global__ __launch_bounds__(256, (DP 
     const T* vrow = seen ? (const T*)a.v + b * a.v_sb + hk * a.v_sh + (long long)key * a.v_st : nullptr;
     TileReader<T, DP> read;
     read.init(lane);
-    Frag8<T> kf[KEEP ? NC : 1];
-    if constexpr (KEEP) {
+    Frag8<T> kf[NC];
 #pragma unroll
-        for (int c = 0; c < NC; ++c) kf[c] = load_frag<T>(krow, 16 * c + 8 * h, a.D);
+    for (int c = 0; c < NC; ++c) kf[c] = load_frag<T>(krow, 16 * c + 8 * h, a.D);
+    if constexpr (KEEP) {
         T* sv = reinterpret_cast<T*>(smem + OFF_V) + wave * 32 * DP;  // rows hidden keys would have are zeros
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
@@ -133,7 +133,7 @@ template <typename T, int DP, bool SPLIT> __global__ __launch_bounds__(256, (DP 
                     mma32(q, kf[c], s);
                     mma32(g, read.rows(lds + wave * TILE, OFF_V, c), dp);
                 } else {
-                    mma32(q, load_frag<T>(krow, 16 * c + 8 * h, a.D), s);
+                    mma32(q, kf[c], s);
                     mma32(g, load_frag<T>(vrow, 16 * c + 8 * h, a.D), dp);
                 }
             }

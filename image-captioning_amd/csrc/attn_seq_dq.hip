@@ -10,7 +10,7 @@
 namespace {
 
 template <typename T, int DP, int BK, bool SPLIT> __global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void attn_seq_dq_kernel(AttnSeqArgs a) {
-    constexpr int NC = DP / 16, ND = DP / 32, KT = BK / 32, NR = InRegs<T, DP>::value ? NC : 1, ES = sizeof(T);
+    constexpr int NC = DP / 16, ND = DP / 32, KT = BK / 32, ES = sizeof(T);
     constexpr bool GLDS = sizeof(T) == 2 && DP == 256;
     constexpr int TILE = BK * DP * ES, OFF_K = 0, OFF_V = 2 * TILE, OFF_G = 4 * TILE;  // two tiles of k, two of v, the waves' g
     __shared__ __attribute__((aligned(16))) unsigned char smem[4 * TILE + (GLDS ? 4 * 32 * DP * ES : 0)];
@@ -27,7 +27,7 @@ template <typename T, int DP, int BK, bool SPLIT> __global__ __launch_bounds__(2
     const T* qrow = row_ok ? (const T*)a.q + b * a.q_sb + qi * a.q_st + qh * a.q_sh : nullptr;
     const T* grow = row_ok ? (const T*)a.g + b * a.g_sb + qi * a.g_st + qh * a.g_sh : nullptr;
     const T* orow = row_ok ? (const T*)a.o + b * a.o_sb + qi * a.o_st + qh * a.o_sh : nullptr;
-    Frag8<T> qf[NR], gf[GLDS ? 1 : NR];
+    Frag8<T> qf[NC], gf[GLDS || !InRegs<T, DP>::value ? 1 : NC];
     TileReader<T, DP> read;
     read.init(lane);
     float delta = 0.f;
@@ -36,10 +36,10 @@ template <typename T, int DP, int BK, bool SPLIT> __global__ __launch_bounds__(2
         const Frag8<T> g = load_frag<T>(grow, 16 * c + 8 * h, a.D), o = load_frag<T>(orow, 16 * c + 8 * h, a.D);
 #pragma unroll
         for (int e = 0; e < 8; ++e) delta = fmaf((float)g.v[e], (float)o.v[e], delta);
+        qf[c] = load_frag<T>(qrow, 16 * c + 8 * h, a.D);
         if constexpr (InRegs<T, DP>::value) {
             if constexpr (GLDS) *reinterpret_cast<uint4*>(smem + OFF_G + (wave * 32 * DP + Tile<T, DP>::at(lane & 31, 2 * c + h)) * ES) = __builtin_bit_cast(uint4, g);
             else gf[c] = g;
-            qf[c] = load_frag<T>(qrow, 16 * c + 8 * h, a.D);
         }
     }
     delta += __shfl_xor(delta, 32, 64);
@@ -120,7 +120,7 @@ template <typename T, int DP, int BK, bool SPLIT> __global__ __launch_bounds__(2
                     mma32(k, qf[c], s);
                     mma32(v, gf[c], dp);
                 } else {
-                    mma32(k, load_frag<T>(qrow, 16 * c + 8 * h, a.D), s);
+                    mma32(k, qf[c], s);
                     mma32(v, load_frag<T>(grow, 16 * c + 8 * h, a.D), dp);
                 }
             }

@@ -8,14 +8,16 @@
 // 2 x 4096 causal queries of 16 heads (2 key heads) of 128 columns, bf16: 190 us, 720 TFLOP/s; matrix and vector instructions (32 exponentials
 // and some 150 others beside 32 products per wave and tile) together fill the time.  One query, 4093 keys, 8 x 8 heads on 2 key
 // heads: 9.9 us for 33.5 MB and 3.9 us to join 64 ranges of keys.  9 x 333 queries, 391 padded keys, 8 heads of 64, fp32: 30 us.
+// 256 columns take one wave per SIMD: with 256 registers a lane bf16 spills (4 x 1024 causal queries, 8 heads: 132 us, with 512 77 us); fp32 with
+// 128 columns is faster with two (148 and 161 us).
 #include "attn_seq.h"
 
 #include <type_traits>
 
 namespace {
 
-template <typename T, int DP, int BK, bool SPLIT> __global__ __launch_bounds__(256, (DP * sizeof(T) <= 512 ? 2 : 1)) void attn_seq_fwd_kernel(AttnSeqArgs a) {
-    constexpr int NC = DP / 16, ND = DP / 32, KT = BK / 32, NR = InRegs<T, DP>::value ? NC : 1, ES = sizeof(T);
+template <typename T, int DP, int BK, bool SPLIT> __global__ __launch_bounds__(256, (DP <= 128 ? 2 : 1)) void attn_seq_fwd_kernel(AttnSeqArgs a) {
+    constexpr int NC = DP / 16, ND = DP / 32, KT = BK / 32, ES = sizeof(T);
     constexpr int TILE = BK * DP * ES, OFF_K = 0, OFF_V = 2 * TILE;  // two tiles of k, two of v
     __shared__ __attribute__((aligned(16))) unsigned char smem[4 * TILE];
     const lds_bytes_t lds = (lds_bytes_t)smem;
@@ -30,9 +32,9 @@ template <typename T, int DP, int BK, bool SPLIT> __global__ __launch_bounds__(2
     const bool row_ok = r < a.R;
     const int qi = row_ok ? r / a.group : 0, qh = hk * a.group + (row_ok ? r - qi * a.group : 0);
     const T* qrow = row_ok ? (const T*)a.q + b * a.q_sb + qi * a.q_st + qh * a.q_sh : nullptr;
-    Frag8<T> qf[NR];
+    Frag8<T> qf[NC];
 #pragma unroll
-    for (int c = 0; c < NR; ++c) qf[c] = load_frag<T>(qrow, 16 * c + 8 * h, a.D);
+    for (int c = 0; c < NC; ++c) qf[c] = load_frag<T>(qrow, 16 * c + 8 * h, a.D);
 
     const int last = min(rt * ATTN_SEQ_BLOCK + ATTN_SEQ_BLOCK, a.R) - 1;
     const int k_end = a.causal ? min(a.Tk, last / a.group + a.off + 1) : a.Tk;  // keys any row of the workgroup may see
@@ -102,7 +104,7 @@ template <typename T, int DP, int BK, bool SPLIT> __global__ __launch_bounds__(2
             for (int c = 0; c < NC; ++c)
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt)
-                    mma32(read.rows(lds, OFF_K + CUR * TILE + kt * 32 * DP * ES, c), InRegs<T, DP>::value ? qf[c % NR] : load_frag<T>(qrow, 16 * c + 8 * h, a.D), s[kt]);
+                    mma32(read.rows(lds, OFF_K + CUR * TILE + kt * 32 * DP * ES, c), qf[c], s[kt]);
             if constexpr (sizeof(T) == 2) reads_ahead<KT, KT, NC>();
             __builtin_amdgcn_s_setprio(0);
 #pragma unroll
