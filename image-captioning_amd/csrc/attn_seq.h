@@ -274,7 +274,7 @@ template <typename T, int DP, int ROWS, typename F> __device__ __forceinline__ v
     }
 }
 
-// The same with offsets that were computed before (tile_offsets), for tiles whose rows lie alike
+// The same with a lane's offsets computed once, for tiles whose rows lie alike
 template <typename T, int DP, int ROWS> struct TileOffsets {
     static constexpr int PIECES = ROWS * DP * (int)sizeof(T) / 1024, PER = (PIECES + 3) / 4;
     unsigned off[PER];

@@ -470,7 +470,7 @@ struct FirstArgs {
     void *d_table, *d_pos;
     float* pos_part;
     long long W;
-    int H, B, slices, rank_blocks, zero_blocks;
+    int H, B, slices, rank_blocks, zero_blocks, sum_blocks;
     long long groups;
 };
 constexpr int SUM_COLUMNS = 16 * VEC;
@@ -530,8 +530,10 @@ template <typename TG, typename TO, bool A> __global__ __launch_bounds__(1024, 8
         }
         return;
     }
-    block -= f.zero_blocks;
-    colsum<TG, TO, 16, VEC, A>(reinterpret_cast<float*>(lds), (const TG*)f.g, (TO*)f.d_pos, f.pos_part, f.B, f.W, f.slices, block % f.groups, (int)(block / f.groups));
+    for (long long i = block - f.zero_blocks; i < f.groups * f.slices; i += f.sum_blocks) {
+        colsum<TG, TO, 16, VEC, A>(reinterpret_cast<float*>(lds), (const TG*)f.g, (TO*)f.d_pos, f.pos_part, f.B, f.W, f.slices, i % f.groups, (int)(i / f.groups));
+        __syncthreads();
+    }
 }
 
 // ---- the gradient's plan: everything that depends on the sizes alone -------------------------------------------------------
@@ -584,7 +586,7 @@ GradPlan grad_plan(long long n, int T, int H, int vocab, bool want_pos) {
     return p;
 }
 
-// columns of a row, and elements of d_pos (a launch has fewer than 2^32 threads)
+// columns of a row, and elements of d_pos
 constexpr int MAX_H = 1 << 20;
 constexpr long long MAX_POS = 1ll << 31;
 
@@ -612,8 +614,10 @@ int launch_grad(const GradPlan& p, const void* ids, int wide, const void* g, voi
         f.W = (long long)T * H;
         f.slices = p.slices;
         f.groups = (f.W + SUM_COLUMNS - 1) / SUM_COLUMNS;
+        const long long sums = f.groups * f.slices;
+        f.sum_blocks = (int)(sums < 1 << 20 ? sums : 1 << 20);  // a launch has fewer than 2^32 threads
     }
-    const long long first = f.rank_blocks + f.zero_blocks + f.groups * f.slices;
+    const long long first = f.rank_blocks + f.zero_blocks + f.sum_blocks;
     if (first > 0) MIC_LAUNCH((embed_first_kernel<TG, TO, A>), dim3((unsigned)first), dim3(1024), 0, s, f);
     if (d_pos && p.slices > 1)
         MIC_LAUNCH((embed_colsum_join_kernel<TO>), dim3((unsigned)((f.W + 63) / 64)), dim3(1024), 0, s, (const float*)f.pos_part, (TO*)d_pos, p.slices, f.W);

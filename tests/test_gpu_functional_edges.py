@@ -198,3 +198,12 @@ def test_vocab_loss_around_the_large_tiles(F, poisoned, N, H, V, bias):  # noqa:
     """bf16 on both sides of the rule for the large tiles, edges of every kind."""
     x, w, b, t, a = vocab_inputs(N, H, V, BF16, bias, seed=67)
     vocab_check(vocab_run(F, *on(x, w, b, t, a), (0,)), vocab_ref(x, w, b, t, a, (0,), BF16))
+
+
+def test_embedding_positions_of_a_very_long_sequence(F):  # noqa: F811
+    """More columns to sum over sequences than one launch has workgroups for: each takes several.  One sequence: the sum is the gradient."""
+    T, H = 1 << 17, 1032
+    g = torch.randn(1, T, H, device=DEV, dtype=BF16)
+    ids = torch.randint(0, 5, (1, T), device=DEV)
+    _, dp = F.embedding_grad(g, ids, 5, positions=T)
+    assert torch.equal(dp, g[0])
