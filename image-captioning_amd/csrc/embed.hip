@@ -56,7 +56,7 @@ template <typename T, bool A> __device__ __forceinline__ void load8_before(const
 }
 // OUT: a result, which is written once, goes past the caches where a lane's eight columns are one access (bf16), so that the rows read again
 // stay in them: 126,821 tokens of 1,024 columns, the table's gradient 102 -> 84 us, lookups repeated on one table 91 -> 55 us.  Eight floats
-// are two accesses 32 bytes apart, and clearing 100,000 rows of 512 took 93 instead of 40 us that way.
+// are two accesses 32 bytes apart, which took twice the time that way.
 template <typename T, bool A, bool OUT> __device__ __forceinline__ void store8(T* p, int n, const float (&v)[VEC]) {
     if constexpr (A && OUT && sizeof(T) == 2) {
         typedef unsigned words_t __attribute__((ext_vector_type(4)));
@@ -82,6 +82,20 @@ template <typename T, bool A, bool OUT> __device__ __forceinline__ void store8(T
         for (int e = 0; e < VEC; ++e)
             if (e < n) p[e] = from_f32<T>(v[e]);
     }
+}
+
+// A wave clears a row that may begin anywhere: whole 16-byte pieces, one to a lane, whatever the row's alignment.  The gradient of 420 tokens
+// for 26,692 rows of 977 floats 31 us, of 100,000 rows of 512 40 us (5.1 TB/s); by eight columns to a lane 54 and 49 us, past the
+// caches 37 and 48.
+template <typename T> __device__ __forceinline__ void clear_row(T* row, int n, int lane) {
+    constexpr int E = Vec16<T>::N;
+    typedef unsigned words_t __attribute__((ext_vector_type(4)));
+    const int head = min(n, (int)((16 - ((uintptr_t)row & 15)) & 15) / (int)sizeof(T)), body = (n - head) / E * E;
+    if (lane < head) row[lane] = (T)0.f;
+    for (int c = lane * E; c < body; c += 64 * E) {
+        *reinterpret_cast<words_t*>(row + head + c) = words_t{0, 0, 0, 0};
+    }
+    if (head + body + lane < n) row[head + body + lane] = (T)0.f;
 }
 
 // ---- lookup: one thread per eight columns of a row ---------------------------------------------------------------------------
@@ -258,11 +272,10 @@ template <typename TG, typename TO, bool A> __global__ __launch_bounds__(256) vo
             absent = p >= (int)a.n || a.key[p] != v;
         }
         unsigned long long todo = __ballot(absent);
-        const float zero[VEC] = {};
         while (todo) {
             const int r = __ffsll((unsigned long long)todo) - 1;
             todo &= todo - 1;
-            for (int c = lane * VEC; c < a.H; c += 64 * VEC) store8<TO, A, true>(dt + (v0 + r) * a.H + c, a.H - c, zero);
+            clear_row(dt + (v0 + r) * a.H, a.H, lane);
         }
         return;
     }
@@ -523,11 +536,8 @@ template <typename TG, typename TO, bool A> __global__ __launch_bounds__(1024, 8
             if (v >= 0 && v < ZERO_ROWS) lds[v] = 1;
         }
         __syncthreads();
-        const float zero[VEC] = {};
-        for (int r = wave; r < ZERO_ROWS && v0 + r < a.vocab; r += 16) {
-            if (lds[r]) continue;
-            for (int c = lane * VEC; c < f.H; c += 64 * VEC) store8<TO, A, true>((TO*)f.d_table + (long long)(v0 + r) * f.H + c, f.H - c, zero);
-        }
+        for (int r = wave; r < ZERO_ROWS && v0 + r < a.vocab; r += 16)
+            if (!lds[r]) clear_row((TO*)f.d_table + (long long)(v0 + r) * f.H, f.H, lane);
         return;
     }
     for (long long i = block - f.zero_blocks; i < f.groups * f.slices; i += f.sum_blocks) {
