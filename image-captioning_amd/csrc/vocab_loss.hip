@@ -455,22 +455,25 @@ struct SplitRule {
 struct Split {
     int tiles, nk, most;    // tiles of the result (dx: per tile of rows), steps of k (dw: 0, by the rows), ranges allowed
 };
-// The pair of numbers that costs least, up to 16 each: a lane looks at one number for x and four for w.  Both products are one launch, whose
+// 1 to 10, 12, 16, 24, 32, 48, 64 ranges (i < 16)
+constexpr int MAX_SLICES = 64;
+__device__ __forceinline__ int slices_at(int i) { return i < 10 ? i + 1 : (i & 1 ? 16 : 12) << ((i - 10) >> 1); }
+// The pair of numbers that costs least: a lane looks at one number for x and four for w.  Both products are one launch, whose
 // tiles are dealt out in turn: the first workgroups have one tile of x more, or the ones behind them one of w.
 __device__ __forceinline__ int2 choose_slices(const SplitRule& r, int tiles_x, int nk_x, int most_x, int tiles_w, int nk_w, int most_w, int lane) {
-    const int sx = (lane & 15) + 1;
+    const int sx = slices_at(lane & 15);
     const float all_x = (float)(tiles_x * sx) / r.capacity, some = floorf(all_x), up = ceilf(all_x), kx = ceilf((float)nk_x / sx) + r.fixed;
     float best = INFINITY;
     int at = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int sw = (lane >> 4) * 4 + i + 1;
+        const int sw = slices_at((lane >> 4) * 4 + i);
         const float all_w = (float)(tiles_w * sw) / r.capacity, rounds = ceilf(all_x + all_w), kw = ceilf((float)nk_w / sw) + r.fixed;
         float cost = fmaxf(up * kx + (rounds - up) * kw, some * kx + (rounds - some) * kw) + (all_x + (sw > 1 ? all_w : 0.f)) * r.traffic;
         if (sx > most_x || sw > most_w) cost = INFINITY;
         if (cost < best) {
             best = cost;
-            at = sw * 32 + sx;
+            at = sw * 128 + sx;
         }
     }
 #pragma unroll
@@ -482,7 +485,7 @@ __device__ __forceinline__ int2 choose_slices(const SplitRule& r, int tiles_x, i
             at = o;
         }
     }
-    return make_int2(at & 31, at >> 5);
+    return make_int2(at & 127, at >> 7);
 }
 enum { COUNT, SX, SX_LAST, SW, SW_LAST, DECISIONS };  // what `count` points to
 struct RowsArgs {
@@ -583,7 +586,7 @@ struct Plan {
 // The most ranges k may be cut into: every one keeps four steps of k.  How many are used is decided when the rows are known.
 int most_slices(long long K, int ks) {
     const long long s = (K + ks - 1) / ks / 4;
-    return (int)(s < 1 ? 1 : s > 16 ? 16 : s);
+    return (int)(s < 1 ? 1 : s > MAX_SLICES ? MAX_SLICES : s);
 }
 
 // Rows kernel: the gathered targets, lse, weights, places and the count
