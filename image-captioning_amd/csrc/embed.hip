@@ -558,7 +558,7 @@ long long up256(long long b) { return (b + 255) / 256 * 256; }
 
 GradPlan grad_plan(long long n, int T, int H, int vocab, bool want_pos) {
     GradPlan p = {};
-    p.rank = n <= RANK_MAX && vocab <= RANK_MAX_VOCAB;
+    p.rank = n > 0 && n <= RANK_MAX && vocab <= RANK_MAX_VOCAB;
     int blocks = (int)((n + SORT_THREADS - 1) / SORT_THREADS);
     blocks = blocks < 1 ? 1 : blocks > MAX_SORT_BLOCKS ? MAX_SORT_BLOCKS : blocks;
     p.per_block = (int)(((n + blocks - 1) / blocks + SORT_THREADS - 1) / SORT_THREADS * SORT_THREADS);
@@ -632,7 +632,7 @@ int launch_grad(const GradPlan& p, const void* ids, int wide, const void* g, voi
     if (d_pos && p.slices > 1)
         MIC_LAUNCH((embed_colsum_join_kernel<TO>), dim3((unsigned)((f.W + 63) / 64)), dim3(1024), 0, s, (const float*)f.pos_part, (TO*)d_pos, p.slices, f.W);
     const int passes = p.rank ? 1 : p.passes;
-    for (int i = 0; i < passes && !p.rank; ++i) {
+    for (int i = 0; i < passes && !p.rank && n > 0; ++i) {
         a.ids = i == 0 ? ids : nullptr;
         a.key_in = (const int*)(ws + p.key[(i + 1) & 1]);
         a.idx_in = (const int*)(ws + p.idx[(i + 1) & 1]);
@@ -642,8 +642,7 @@ int launch_grad(const GradPlan& p, const void* ids, int wide, const void* g, voi
         MIC_LAUNCH(embed_hist_kernel, dim3(p.sort_blocks), dim3(SORT_THREADS), 0, s, a);
         MIC_LAUNCH(embed_scatter_kernel, dim3(p.sort_blocks), dim3(SORT_THREADS), 0, s, a);
     }
-    if (n == 0) return 0;
-    SumArgs m = {};
+    SumArgs m = {};  // (no tokens: no chunks, and every row is one of a word that does not occur)
     m.key = (const int*)(ws + p.key[(passes - 1) & 1]);
     m.idx = (const int*)(ws + p.idx[(passes - 1) & 1]);
     m.g = g; m.d_table = d_table;

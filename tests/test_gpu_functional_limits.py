@@ -1,0 +1,36 @@
+"""The teacher-forced operators at the limits of what their documentation allows: nothing to do, the largest sizes, values of the
+type's lowest, rows that take part in nothing.  Bounds and references are those of test_gpu_functional.py."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_functional import BF16, DEV, F, F32, U, attn_check, attn_inputs, attn_ref, attn_run, gen, on, vocab_inputs, vocab_ref, vocab_run, within  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def nan(*shape, dtype=F32):
+    return torch.full(shape, math.nan, dtype=dtype, device=DEV)
+
+
+@pytest.mark.parametrize("V", [9, 1 << 18, (1 << 18) + 1, 1_000_003])
+@pytest.mark.parametrize("positions", [0, 5])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_embedding_gradient_of_no_tokens_is_written(F, V, positions, dtype):  # noqa: F811
+    """The entry point itself, on results full of NaN: no sequence of `positions` tokens, a vocabulary on both sides of the border of the
+    two sorts."""
+    import image_captioning_amd as m
+    L, H = m._lib, 12
+    code = L.F32 if dtype == F32 else L.BF16
+    d, p = nan(V, H, dtype=dtype), nan(max(positions, 1), H, dtype=dtype)
+    T = max(positions, 1)
+    size = L.lib.mic_embed_grad_workspace_bytes(0, T, H, V, 1 if positions else 0)
+    ws = torch.empty(max(size, 16), dtype=torch.uint8, device=DEV)
+    L.check(L.lib.mic_embed_grad(None, 64, None, d.data_ptr(), p.data_ptr() if positions else None, code, code, 1.0, 0, T, H, V, ws.data_ptr(), size,
+                                 torch.cuda.current_stream().cuda_stream), "mic_embed_grad")
+    assert not d.isnan().any() and not d.any()
+    assert not positions or (not p.isnan().any() and not p.any())
+    none = torch.zeros(0, T, dtype=torch.long, device=DEV)
+    for r in F.embedding_grad(torch.zeros(0, T, H, device=DEV, dtype=dtype), none, V, positions=positions):
+        assert r is None or not r.any()
