@@ -649,7 +649,7 @@ int launch_grad(const GradPlan& p, const void* ids, int wide, const void* g, voi
     m.head = (float*)(ws + p.head); m.tail = (float*)(ws + p.tail);
     m.n = n; m.H = H; m.Hs = (H + VEC - 1) / VEC * VEC; m.vocab = vocab; m.chunk = p.chunk; m.chunks = p.chunks; m.scale = scale; m.cleared = p.rank;
     m.slabs = (H + 64 * VEC - 1) / (64 * VEC);
-    const long long units = (long long)p.chunks * m.slabs + (p.rank ? 0 : (vocab + 63) / 64);
+    const long long units = (long long)p.chunks * m.slabs + (p.rank ? 0 : ((long long)vocab + 63) / 64);
     MIC_LAUNCH((embed_sum_kernel<TG, TO, A>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, s, m);
     if (p.chunks > 1) {
         const int long_blocks = (p.chunks - 1) / JOIN_LONG * ((H + 63) / 64);

@@ -34,3 +34,18 @@ def test_embedding_gradient_of_no_tokens_is_written(F, V, positions, dtype):  # 
     none = torch.zeros(0, T, dtype=torch.long, device=DEV)
     for r in F.embedding_grad(torch.zeros(0, T, H, device=DEV, dtype=dtype), none, V, positions=positions):
         assert r is None or not r.any()
+
+
+def test_embedding_with_the_most_words_there_can_be(F):  # noqa: F811
+    """2^31 - 1 rows of one column: the last word and the first, and no token at all."""
+    V = (1 << 31) - 1
+    ids = torch.tensor([[V - 1, 0, 5, V - 1, 1 << 40]], device=DEV)
+    g = torch.tensor([1.0, 2, 4, 8, 16], device=DEV).view(1, 5, 1).to(BF16)
+    d, _ = F.embedding_grad(g, ids, V)
+    assert int(torch.count_nonzero(d)) == 3
+    assert [float(d[i, 0]) for i in (V - 1, 0, 5)] == [25.0, 2.0, 4.0]  # a word outside is the nearest one
+    assert F.embedding_forward(ids, d).flatten().tolist() == [25.0, 2.0, 4.0, 25.0, 25.0]
+    d.fill_(math.nan)
+    del d
+    d, _ = F.embedding_grad(g[:, :0], ids[:, :0], V)
+    assert not torch.count_nonzero(d)
