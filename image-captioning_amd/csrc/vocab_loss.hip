@@ -607,7 +607,9 @@ Plan make_plan(const mic_vocab_loss_desc* d, bool grad) {
     // us, on the larger 746), and in fp32 also the last round of them: a small tile costs 8 % more there (4096 x 512 x 16384: 2663 and
     // 2443 us), 1111 x 300 x 10007 is 1.4 rounds of large tiles and 2.8 of small ones (266 and 302 us)
     const long long large = (long long)edge_tiles(N, 128) * edge_tiles(V, 128), small = (long long)edge_tiles(N, 64) * edge_tiles(V, 64);
-    p.edge = p.big ? 256 : large < 512 || H <= 64 || N <= 64 || (d->dtype == MIC_F32 && 1.08 * filled(large, 512) < filled(small, 1024)) ? 64 : 128;
+    // (from 2^24 of the small ones on the larger alone: a tile is a workgroup of 256 threads, and a launch has fewer than 2^32)
+    const bool fine = small < 1 << 24 && (large < 512 || H <= 64 || N <= 64 || (d->dtype == MIC_F32 && 1.08 * filled(large, 512) < filled(small, 1024)));
+    p.edge = p.big ? 256 : fine ? 64 : 128;
     p.copy_x = p.pad || grad;
     long long o = 0;
     p.xpad = o;
@@ -655,7 +657,7 @@ int check_desc(const char* who, const mic_vocab_loss_desc* d) {
     MIC_ARG_CHECK(d, "%s: null descriptor", who);
     MIC_ARG_CHECK(d->dtype == MIC_F32 || d->dtype == MIC_BF16, "%s: bad dtype %d", who, d->dtype);
     MIC_ARG_CHECK(d->N >= 0 && d->H > 0 && d->V > 0, "%s: bad sizes N=%d H=%d V=%d", who, d->N, d->H, d->V);
-    // launches and tile numbers have 32 bits: at most 2^37 logits, 2^33 elements of x or w
+    // tile numbers have 32 bits: at most 2^37 logits (2^23 tiles of 128 x 128), 2^33 elements of x or w
     const long long N = d->N / 64 + 2ll, H = d->H / 64 + 2ll, V = d->V / 64 + 2ll;
     MIC_ARG_CHECK(N <= 1 << 19 && H <= 1 << 21 && V <= 1 << 21 && N * V < 1 << 25 && N * H < 1 << 21 && V * H < 1 << 21, "%s: sizes out of range N=%d H=%d V=%d", who, d->N,
                   d->H, d->V);

@@ -232,3 +232,18 @@ def test_sizes_beyond_a_launch_are_refused(L):
             assert L.lib.mic_vocab_loss_workspace_bytes(C.byref(v), grad) == -1 and b"sizes out of range" in L.lib.mic_last_error()
     v.N, v.H, v.V, v.ld_x, v.ld_w = 1 << 17, 1 << 10, 1 << 17, 1 << 10, 1 << 10
     assert L.lib.mic_vocab_loss_workspace_bytes(C.byref(v), 1) < 16 << 30  # d and the partial dx share a few GiB
+
+
+def test_vocab_loss_of_many_small_tiles_takes_larger_ones(L):
+    """2^36 logits on tiles of 64 x 64 would be a launch of 2^32 threads; a row's statistics are kept for every half tile of columns, so
+    the scratch tells the tile."""
+    import ctypes as C
+    v = L.VocabLossDesc()
+    v.V, v.target_bits = 4096, 32
+    for dtype, H in ((L.BF16, 8), (L.F32, 64)):
+        v.dtype, v.H, v.ld_x, v.ld_w = dtype, H, H, H
+        for N, half_tile in (((1 << 24) - 64, 32), (1 << 24, 64), ((1 << 24) + 5, 64)):
+            v.N = N
+            parts = v.V // half_tile
+            need = L.lib.mic_vocab_loss_workspace_bytes(C.byref(v), 0)
+            assert abs(need - N * (parts * 8 + 4)) <= 1024, (dtype, N, need)

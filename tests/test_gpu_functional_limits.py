@@ -49,3 +49,21 @@ def test_embedding_with_the_most_words_there_can_be(F):  # noqa: F811
     del d
     d, _ = F.embedding_grad(g[:, :0], ids[:, :0], V)
     assert not torch.count_nonzero(d)
+
+
+def test_vocab_loss_of_2_to_the_36_logits(F):  # noqa: F811
+    """Narrow rows, so many of them that tiles of 64 x 64 would be 2^32 threads: some rows' results against their definition."""
+    N, H, V = (1 << 24) + 3, 8, 4096
+    g = torch.Generator(device=DEV).manual_seed(85)
+    x = torch.randn(N, H, device=DEV, generator=g).to(BF16)
+    w = torch.randn(V, H, device=DEV, generator=g).to(BF16)
+    t = torch.randint(0, V, (N,), device=DEV, generator=g)
+    loss, lse = F.vocab_loss_forward(x, w, t, ignore=(0,))
+    rows = torch.cat([torch.tensor([0, 1, 63, 64, 127, 128, N - 4, N - 1]), torch.randint(0, N, (500,), generator=gen(86))])
+    xs, ts = x[rows.to(DEV)].cpu(), t[rows.to(DEV)].cpu()
+    a = torch.randn(N, device=DEV, generator=g)
+    ref = vocab_ref(xs, w.cpu(), None, ts, a[rows.to(DEV)].cpu(), (0,), BF16)
+    within(F.vocab_loss_grad(a, x, w, t, lse, ignore=(0,))[0][rows.to(DEV)], *ref["dx"], "dx")
+    within(loss[rows.to(DEV)], *ref["loss"], "loss")
+    within(lse[rows.to(DEV)], *ref["lse"], "lse")
+    assert torch.isfinite(lse).all() and (lse > 0).all()
