@@ -256,10 +256,17 @@ struct StatsEpi8 {
                     for (int e = 0; e < 4; ++e) z = tc == 16 * j + e ? acc[j][i][e] : z;
                 a.zt[q0 + ql + 16 * i] = z;
             }
+            if (fabsf(m[i]) < 1e38f || m[i] == -INFINITY) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+                for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[i] += __builtin_amdgcn_exp2f(fmaf(acc[j][i][e], ATTN_LOG2E, -m2));
+                    for (int e = 0; e < 4; ++e) s[i] += __builtin_amdgcn_exp2f(fmaf(acc[j][i][e], ATTN_LOG2E, -m2));
+            } else {  // all hidden by the type's lowest value: m2 would be infinite
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[i] += __builtin_amdgcn_exp2f((acc[j][i][e] - m[i]) * ATTN_LOG2E);
+            }
         }
 #pragma unroll
         for (int d = 16; d < 64; d <<= 1) {

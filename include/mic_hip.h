@@ -556,7 +556,7 @@ int mic_attn_seq_grad(const mic_attn_seq_desc* d, void* stream);
  * A row whose target is one of the `ignore` words or outside [0, V) has loss 0 and no gradient, whatever x and grad_rows hold there; its
  * lse is computed all the same.
  * x [N][ld_x], w [V][ld_w] of dtype, bias fp32 [V] or NULL, targets int32 / int64; loss, lse, grad_rows fp32 [N]; dx [N][H] and
- * dw [V][H] of dtype, db fp32 [V] or NULL (not wanted), written whole.  A bias may hide words with -infinity.  The gradient takes
+ * dw [V][H] of dtype, db fp32 [V] or NULL (not wanted), written whole.  A bias may hide words with -infinity or the lowest float.  The gradient takes
  * x, w, targets, bias and ignore as the loss did, and its lse; it computes the logits again, a piece of the vocabulary at a time
  * (a piece of d takes up to 256 MiB of the workspace, more where the partial sums of dx, N * H * 4 bytes a piece, would outgrow it).  At
  * most 2^25 rows, 2^37 logits, 2^33 elements of x or w.  bf16: products and sums in fp32, d rounded to bf16 for the products with w and x,

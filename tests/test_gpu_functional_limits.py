@@ -67,3 +67,24 @@ def test_vocab_loss_of_2_to_the_36_logits(F):  # noqa: F811
     within(loss[rows.to(DEV)], *ref["loss"], "loss")
     within(lse[rows.to(DEV)], *ref["lse"], "lse")
     assert torch.isfinite(lse).all() and (lse > 0).all()
+
+
+LOWEST = torch.finfo(F32).min
+
+
+@pytest.mark.parametrize("N,H,V,dtype", [(256, 64, 24700, BF16), (2100, 136, 3119, BF16), (150, 96, 400, BF16), (150, 96, 400, F32)])
+def test_vocab_loss_words_hidden_by_the_lowest_value(F, N, H, V, dtype):  # noqa: F811
+    """A bias of the type's lowest value hides words like one of -infinity, also all words of a tile's columns; large and small tiles."""
+    x, w, b, t, a = vocab_inputs(N, H, V, dtype, True, seed=80)
+    hide = torch.rand(V, generator=gen(81)) < 0.2
+    hide[64:330] = True
+    hide[V - 70:] = True
+    hide[:3] = False
+    t = torch.where(hide[t], torch.full_like(t, 2), t)
+    ref = vocab_ref(x, w, b.masked_fill(hide, -math.inf), t, a, (0,), dtype)
+    got = vocab_run(F, *on(x, w, b.masked_fill(hide, LOWEST), t, a), (0,))
+    for n in ("loss", "lse", "dx", "dw", "db"):
+        within(got[n], *ref[n], n)
+    same = vocab_run(F, *on(x, w, b.masked_fill(hide, -math.inf), t, a), (0,))
+    for n in same:
+        assert torch.equal(got[n], same[n]), n
