@@ -12,6 +12,9 @@
 
 namespace {
 
+// (a lambda that stays a call has its captures in scratch memory: fp32 with 256 columns 700 bytes a lane instead of 140)
+#define INLINE __attribute__((always_inline))
+
 template <typename T, int DP, bool SPLIT> __global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void attn_seq_dkv_kernel(AttnSeqArgs a) {
     constexpr int NC = DP / 16, ND = DP / 32, ES = sizeof(T);
     constexpr bool KEEP = InRegs<T, DP>::value;  // else v is read from memory for every tile
@@ -56,9 +59,14 @@ template <typename T, int DP, bool SPLIT> __global__ __launch_bounds__(256, (DP 
     const int w_all = a.causal ? max(0, k0 + 31 - a.off) * a.group : 0;
     const unsigned w_seen = (unsigned)__ballot(seen);
     const bool all_seen = w_seen == 0xffffffffu;
-    unsigned b_seen = w_seen;  // does any wave of the workgroup have a key to work for?
+    int b_first = 0x7fffffff;  // the first key that is seen, of all the workgroup's
 #pragma unroll
-    for (int w = 1; w < 4; ++w) b_seen |= key_bits(a, b, kt * ATTN_SEQ_BLOCK + (wave + w) % 4 * 32, lane);
+    for (int w = 3; w >= 0; --w) {
+        const unsigned bits = key_bits(a, b, kt * ATTN_SEQ_BLOCK + w * 32, lane);
+        if (bits) b_first = kt * ATTN_SEQ_BLOCK + w * 32 + __builtin_ctz(bits);
+    }
+    // Rows below this see none of them.  Those that share a tile with rows that do are fetched as zeros, whatever q and g hold there.
+    const int blind = a.causal && b_first != 0x7fffffff ? min(max(0, b_first - a.off) * a.group, a.R) : 0;
     // a row sees this lane's key from row (key - off) * group on
     const int from = !seen ? 0x7fffffff : a.causal ? max(0, key - a.off) * a.group : 0;
     int t0 = min(first, a.R) / 32, t1 = (a.R + 31) / 32;
@@ -67,7 +75,7 @@ template <typename T, int DP, bool SPLIT> __global__ __launch_bounds__(256, (DP 
         if (split > 0 && t0 >= t1) return;  // this key tile needs fewer workgroups
         t1 = min(t1, t0 + a.tiles_per_split);
     }
-    if (b_seen == 0) t1 = t0;
+    if (b_first == 0x7fffffff) t1 = t0;
     const unsigned q_row = (unsigned)(a.q_st * ES), q_head = (unsigned)(a.q_sh * ES), g_row = (unsigned)(a.g_st * ES), g_head = (unsigned)(a.g_sh * ES);
     const unsigned lds0 = lds_address(smem);
     TileOffsets<T, DP, 32> at_q, at_g;
@@ -76,12 +84,12 @@ template <typename T, int DP, bool SPLIT> __global__ __launch_bounds__(256, (DP 
     const bool even = 32 % a.group == 0;  // every tile then begins with a query's first head, and a lane's offsets never change
     const int step_i = even ? 32 / a.group : 0;
     long long at_stats;  // lse and delta of the lane's row: 32 threads, loaded a tile ahead
-    // row x of a tile: query (rest + x) / group from the tile's first on, of `rows` that there are
-    auto places = [&](int rest, int rows) {
+    // row x of a tile: query (rest + x) / group from the tile's first on, of `rows` that there are, the first `none` of them left out
+    auto places = [&](int rest, int rows, int none) INLINE {
         auto row = [&](unsigned per_row, unsigned per_head) {
             return [&, per_row, per_head](int x) {
                 const unsigned y = rest + x, i = a.group == 1 ? y : by_group(a, y);
-                return x < rows ? i * per_row + (y - i * a.group) * per_head : 0x80000000u;
+                return x >= none && x < rows ? i * per_row + (y - i * a.group) * per_head : 0x80000000u;
             };
         };
         at_q.set(a.D, wave, lane, row(q_row, q_head));
@@ -89,11 +97,12 @@ template <typename T, int DP, bool SPLIT> __global__ __launch_bounds__(256, (DP 
         const unsigned y = rest + (lane & 31), i = a.group == 1 ? y : by_group(a, y);
         at_stats = ((long long)b * a.Hq + hk * a.group + (y - i * a.group)) * a.Tq + i;
     };
-    if (even) places(0, 32);
+    if (even) places(0, 32, 0);
     float lse2 = INFINITY, delta = 0.f;
-    auto request = [&](int t, int buf) {
+    auto request = [&](int t, int buf) INLINE {
         const int r0 = t * 32, i0 = even ? t * step_i : r0 / a.group;
-        if (!even || r0 + 32 > a.R) places(even ? 0 : r0 - i0 * a.group, a.R - r0);
+        // (the tile behind one with such rows takes its offsets anew)
+        if (!even || r0 + 32 > a.R || r0 < blind + 32) places(even ? 0 : r0 - i0 * a.group, a.R - r0, blind - r0);
         at_q.request(qb + (long long)i0 * a.q_st, lds0 + OFF_Q + buf * TILE, wave);
         at_g.request(gb + (long long)i0 * a.g_st, lds0 + OFF_G + buf * TILE, wave);
         lse2 = INFINITY;
@@ -117,7 +126,7 @@ template <typename T, int DP, bool SPLIT> __global__ __launch_bounds__(256, (DP 
         put_stats(0);
     }
     // one tile out of buffer CUR
-    auto step = [&](auto which, int t) {
+    auto step = [&](auto which, int t) INLINE {
         constexpr int CUR = decltype(which)::value;
         const int r0 = t * 32;
         tile_landed();

@@ -140,8 +140,15 @@ __global__ __launch_bounds__(256, (GradOccupancy<T, DP, KT, ROWS>::value)) void 
     const T* urow = key_seen(a, b, ukey) ? (utype ? vb + (long long)ukey * a.v_st : kb + (long long)ukey * a.k_st) : nullptr;
     stage<T, DP, KP, 256>(sk, a.D, [&](int x) { return key_seen(a, b, x) ? kb + (long long)x * a.k_st : nullptr; });
     unsigned bits[KT];
+    int first = KP;  // the first key that is seen
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt) bits[kt] = key_bits(a, b, kt * 32, lane) >> (4 * h);
+    for (int kt = KT - 1; kt >= 0; --kt) {
+        const unsigned all = key_bits(a, b, kt * 32, lane);
+        if (all) first = kt * 32 + __builtin_ctz(all);
+        bits[kt] = all >> (4 * h);
+    }
+    // rows below this see nothing: zeros, whatever q and g hold there
+    const int blind = first == KP ? a.R : a.causal ? max(0, first - a.off) * a.group : 0;
     auto store = [&](int d, int kt, const f32x16_t& x, const f32x16_t& y) {
         const int key = kt * 32 + (lane & 31);
         if (key >= a.Tk) return;
@@ -173,7 +180,7 @@ __global__ __launch_bounds__(256, (GradOccupancy<T, DP, KT, ROWS>::value)) void 
     for (int t = t0; t < t1; ++t) {
         auto row_of = [&](const void* p, long long sb, long long st, long long sh, int x) -> const T* {
             const int r = t * 32 + x;
-            if (r >= a.R) return nullptr;
+            if (r < blind || r >= a.R) return nullptr;
             const int qi = r / a.group;
             return (const T*)p + b * sb + qi * st + (hk * a.group + r - qi * a.group) * sh;
         };

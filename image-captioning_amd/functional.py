@@ -258,7 +258,7 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, caus
     q (B, Tq, Hq, D); k, v (B, Tk, Hkv, D), Hq a multiple of Hkv (query head h reads key head h // (Hq // Hkv)); any strides, e.g.
     slices of one packed projection.  ``causal``: query i sees keys up to i + Tk - Tq.  key_mask (B, Tk) bool: True where a key may
     be seen; what k and v hold elsewhere is never used.  (A key hidden from a query by causality alone takes part in its products with
-    weight zero, so it has to be finite.)  A query that sees nothing gets zeros.  scale defaults to D ** -0.5.
+    weight zero, so it has to be finite.)  A query that sees nothing gets zeros, whatever it holds.  scale defaults to D ** -0.5.
     o (B, Tq, Hq, D) in q's dtype, lse (B, Hq, Tq) fp32.  D at most 256 and a multiple of 8 (bf16) or 4 (fp32)."""
     name = "attention_forward"
     dev = _device(name, q, k, v, key_mask)

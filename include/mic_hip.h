@@ -522,7 +522,8 @@ int mic_embed_grad(const void* ids, int ids_bits, const void* g, void* d_table, 
  *     o[b, i, h] = sum_j p_ij v[b, j, h / (Hq/Hkv)],   p_ij = exp(scale * q_i . k_j - lse_i) over the keys j that i sees,
  *     lse[b, h, i] = log sum_j exp(scale * q_i . k_j).
  * Query i sees key j when key_mask[b, j] != 0 (NULL: always) and, with causal != 0, j <= i + Tk - Tq (the last query sees every
- * key).  A row that sees no key has o = 0, lse = -infinity and zero gradients.  Keys hidden by key_mask never enter a product,
+ * key).  A row that sees no key has o = 0, lse = -infinity and zero gradients, and no part in any other result, whatever q and grad_o
+ * hold there.  Keys hidden by key_mask never enter a product,
  * whatever k and v hold there (infinities and NaN included); k and v of every other key must be finite, also where causality
  * hides them from some rows.
  * q, o, grad_o [B][Tq][Hq][D], k, v [B][Tk][Hkv][D] of dtype, addressed by element strides (batch, position, head), the D columns of

@@ -88,3 +88,56 @@ def test_vocab_loss_words_hidden_by_the_lowest_value(F, N, H, V, dtype):  # noqa
     same = vocab_run(F, *on(x, w, b.masked_fill(hide, -math.inf), t, a), (0,))
     for n in same:
         assert torch.equal(got[n], same[n]), n
+
+
+BLIND = [
+    # B, Tq, Tk, Hq, Hkv, D, how many of the first keys are hidden
+    (2, 150, 100, 2, 1, 64, 0),     # more queries than keys: the first ones see nothing
+    (2, 40, 30, 2, 2, 256, 0),      # the kernels for one tile of keys
+    (3, 29, 29, 2, 2, 256, 11),     # captions padded on the left
+    (3, 60, 60, 3, 1, 40, 33),
+    (2, 300, 300, 2, 2, 128, 150),
+    (2, 333, 333, 6, 2, 72, 47),    # three query heads to a key head
+    (1, 520, 520, 2, 1, 32, 129),   # ranges of rows
+    (1, 270, 270, 40, 1, 64, 5),    # more query heads than a tile of rows
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("B,Tq,Tk,Hq,Hkv,D,hidden", BLIND)
+def test_attention_rows_that_see_nothing_may_hold_anything(F, B, Tq, Tk, Hq, Hkv, D, hidden, dtype):  # noqa: F811
+    """Causal queries before the first key that is seen: what q and the output's gradient hold there enters no result."""
+    q, k, v, go, _ = attn_inputs(B, Tq, Tk, Hq, Hkv, D, dtype, None, seed=82)
+    m = None
+    if hidden:
+        m = (torch.arange(Tk) >= hidden).repeat(B, 1)
+        if B > 1:
+            m[-1] = True  # one sequence is not padded
+        m[0, hidden + 1] = False
+    first = [(int(m[b].int().argmax()) if hidden else 0) - (Tk - Tq) for b in range(B)]
+    blind = torch.arange(Tq)[None] < torch.tensor(first)[:, None]
+    assert blind.any() and not blind.all()
+    ref = attn_ref(q, k, v, go, True, m, 1 / math.sqrt(D), dtype)
+    bad = torch.tensor([math.nan, math.inf, -math.inf, torch.finfo(dtype).min])
+    for seed, x in ((83, q), (84, go)):
+        x[blind] = bad[torch.randint(0, 4, x[blind].shape, generator=gen(seed))].to(dtype)
+    got = attn_run(F, *on(q, k, v, go), True, None if m is None else m.to(DEV))
+    attn_check(got, ref)
+    assert not got["o"][blind.to(DEV)].any() and not got["dq"][blind.to(DEV)].any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("Tk", [20, 49, 130])
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_sequence_without_a_key_may_hold_anything(F, Tk, causal, dtype):  # noqa: F811
+    """All keys of one sequence are hidden: none of its inputs enters a result, and all its results are zero."""
+    q, k, v, go, _ = attn_inputs(3, 40, Tk, 4, 2, 64, dtype, None, seed=87)
+    m = torch.ones(3, Tk, dtype=torch.bool)
+    m[1] = False
+    ref = attn_ref(q, k, v, go, causal, m, 0.125, dtype)
+    bad = torch.tensor([math.nan, math.inf, -math.inf, torch.finfo(dtype).min])
+    for seed, x in ((88, q), (89, go), (90, k), (91, v)):
+        x[1] = bad[torch.randint(0, 4, x[1].shape, generator=gen(seed))].to(dtype)
+    got = attn_run(F, *on(q, k, v, go), causal, m.to(DEV))
+    attn_check(got, ref)
+    assert not any(got[n][1].any() for n in ("o", "dq", "dk", "dv"))
