@@ -236,7 +236,7 @@ def _attn_check(name, dev, q, k, v, key_mask):
     Bk, Tk, Hkv, Dk = k.shape
     if Bk != B or Dk != D or Hq < 1 or Hkv < 1 or D < 1:
         raise ValueError(f"{name}: q {tuple(q.shape)} and k {tuple(k.shape)} do not fit")
-    _small(name, B, Tq, Tk, Hq, Hkv)
+    _small(name, B, Tq, Tk, Hq, Hkv, D)
     dtype = q.dtype
     if k.dtype is not dtype or v.dtype is not dtype:
         raise ValueError(f"{name}: q, k and v are {dtype}, {k.dtype} and {v.dtype}")

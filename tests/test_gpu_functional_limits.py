@@ -141,3 +141,11 @@ def test_attention_sequence_without_a_key_may_hold_anything(F, Tk, causal, dtype
     got = attn_run(F, *on(q, k, v, go), causal, m.to(DEV))
     attn_check(got, ref)
     assert not any(got[n][1].any() for n in ("o", "dq", "dk", "dv"))
+
+
+def test_attention_columns_past_32_bits_are_refused(F):  # noqa: F811
+    q = torch.empty(0, 1, 1, 1 << 31, device=DEV)
+    with pytest.raises(ValueError):
+        F.attention_forward(q, q, q)
+    with pytest.raises(ValueError):
+        F.attention_grad(q, q, q, q, q, torch.empty(0, 1, 1, device=DEV))
