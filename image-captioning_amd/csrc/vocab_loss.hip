@@ -170,32 +170,39 @@ template <typename T> struct GradEpi {
 // ---- epilogue: fp32 partial results of a slice, or the rounded result ---------------------------------------------------------
 template <typename T> struct OutEpi {
     struct Args {
-        T* out;       // [Nq][ld] rounded, used with one slice
-        float* part;  // [slices][Nq][Np] fp32 otherwise
-        long long ld;
+        T* out;        // [Nq][Np] rounded, taken where there is one slice; or NULL
+        float* part;   // fp32 [Nq][Np] per slice otherwise, each slice before the last; without `out` one after the other, of *count rows
+        const int* count;  // on the device: with `out` the slices, without it the rows there are
         int Np, Nq;
     };
+    // the rows to write, and the slice's partial matrix (NULL: write the result)
+    __device__ static __forceinline__ int rows(const Args& a) { return a.out ? a.Nq : __builtin_amdgcn_readfirstlane(*a.count); }
+    __device__ static __forceinline__ float* part(const Args& a, int slice) {
+        if (a.out) return a.part && __builtin_amdgcn_readfirstlane(*a.count) != 1 ? a.part - (long long)slice * a.Nq * a.Np : nullptr;
+        return a.part + (long long)slice * rows(a) * a.Np;
+    }
     template <int S> __device__ static __forceinline__ void run(const Args& a, f32x16_t (&acc)[S][S], int p0, int q0, int lane, int, int, int slice) {
-        const int h = lane >> 5;
-        const bool whole = a.Np % 4 == 0 && a.ld % 4 == 0;
+        const int h = lane >> 5, nq = rows(a);
+        float* to = part(a, slice);
+        const bool whole = a.Np % 4 == 0;
 #pragma unroll
         for (int j = 0; j < S; ++j) {
             const int row = q0 + j * 32 + (lane & 31);
-            if (row >= a.Nq) continue;
+            if (row >= nq) continue;
 #pragma unroll
             for (int i = 0; i < S; ++i)
 #pragma unroll
                 for (int e4 = 0; e4 < 4; ++e4) {
                     const int c = p0 + i * 32 + 8 * e4 + 4 * h;
                     const float v[4] = {acc[i][j][4 * e4], acc[i][j][4 * e4 + 1], acc[i][j][4 * e4 + 2], acc[i][j][4 * e4 + 3]};
-                    if (a.part) {
-                        float* o = a.part + ((long long)slice * a.Nq + row) * a.Np + c;
+                    if (to) {
+                        float* o = to + (long long)row * a.Np + c;
                         if (whole && c < a.Np) store4<float>(o, v[0], v[1], v[2], v[3]);
                         else if (!whole)
                             for (int e = 0; e < 4; ++e)
                                 if (c + e < a.Np) o[e] = v[e];
                     } else {
-                        T* o = a.out + (long long)row * a.ld + c;
+                        T* o = a.out + (long long)row * a.Np + c;
                         if (whole && c < a.Np) store4<T>(o, v[0], v[1], v[2], v[3]);
                         else if (!whole)
                             for (int e = 0; e < 4; ++e)
@@ -349,24 +356,25 @@ struct OutEpi8 {
     typedef OutEpi<bf16_t>::Args Args;
     __device__ static __forceinline__ void side(const Args&, int, int, int, float*) {}
     __device__ static __forceinline__ void run(const Args& a, f32x4_t (&acc)[4][8], int p0, int q0, int lane, int wave, int, int, int slice, const float*) {
-        const int pw = p0 + 64 * (wave & 3) + 4 * (lane >> 4), qw = q0 + 128 * (wave >> 2) + (lane & 15);
-        const bool whole = a.Np % 4 == 0 && a.ld % 4 == 0;
+        const int pw = p0 + 64 * (wave & 3) + 4 * (lane >> 4), qw = q0 + 128 * (wave >> 2) + (lane & 15), nq = OutEpi<bf16_t>::rows(a);
+        float* to = OutEpi<bf16_t>::part(a, slice);
+        const bool whole = a.Np % 4 == 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int row = qw + 16 * i;
-            if (row >= a.Nq) continue;
+            if (row >= nq) continue;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int c = pw + 16 * j;
                 const f32x4_t& v = acc[j][i];
-                if (a.part) {
-                    float* o = a.part + ((long long)slice * a.Nq + row) * a.Np + c;
+                if (to) {
+                    float* o = to + (long long)row * a.Np + c;
                     if (whole && c < a.Np) store4<float>(o, v[0], v[1], v[2], v[3]);
                     else if (!whole)
                         for (int e = 0; e < 4; ++e)
                             if (c + e < a.Np) o[e] = v[e];
                 } else {
-                    bf16_t* o = a.out + (long long)row * a.ld + c;
+                    bf16_t* o = a.out + (long long)row * a.Np + c;
                     if (whole && c < a.Np) store4<bf16_t>(o, v[0], v[1], v[2], v[3]);
                     else if (!whole)
                         for (int e = 0; e < 4; ++e)
@@ -378,36 +386,39 @@ struct OutEpi8 {
 };
 
 // ---- the sums of partial results, by block number in one launch ---------------------------------------------------------------------
-// out[row] = the sum of fp32 rows at[row] (NULL: the row itself; negative: zeros) of the partial matrices, in order: `pieces` groups of
-// `most` matrices `stride` elements apart, of which the first *slices (of the last group: *slices_last) were written
+// out[row] = the sum of fp32 rows at[row] (negative: zeros) of the partial matrices, in order: `pieces` groups of *slices matrices (the
+// last: *slices_last), `room` elements apart, of *counted rows each.  Without `at`: row `row` of *slices_last matrices `stride` elements
+// apart, where there are several (one is the result already).
 struct SumParts {
     const float* part;
     void* out;
-    const int *at, *slices, *slices_last;
-    long long stride;
-    int rows, cols, pieces, most;
+    const int *at, *slices, *slices_last, *counted;
+    long long stride, room;
+    int rows, cols, pieces;
     unsigned blocks;  // 0: nothing to do
 };
 template <typename T> __device__ __forceinline__ void sum_parts(const SumParts& a, unsigned block) {
     const int quads = (a.cols + 3) / 4;
     const long long i = (long long)block * 256 + threadIdx.x;
     const int row = (int)(i / quads), c = (int)(i - (long long)row * quads) * 4;
-    if (row >= a.rows) return;
-    const int src = a.at ? a.at[row] : row, whole = *a.slices, last = *a.slices_last;
+    const int whole = *a.slices, last = *a.slices_last;
+    if (row >= a.rows || (!a.at && last == 1)) return;
+    const int src = a.at ? a.at[row] : row;
+    const long long stride = a.at ? (long long)*a.counted * a.cols : a.stride;
     float s[4] = {};
     if (src >= 0) {
         for (int g = 0; g < a.pieces; ++g) {
-            const float* p = a.part + (long long)g * a.most * a.stride + (long long)src * a.cols + c;
+            const float* p = a.part + g * a.room + (long long)src * a.cols + c;
             const int parts = g == a.pieces - 1 ? last : whole;
             if (a.cols % 4 == 0) {
 #pragma unroll 8
                 for (int k = 0; k < parts; ++k) {
-                    const float4 x = *reinterpret_cast<const float4*>(p + k * a.stride);
+                    const float4 x = *reinterpret_cast<const float4*>(p + k * stride);
                     s[0] += x.x; s[1] += x.y; s[2] += x.z; s[3] += x.w;
                 }
             } else {
                 for (int e = 0; e < 4 && c + e < a.cols; ++e)
-                    for (int k = 0; k < parts; ++k) s[e] += p[k * a.stride + e];
+                    for (int k = 0; k < parts; ++k) s[e] += p[k * stride + e];
             }
         }
     }
@@ -461,13 +472,16 @@ struct SplitRule {
 };
 struct Split {
     int tiles, nk, most;    // tiles of the result (dx: per tile of rows), steps of k (dw: 0, by the rows), ranges allowed
+    long long elements;     // of one partial matrix (dx: per row)
 };
 // 1 to 10, 12, 16, 24, 32, 48, 64 ranges (i < 16)
 constexpr int MAX_SLICES = 64;
 __device__ __forceinline__ int slices_at(int i) { return i < 10 ? i + 1 : (i & 1 ? 16 : 12) << ((i - 10) >> 1); }
 // The pair of numbers that costs least: a lane looks at one number for x and four for w.  Both products are one launch, whose
 // tiles are dealt out in turn: the first workgroups have one tile of x more, or the ones behind them one of w.
-__device__ __forceinline__ int2 choose_slices(const SplitRule& r, int tiles_x, int nk_x, int most_x, int tiles_w, int nk_w, int most_w, int lane) {
+// The partial matrices of both have to fit `room` elements; one of x alone does.
+__device__ __forceinline__ int2 choose_slices(const SplitRule& r, int tiles_x, int nk_x, int most_x, long long elements_x, int tiles_w, int nk_w, int most_w, long long elements_w,
+                                              long long room, int lane) {
     const int sx = slices_at(lane & 15);
     const float all_x = (float)(tiles_x * sx) / r.capacity, some = floorf(all_x), up = ceilf(all_x), kx = ceilf((float)nk_x / sx) + r.fixed;
     float best = INFINITY;
@@ -477,7 +491,7 @@ __device__ __forceinline__ int2 choose_slices(const SplitRule& r, int tiles_x, i
         const int sw = slices_at((lane >> 4) * 4 + i);
         const float all_w = (float)(tiles_w * sw) / r.capacity, rounds = ceilf(all_x + all_w), kw = ceilf((float)nk_w / sw) + r.fixed;
         float cost = fmaxf(up * kx + (rounds - up) * kw, some * kx + (rounds - some) * kw) + (all_x + (sw > 1 ? all_w : 0.f)) * r.traffic;
-        if (sx > most_x || sw > most_w) cost = INFINITY;
+        if (sx > most_x || sw > most_w || sx * elements_x + (sw > 1 ? sw * elements_w : 0) > room) cost = INFINITY;
         if (cost < best) {
             best = cost;
             at = sw * 128 + sx;
@@ -503,6 +517,7 @@ struct RowsArgs {
     int N, per_block;
     SplitRule rule;
     Split dx[2], dw[2];     // whole pieces, the last one
+    long long room;         // elements for the partial matrices of a piece
     int edge, ks;
 };
 __global__ __launch_bounds__(1024) void vocab_rows_kernel(RowsArgs a) {
@@ -538,7 +553,8 @@ __global__ __launch_bounds__(1024) void vocab_rows_kernel(RowsArgs a) {
     }
     if (blockIdx.x == gridDim.x - 1 && wave < 2) {  // whole pieces, the last one
         const int rows = base, i = wave;
-        const int2 n = choose_slices(a.rule, a.dx[i].tiles * ((rows + a.edge - 1) / a.edge), a.dx[i].nk, a.dx[i].most, a.dw[i].tiles, (rows + a.ks - 1) / a.ks, a.dw[i].most, lane);
+        const int2 n = choose_slices(a.rule, a.dx[i].tiles * ((rows + a.edge - 1) / a.edge), a.dx[i].nk, a.dx[i].most, rows * a.dx[i].elements, a.dw[i].tiles,
+                                     (rows + a.ks - 1) / a.ks, a.dw[i].most, a.dw[i].elements, a.room, lane);
         if (lane == 0) {
             a.count[i ? SX_LAST : SX] = n.x;
             a.count[i ? SW_LAST : SW] = n.y;
@@ -585,8 +601,9 @@ struct Plan {
     int edge;               // tile edge
     int parts;              // forward: column parts per row
     int Vc, pieces, ld;     // gradient: words per piece, row stride of d
-    int sx, sw;             // slices of k of dx (per piece) and dw
-    long long xpad, wpad, part, zt, d, dx, dw, db, rows, bytes;
+    int sx, sw;             // at most so many slices of k of dx (per piece) and dw
+    long long room;         // elements for the partial sums of a piece: dx from the front, dw from the end
+    long long xpad, wpad, part, zt, d, sums, db, rows, bytes;
 };
 
 
@@ -649,10 +666,12 @@ Plan make_plan(const mic_vocab_loss_desc* d, bool grad) {
         while (p.sw > 1 && p.sw * tw > wide) --p.sw;
         p.rows = o; o += rows_bytes(N);
         p.d = o; o += up256(N * p.ld * es);
-        p.dx = o;
-        o += up256((long long)p.sx * p.pieces * N * H * 4);
-        p.dw = o;
-        if (p.sw > 1) o += up256((long long)p.sw * p.Vc * H * 4);
+        // One copy of dx (its pieces are added at the end) and the partial tiles of one round of workgroups, if that many can be: the rule that
+        // chooses the slices keeps to it, and the copies of dx have the counted rows alone.  7424 x 512 x 3500 in bf16, half counted: the rule
+        // without a limit chooses 4 and 4 slices, 56 MB of the 82.
+        const long long round = (p.big ? 256ll : p.edge == 128 ? 512 : 1024) * p.edge * p.edge, most = (p.sx * N + (p.sw > 1 ? p.sw * (long long)p.Vc : 0)) * H;
+        p.room = ((N * H + round < most ? N * H + round : most) + 63) / 64 * 64;
+        p.sums = o; o += p.pieces * p.room * 4;
         p.db = o;
         if (d->db) o += up256((long long)edge_tiles(N, p.edge) * 2 * p.Vc * 4);
     }
@@ -787,19 +806,20 @@ template <typename T> int gradient(const mic_vocab_loss_desc* d, const Plan& p, 
     ra.edge = p.edge;
     ra.ks = 128 / (int)sizeof(T);
     const int last = d->V - (p.pieces - 1) * p.Vc, th = edge_tiles(H, p.edge);
-    ra.dx[0] = {th, (p.Vc + ra.ks - 1) / ra.ks, p.sx};
-    ra.dx[1] = {th, (last + ra.ks - 1) / ra.ks, p.sx};
-    ra.dw[0] = {th * edge_tiles(p.Vc, p.edge), 0, p.sw};
-    ra.dw[1] = {th * edge_tiles(last, p.edge), 0, p.sw};
+    ra.dx[0] = {th, (p.Vc + ra.ks - 1) / ra.ks, p.sx, H};
+    ra.dx[1] = {th, (last + ra.ks - 1) / ra.ks, p.sx, H};
+    ra.dw[0] = {th * edge_tiles(p.Vc, p.edge), 0, p.sw, p.Vc * H};
+    ra.dw[1] = {th * edge_tiles(last, p.edge), 0, p.sw, last * H};
+    ra.room = p.room;
     MIC_LAUNCH(vocab_rows_kernel, dim3((unsigned)((N + ra.per_block - 1) / ra.per_block)), dim3(1024), 0, s, ra);
     const int *at = ra.at, *count = ra.count;
     Operand x, w;
     MIC_TRY(operands<T>(d, p, ws, at, x, w, s));
     T* dl = (T*)(ws + p.d);
-    float *part_dx = (float*)(ws + p.dx), *part_dw = (float*)(ws + p.dw), *part_db = (float*)(ws + p.db);
-    auto parts_of = [&](const float* part, T* out, const int* where, int rows, long long stride, int pieces, int most, int whole, int end) {
+    float *sums = (float*)(ws + p.sums), *part_db = (float*)(ws + p.db);
+    auto parts_of = [&](const float* part, T* out, const int* where, int rows, long long stride, int pieces, int whole, int end) {
         const long long quads = (long long)rows * ((H + 3) / 4);
-        return SumParts{part, out, where, ra.count + whole, ra.count + end, stride, rows, d->H, pieces, most, (unsigned)((quads + 255) / 256)};
+        return SumParts{part, out, where, ra.count + whole, ra.count + end, count, stride, p.room, rows, d->H, pieces, (unsigned)((quads + 255) / 256)};
     };
     auto finish = [&](const SumParts& x1, const SumParts& x2, const ColSum& c) -> int {
         const unsigned blocks = x1.blocks + x2.blocks + c.blocks;
@@ -818,22 +838,23 @@ template <typename T> int gradient(const mic_vocab_loss_desc* d, const Plan& p, 
         MIC_TRY((product<T, GradEpi<T>, GradEpi8>(p, wi, x, Rows{count, 0, nullptr, 1}, d->H, ga, s)));
         // dx += d w: k runs over the words of the piece
         typename OutEpi<T>::Args xa = {};
-        xa.ld = H; xa.Np = d->H; xa.Nq = d->N;
-        xa.part = part_dx + (long long)i * p.sx * N * H;  // rows of the gathered order
+        xa.Np = d->H; xa.Nq = d->N;
+        xa.part = sums + i * p.room; xa.count = count;  // rows of the gathered order
         const Operand wc = {wi.p, wi.ld, d->H}, dr = {dl, p.ld, d->N};
         const Rows rx = {count, 0, ra.count + (end ? SX_LAST : SX), p.sx};
         // dw = d^T x: k runs over the rows
         typename OutEpi<T>::Args wa = {};
-        wa.out = (T*)d->dw + v0 * H; wa.ld = H; wa.Np = d->H; wa.Nq = vc;
-        if (p.sw > 1) wa.part = part_dw;
+        wa.out = (T*)d->dw + v0 * H; wa.Np = d->H; wa.Nq = vc;
+        if (p.sw > 1) wa.part = sums + (i + 1) * p.room - vc * H;
         const Operand xc = {x.p, x.ld, d->H}, dc = {dl, p.ld, vc};
         const Rows rw = {count, 1, ra.count + (end ? SW_LAST : SW), p.sw};
+        wa.count = rw.slices;
         MIC_TRY((products<T>(p, {wc, dr, rx, vc}, xa, {xc, dc, rw, d->N}, wa, s)));
         SumParts sw = {}, sx = {};
         ColSum sb = {};
-        if (p.sw > 1) sw = parts_of(part_dw, wa.out, nullptr, vc, vc * H, 1, p.sw, SW, end ? SW_LAST : SW);
+        if (p.sw > 1) sw = parts_of(wa.part, wa.out, nullptr, vc, -(vc * H), 1, SW, end ? SW_LAST : SW);
         if (d->db) sb = {part_db, d->db + v0, count, vc, edge_tiles(N, p.edge) * 2, p.edge / 2, (unsigned)((vc + 15) / 16)};
-        if (end) sx = parts_of(part_dx, (T*)d->dx, at, d->N, N * H, p.pieces, p.sx, SX, SX_LAST);
+        if (end) sx = parts_of(sums, (T*)d->dx, at, d->N, 0, p.pieces, SX, SX_LAST);
         MIC_TRY(finish(sx, sw, sb));
     }
     return 0;

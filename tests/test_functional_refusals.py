@@ -247,3 +247,20 @@ def test_vocab_loss_of_many_small_tiles_takes_larger_ones(L):
             parts = v.V // half_tile
             need = L.lib.mic_vocab_loss_workspace_bytes(C.byref(v), 0)
             assert abs(need - N * (parts * 8 + 4)) <= 1024, (dtype, N, need)
+
+
+def test_vocab_loss_gradient_scratch(L):
+    """Beside the gathered rows, a piece of d and the column sums: per piece a copy of dx and the partial tiles of one round of workgroups
+    (256 of 256 x 256, 512 of 128 x 128 or 1024 of 64 x 64) at most."""
+    import ctypes as C
+    v = L.VocabLossDesc()
+    v.target_bits, v.db = 64, P
+    for dtype, N, H, V, pieces, width, tile in ((L.BF16, 7424, 512, 3500, 1, 3500, 256), (L.BF16, 256, 2048, 65536, 1, 65536, 256),
+                                                (L.BF16, 4096, 2048, 32000, 1, 32000, 256), (L.BF16, 8192, 2048, 65536, 4, 16384, 256),
+                                                (L.F32, 7424, 512, 3500, 1, 3500, 64), (L.F32, 1111, 300, 10007, 1, 10007, 64),
+                                                (L.BF16, 100, 1024, 70000, 1, 70000, 128), (L.BF16, 24, 512, 32000, 1, 32000, 64)):
+        v.dtype, v.N, v.H, v.V, v.ld_x, v.ld_w = dtype, N, H, V, H, H
+        size = 4 if dtype == L.F32 else 2
+        round_ = {256: 256, 128: 512, 64: 1024}[tile] * tile * tile
+        most = N * H * size + N * (width + 8) * size + pieces * (N * H + round_) * 4 + -(-N // tile) * 2 * width * 4 + 16 * N + (1 << 16)
+        assert L.lib.mic_vocab_loss_workspace_bytes(C.byref(v), 1) <= most, (dtype, N, H, V)

@@ -5,6 +5,7 @@ import math
 import pytest
 import torch
 
+from test_gpu_functional_edges import poisoned  # noqa: F401
 from test_gpu_functional import BF16, DEV, F, F32, U, attn_check, attn_inputs, attn_ref, attn_run, gen, on, vocab_inputs, vocab_ref, vocab_run, within  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -149,3 +150,18 @@ def test_attention_columns_past_32_bits_are_refused(F):  # noqa: F811
         F.attention_forward(q, q, q)
     with pytest.raises(ValueError):
         F.attention_grad(q, q, q, q, q, torch.empty(0, 1, 1, device=DEV))
+
+
+@pytest.mark.parametrize("dtype,N,H,V", [(F32, 40_000, 72, 3500), (F32, 40_000, 41, 3500), (BF16, 90_000, 64, 3500), (F32, 1111, 300, 10007), (BF16, 2600, 520, 3500)])
+@pytest.mark.parametrize("counted", [0.0, 0.01, 0.5, 1.0])
+def test_vocab_loss_pieces_and_ranges(F, poisoned, dtype, N, H, V, counted):  # noqa: F811
+    """Several pieces of the vocabulary, ranges of k in both products, and so many of the rows counted: partial sums share the scratch."""
+    x, w, b, t, a = vocab_inputs(N, H, V, dtype, True, seed=90, ignore_share=0.0)
+    t = torch.where(torch.rand(N, generator=gen(92)) < counted, t.clamp_min(1), torch.zeros_like(t))
+    args = on(x, w, b, t, a / N)
+    ref = {n: [v.cpu() for v in r] for n, r in vocab_ref(*args, (0,), dtype).items()}
+    got = vocab_run(F, *args, (0,))
+    for n, r in ref.items():
+        within(got[n], *r, n)
+    again = vocab_run(F, *args, (0,))
+    assert all(torch.equal(got[n], again[n]) for n in got)
