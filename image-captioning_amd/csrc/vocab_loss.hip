@@ -241,6 +241,7 @@ struct StatsEpi8 {
                 m[i] = fmaxf(m[i], fmaxf(fmaxf(acc[j][i][0], acc[j][i][1]), fmaxf(acc[j][i][2], acc[j][i][3])));
             }
         }
+        bool far = false;
         // the four lanes of a row, all rows at once: an exchange's latency is paid four times, not 32
 #pragma unroll
         for (int d = 16; d < 64; d <<= 1) {
@@ -263,18 +264,22 @@ struct StatsEpi8 {
                     for (int e = 0; e < 4; ++e) z = tc == 16 * j + e ? acc[j][i][e] : z;
                 a.zt[q0 + ql + 16 * i] = z;
             }
-            if (fabsf(m[i]) < 1e38f || m[i] == -INFINITY) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < 4; ++j)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[i] += __builtin_amdgcn_exp2f(fmaf(acc[j][i][e], ATTN_LOG2E, -m2));
-            } else {  // all hidden by the type's lowest value: m2 would be infinite
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s[i] += __builtin_amdgcn_exp2f((acc[j][i][e] - m[i]) * ATTN_LOG2E);
-            }
+                for (int e = 0; e < 4; ++e) s[i] += __builtin_amdgcn_exp2f(fmaf(acc[j][i][e], ATTN_LOG2E, -m2));
+            far |= fabsf(m2) == INFINITY;
         }
+        if (__any(far))  // all hidden by the type's lowest value, the exponent's maximum is not a number of 32 bits: by differences
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float top = m[i] == -INFINITY ? 0.f : m[i];
+                s[i] = 0.f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[i] += __builtin_amdgcn_exp2f((acc[j][i][e] - top) * ATTN_LOG2E);
+            }
 #pragma unroll
         for (int d = 16; d < 64; d <<= 1) {
             float o[8];
