@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from test_gpu_functional_edges import poisoned  # noqa: F401
-from test_gpu_functional import BF16, DEV, F, F32, U, attn_check, attn_inputs, attn_ref, attn_run, gen, on, vocab_inputs, vocab_ref, vocab_run, within  # noqa: F401
+from test_gpu_functional import BF16, DEV, F, F32, U, attn_check, attn_inputs, attn_ref, attn_run, embed_inputs, gen, on, vocab_inputs, vocab_ref, vocab_run, within  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -165,3 +165,54 @@ def test_vocab_loss_pieces_and_ranges(F, poisoned, dtype, N, H, V, counted):  # 
         within(got[n], *r, n)
     again = vocab_run(F, *args, (0,))
     assert all(torch.equal(got[n], again[n]) for n in got)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_vocab_loss_one_gradient_for_every_row(F, dtype):  # noqa: F811
+    """A scalar tensor, and the expanded one that a sum or a mean leaves: the bits that a gradient per row gives."""
+    x, w, b, t, _ = vocab_inputs(70, 96, 500, dtype, True, seed=93)
+    a = torch.full((70,), 0.37)
+    ref = vocab_ref(x, w, b, t, a, (0,), dtype)
+    args = on(x, w, b, t, a)
+    rows = vocab_run(F, *args, (0,))
+    for n, r in ref.items():
+        within(rows[n], *r, n)
+    scalar = vocab_run(F, *args[:4], torch.tensor(0.37, device=DEV), (0,))
+    assert all(torch.equal(rows[n], scalar[n]) for n in rows)
+    for scale, reduce in ((1.0, torch.sum), (70.0, torch.mean)):
+        leaves = [v.clone().requires_grad_() for v in args[:3]]
+        loss = reduce(F.vocab_loss(leaves[0], leaves[1], args[3], bias=leaves[2], ignore=(0,)))
+        loss.backward(torch.tensor(scale, device=DEV))
+        one = vocab_run(F, *args[:4], torch.tensor(1.0, device=DEV), (0,))
+        for n, v in zip(("dx", "dw", "db"), leaves):
+            if scale == 1.0:
+                assert torch.equal(v.grad, one[n]), n
+            else:  # 70 / 70 in fp32
+                within(v.grad, *vocab_ref(x, w, b, t, torch.ones(70), (0,), dtype)[n], n)
+
+
+def test_frozen_operands(F):  # noqa: F811
+    """Gradients of what needs one, whichever that is, are those of the plain calls; what is frozen gets none."""
+    ids, table, p, g = embed_inputs(3, 6, 11, 16, F32, F32, True, seed=94)
+    ids, table, p, g = on(ids, table, p, g)
+    d_table, d_pos = F.embedding_grad(g, ids, 11, scale=2.0, positions=6)
+    for need in ((True, False), (False, True)):
+        leaves = [v.clone().requires_grad_(n) for v, n in zip((table, p), need)]
+        F.embedding(ids, *leaves, scale=2.0).backward(g)
+        for v, n, r in zip(leaves, need, (d_table, d_pos)):
+            assert torch.equal(v.grad, r) if n else v.grad is None
+    q, k, v, go, _ = attn_inputs(2, 9, 70, 4, 2, 32, F32, None, seed=95)
+    q, k, v, go = on(q, k, v, go)
+    plain = attn_run(F, q, k, v, go, False, None)
+    for need in ((True, False, False), (False, True, False), (False, False, True)):
+        leaves = [x.clone().requires_grad_(n) for x, n in zip((q, k, v), need)]
+        F.attention(*leaves).backward(go)
+        for x, n, r in zip(leaves, need, ("dq", "dk", "dv")):
+            assert torch.equal(x.grad, plain[r]) if n else x.grad is None
+    x, w, b, t, a = on(*vocab_inputs(40, 32, 90, F32, True, seed=96))
+    plain = vocab_run(F, x, w, b, t, a, (0,))
+    for need in ((True, False, False), (False, True, False), (False, False, True)):
+        leaves = [y.clone().requires_grad_(n) for y, n in zip((x, w, b), need)]
+        F.vocab_loss(leaves[0], leaves[1], t, bias=leaves[2], ignore=(0,)).backward(a)
+        for y, n, r in zip(leaves, need, ("dx", "dw", "db")):
+            assert torch.equal(y.grad, plain[r]) if n else y.grad is None
