@@ -187,7 +187,8 @@ template <int DP> struct TileReader<float, DP> {
 };
 
 // fp32 with more than 128 columns: the second of a wave's own operands in the gradients (g, v) does not fit the registers next to the first
-// and the sums, it is read again for every tile (4 x 1024 causal queries, 8 heads of 256: 1165 us, with both read again 1355)
+// and the sums, it is read again for every tile (4 x 1024 causal queries, 8 heads of 256: 1165 us, with both read again 1355).  What is left
+// still spills: 130 registers in the key gradients, 28 to 60 in the query gradients.
 template <typename T, int DP> struct InRegs {
     static constexpr bool value = sizeof(T) == 2 || DP <= 128;
 };

@@ -4,7 +4,8 @@
 // and dP = G V^T come out with a lane per key, and P and dS are the B operands of dV^T = G^T P and dK^T = Q^T dS.  The workgroup's
 // four waves walk the same tiles of 32 rows.
 // 2 x 4096 causal queries of 16 heads on 2 key heads of 128 columns, bf16: 350 us, 790 TFLOP/s, the matrix units 45 % busy: 250 registers a lane
-// leave two waves to a SIMD and operands that are read one step ahead.
+// leave two waves to a SIMD and operands that are read one step ahead (the form without `splits` needs 3 more and spills them; fp32 with
+// 256 columns spills 130 at one wave per SIMD).
 // With `splits` the rows are shared out over several workgroups, which leave fp32 partial sums that a second launch adds in order.
 #include "attn_seq.h"
 

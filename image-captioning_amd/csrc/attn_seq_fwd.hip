@@ -7,9 +7,9 @@
 //
 // 2 x 4096 causal queries of 16 heads (2 key heads) of 128 columns, bf16: 190 us, 720 TFLOP/s; matrix and vector instructions (32 exponentials
 // and some 150 others beside 32 products per wave and tile) together fill the time.  One query, 4093 keys, 8 x 8 heads on 2 key
-// heads: 9.9 us for 33.5 MB and 3.9 us to join 64 ranges of keys.  9 x 333 queries, 391 padded keys, 8 heads of 64, fp32: 30 us.
+// heads: 9.5 us for 33.5 MB and 3.9 us to join 32 ranges of keys.  9 x 333 queries, 391 padded keys, 8 heads of 64, fp32: 30 us.
 // 256 columns take one wave per SIMD: with 256 registers a lane bf16 spills (4 x 1024 causal queries, 8 heads: 132 us, with 512 77 us); fp32 with
-// 128 columns is faster with two (148 and 161 us).
+// 128 columns is faster with two (148 and 161 us), though its form for shared keys spills 14 registers then, and fp32 with 256 columns 6 to 9.
 #include "attn_seq.h"
 
 #include <type_traits>

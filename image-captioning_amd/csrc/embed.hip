@@ -422,8 +422,8 @@ template <typename TO, bool A> __global__ __launch_bounds__(1024) void embed_joi
 
 // ---- sum over sequences: columns of a [B][W] matrix, W = T*H; `slices` of the rows leave fp32 partial rows when there are several
 // A workgroup takes L * N columns, N to a lane; its 1024 / L groups of L lanes share the rows.  With L = 16 and N = 8 a batch of 256 captions
-// of 30 x 512 columns is 120 workgroups with one round of loads each, two to a compute unit: the first launch of the gradient takes 8.6 us, with L = 64 and one
-// workgroup to a compute unit it took 13.9 us.
+// of 30 x 512 columns is 120 workgroups with one round of loads each, two to a compute unit: the first launch of the gradient takes 11 us, with L = 64
+// and one workgroup to a compute unit it took 5 us more.
 template <typename TG, typename TO, int L, int N, bool A>
 __device__ __forceinline__ void colsum(float* lds, const TG* __restrict__ g, TO* __restrict__ out, float* __restrict__ part_out, int B, long long W, int slices,
                                        long long group, int slice) {

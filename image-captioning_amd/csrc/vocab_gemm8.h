@@ -9,7 +9,8 @@
 // A workgroup stays and takes every 256th tile: the next tile's first requests are under way while the epilogue of the last one
 // computes (epilogues leave LDS alone; what they need of bias and rows is put into a small side buffer beforehand).  With H = 512 a
 // tile is 13 us of products, and its start and end used to cost 17 us more.  8192 x 2048 x 65536: 1628 us, 1350 TFLOP/s (the library's
-// product of 8192^3 runs at 1408); 7424 x 512 x 3500: 35 us, 750, as 406 tiles are 1.6 rounds of 256.
+// product of 8192^3 runs at 1408); 7424 x 512 x 3500: 35 us, 750, as 406 tiles are 1.6 rounds of 256.  (The gradient's logits spill 6 registers
+// around the epilogue.)
 // Requests go straight to LDS through a buffer descriptor whose base is the K-tile's, so a lane's offset never changes and no
 // operand is too long; an index outside the operand or a k past the end is bit 31 of the offset, which returns zeros without
 // touching memory.

@@ -1,7 +1,8 @@
 // Softmax cross entropy of a linear layer over the vocabulary, without keeping the logits:
 //   z = x w^T + bias     lse = log sum_v exp z_v     loss = lse - z_target
 //   d = weight * (exp(z - lse) - onehot(target))     dx = d w     dw = d^T x     dbias = column sums of d
-// Forward: the logits' tiles end in the statistics (maximum, sum) of their 64 columns; a second launch joins a row's parts.
+// Forward: a wave's part of a logits' tile ends in the statistics (maximum, sum) of its columns (64, 32 on the smallest tiles); a second
+// launch joins a row's parts.
 // Gradient: piece by piece of the vocabulary the logits are computed again, their epilogue turns them into d (rounded to bf16 for
 // bf16 operands: both remaining products take it as a matrix-core operand; dbias is summed before the rounding), and two more
 // products use the piece.  dw's rows of a piece are complete; dx is summed over the pieces in fp32.
@@ -31,7 +32,7 @@ __device__ __forceinline__ int target_of(const Targets& t, int row) {
     return (int)v;
 }
 
-// ---- epilogue: statistics of 64 columns of logits per row -------------------------------------------------------------------
+// ---- epilogue: statistics of a wave's columns of logits (half a tile) per row -------------------------------------------------
 struct StatsEpi {
     struct Args {
         const float* bias;
@@ -628,9 +629,13 @@ Plan make_plan(const mic_vocab_loss_desc* d, bool grad) {
     p.e = 16 / (int)es;
     p.Hp = (int)((H + p.e - 1) / p.e * p.e);
     p.pad = p.Hp != H || d->ld_x % p.e || d->ld_w % p.e || (((uintptr_t)d->x | (uintptr_t)d->w) & 15);
-    // The large tiles from 128 rows and as many logits as 96 full tiles on.  V = 3500, H = 512, all rows counted, forward and gradient: 2,400
-    // rows 97 us on large tiles and 121 us on small ones, 1,800 rows 92 and 99, 1,200 rows 88 and 80; 100 rows, H = 1024, V = 70000: 273 and
-    // 217.  They address 256 rows (64 of k) with 31 bits.
+    // The large tiles from 128 rows and as many logits as 96 full tiles on.  Forward + gradient on large and on small ones, all rows counted:
+    //   2,400 rows x 3500   H = 64: 18+50 18+42   128: 18+51 25+54   512: 22+74 36+84   1024: 32+102 52+132   2048: 50+158 82+219
+    //   1,800 rows x 3500           17+51 18+38        17+52 18+45        22+70 24+73         31+94  37+116         49+130 61+196
+    //   1,200 rows x 3500           17+46 18+35        17+49 18+41        22+66 22+60         31+86  30+88          49+114 52+147
+    //   512 rows x 16000            19+51 17+39        18+52 19+47        23+74 27+92         33+113 43+142         53+169 72+243
+    // and 100 rows x 70000 with H = 1024 273 and 217 in all.  So the border fits H of some hundred columns; with H <= 128 the small tiles'
+    // gradient would be better up to about 250 tiles, from H = 1024 on the large ones are from 64.  They address 256 rows (64 of k) with 31 bits.
     p.big = d->dtype == MIC_BF16 && N >= 128 && N * V >= 96ll << 16 && H >= 64 && H < (1 << 21) && d->ld_x < (1 << 21) && d->ld_w < (1 << 21);
     // 64 x 64 tiles where 128 x 128 ones would leave compute units idle, half of each tile (H = 64: 20,000 x 3500 forward and gradient 533
     // us, on the larger 746), and in fp32 also the last round of them: a small tile costs 8 % more there (4096 x 512 x 16384: 2663 and

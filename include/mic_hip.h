@@ -558,9 +558,10 @@ int mic_attn_seq_grad(const mic_attn_seq_desc* d, void* stream);
  * lse is computed all the same.
  * x [N][ld_x], w [V][ld_w] of dtype, bias fp32 [V] or NULL, targets int32 / int64; loss, lse, grad_rows fp32 [N]; dx [N][H] and
  * dw [V][H] of dtype, db fp32 [V] or NULL (not wanted), written whole.  A bias may hide words with -infinity or the lowest float.  The gradient takes
- * x, w, targets, bias and ignore as the loss did, and its lse; it computes the logits again, a piece of the vocabulary at a time
- * (a piece of d takes up to 256 MiB of the workspace, more where the partial sums of dx, N * H * 4 bytes a piece, would outgrow it).  At
- * most 2^25 rows, 2^37 logits, 2^33 elements of x or w.  bf16: products and sums in fp32, d rounded to bf16 for the products with w and x,
+ * x, w, targets, bias and ignore as the loss did, and its lse; it computes the logits again, a piece of the vocabulary at a time.
+ * Its workspace holds x, a piece of d (up to 256 MiB, more where the sums of many pieces would outgrow it) and per piece the partial sums:
+ * N * H * 4 bytes and 64 MiB at most.  That can be more than all logits would take where they are few: bf16, 7,424 x 512 x 3500 143 MB
+ * (logits 52), 8,192 x 2048 x 65536 843 MB (logits 1,074).  At most 2^25 rows, 2^37 logits, 2^33 elements of x or w.  bf16: products and sums in fp32, d rounded to bf16 for the products with w and x,
  * db summed before that.  H of any size; x and w whose rows are not whole 16 bytes on 16-byte boundaries are copied into
  * the workspace first.  mic_vocab_loss_workspace_bytes(d, grad) looks at dtype, sizes, strides and the alignment of x, w and
  * whether db is NULL (an argument error is negative). */
