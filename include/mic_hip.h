@@ -561,8 +561,10 @@ int mic_attn_seq_grad(const mic_attn_seq_desc* d, void* stream);
  * x, w, targets, bias and ignore as the loss did, and its lse; it computes the logits again, a piece of the vocabulary at a time.
  * Its workspace holds x, a piece of d (up to 256 MiB, more where the sums of many pieces would outgrow it) and per piece the partial sums:
  * N * H * 4 bytes and 64 MiB at most.  That can be more than all logits would take where they are few: bf16, 7,424 x 512 x 3500 143 MB
- * (logits 52), 8,192 x 2048 x 65536 843 MB (logits 1,074).  At most 2^25 rows, 2^37 logits, 2^33 elements of x or w.  bf16: products and sums in fp32, d rounded to bf16 for the products with w and x,
- * db summed before that.  H of any size; x and w whose rows are not whole 16 bytes on 16-byte boundaries are copied into
+ * (logits 52), 8,192 x 2048 x 65536 843 MB (logits 1,074).  Sizes are limited in tiles: with n = N / 64 + 2
+ * and h, v likewise, n <= 2^19, h, v <= 2^21, n * v < 2^25, n * h and v * h < 2^21 (2^37 logits and 2^33 elements of x or w where they
+ * are wide, 2^26 words of 8 columns).  bf16: products and sums in fp32, d rounded to bf16 for the products with w and x, db summed before
+ * that.  H of any size; x and w whose rows are not whole 16 bytes on 16-byte boundaries are copied into
  * the workspace first.  mic_vocab_loss_workspace_bytes(d, grad) looks at dtype, sizes, strides and the alignment of x, w and
  * whether db is NULL (an argument error is negative). */
 typedef struct mic_vocab_loss_desc {

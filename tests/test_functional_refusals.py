@@ -264,3 +264,23 @@ def test_vocab_loss_gradient_scratch(L):
         round_ = {256: 256, 128: 512, 64: 1024}[tile] * tile * tile
         most = N * H * size + N * (width + 8) * size + pieces * (N * H + round_) * 4 + -(-N // tile) * 2 * width * 4 + 16 * N + (1 << 16)
         assert L.lib.mic_vocab_loss_workspace_bytes(C.byref(v), 1) <= most, (dtype, N, H, V)
+
+
+def test_vocab_loss_limits_are_those_of_the_header(L):
+    """Each size alone at its limit, and one step of 64 beyond it."""
+    import ctypes as C
+    v = L.VocabLossDesc()
+    v.dtype, v.target_bits = L.BF16, 64
+    edge = lambda units: (units - 2) * 64 + 63  # noqa: E731  (the largest size of so many units)
+    for N, H, V in ((edge(1 << 19), 8, 8), (8, edge((1 << 20) - 1), 8), (8, 8, edge((1 << 20) - 1)), (edge(1 << 14), 8, edge((1 << 11) - 1)),
+                    (edge(1 << 11), edge((1 << 10) - 1), 8)):
+        for k in range(4):
+            sizes = [N, H, V]
+            if k:
+                sizes[k - 1] += 64
+            v.N, v.H, v.V, v.ld_x, v.ld_w = *sizes, sizes[1], sizes[1]
+            n, h, w = (s // 64 + 2 for s in sizes)
+            fits = n <= 1 << 19 and h <= 1 << 21 and w <= 1 << 21 and n * w < 1 << 25 and n * h < 1 << 21 and w * h < 1 << 21
+            assert k or fits
+            for grad in (0, 1):
+                assert (L.lib.mic_vocab_loss_workspace_bytes(C.byref(v), grad) >= 0) == fits, sizes

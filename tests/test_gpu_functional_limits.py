@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from test_gpu_functional_edges import poisoned  # noqa: F401
-from test_gpu_functional import BF16, DEV, F, F32, U, attn_check, attn_inputs, attn_ref, attn_run, embed_inputs, gen, on, vocab_inputs, vocab_ref, vocab_run, within  # noqa: F401
+from test_gpu_functional import BF16, DEV, F, F32, U, attn_check, attn_inputs, attn_ref, attn_run, embed_inputs, gen, half, on, vocab_inputs, vocab_ref, vocab_run, within  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -216,3 +216,145 @@ def test_frozen_operands(F):  # noqa: F811
         F.vocab_loss(leaves[0], leaves[1], t, bias=leaves[2], ignore=(0,)).backward(a)
         for y, n, r in zip(leaves, need, ("dx", "dw", "db")):
             assert torch.equal(y.grad, plain[r]) if n else y.grad is None
+
+
+# ---- tensors of more than 2^31 elements, and the longest of each size ------------------------------------------------------------
+def test_attention_over_a_cache_past_32_bits(F):  # noqa: F811
+    """One query on 2^24 + 5 keys of 128 columns: the last ones lie behind 2^31 elements.  A few keys, those among them, carry the softmax."""
+    T, D = (1 << 24) + 5, 128
+    scale, h = 1 / math.sqrt(D), 2.0 ** -9
+    torch.manual_seed(100)
+    q, g = (torch.randn(1, 1, 1, D, device=DEV).to(BF16) for _ in range(2))
+    k, v = (torch.empty(1, T, 1, D, dtype=BF16, device=DEV).normal_(0, s) for s in (0.02, 1.0))
+    heavy = torch.tensor([0, 1000, 1 << 23, (1 << 24) - 1, 1 << 24, T - 1], device=DEV)
+    k[0, heavy, 0] += (torch.linspace(2.3, 2.6, 6, device=DEV)[:, None] * q[0, 0]).to(BF16)
+    o, lse = F.attention_forward(q, k, v, causal=True)
+    dq, dk, dv = F.attention_grad(g, q, k, v, o, lse, causal=True)
+    Q, G = q.double().view(D), g.double().view(D)
+
+    def blocks():
+        for lo in range(0, T, 1 << 20):
+            yield slice(lo, lo + (1 << 20)), k[0, lo:lo + (1 << 20), 0].double(), v[0, lo:lo + (1 << 20), 0].double()
+    z = torch.cat([K @ Q for _, K, _ in blocks()]) * scale
+    L = torch.logsumexp(z, 0)
+    p = torch.exp(z - L)
+    dP = torch.cat([V @ G for *_, V in blocks()])
+    out, mag = sum(p[r] @ V for r, _, V in blocks()), sum(p[r] @ V.abs() for r, _, V in blocks())
+    delta = (p * dP).sum()
+    # a score is a sum of 128 products; a range's sum l takes at most 2^14 additions
+    e = 2 * (D + 3) * U * scale * (k[0, heavy, 0].double().abs() @ Q.abs()).max() + 200 * U + 2.0 ** -10
+    near = lambda got, ref, tol, what: within(got.reshape(ref.shape), ref.cpu(), 1.01 * tol.cpu() + 1e-30, what)  # noqa: E731
+    near(lse, L.view(1), (e + 2 * U * L.abs()).view(1), "lse")
+    near(o, out, (2 * h + 2 * e) * mag, "o")
+    e_delta = (3 * h + 2 * e) * (mag @ G.abs())
+    e_ds = p * ((h + e) * (dP - delta).abs() + e_delta + 200 * U * (dP.abs() + delta.abs()))
+    ds = p * (dP - delta)
+    near(dq, scale * sum(ds[r] @ K for r, K, _ in blocks()), scale * (1 + h) * sum((e_ds[r] + (h + e) * ds[r].abs()) @ K.abs() for r, K, _ in blocks()), "dq")
+    rows = torch.cat([heavy, torch.randint(0, T, (1000,), device=DEV), torch.arange(T - 200, T, device=DEV)])
+    near(dk[0, rows, 0], scale * ds[rows, None] * Q, scale * (e_ds + h * ds.abs())[rows, None] * (1 + h) * Q.abs(), "dk")
+    near(dv[0, rows, 0], p[rows, None] * G, (2 * h + 2 * e) * p[rows, None] * G.abs(), "dv")
+    light = torch.ones(T, dtype=torch.bool, device=DEV)
+    light[heavy] = False
+    assert float(dv[0, :, 0].abs().amax(1)[light].max()) <= 1.1 * float((p[light]).max() * G.abs().max())
+
+
+def test_embedding_past_32_bits(F):  # noqa: F811
+    """2^21 + 3 tokens of 1,024 columns: result and gradient have more than 2^31 elements."""
+    n, H, V = (1 << 21) + 3, 1024, 1000
+    torch.manual_seed(101)
+    ids = torch.randint(0, V, (n,), device=DEV)
+    table = torch.randn(V, H, device=DEV).to(BF16)
+    out = F.embedding_forward(ids, table)
+    assert all(torch.equal(out[lo:lo + (1 << 18)], table[ids[lo:lo + (1 << 18)]]) for lo in range(0, n, 1 << 18))
+    d, _ = F.embedding_grad(out, ids, V, dtype=F32)  # the gradient of a word's row: its count times the row
+    m = torch.bincount(ids, minlength=V).double()[:, None].cpu()
+    ref = m * table.double().cpu()
+    within(d, ref, 1.01 * ((m + 2) * U * ref.abs()) + 1e-30, "d_table")
+
+
+def test_vocab_loss_rows_past_32_bits(F):  # noqa: F811
+    """2^21 + 1 rows of 1,032 columns: x and dx have more than 2^31 elements."""
+    N, H, V = (1 << 21) + 1, 1032, 260
+    torch.manual_seed(102)
+    x = torch.empty(N, H, dtype=BF16, device=DEV).normal_()
+    w, b = (2 / math.sqrt(H) * torch.randn(V, H, device=DEV)).to(BF16), torch.randn(V, device=DEV)
+    t = torch.randint(0, V, (N,), device=DEV)
+    a = torch.randn(N, device=DEV) / N
+    got = vocab_run(F, x, w, b, t, a, (0,))
+    rows = torch.cat([torch.arange(130), torch.arange(N - 300, N), torch.randint(0, N, (300,), generator=gen(103))]).to(DEV)
+    ref = vocab_ref(x[rows].cpu(), w.cpu(), b.cpu(), t[rows].cpu(), a[rows].cpu(), (0,), BF16)
+    for n in ("loss", "lse", "dx"):
+        within(got[n][rows], *ref[n], n)
+    dw, db = torch.zeros(V, H, dtype=torch.float64, device=DEV), torch.zeros(V, dtype=torch.float64, device=DEV)
+    mag_w, mag_b = torch.zeros_like(dw), torch.zeros_like(db)
+    W, B = w.double().t().contiguous(), b.double()
+    for lo in range(0, N, 1 << 17):
+        r = slice(lo, lo + (1 << 17))
+        X = x[r].double()
+        d = torch.softmax(X @ W + B, 1)
+        d[torch.arange(d.shape[0]), t[r]] -= 1
+        d *= (a[r].double() * (t[r] != 0))[:, None]
+        D = d.t().contiguous()
+        dw += D @ X; db += d.sum(0)
+        mag_w += D.abs() @ X.abs(); mag_b += d.abs().sum(0)
+    # A logit: 1,035 U times sum |x w|, below 64 here.  A sum over the rows in fp32: at most 64 ranges of N / 64 / 64 tiles of 64 k, four additions each,
+    # and the join; the column sums: 2^14 partial sums of 128 rows, by 16
+    e = 2 * 1035 * U * 64 + 400 * U
+    within(got["dw"], dw.cpu(), (1.01 * ((half(BF16) + e + 2200 * U) * mag_w + half(BF16) * dw.abs())).cpu(), "dw")
+    within(got["db"], db.cpu(), (1.01 * (e + 1300 * U) * mag_b).cpu(), "db")
+
+
+@pytest.mark.parametrize("N,H,V,dtype", [(3, 8, (1 << 23) + 5, BF16), (5, (1 << 20) + 8, 7, BF16), (70, (1 << 18) + 4, 40, F32), ((1 << 20) + 9, 12, 33, F32)])
+def test_vocab_loss_with_one_very_long_size(F, N, H, V, dtype):  # noqa: F811
+    g = torch.Generator(device=DEV).manual_seed(104)
+    x = torch.randn(N, H, device=DEV, generator=g).to(dtype)
+    w = (2.0 / math.sqrt(H) * torch.randn(V, H, device=DEV, generator=g)).to(dtype)
+    t, a = torch.randint(0, V, (N,), device=DEV, generator=g), torch.randn(N, device=DEV, generator=g)
+    got = vocab_run(F, x, w, None, t, a, ())
+    ref = vocab_ref(x, w, None, t, a, (), dtype)
+    for n, r in ref.items():
+        if r is not None:
+            within(got[n], r[0].cpu(), r[1].cpu(), n)
+
+
+@pytest.mark.parametrize("dtype,N,H,V", [(BF16, 2600, 520, 3500), (F32, 700, 96, 4000)])
+def test_vocab_loss_in_a_graph_with_other_rows_counted(F, dtype, N, H, V):  # noqa: F811
+    """How many rows count is known on the device alone: one capture, replayed for none, one, some and all of them."""
+    x, w, b, t, a = on(*vocab_inputs(N, H, V, dtype, True, seed=97, ignore_share=0.0))
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        vocab_run(F, x, w, b, t, a, (0,))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = vocab_run(F, x, w, b, t, a, (0,))
+    words = t.clamp_min(1)
+    for seed, share in enumerate((0.5, 0.0, 1.0, 1.5 / N, 0.1)):
+        rows = torch.rand(N, generator=gen(98 + seed)) < share
+        t.copy_(torch.where(rows.to(DEV), words, torch.zeros_like(words)))
+        graph.replay()
+        eager = vocab_run(F, x, w, b, t, a, (0,))
+        torch.cuda.synchronize()
+        assert all(torch.equal(held[n], eager[n]) for n in held), share
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_attention_left_padding_in_a_graph(F, dtype):  # noqa: F811
+    """One capture, replayed for other paddings: rows without a key hold NaN."""
+    q, k, v, go, _ = on(*attn_inputs(2, 90, 90, 4, 2, 64, dtype, None, seed=99))
+    m = torch.ones(2, 90, dtype=torch.bool, device=DEV)
+    Q, G = q.clone(), go.clone()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        attn_run(F, Q, k, v, G, True, m)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = attn_run(F, Q, k, v, G, True, m)
+    for hidden in ((0, 0), (3, 61), (89, 1), (33, 90)):
+        m.copy_(torch.arange(90, device=DEV)[None] >= torch.tensor(hidden, device=DEV)[:, None])
+        for x, y in ((Q, q), (G, go)):
+            x.copy_(y.masked_fill(~m[:, :, None, None], math.nan))
+        graph.replay()
+        torch.cuda.synchronize()
+        attn_check(held, attn_ref(q.cpu(), k.cpu(), v.cpu(), go.cpu(), True, m.cpu(), 0.125, dtype))
